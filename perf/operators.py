@@ -262,7 +262,7 @@ def _plan_plain(s):
     need = torch.where(fits, torch.div(past + new + page - 1, page, rounding_mode="floor") - have, torch.zeros_like(have))
     upto = torch.cumsum(need, 0)
     ok = fits & ((need == 0) | (upto <= count))
-    popped = torch.where(ok, upto, torch.zeros_like(upto)).max()
+    popped = torch.where(ok & (need > 0), upto, torch.zeros_like(upto)).max()
     k = cols[None, :] - have[:, None]
     fresh = ok[:, None] & (k >= 0) & (k < need[:, None])
     page_id = ring[(head + (upto - need)[:, None] + k.clamp(min=0)) % n].long()
