@@ -264,6 +264,106 @@ int sqa_out_proj(const sqa_tensor *w, const sqa_tensor *x, const sqa_tensor *gat
                  void *workspace, size_t workspace_bytes, void *stream);
 
 /* ------------------------------------------------------------------------ */
+/* A batch of requests over one paged pool                                   */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * The pool of a layer holds n_pages pages of `page` token rows for K and the same
+ * for V, each row the cache's Hkv x 144 bytes of q4_0 blocks. A request owns the
+ * pages that its row of the page table lists, token p in page table[p / page]
+ * at row p % page. The three operators below are a step's way through it: the
+ * plan (which page and row every new token goes to), the writes (the existing
+ * sqa_set_rows_q4_0 and sqa_rope_norm_set_rows_q4_0 with the plan's slots as idx
+ * over the pool as n_pages * page rows; a slot of -1 is skipped there), the
+ * attention, and the adapters beside the W_o projection. The lengths stay on
+ * the device: a step can be captured into a graph once and replayed.
+ */
+
+/*
+ * Plan of one step for B places of the batch.
+ *   n_past     I32 [B]     tokens that each request has in the cache
+ *   n_new      I32 [B]     its new tokens; 0: none in this step; < 0: it has ended
+ *                          and its pages return to the pool
+ *   table      I32 [W, B]  page table, row stride nb[1] (updated)
+ *   ring       I32 [n_pages] the free pages, a ring (updated)
+ *   state      I32 [4]     {first free place of the ring, free pages, ., .}
+ *   page       tokens per page, a power of two in [16, 65536]
+ *   state_out  I32 [4]     {first, free, requests refused, tokens planned}
+ *   n_past_out I32 [B]     lengths after the step
+ *   q_start    I32 [B + 1] request b's tokens are rows q_start[b] .. q_start[b + 1] - 1
+ *   kv_len     I32 [B]     cached plus new tokens; 0 for refused and ended requests
+ *   slots      I64 [T]     pool row of every token, -1 for a refused one and behind the last
+ *   pos        I32 [4 * T] rotary positions t, h, w, e of every token (text: all equal)
+ * The pages of ended requests join the ring first (in the order of requests and
+ * table entries), then pages leave it in the order of requests. A request whose
+ * new pages are not all there, whose tokens pass the table's W pages or the T rows
+ * is refused: it gets no page, its slots are -1, its length stays. state_out and
+ * n_past_out must not overlap state and n_past (the caller swaps them or copies).
+ * All arrays contiguous but table. B <= 4096, W <= 2^18, W * page < 2^31, T <= 2^29.
+ */
+int sqa_paged_plan(const sqa_tensor *n_past, const sqa_tensor *n_new, const sqa_tensor *table,
+                   const sqa_tensor *ring, const sqa_tensor *state, int32_t page,
+                   const sqa_tensor *state_out, const sqa_tensor *n_past_out,
+                   const sqa_tensor *q_start, const sqa_tensor *kv_len, const sqa_tensor *slots,
+                   const sqa_tensor *pos, void *stream);
+
+/*
+ * Attention of every request's new tokens over its pages.
+ *   q       F32  [D, n_tok, H, 1]   as in sqa_flash_attn_ext, all requests' tokens
+ *   k, v    Q4_0 [D, Hkv, page, n_pages]  nb = 18, 144, Hkv * 144, page stride (a
+ *           multiple of 16, at least a page); 16-byte aligned
+ *   table   I32  [W, B]  row stride nb[1]
+ *   q_start I32  [B + 1], kv_len I32 [B]   as sqa_paged_plan writes them
+ *   prefix  I32  [B] or NULL: keys below prefix[b] are seen by every token of b
+ *   max_q   no request of the call has more new tokens than this
+ *   dst     F32  [D, H, n_tok, 1]   contiguous, 16-byte aligned
+ * Token i of request b (n = q_start[b + 1] - q_start[b] of them) sits at position
+ * p = kv_len[b] - n + i and sees key j < kv_len[b] where j <= p or j < prefix[b].
+ * Its logits are those of sqa_flash_attn_ext, s = scale * q8_0(Q) . K, then
+ *   s = logit_softcap * tanh(s / logit_softcap)       where logit_softcap > 0
+ *   s = s - slope(h) * |p - j|                         where max_bias > 0
+ * with ggml's slopes: for n = 2^floor(log2 H), 2^(-max_bias (h + 1) / n) for h < n
+ * and 2^(-max_bias / 2 (2 (h - n) + 1) / n) for the others. gate as in
+ * sqa_flash_attn_ext_causal. A token that sees no key gets zeros; rows of dst
+ * outside [q_start[0], q_start[B]) are left as they were. Keys of a page whose
+ * table entry is outside [0, n_pages) are not seen; no byte of keys that no token
+ * sees enters the result. The results of a call repeat bit for bit.
+ * D == 256, H / Hkv <= 16, page, B and W as for the plan. Requests with more than
+ * max_q tokens may be left as they were.
+ * workspace: sqa_paged_attn_workspace_size bytes; a smaller one (at least
+ * sqa_paged_attn_workspace_least) takes fewer splits of the keys.
+ */
+int sqa_paged_attn(const sqa_tensor *q, const sqa_tensor *k, const sqa_tensor *v,
+                   const sqa_tensor *table, const sqa_tensor *q_start, const sqa_tensor *kv_len,
+                   const sqa_tensor *prefix, int64_t max_q, float scale, float max_bias,
+                   float logit_softcap, const sqa_tensor *gate, const sqa_tensor *dst,
+                   void *workspace, size_t workspace_bytes, void *stream);
+size_t sqa_paged_attn_workspace_size(const sqa_tensor *q, const sqa_tensor *k, const sqa_tensor *table,
+                                     int64_t max_q);
+int sqa_supports_paged_attn(const sqa_tensor *q, const sqa_tensor *k, const sqa_tensor *v,
+                            const sqa_tensor *table, int64_t max_q, float scale, float max_bias,
+                            float logit_softcap, const sqa_tensor *dst);
+
+/*
+ * Low-rank adapters of many requests beside a shared projection:
+ *   dst[:, m] = base[:, m] + scale[i] * B_i (A_i (x[:, m] * sigmoid(gate[:, m]))),  i = ids[m]
+ *   base  F32 [N, M]  the shared projection's output; may be dst itself (no other overlap with dst)
+ *   x     F32 [K, M], gate F32 [K, M] or NULL (unit element stride)
+ *   a     F16 [K, r, n_adapters], b F16 [r, N, n_adapters]  contiguous, 16-byte aligned
+ *   ids   I32 [M]; an id outside [0, n_adapters) is a token without adapter
+ *   scale F32 [n_adapters] or NULL (1)
+ *   dst   F32 [N, M]
+ * Products are exact and sums fp32 where a token's own few rows are summed, and an
+ * fp16 hi + lo pair of x and of A x elsewhere (22 bits; |x|, |A x| < 65504).
+ * K % 256 == 0, N % 16 == 0, r % 8 == 0, r <= 128; base and dst rows 16-byte aligned.
+ */
+int sqa_lora_add(const sqa_tensor *base, const sqa_tensor *x, const sqa_tensor *gate, const sqa_tensor *a,
+                 const sqa_tensor *b, const sqa_tensor *ids, const sqa_tensor *scale,
+                 const sqa_tensor *dst, void *stream);
+int sqa_supports_lora_add(const sqa_tensor *base, const sqa_tensor *x, const sqa_tensor *gate,
+                          const sqa_tensor *a, const sqa_tensor *b, const sqa_tensor *dst);
+
+/* ------------------------------------------------------------------------ */
 /* KV cache bookkeeping (host only: no device calls)                         */
 /* ------------------------------------------------------------------------ */
 

@@ -13,7 +13,10 @@ Tensor conventions (torch shapes, C order, all on the GPU):
   cache   uint8   (rows, Hkv, D//32*18)   one q4_0 K or V cache (kv.rs:95-148)
   mask    float16 (n_q_pad, n_kv)         0 / -inf, or None
   out     float32 (n_q, H, D)             [D, H, n_q] attention output
+  pool    uint8   (n_pages, page, Hkv, D//32*18)  one paged q4_0 K or V cache of a batch
+  table   int32   (B, W)                  page ids of every request
 """
+import collections
 import ctypes
 import importlib.machinery
 import importlib.util
@@ -27,6 +30,8 @@ __all__ = [
     "flash_attn_ext_causal", "flash_attn_ext_static", "sigmoid_mul", "fill_causal_mask", "supports_flash_attn_ext",
     "flash_attn_workspace_size", "out_proj", "out_proj_workspace_size", "KvCache", "cache_view", "row_bytes", "profile_begin", "profile_end",
     "profile_get", "Rope", "rope_params", "rope_norm_set_rows_q4_0", "rope_norm_f32",
+    "paged_plan", "paged_attn", "paged_attn_workspace_size", "supports_paged_attn", "PagedStep", "PagedKvCache",
+    "lora_add", "supports_lora_add",
 ]
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -139,6 +144,12 @@ def lib():
             "sqa_kv_cache_k_view": (ctypes.c_int, [vp, i32, P]),
             "sqa_kv_cache_v_view": (ctypes.c_int, [vp, i32, P]),
             "sqa_kv_cache_append": (ctypes.c_int, [vp, i32, P, P, P, vp]),
+            "sqa_paged_plan": (ctypes.c_int, [P, P, P, P, P, i32, P, P, P, P, P, P, vp]),
+            "sqa_paged_attn": (ctypes.c_int, [P, P, P, P, P, P, P, i64, f32, f32, f32, P, P, vp, sz, vp]),
+            "sqa_paged_attn_workspace_size": (sz, [P, P, P, i64]),
+            "sqa_supports_paged_attn": (ctypes.c_int, [P, P, P, P, i64, f32, f32, f32, P]),
+            "sqa_lora_add": (ctypes.c_int, [P, P, P, P, P, P, P, P, vp]),
+            "sqa_supports_lora_add": (ctypes.c_int, [P, P, P, P, P, P]),
             "sqa_profile_begin": (ctypes.c_int, [i32]),
             "sqa_profile_end": (ctypes.c_int, []),
             "sqa_profile_get": (ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(ctypes.c_double),
@@ -461,6 +472,197 @@ def fill_causal_mask(mask, step_start, stream=None):
     return mask
 
 
+# ------------------------------------------- a batch over one paged pool --
+
+def _need(ok, msg):
+    if not ok:
+        raise SqaError(1, msg)
+
+
+def _on(device, **tensors):
+    """The tensors (None left out) are on one GPU; what follows runs with it as the current device."""
+    for name, t in tensors.items():
+        if t is not None:
+            _need(isinstance(t, torch.Tensor) and t.device == device, f"{name} must be a tensor on {device}")
+    _need(device.type == "cuda", "tensors must be on the GPU")
+    return torch.cuda.device(device)
+
+
+def _vec(t, dtype, name):
+    _need(t.dim() == 1 and t.dtype == dtype and t.is_contiguous(), f"{name} must be a contiguous 1-D {dtype} tensor")
+    code, size = (TYPE_I64, 8) if dtype == torch.int64 else (TYPE_F32 if dtype == torch.float32 else TYPE_I32, 4)
+    return Tensor.make(code, [t.shape[0]], [size], t.data_ptr())
+
+
+def _table_desc(table):
+    _need(table.dim() == 2 and table.dtype == torch.int32 and (table.shape[1] <= 1 or table.stride(1) == 1),
+          "table must be int32 (B, W) with contiguous rows")
+    return Tensor.make(TYPE_I32, [table.shape[1], table.shape[0]], [4, table.stride(0) * 4], table.data_ptr())
+
+
+def _pool_desc(pool, name):
+    _need(pool.dim() == 4 and pool.dtype == torch.uint8 and pool.shape[3] % Q4_0_BLOCK == 0 and
+          (pool.shape[0] <= 1 or pool.stride(0) > 0) and (pool.numel() == 0 or pool[0].is_contiguous()),
+          f"{name} must be uint8 (n_pages, page, Hkv, D // 32 * 18) with contiguous pages")
+    n_pages, page, Hkv, rb = pool.shape
+    step = pool.stride(0) if n_pages > 1 else page * Hkv * rb
+    return Tensor.make(TYPE_Q4_0, [rb // Q4_0_BLOCK * QK4_0, Hkv, page, n_pages], [Q4_0_BLOCK, rb, Hkv * rb, step],
+                       pool.data_ptr())
+
+
+def _tokens_desc(t, name):
+    """(n_tok, H, D) float32 -> [D, n_tok, H], any strides with contiguous elements."""
+    _need(t.dim() == 3 and t.dtype == torch.float32, f"{name} must be float32 (n_tok, H, D)")
+    return q_desc(t)
+
+
+def paged_plan(state, ring, table, n_past, n_new, page, slots, pos=None, state_out=None, n_past_out=None, q_start=None,
+               kv_len=None, stream=None):
+    """One step's plan for a batch, on the GPU: pages of ended requests (n_new < 0) return
+    to the ring of free ones, new tokens get their pages, every token its pool row
+    (slots, -1: none) and rotary positions. table and ring are updated in place; the
+    other results are (state_out, n_past_out, q_start, kv_len, slots, pos), made here
+    where they are not given, and returned as a PagedStep.
+
+    state: int32 (4,) {first free place of the ring, free pages, ., .}; ring: int32
+    (n_pages,); table: int32 (B, W); n_past, n_new: int32 (B,); slots: int64 (T,);
+    pos: int32 (4 * T,). A request that finds too few pages, too little room in its
+    table row or in slots is refused whole: state_out[2] counts them."""
+    def new(t, n):
+        return t if t is not None else torch.empty(n, dtype=torch.int32, device=slots.device)
+
+    B, T = table.shape[0], slots.shape[0]
+    step = PagedStep(new(state_out, 4), new(n_past_out, B), new(q_start, B + 1), new(kv_len, B), slots, new(pos, 4 * T))
+    if stream is None:
+        rc = (_host or _load_host()).plan(state, ring, table, n_past, n_new, page, *step)
+        if rc is not None:
+            if rc:
+                _check(rc)
+            return step
+    i32 = torch.int32
+    with _on(slots.device, state=state, ring=ring, table=table, n_past=n_past, n_new=n_new, state_out=step.state,
+             n_past_out=step.n_past, q_start=step.q_start, kv_len=step.kv_len, pos=step.pos):
+        d = [_vec(n_past, i32, "n_past"), _vec(n_new, i32, "n_new"), _table_desc(table), _vec(ring, i32, "ring"),
+             _vec(state, i32, "state")]
+        o = [_vec(step.state, i32, "state_out"), _vec(step.n_past, i32, "n_past_out"), _vec(step.q_start, i32, "q_start"),
+             _vec(step.kv_len, i32, "kv_len"), _vec(slots, torch.int64, "slots"), _vec(step.pos, i32, "pos")]
+        _check(lib().sqa_paged_plan(*[ctypes.byref(t) for t in d], int(page), *[ctypes.byref(t) for t in o],
+                                    _stream(stream)))
+    return step
+
+
+class PagedStep(collections.namedtuple("PagedStep", "state n_past q_start kv_len slots pos")):
+    """What paged_plan gives for one step (q_start, kv_len, slots and pos are the
+    operands of paged_attn, set_rows_q4_0 and the producers)."""
+
+    __slots__ = ()
+
+
+def paged_attn_workspace_size(q, k_pool, table, max_q):
+    """Workspace bytes of paged_attn for these shapes (a smaller one takes fewer splits)."""
+    tq, tk, tt = _tokens_desc(q, "q"), _pool_desc(k_pool, "k_pool"), _table_desc(table)
+    return int(lib().sqa_paged_attn_workspace_size(ctypes.byref(tq), ctypes.byref(tk), ctypes.byref(tt), int(max_q)))
+
+
+def supports_paged_attn(q, k_pool, table, max_q, scale=None, max_bias=0.0, softcap=0.0):
+    n_tok, H, D = q.shape
+    scale = D ** -0.5 if scale is None else scale
+    tq, tk, tt = _tokens_desc(q, "q"), _pool_desc(k_pool, "k_pool"), _table_desc(table)
+    to = Tensor.make(TYPE_F32, [D, H, n_tok, 1], [4, D * 4, H * D * 4], 16)
+    return bool(lib().sqa_supports_paged_attn(ctypes.byref(tq), ctypes.byref(tk), ctypes.byref(tk), ctypes.byref(tt),
+                                              int(max_q), scale, max_bias, softcap, ctypes.byref(to)))
+
+
+def paged_attn(q, k_pool, v_pool, table, q_start, kv_len, max_q, scale=None, max_bias=0.0, softcap=0.0, prefix=None,
+               gate=None, out=None, workspace=None, stream=None):
+    """Causal attention of every request's new tokens over its pages of one q4_0 pool.
+
+    q: float32 (n_tok, H, 256), request b's tokens in rows q_start[b] .. q_start[b + 1] - 1
+    at positions kv_len[b] - n .. kv_len[b] - 1; table, q_start, kv_len: int32 as
+    paged_plan writes them; max_q: the most new tokens of a request; prefix: int32 (B,),
+    keys that every token of the request sees; softcap, max_bias: tanh cap and distance
+    bias of the logits; gate: float32 like q, out *= sigmoid(gate). Rows of no request
+    are left as they were (zeros in an out made here)."""
+    if stream is None and out is not None and workspace is not None:
+        rc = (_host or _load_host()).paged_attn(q, k_pool, v_pool, table, q_start, kv_len, prefix, max_q, scale,
+                                                max_bias, softcap, gate, out, workspace)
+        if rc is not None:
+            if rc:
+                _check(rc)
+            return out
+    with _on(q.device, k_pool=k_pool, v_pool=v_pool, table=table, q_start=q_start, kv_len=kv_len, prefix=prefix,
+             gate=gate, out=out, workspace=workspace):
+        tq, tk, tv = _tokens_desc(q, "q"), _pool_desc(k_pool, "k_pool"), _pool_desc(v_pool, "v_pool")
+        n_tok, H, D = q.shape
+        scale = D ** -0.5 if scale is None else scale
+        if out is None:
+            out = torch.zeros((n_tok, H, D), dtype=torch.float32, device=q.device)
+        _need(out.dtype == torch.float32 and out.dim() == 3 and out.is_contiguous(), "out must be contiguous float32 (n_tok, H, D)")
+        tt, to = _table_desc(table), out_desc(out)
+        ts, tl = _vec(q_start, torch.int32, "q_start"), _vec(kv_len, torch.int32, "kv_len")
+        tp = None if prefix is None else _vec(prefix, torch.int32, "prefix")
+        tg = None
+        if gate is not None:
+            _need(gate.dim() == 3 and gate.dtype == torch.float32 and gate.shape == q.shape and
+                  (gate.shape[2] <= 1 or gate.stride(2) == 1), "gate must be float32 like q")
+            tg = Tensor.make(TYPE_F32, [D, H, n_tok, 1], [4, gate.stride(1) * 4, gate.stride(0) * 4], gate.data_ptr())
+        _need(q.shape[2] <= 1 or q.stride(2) == 1, "q rows must have unit element stride")
+        if workspace is None:
+            need = int(lib().sqa_paged_attn_workspace_size(ctypes.byref(tq), ctypes.byref(tk), ctypes.byref(tt), int(max_q)))
+            workspace, _ = _workspace(need, q.device)
+        _need(workspace is None or workspace.is_contiguous(), "workspace must be contiguous")
+        _check(lib().sqa_paged_attn(ctypes.byref(tq), ctypes.byref(tk), ctypes.byref(tv), ctypes.byref(tt), ctypes.byref(ts),
+                                    ctypes.byref(tl), _ref(tp), int(max_q), scale, max_bias, softcap, _ref(tg),
+                                    ctypes.byref(to), workspace.data_ptr() if workspace is not None else None,
+                                    workspace.numel() * workspace.element_size() if workspace is not None else 0,
+                                    _stream(stream)))
+    return out
+
+
+def _lora_descs(base, x, a, b, gate, out):
+    for t, name in ((base, "base"), (x, "x"), (gate, "gate"), (out, "out")):
+        _need(t is None or (t.dim() == 2 and t.dtype == torch.float32 and (t.shape[1] <= 1 or t.stride(1) == 1)),
+              f"{name} must be float32 rows with contiguous elements")
+    for t, name in ((a, "a"), (b, "b")):
+        _need(t.dim() == 3 and t.dtype == torch.float16 and t.is_contiguous(), f"{name} must be contiguous float16 of 3 dims")
+
+    def rows(t):
+        return None if t is None else Tensor.make(TYPE_F32, [t.shape[1], t.shape[0]], [4, t.stride(0) * 4], t.data_ptr())
+
+    ta, tb = (Tensor.make(TYPE_F16, [t.shape[2], t.shape[1], t.shape[0]],
+                          [2, 2 * t.shape[2], 2 * t.shape[2] * t.shape[1]], t.data_ptr()) for t in (a, b))
+    return rows(base), rows(x), rows(gate), ta, tb, rows(out)
+
+
+def supports_lora_add(base, x, a, b, gate=None, out=None):
+    td, tx, tg, ta, tb, to = _lora_descs(base, x, a, b, gate, base if out is None else out)
+    return bool(lib().sqa_supports_lora_add(_ref(td), _ref(tx), _ref(tg), _ref(ta), _ref(tb), _ref(to)))
+
+
+def lora_add(base, x, a, b, ids, scale=None, gate=None, out=None, stream=None):
+    """out = base + scale[i] * (x * sigmoid(gate)) @ a[i]^T @ b[i]^T with i = ids[m] for token m:
+    the low-rank adapters of a batch's requests beside a shared projection (out_proj).
+
+    base: float32 (M, N), may be out; x, gate: float32 (M, K); a: float16 (n, r, K);
+    b: float16 (n, N, r); ids: int32 (M,), an id outside [0, n) is a token without
+    adapter; scale: float32 (n,) or None."""
+    if stream is None and out is not None:
+        rc = (_host or _load_host()).lora(base, x, a, b, ids, scale, gate, out)
+        if rc is not None:
+            if rc:
+                _check(rc)
+            return out
+    with _on(x.device, base=base, a=a, b=b, ids=ids, scale=scale, gate=gate, out=out):
+        if out is None:
+            out = torch.empty_like(base, memory_format=torch.contiguous_format)
+        td, tx, tg, ta, tb, to = _lora_descs(base, x, a, b, gate, out)
+        ti = _vec(ids, torch.int32, "ids")
+        ts = None if scale is None else _vec(scale, torch.float32, "scale")
+        _check(lib().sqa_lora_add(_ref(td), _ref(tx), _ref(tg), _ref(ta), _ref(tb), _ref(ti), _ref(ts), _ref(to),
+                                  _stream(stream)))
+    return out
+
+
 def profile_begin(max_records=4096):
     """Bracket every kernel launch with HIP events until profile_end()."""
     _check(lib().sqa_profile_begin(max_records))
@@ -579,3 +781,70 @@ class KvCache:
         _check(lib().sqa_flash_attn_ext(ctypes.byref(tq), ctypes.byref(tk), ctypes.byref(tv), _ref(tm), scale,
                                         0.0, 0.0, ctypes.byref(to), wptr, wbytes, _stream(stream)))
         return out
+
+
+# ----------------------------------------------------------- PagedKvCache ---
+
+class PagedKvCache:
+    """q4_0 KV cache of many requests in pages of one pool, KvCache's counterpart for a batch.
+
+    Owns one K and one V pool per layer, uint8 (n_pages, page, Hkv, D//32*18), the page
+    table (max_requests, max_pages) and the lengths; a request is a place of the batch.
+    All bookkeeping runs on the GPU: plan() then append() and attend() of every layer
+    make up a step that can be captured into a graph and replayed with other n_new."""
+
+    def __init__(self, n_layers, head_dim, n_head_kv, n_pages, page, max_requests, max_pages, device="cuda"):
+        _need(n_layers >= 1 and n_pages >= 1 and max_requests >= 1 and max_pages >= 1 and n_head_kv >= 1 and
+              head_dim % QK4_0 == 0 and page >= 16 and page & (page - 1) == 0, "invalid paged KV cache geometry")
+        self.head_dim, self.n_head_kv, self.page = head_dim, n_head_kv, page
+        shape = (n_pages, page, n_head_kv, row_bytes(head_dim))
+        self.k = [torch.empty(shape, dtype=torch.uint8, device=device) for _ in range(n_layers)]
+        self.v = [torch.empty(shape, dtype=torch.uint8, device=device) for _ in range(n_layers)]
+        i32 = dict(dtype=torch.int32, device=device)
+        self.table = torch.full((max_requests, max_pages), -1, **i32)
+        self.ring = torch.arange(n_pages, **i32)
+        # {first, free, refused, tokens} and the lengths, and the same after the step being planned
+        self._now, self._next = torch.zeros(4 + max_requests, **i32), torch.zeros(4 + max_requests, **i32)
+        self._now[1] = n_pages
+
+    @property
+    def state(self):
+        """int32 (4,) on the GPU: first free place of the ring, free pages, requests the last plan refused, its tokens."""
+        return self._now[:4]
+
+    @property
+    def n_past(self):
+        """int32 (max_requests,) on the GPU: tokens of every request."""
+        return self._now[4:]
+
+    def new_step(self, n_rows):
+        """Buffers of a step of up to n_rows tokens (kept by the caller, reused step after step)."""
+        i32, B, dev = torch.int32, self.table.shape[0], self.table.device
+        return PagedStep(self._next[:4], self._next[4:], torch.zeros(B + 1, dtype=i32, device=dev),
+                         torch.zeros(B, dtype=i32, device=dev), torch.zeros(n_rows, dtype=torch.int64, device=dev),
+                         torch.zeros(4 * n_rows, dtype=i32, device=dev))
+
+    def plan(self, n_new, step):
+        """Gives the step's new tokens (n_new: int32 (max_requests,), < 0 ends a request) their pages."""
+        with torch.cuda.device(self.table.device):
+            paged_plan(self.state, self.ring, self.table, self.n_past, n_new, self.page, step.slots, step.pos,
+                       step.state, step.n_past, step.q_start, step.kv_len)
+            self._now.copy_(self._next)
+        return step
+
+    def rows(self, layer, which="k"):
+        """Layer's K or V pool as cache rows (n_pages * page, Hkv, bytes): where slots point."""
+        return (self.k if which == "k" else self.v)[layer].view(-1, self.n_head_kv, row_bytes(self.head_dim))
+
+    def append(self, layer, k_cur, v_cur, step, stream=None):
+        """Quantize the step's K and V rows, float32 (n_rows, Hkv*D), into the layer's pages."""
+        set_rows_q4_0(self.rows(layer, "k"), k_cur, step.slots, stream)
+        set_rows_q4_0(self.rows(layer, "v"), v_cur, step.slots, stream)
+
+    def workspace_size(self, q, max_q):
+        return paged_attn_workspace_size(q, self.k[0], self.table, max_q)
+
+    def attend(self, layer, q, step, max_q, **options):
+        """paged_attn of the step's tokens over the layer's pages (options: scale, max_bias, softcap, prefix, gate,
+        out, workspace, stream)."""
+        return paged_attn(q, self.k[layer], self.v[layer], self.table, step.q_start, step.kv_len, max_q, **options)

@@ -13,7 +13,9 @@
 #include <Python.h>
 
 #include <cmath>
+#include <initializer_list>
 
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -252,10 +254,121 @@ PyObject *append(PyObject *, PyObject *const *a, Py_ssize_t n) {
     });
 }
 
+// one-dimensional contiguous tensor
+sqa_tensor vec(const at::Tensor &t, at::ScalarType dtype, int type) {
+    need(t.dim() == 1 && t.scalar_type() == dtype && t.is_contiguous());
+    const int64_t n = t.size(0), e = (int64_t)t.element_size();
+    return make(type, t, n, 1, 1, e, e * n, e * n, e * n);
+}
+sqa_tensor ints(const at::Tensor &t) { return vec(t, at::kInt, SQA_TYPE_I32); }
+
+sqa_tensor table_view(const at::Tensor &t) {  // (B, W) -> [W, B]
+    need(t.dim() == 2 && t.scalar_type() == at::kInt && (t.size(1) <= 1 || t.stride(1) == 1));
+    const int64_t s = t.stride(0) * 4;
+    return make(SQA_TYPE_I32, t, t.size(1), t.size(0), 1, 4, s, s * t.size(0), s * t.size(0));
+}
+
+sqa_tensor pool_view(const at::Tensor &t) {  // (n_pages, page, Hkv, bytes) -> [D, Hkv, page, n_pages]
+    need(t.dim() == 4 && t.scalar_type() == at::kByte);
+    const int64_t n = t.size(0), page = t.size(1), Hkv = t.size(2), rb = t.size(3);
+    need(n >= 1 && rb % SQA_Q4_0_BLOCK_BYTES == 0 && t.stride(3) == 1 && (Hkv == 1 || t.stride(2) == rb) &&
+         (page == 1 || t.stride(1) == Hkv * rb) && (n == 1 || t.stride(0) > 0));
+    sqa_tensor d = make(SQA_TYPE_Q4_0, t, rb / SQA_Q4_0_BLOCK_BYTES * SQA_QK4_0, Hkv, page, SQA_Q4_0_BLOCK_BYTES, rb,
+                        Hkv * rb, n == 1 ? page * Hkv * rb : t.stride(0));
+    d.ne[3] = n;
+    return d;
+}
+
+// every tensor of a call on the current device (the general path switches to theirs)
+void here(std::initializer_list<PyObject *> ts) {
+    const int dev = (int)c10::hip::current_device();
+    for (PyObject *o : ts) {
+        if (o == Py_None) continue;
+        const at::Tensor &t = tensor(o);
+        need(t.is_cuda() && t.get_device() == dev);
+    }
+}
+
+// state, ring, table, n_past, n_new, page, then the step: state, n_past, q_start, kv_len, slots, pos
+PyObject *plan(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    return answer([&]() -> int {
+        need(n == 12);
+        here({a[0], a[1], a[2], a[3], a[4], a[6], a[7], a[8], a[9], a[10], a[11]});
+        const sqa_tensor st = ints(tensor(a[0])), ring = ints(tensor(a[1])), tab = table_view(tensor(a[2])),
+                         past = ints(tensor(a[3])), fresh = ints(tensor(a[4])), so = ints(tensor(a[6])),
+                         po = ints(tensor(a[7])), qs = ints(tensor(a[8])), kl = ints(tensor(a[9])),
+                         sl = vec(tensor(a[10]), at::kLong, SQA_TYPE_I64), pos = ints(tensor(a[11]));
+        const int64_t page = integer(a[5]);
+        need(page == (int64_t)(int32_t)page);
+        void *s = stream();
+        return without_gil([&] {
+            return sqa_paged_plan(&past, &fresh, &tab, &ring, &st, (int32_t)page, &so, &po, &qs, &kl, &sl, &pos, s);
+        });
+    });
+}
+
+// q, k_pool, v_pool, table, q_start, kv_len, prefix, max_q, scale, max_bias, softcap, gate, out, workspace
+PyObject *paged_attn(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    return answer([&]() -> int {
+        need(n == 14);
+        here({a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[11], a[12], a[13]});
+        const at::Tensor &q = tensor(a[0]), &o = tensor(a[12]), &ws = tensor(a[13]);
+        need(q.dim() == 3 && q.scalar_type() == at::kFloat && o.scalar_type() == at::kFloat && ws.is_contiguous() &&
+             (q.size(2) <= 1 || q.stride(2) == 1));
+        const sqa_tensor tq = q_view(q), tk = pool_view(tensor(a[1])), tv = pool_view(tensor(a[2])),
+                         tt = table_view(tensor(a[3])), ts = ints(tensor(a[4])), tl = ints(tensor(a[5])), to = out_view(o);
+        sqa_tensor tp, tg;
+        const bool prefix = a[6] != Py_None, gate = a[11] != Py_None;
+        if (prefix) tp = ints(tensor(a[6]));
+        if (gate) {
+            const at::Tensor &t = tensor(a[11]);
+            need(t.dim() == 3 && t.scalar_type() == at::kFloat && t.sizes() == q.sizes() && (t.size(2) <= 1 || t.stride(2) == 1));
+            tg = make(SQA_TYPE_F32, t, q.size(2), q.size(1), q.size(0), 4, t.stride(1) * 4, t.stride(0) * 4,
+                      t.stride(0) * 4 * q.size(0));
+        }
+        const int64_t max_q = integer(a[7]);
+        const float scale = scale_of(a[8], q), bias = (float)real(a[9]), cap = (float)real(a[10]);
+        void *wp = ws.data_ptr(), *st = stream();
+        const size_t wb = (size_t)ws.nbytes();
+        return without_gil([&] {
+            return sqa_paged_attn(&tq, &tk, &tv, &tt, &ts, &tl, prefix ? &tp : nullptr, max_q, scale, bias, cap,
+                                  gate ? &tg : nullptr, &to, wp, wb, st);
+        });
+    });
+}
+
+// base, x, a, b, ids, scale, gate, out
+PyObject *lora(PyObject *, PyObject *const *p, Py_ssize_t n) {
+    return answer([&]() -> int {
+        need(n == 8);
+        here({p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]});
+        auto rows = [](const at::Tensor &t) {
+            need(t.dim() == 2 && t.scalar_type() == at::kFloat && (t.size(1) <= 1 || t.stride(1) == 1));
+            return rows2(t, t.size(1), t.size(0));
+        };
+        auto half3 = [](const at::Tensor &t) {
+            need(t.dim() == 3 && t.scalar_type() == at::kHalf && t.is_contiguous());
+            const int64_t n0 = t.size(2), n1 = t.size(1), n2 = t.size(0);
+            return make(SQA_TYPE_F16, t, n0, n1, n2, 2, 2 * n0, 2 * n0 * n1, 2 * n0 * n1 * n2);
+        };
+        const sqa_tensor td = rows(tensor(p[0])), tx = rows(tensor(p[1])), ta = half3(tensor(p[2])), tb = half3(tensor(p[3])),
+                         ti = ints(tensor(p[4])), to = rows(tensor(p[7]));
+        sqa_tensor ts, tg;
+        const bool scale = p[5] != Py_None, gate = p[6] != Py_None;
+        if (scale) ts = vec(tensor(p[5]), at::kFloat, SQA_TYPE_F32);
+        if (gate) tg = rows(tensor(p[6]));
+        void *st = stream();
+        return without_gil([&] {
+            return sqa_lora_add(&td, &tx, gate ? &tg : nullptr, &ta, &tb, &ti, scale ? &ts : nullptr, &to, st);
+        });
+    });
+}
+
 PyMethodDef methods[] = {
 #define SQA_FN(f) {#f, (PyCFunction)(void (*)(void))f, METH_FASTCALL, nullptr}
     SQA_FN(fa),        SQA_FN(fa_causal), SQA_FN(fill_mask), SQA_FN(set_rows),
-    SQA_FN(rope_norm), SQA_FN(out_proj),  SQA_FN(append),    {nullptr, nullptr, 0, nullptr},
+    SQA_FN(rope_norm), SQA_FN(out_proj),  SQA_FN(append),    SQA_FN(plan),
+    SQA_FN(paged_attn), SQA_FN(lora),     {nullptr, nullptr, 0, nullptr},
 #undef SQA_FN
 };
 
