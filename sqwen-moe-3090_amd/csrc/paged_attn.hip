@@ -1,33 +1,15 @@
-// paged_attn.hip - attention of a batch of requests over a paged q4_0 pool.
+// paged_attn.hip - attention of a batch of requests over a paged q4_0 pool: what a
+// call launches, its workspace, and the merge of split partials.
 //
-// One workgroup per (token, query head): its 4 wavefronts walk the keys in turn, a
-// lane holding 4 of the 256 dims, each with a softmax of its own that is kept
-// online (running maximum and sum); the four are merged through LDS.
-#include "paged.hpp"
+// Requests of few query rows (up to 16 per KV head) go to paged_decode.hip, the
+// others to one workgroup per (token, query head).
+#include "paged_attn.hpp"
 
 namespace sqa {
+namespace paged {
 namespace {
 
 constexpr int kThreads = 256;
-
-struct Params {
-    const char *q;
-    int64_t q_nb1, q_nb2;
-    const uint8_t *k, *v;
-    int64_t row_bytes, k_page, v_page;
-    int32_t n_pages;
-    int page, lp;
-    const int32_t *table;
-    int64_t table_stride;
-    int W, B;
-    const int32_t *q_start, *kv_len, *prefix;
-    int n_tok, H, G;
-    float scale, cap, bias;
-    int nl2;
-    const char *gate;
-    int64_t gate_nb1, gate_nb2;
-    float *dst;
-};
 
 __device__ __forceinline__ float h2f(uint16_t b) {
     _Float16 f;
@@ -35,7 +17,7 @@ __device__ __forceinline__ float h2f(uint16_t b) {
     return (float)f;
 }
 
-__global__ __launch_bounds__(kThreads) void paged_attn_kernel(Params p) {
+__global__ __launch_bounds__(kThreads) void token_kernel(Call p) {
     __shared__ int found;
     __shared__ float xo[4][256], xm[4], xl[4];
     const int t = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
@@ -47,11 +29,10 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(Params p) {
     const int b = found;
     if (b < 0) return;
     const int kvh = h / p.G;
-    const int64_t kv = min((int64_t)max(p.kv_len[b], 0), (int64_t)p.W << p.lp);
-    const int64_t pos = (int64_t)p.kv_len[b] - p.q_start[b + 1] + t;
-    int64_t see = pos + 1;
-    if (p.prefix) see = max(see, (int64_t)p.prefix[b]);
-    see = min(see, kv);
+    const Request rq = request(p, b);
+    if (rq.n * p.G <= p.most_d) return;
+    if (h == 0 && tid == 0) p.where[t] = make_int4(0, 0, 0, kDone);
+    const int64_t pos = rq.pos0 + t - rq.q0, see = sees(rq, t - rq.q0);
     // dims of the lane: elements 2i, 2i + 1, 16 + 2i, 17 + 2i of block blk
     const int blk = lane >> 3, i = lane & 7;
     const float *qr = reinterpret_cast<const float *>(p.q + t * p.q_nb1 + h * p.q_nb2) + 32 * blk + 2 * i;
@@ -60,11 +41,9 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(Params p) {
     for (int j = 0; j < 4; ++j) amax = fmaxf(amax, fabsf(q[j]));
     for (int o = 1; o < 8; o <<= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
     const float id = amax != 0.0f ? 127.f / amax : 0.0f;
-    const float qd = (float)(_Float16)(amax / 127.f) * p.scale;
+    const float qd = (float)(_Float16)(amax / 127.f) * (p.qscale / kLog2e);
     for (int j = 0; j < 4; ++j) q[j] = rintf(q[j] * id) * qd;
-    const float slope = p.bias == 0.0f ? 0.0f
-                        : h < p.nl2    ? exp2f(-p.bias * (float)(h + 1) / (float)p.nl2)
-                                       : exp2f(-0.5f * p.bias * (float)(2 * (h - p.nl2) + 1) / (float)p.nl2);
+    const float slope = p.bias == 0.0f ? 0.0f : slope2(p, h) / kLog2e;
     float m = -INFINITY, l = 0.0f, o[4] = {0.f, 0.f, 0.f, 0.f};
     for (int64_t j = wave; j < see; j += 4) {
         const int32_t id_p = p.table[b * p.table_stride + (j >> p.lp)];
@@ -77,7 +56,7 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(Params p) {
         float s = kd * (q[0] * (float)((int)(kc & 15) - 8) + q[1] * (float)((int)(kc >> 8 & 15) - 8) +
                         q[2] * (float)((int)(kc >> 4 & 15) - 8) + q[3] * (float)((int)(kc >> 12) - 8));
         for (int x = 1; x < 64; x <<= 1) s += __shfl_xor(s, x);
-        if (p.cap != 0.0f) s = p.cap * tanhf(s / p.cap);
+        if (p.cap2 != 0.0f) s = p.cap2 / kLog2e * tanhf(s * kLog2e * p.cap_inv);
         s -= slope * fabsf((float)(pos - j));
         const float mn = fmaxf(m, s), al = expf(m - mn), w = expf(s - mn);
         m = mn;
@@ -108,33 +87,235 @@ __global__ __launch_bounds__(kThreads) void paged_attn_kernel(Params p) {
     p.dst[((int64_t)t * p.H + h) * kHeadDim + tid] = r;
 }
 
+
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+// Merge of a row's partials: out = sum_s acc_s e^(m_s - M) / sum_s l_s e^(m_s - M), M = max m_s,
+// then the gate. A partial whose m is -inf (no key seen) may hold anything.
+struct Row {
+    const float *acc, *ml;  // of the row in its first slot
+    int64_t step;           // floats of acc between its splits (ml: step / 128)
+    int n;                  // 0: nothing to do
+};
+
+__device__ __forceinline__ Row row_of(const Call &c, int t, int h) {
+    Row r{nullptr, nullptr, 0, 0};
+    const int4 w = c.where[t];
+    if (t < c.q_start[0] || t >= c.q_start[c.B]) return r;  // of no request: w was not written
+    const int form = w.w & 3, step = w.w >> 2, kvh = h / c.G, row = w.z + h - kvh * c.G;
+    const int heads = form == kFew ? 1 : w.y * step, rows = form == kFew ? c.rows_d : c.rows_c;
+    const int64_t first = w.x + (int64_t)kvh * heads;
+    // (arrays that are no plan's may leave an entry of an earlier call here)
+    if (form == kDone || w.x < 0 || step < 1 || w.y < 1 || w.y > 256 || row < 0 || row >= rows ||
+        first + (int64_t)(w.y - 1) * step >= (form == kFew ? c.slots_d : c.slots_c))
+        return r;
+    const int64_t at = first * rows + row;
+    r.acc = (form == kFew ? c.acc_d : c.acc_c) + at * 256;
+    r.ml = (form == kFew ? c.ml_d : c.ml_c) + at * 2;
+    r.step = (int64_t)step * rows * 256;
+    r.n = w.y;
+    return r;
+}
+
+__device__ __forceinline__ float gated(const Call &c, int t, int h, int d, float r) {
+    if (!c.gate) return r;
+    const float g = reinterpret_cast<const float *>(c.gate + t * c.gate_nb2 + h * c.gate_nb1)[d];
+    return r * (1.0f / (1.0f + expf(-g)));
+}
+
+// Few rows of many splits: 16 workgroups per row, 16 dims each; a thread holds one dim
+// of every 16th split, all its loads in flight together.
+__global__ __launch_bounds__(kThreads) void merge_dims_kernel(Call c) {
+    __shared__ float xm[4], xl[4], xo[4][16];
+    const int t = blockIdx.x / c.H, h = blockIdx.x - t * c.H;
+    const Row r = row_of(c, t, h);
+    if (r.n == 0) return;
+    const int tid = threadIdx.x, dl = tid & 15, sg = tid >> 4, d = blockIdx.y * 16 + dl;
+    float acc[16];
+    float2 ml[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        const int s = sg + 16 * j;
+        const bool ok = s < r.n;
+        acc[j] = ok ? r.acc[s * r.step + d] : 0.0f;
+        ml[j] = ok ? *reinterpret_cast<const float2 *>(r.ml + s * (r.step / 128)) : make_float2(-INFINITY, 0.0f);
+    }
+    float m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) m = fmaxf(m, ml[j].x);
+    m = fmaxf(m, __shfl_xor(m, 16));
+    m = fmaxf(m, __shfl_xor(m, 32));
+    if ((tid & 63) == 0) xm[tid >> 6] = m;
+    __syncthreads();
+    const float M = fmaxf(fmaxf(xm[0], xm[1]), fmaxf(xm[2], xm[3]));
+    float o = 0.0f, l = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        const bool dead = ml[j].x == -INFINITY;
+        const float w = dead ? 0.0f : __builtin_amdgcn_exp2f((ml[j].x - M) * kLog2e);
+        o = dead ? o : fmaf(acc[j], w, o);
+        l = dead ? l : fmaf(ml[j].y, w, l);
+    }
+    o += __shfl_xor(o, 16);
+    o += __shfl_xor(o, 32);
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if ((tid & 63) < 16) xo[tid >> 6][dl] = o;
+    if ((tid & 63) == 0) xl[tid >> 6] = l;
+    __syncthreads();
+    if (tid < 16) {
+        const float L = (xl[0] + xl[1]) + (xl[2] + xl[3]), O = (xo[0][dl] + xo[1][dl]) + (xo[2][dl] + xo[3][dl]);
+        c.dst[((int64_t)t * c.H + h) * kHeadDim + d] = gated(c, t, h, d, L == 0.0f ? 0.0f : O / L);
+    }
+}
+
+// Many rows: a wavefront per row, 4 dims a lane; the heads of a token in turn.
+__global__ __launch_bounds__(kThreads) void merge_rows_kernel(Call c, int heads) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int groups = (c.H + heads - 1) / heads;  // of a token
+    const int id = (int)blockIdx.x * 4 + wave;
+    const int t = id / groups, h0 = (id - t * groups) * heads;
+    if (t >= c.n_tok) return;
+    for (int h = h0; h < min(h0 + heads, c.H); ++h) {
+        const Row r = row_of(c, t, h);
+        if (r.n == 0) return;
+        constexpr int kBatch = 8;
+        float M = -INFINITY, L = 0.0f;
+        floatx4 o = {0.f, 0.f, 0.f, 0.f};
+        for (int s0 = 0; s0 < r.n; s0 += 64) {  // 64 splits' weights at a time
+            const int s = s0 + lane;
+            const float2 ml = s < r.n ? *reinterpret_cast<const float2 *>(r.ml + s * (r.step / 128)) : make_float2(-INFINITY, 0.0f);
+            float m = ml.x;
+#pragma unroll
+            for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
+            if (m == -INFINITY) continue;
+            const float Mn = fmaxf(M, m), al = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((M - Mn) * kLog2e);
+            const float w = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((ml.x - Mn) * kLog2e);
+            float l = ml.x == -INFINITY ? 0.0f : ml.y * w;
+#pragma unroll
+            for (int x = 1; x < 64; x <<= 1) l += __shfl_xor(l, x);
+            L = L * al + l;
+            o *= al;
+            M = Mn;
+            const int end = min(r.n - s0, 64);
+            for (int s1 = 0; s1 < end; s1 += kBatch) {
+                floatx4 a[kBatch];
+                float wt[kBatch];
+#pragma unroll
+                for (int j = 0; j < kBatch; ++j) {
+                    wt[j] = s1 + j < end ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), s1 + j)) : 0.0f;
+                    if (wt[j] != 0.0f) a[j] = *reinterpret_cast<const floatx4 *>(r.acc + (s0 + s1 + j) * r.step + 4 * lane);
+                }
+#pragma unroll
+                for (int j = 0; j < kBatch; ++j)
+                    if (wt[j] != 0.0f) o += a[j] * wt[j];
+            }
+        }
+        float *out = c.dst + ((int64_t)t * c.H + h) * kHeadDim + 4 * lane;
+        floatx4 x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = gated(c, t, h, 4 * lane + i, L == 0.0f ? 0.0f : o[i] / L);
+        *reinterpret_cast<floatx4 *>(out) = x;
+    }
+}
+
+size_t al256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+// Workspace of a call: the tokens' entries, then the slots of the few-row kernel.
+struct Plan {
+    int most_d, rows_d;   // of Call
+    bool few, many;       // which kernels run
+    int64_t slots_d, least_d;
+    size_t where, slot_d;
+};
+
+Plan plan(int64_t n_tok, int64_t H, int64_t Hkv, int64_t B, int64_t max_q) {
+    Plan p{};
+    const int64_t G = H / Hkv, rows = (max_q < n_tok ? max_q : n_tok) * G;
+    p.most_d = rows <= 8 || (rows > 16 && G <= 8) ? 8 : 16;
+    p.rows_d = p.most_d;
+    p.many = rows > p.most_d;
+    p.few = true;
+    const int64_t active = B < n_tok ? B : n_tok;
+    int64_t P = 2 * device_cu_count() / Hkv;
+    if (P < 1) P = 1;
+    p.slots_d = (P + active) * Hkv;
+    p.least_d = (1 + active) * Hkv;
+    p.where = al256((size_t)n_tok * 16);
+    p.slot_d = (size_t)p.rows_d * (kHeadDim + 2) * 4;
+    return p;
+}
+
 }  // namespace
 
-size_t paged_attn_workspace(int64_t, int64_t, int64_t, int64_t, int64_t) { return 0; }
+int launch_combine(const Call &c, hipStream_t s) {
+    const int prof = profile_start("paged_merge", s);
+    const int64_t rows = (int64_t)c.n_tok * c.H;
+    if (rows <= 128) {
+        merge_dims_kernel<<<dim3((unsigned)rows, 16), dim3(kThreads), 0, s>>>(c);
+    } else {
+        const int heads = c.n_tok <= 1024 ? 1 : c.H;
+        const int64_t waves = (int64_t)c.n_tok * ((c.H + heads - 1) / heads);
+        merge_rows_kernel<<<dim3((unsigned)((waves + 3) / 4)), dim3(kThreads), 0, s>>>(c, heads);
+    }
+    profile_stop(prof, s);
+    return hip_status(hipGetLastError(), "paged_attn merge launch");
+}
+
+}  // namespace paged
+
+using namespace paged;
+
+size_t paged_attn_workspace(int64_t n_tok, int64_t H, int64_t Hkv, int64_t B, int64_t max_q) {
+    if (n_tok < 1) return 0;
+    const Plan p = plan(n_tok, H, Hkv, B, max_q);
+    return p.where + al256((size_t)p.slots_d * p.slot_d) + 256;
+}
 
 int launch_paged_attn(const PagedArgs &a, hipStream_t s) {
     const sqa_tensor &q = *a.q, &k = *a.k;
-    Params p{};
-    p.q = (const char *)q.data, p.q_nb1 = (int64_t)q.nb[1], p.q_nb2 = (int64_t)q.nb[2];
-    p.k = (const uint8_t *)k.data, p.v = (const uint8_t *)a.v->data;
-    p.row_bytes = (int64_t)k.nb[2], p.k_page = (int64_t)k.nb[3], p.v_page = (int64_t)a.v->nb[3];
-    p.n_pages = (int32_t)k.ne[3], p.page = (int)k.ne[2];
-    while ((1 << p.lp) < p.page) ++p.lp;
-    p.table = (const int32_t *)a.table->data, p.table_stride = (int64_t)a.table->nb[1] / 4;
-    p.W = (int)a.table->ne[0], p.B = (int)a.table->ne[1];
-    p.q_start = (const int32_t *)a.q_start->data, p.kv_len = (const int32_t *)a.kv_len->data;
-    p.prefix = a.prefix ? (const int32_t *)a.prefix->data : nullptr;
-    p.n_tok = (int)q.ne[1], p.H = (int)q.ne[2], p.G = (int)(q.ne[2] / k.ne[1]);
-    p.scale = a.scale, p.cap = a.softcap, p.bias = a.max_bias;
-    p.nl2 = 1;
-    while (2 * p.nl2 <= p.H) p.nl2 *= 2;
-    p.gate = a.gate ? (const char *)a.gate->data : nullptr;
-    p.gate_nb1 = a.gate ? (int64_t)a.gate->nb[1] : 0, p.gate_nb2 = a.gate ? (int64_t)a.gate->nb[2] : 0;
-    p.dst = (float *)a.dst->data;
-    const int prof = profile_start("paged_attn", s);
-    paged_attn_kernel<<<dim3((unsigned)p.n_tok, (unsigned)p.H), dim3(kThreads), 0, s>>>(p);
-    profile_stop(prof, s);
-    return hip_status(hipGetLastError(), "paged_attn launch");
+    Call c{};
+    c.q = (const char *)q.data, c.q_nb1 = (int64_t)q.nb[1], c.q_nb2 = (int64_t)q.nb[2];
+    c.k = (const uint8_t *)k.data, c.v = (const uint8_t *)a.v->data;
+    c.k_page = (int64_t)k.nb[3], c.v_page = (int64_t)a.v->nb[3];
+    c.row_bytes = (int)k.nb[2];
+    c.n_pages = (int)k.ne[3], c.page = (int)k.ne[2];
+    while ((1 << c.lp) < c.page) ++c.lp;
+    c.table = (const int32_t *)a.table->data, c.table_stride = (int64_t)a.table->nb[1] / 4;
+    c.most_kv = a.table->ne[0] << c.lp;
+    c.B = (int)a.table->ne[1];
+    c.q_start = (const int32_t *)a.q_start->data, c.kv_len = (const int32_t *)a.kv_len->data;
+    c.prefix = a.prefix ? (const int32_t *)a.prefix->data : nullptr;
+    c.n_tok = (int)q.ne[1], c.H = (int)q.ne[2], c.Hkv = (int)k.ne[1], c.G = c.H / c.Hkv;
+    c.qscale = a.scale * kLog2e;
+    c.cap2 = a.softcap * kLog2e, c.cap_inv = a.softcap > 0.0f ? 1.0f / c.cap2 : 0.0f;
+    c.bias = a.max_bias;
+    c.nl2 = 1;
+    while (2 * c.nl2 <= c.H) c.nl2 *= 2;
+    c.gate = a.gate ? (const char *)a.gate->data : nullptr;
+    c.gate_nb1 = a.gate ? (int64_t)a.gate->nb[1] : 0, c.gate_nb2 = a.gate ? (int64_t)a.gate->nb[2] : 0;
+    c.dst = (float *)a.dst->data;
+    c.cus = device_cu_count();
+
+    const Plan p = plan(c.n_tok, c.H, c.Hkv, c.B, a.max_q);
+    const size_t need = p.where + al256((size_t)p.least_d * p.slot_d) + 256;
+    if (!a.ws || a.ws_bytes < need)
+        return set_error(SQA_ERR_WORKSPACE, "paged_attn: workspace %zu bytes < %zu needed", a.ws ? a.ws_bytes : (size_t)0, need);
+    const size_t left = a.ws_bytes - 512 - p.where;
+    c.most_d = p.most_d, c.rows_d = p.rows_d, c.rows_c = p.many ? 1 : 0;
+    c.slots_d = (int)((size_t)p.slots_d * p.slot_d <= left ? p.slots_d : (int64_t)(left / p.slot_d));
+    uint8_t *base = reinterpret_cast<uint8_t *>(((uintptr_t)a.ws + 255) & ~(uintptr_t)255);
+    c.where = reinterpret_cast<int4 *>(base);
+    c.acc_d = reinterpret_cast<float *>(base + p.where);
+    c.ml_d = c.acc_d + (size_t)c.slots_d * c.rows_d * kHeadDim;
+
+    int rc = launch_few(c, s);
+    if (rc) return rc;
+    if (p.many) {
+        token_kernel<<<dim3((unsigned)c.n_tok, (unsigned)c.H), dim3(kThreads), 0, s>>>(c);
+        rc = hip_status(hipGetLastError(), "paged_attn launch");
+        if (rc) return rc;
+    }
+    return launch_combine(c, s);
 }
 
 }  // namespace sqa
