@@ -37,11 +37,12 @@ def sources():
     return sorted(glob.glob(os.path.join(csrc, "*.hip")) + glob.glob(os.path.join(csrc, "*.cpp")))
 
 
-# Per-source extra flags. fa_prefill.hip: its MFMA accumulators are read and
+# Per-source extra flags. The prefill and chunk kernels: their MFMA accumulators are read and
 # rescaled by VALU code, so keep every MFMA result in VGPRs (the AGPR form makes
 # the register allocator copy the 128-register accumulator on every tile).
 EXTRA_FLAGS = {
     "fa_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
+    "paged_chunk.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
 }
 
 

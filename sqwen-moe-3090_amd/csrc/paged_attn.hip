@@ -1,8 +1,8 @@
 // paged_attn.hip - attention of a batch of requests over a paged q4_0 pool: what a
 // call launches, its workspace, and the merge of split partials.
 //
-// Requests of few query rows (up to 16 per KV head) go to paged_decode.hip, the
-// others to one workgroup per (token, query head).
+// Requests of few query rows (up to 16 per KV head; up to 8 where larger ones may be
+// in the call) go to paged_decode.hip, the others to paged_chunk.hip.
 #include "paged_attn.hpp"
 
 namespace sqa {
@@ -10,83 +10,6 @@ namespace paged {
 namespace {
 
 constexpr int kThreads = 256;
-
-__device__ __forceinline__ float h2f(uint16_t b) {
-    _Float16 f;
-    __builtin_memcpy(&f, &b, 2);
-    return (float)f;
-}
-
-__global__ __launch_bounds__(kThreads) void token_kernel(Call p) {
-    __shared__ int found;
-    __shared__ float xo[4][256], xm[4], xl[4];
-    const int t = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-    if (tid == 0) found = -1;
-    __syncthreads();
-    for (int b = tid; b < p.B; b += kThreads)
-        if (p.q_start[b] <= t && t < p.q_start[b + 1]) found = b;
-    __syncthreads();
-    const int b = found;
-    if (b < 0) return;
-    const int kvh = h / p.G;
-    const Request rq = request(p, b);
-    if (rq.n * p.G <= p.most_d) return;
-    if (h == 0 && tid == 0) p.where[t] = make_int4(0, 0, 0, kDone);
-    const int64_t pos = rq.pos0 + t - rq.q0, see = sees(rq, t - rq.q0);
-    // dims of the lane: elements 2i, 2i + 1, 16 + 2i, 17 + 2i of block blk
-    const int blk = lane >> 3, i = lane & 7;
-    const float *qr = reinterpret_cast<const float *>(p.q + t * p.q_nb1 + h * p.q_nb2) + 32 * blk + 2 * i;
-    float q[4] = {qr[0], qr[1], qr[16], qr[17]};
-    float amax = 0.0f;
-    for (int j = 0; j < 4; ++j) amax = fmaxf(amax, fabsf(q[j]));
-    for (int o = 1; o < 8; o <<= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
-    const float id = amax != 0.0f ? 127.f / amax : 0.0f;
-    const float qd = (float)(_Float16)(amax / 127.f) * (p.qscale / kLog2e);
-    for (int j = 0; j < 4; ++j) q[j] = rintf(q[j] * id) * qd;
-    const float slope = p.bias == 0.0f ? 0.0f : slope2(p, h) / kLog2e;
-    float m = -INFINITY, l = 0.0f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int64_t j = wave; j < see; j += 4) {
-        const int32_t id_p = p.table[b * p.table_stride + (j >> p.lp)];
-        if (id_p < 0 || id_p >= p.n_pages) continue;
-        const int64_t row = (j & (p.page - 1)) * p.row_bytes + kvh * kHeadRowBytes + 18 * blk;
-        const uint16_t *kb = reinterpret_cast<const uint16_t *>(p.k + id_p * p.k_page + row);
-        const uint16_t *vb = reinterpret_cast<const uint16_t *>(p.v + id_p * p.v_page + row);
-        const uint32_t kc = kb[1 + i], vc = vb[1 + i];
-        const float kd = h2f(kb[0]), vd = h2f(vb[0]);
-        float s = kd * (q[0] * (float)((int)(kc & 15) - 8) + q[1] * (float)((int)(kc >> 8 & 15) - 8) +
-                        q[2] * (float)((int)(kc >> 4 & 15) - 8) + q[3] * (float)((int)(kc >> 12) - 8));
-        for (int x = 1; x < 64; x <<= 1) s += __shfl_xor(s, x);
-        if (p.cap2 != 0.0f) s = p.cap2 / kLog2e * tanhf(s * kLog2e * p.cap_inv);
-        s -= slope * fabsf((float)(pos - j));
-        const float mn = fmaxf(m, s), al = expf(m - mn), w = expf(s - mn);
-        m = mn;
-        l = l * al + w;
-        const float wd = w * vd;
-        o[0] = o[0] * al + wd * (float)((int)(vc & 15) - 8);
-        o[1] = o[1] * al + wd * (float)((int)(vc >> 8 & 15) - 8);
-        o[2] = o[2] * al + wd * (float)((int)(vc >> 4 & 15) - 8);
-        o[3] = o[3] * al + wd * (float)((int)(vc >> 12) - 8);
-    }
-    const int d = 32 * blk + 2 * i;
-    xo[wave][d] = o[0], xo[wave][d + 1] = o[1], xo[wave][d + 16] = o[2], xo[wave][d + 17] = o[3];
-    if (lane == 0) xm[wave] = m, xl[wave] = l;
-    __syncthreads();
-    const float M = fmaxf(fmaxf(xm[0], xm[1]), fmaxf(xm[2], xm[3]));
-    float r = 0.0f, L = 0.0f;
-    if (M != -INFINITY)
-        for (int w = 0; w < 4; ++w) {
-            const float f = expf(xm[w] - M);
-            r += f * xo[w][tid];
-            L += f * xl[w];
-        }
-    r = L == 0.0f ? 0.0f : r / L;
-    if (p.gate) {
-        const float g = reinterpret_cast<const float *>(p.gate + t * p.gate_nb2 + h * p.gate_nb1)[tid];
-        r *= 1.0f / (1.0f + expf(-g));
-    }
-    p.dst[((int64_t)t * p.H + h) * kHeadDim + tid] = r;
-}
-
 
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 // Merge of a row's partials: out = sum_s acc_s e^(m_s - M) / sum_s l_s e^(m_s - M), M = max m_s,
@@ -220,28 +143,33 @@ __global__ __launch_bounds__(kThreads) void merge_rows_kernel(Call c, int heads)
 
 size_t al256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-// Workspace of a call: the tokens' entries, then the slots of the few-row kernel.
+// What a call launches, and its workspace: the tokens' entries, then the slots of the
+// few-row kernel, then those of the many-row kernel.
 struct Plan {
-    int most_d, rows_d;   // of Call
-    bool few, many;       // which kernels run
-    int64_t slots_d, least_d;
-    size_t where, slot_d;
+    int most_d, rows_d, rows_c;  // of Call
+    int64_t slots_d, least_d, slots_c, grid_c;
+    size_t where, slot_d, slot_c;
 };
 
 Plan plan(int64_t n_tok, int64_t H, int64_t Hkv, int64_t B, int64_t max_q) {
     Plan p{};
-    const int64_t G = H / Hkv, rows = (max_q < n_tok ? max_q : n_tok) * G;
+    const int64_t G = H / Hkv, rows = (max_q < n_tok ? max_q : n_tok) * G, cus = device_cu_count();
+    const int64_t active = B < n_tok ? B : n_tok;
     p.most_d = rows <= 8 || (rows > 16 && G <= 8) ? 8 : 16;
     p.rows_d = p.most_d;
-    p.many = rows > p.most_d;
-    p.few = true;
-    const int64_t active = B < n_tok ? B : n_tok;
-    int64_t P = 2 * device_cu_count() / Hkv;
-    if (P < 1) P = 1;
-    p.slots_d = (P + active) * Hkv;
+    const int64_t P = 2 * cus / Hkv;  // pieces that are wanted at most
+    p.slots_d = ((P < 1 ? 1 : P) + active) * Hkv;
     p.least_d = (1 + active) * Hkv;
     p.where = al256((size_t)n_tok * 16);
     p.slot_d = (size_t)p.rows_d * (kHeadDim + 2) * 4;
+    if (rows > p.most_d) {
+        p.rows_c = rows <= 64 ? 64 : 128;
+        // whole query tiles and a last one of every request; three rounds where that is less
+        const int64_t wgs = (n_tok / (p.rows_c / G) + active) * Hkv;
+        p.grid_c = (wgs + cus > 3 * cus ? wgs + cus : 3 * cus) + 7 & ~(int64_t)7;
+        p.slots_c = 3 * cus;
+        p.slot_c = (size_t)p.rows_c * (kHeadDim + 2) * 4;
+    }
     return p;
 }
 
@@ -268,7 +196,7 @@ using namespace paged;
 size_t paged_attn_workspace(int64_t n_tok, int64_t H, int64_t Hkv, int64_t B, int64_t max_q) {
     if (n_tok < 1) return 0;
     const Plan p = plan(n_tok, H, Hkv, B, max_q);
-    return p.where + al256((size_t)p.slots_d * p.slot_d) + 256;
+    return p.where + (size_t)p.slots_d * p.slot_d + (size_t)p.slots_c * p.slot_c + 512;
 }
 
 int launch_paged_attn(const PagedArgs &a, hipStream_t s) {
@@ -297,22 +225,30 @@ int launch_paged_attn(const PagedArgs &a, hipStream_t s) {
     c.cus = device_cu_count();
 
     const Plan p = plan(c.n_tok, c.H, c.Hkv, c.B, a.max_q);
-    const size_t need = p.where + al256((size_t)p.least_d * p.slot_d) + 256;
+    const size_t need = p.where + (size_t)p.least_d * p.slot_d + 512;
     if (!a.ws || a.ws_bytes < need)
         return set_error(SQA_ERR_WORKSPACE, "paged_attn: workspace %zu bytes < %zu needed", a.ws ? a.ws_bytes : (size_t)0, need);
-    const size_t left = a.ws_bytes - 512 - p.where;
-    c.most_d = p.most_d, c.rows_d = p.rows_d, c.rows_c = p.many ? 1 : 0;
-    c.slots_d = (int)((size_t)p.slots_d * p.slot_d <= left ? p.slots_d : (int64_t)(left / p.slot_d));
+    if (p.grid_c > INT32_MAX) return set_error(SQA_ERR_UNSUPPORTED, "paged_attn: too many query tiles");
+    size_t left = a.ws_bytes - 512 - p.where;
+    c.most_d = p.most_d, c.rows_d = p.rows_d, c.rows_c = p.rows_c, c.grid_c = (int)p.grid_c;
+    auto take = [&left](int64_t slots, size_t bytes) {
+        if (!slots || (size_t)slots > left / bytes) slots = slots ? (int64_t)(left / bytes) : 0;
+        left -= (size_t)slots * bytes;
+        return (int)slots;
+    };
+    c.slots_d = take(p.slots_d, p.slot_d);
+    c.slots_c = take(p.slots_c, p.slot_c);
     uint8_t *base = reinterpret_cast<uint8_t *>(((uintptr_t)a.ws + 255) & ~(uintptr_t)255);
     c.where = reinterpret_cast<int4 *>(base);
     c.acc_d = reinterpret_cast<float *>(base + p.where);
-    c.ml_d = c.acc_d + (size_t)c.slots_d * c.rows_d * kHeadDim;
+    c.acc_c = c.acc_d + (size_t)c.slots_d * c.rows_d * kHeadDim;
+    c.ml_d = c.acc_c + (size_t)c.slots_c * c.rows_c * kHeadDim;
+    c.ml_c = c.ml_d + (size_t)c.slots_d * c.rows_d * 2;
 
     int rc = launch_few(c, s);
     if (rc) return rc;
-    if (p.many) {
-        token_kernel<<<dim3((unsigned)c.n_tok, (unsigned)c.H), dim3(kThreads), 0, s>>>(c);
-        rc = hip_status(hipGetLastError(), "paged_attn launch");
+    if (p.rows_c) {
+        rc = launch_many(c, s);
         if (rc) return rc;
     }
     return launch_combine(c, s);

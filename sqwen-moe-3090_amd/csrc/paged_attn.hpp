@@ -44,6 +44,7 @@ struct Call {
     float *acc_c, *ml_c;         // [slot][rows_c][256], ...
     int rows_d, rows_c;          // rows of a slot
     int slots_d, slots_c;        // slots of the workspace
+    int grid_c;                  // workgroups of the many-row kernel
     int most_d;                  // query rows per KV head that the few-row kernel takes (0: it does not run)
     int cus;
 };
@@ -138,6 +139,7 @@ __device__ __forceinline__ void cap_logits(float (&s)[N], float cap2, float cap_
 }
 
 int launch_few(const Call &c, hipStream_t s);      // paged_decode.hip
+int launch_many(const Call &c, hipStream_t s);     // paged_chunk.hip
 int launch_combine(const Call &c, hipStream_t s);  // paged_attn.hip
 
 }  // namespace paged

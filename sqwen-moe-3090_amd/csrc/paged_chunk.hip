@@ -1,0 +1,816 @@
+// paged_chunk.hip - attention of requests with many new tokens (more than 16 query
+// rows per KV head, or more than 8 beside larger ones) over a paged q4_0 pool.
+//
+// A workgroup takes 128 (or 64) query rows of one request and KV head (GQA packed: row
+// r is token r / G, head kvh * G + r % G) and a range of its keys, 32 at a time. Its 8
+// wavefronts split the work by kind as in the contiguous prefill kernel: four score
+// wavefronts hold Q' (hi and lo) of 32 rows each and make the logits and P of tile t,
+// four value wavefronts hold O of the same rows and add P V of tile t - 1.
+//   S^T = sum over q4_0 blocks b of d_k[b] (Kc_b . Q'h_b + Kc_b . Q'l_b): exact codes as
+//   fp16 on v_mfma_f32_16x16x32_f16, Q' = q8_0(Q) * scale * log2(e) as an fp16 hi + lo
+//   pair, the scaling by d_k in fp32; softmax base 2 with a reference maximum that
+//   moves only when a logit passes it by kSlack; O += (P d_v) V with P d_v as an fp16
+//   hi + lo pair and exact codes.
+//
+// There is no pre-pass: the contiguous kernel expands K and V into 2112 bytes per key
+// in its workspace, which for a batch would have to hold every request's keys. Here
+// the value wavefronts bring the q4_0 rows themselves into LDS (288 bytes per key and
+// head; a 16-key group lies on one page, so its id is one scalar load and its rows a
+// scalar base plus constant offsets) and expand them there for all 128 rows:
+//   iteration t: rows of K tile t + 2 and V tile t + 1 are on their way; K tile t + 1
+//   and V tile t are expanded; P V of tile t - 1.
+// K codes leave a dword of nibbles by shifts and masks alone: the 8 values of a chunk
+// are its dims in the order 0 2 1 3 16 18 17 19, and Q' is laid out in the same order.
+// V needs the codes of 8 keys side by side: 16-bit reads of 8 rows, packed in pairs.
+//
+// d_v enters as d_v 2^E with E from the largest |d_v| of the keys so far (in [1/2, 1)
+// there; O is rescaled when it falls), and P as P 2^kEp, so that A = P d_v stays below
+// 2^14 and the parts that count stay clear of fp16's subnormals for V of any size.
+#include <mutex>
+
+#include "paged_attn.hpp"
+
+namespace sqa {
+namespace paged {
+namespace {
+
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+
+constexpr int kPK = 32;                  // keys per tile
+constexpr int kScoreWaves = 4;
+constexpr int kValueWaves = 4;
+constexpr int kThreads = 64 * (kScoreWaves + kValueWaves);
+constexpr int kMaxRG = 2;                // 16-row groups per score wave: 1 or 2 (kRG in the kernel)
+constexpr int rows_per_wg(int rg) { return kScoreWaves * rg * 16; }
+constexpr int kOffDk = kPK * 512;        // K stage: Kc, Dk
+constexpr int kKStage = kOffDk + 8 * kPK * 2;
+constexpr int kOffDv = kHeadDim * kPK * 2;  // V stage: Vc, Dv
+constexpr int kVStage = kOffDv + 8 * kPK * 2;
+constexpr int kRawTile = kPK * kHeadRowBytes;  // q4_0 rows of a tile
+// LDS map: 2 K stages | 2 V stages | 2 P buffers | 2 rescale buffers | raw K, V tiles, 2 each
+constexpr int kLdsV = 2 * kKStage;
+constexpr int kLdsP = kLdsV + 2 * kVStage;        // [4 waves][kRG][2 halves][64 lanes][16 B]
+constexpr int kPBuf = kScoreWaves * kMaxRG * 2 * 1024;
+constexpr int kLdsA = kLdsP + 2 * kPBuf;          // [4 waves][kRG][16 rows] f32
+constexpr int kABuf = kScoreWaves * kMaxRG * 16 * 4;
+constexpr int kLdsRaw = kLdsA + 2 * kABuf;        // [K, V][2][32 rows][144 B]
+constexpr int kLdsBytes = kLdsRaw + 4 * kRawTile + 16;
+static_assert(kLdsBytes <= 160 * 1024, "LDS budget");
+static_assert(kLdsRaw % 16 == 0 && kKStage % 16 == 0 && kVStage % 16 == 0, "alignment of the stages");
+constexpr int kSlack = 8;  // log2 of the largest P the lazy rescale admits
+constexpr int kEp = 6;     // P travels as P 2^kEp (at most 2^14)
+constexpr int kMaxE = 24;  // of the V scales: makes the smallest fp16 one
+
+__device__ __forceinline__ uint4 swap_halves(uint4 v, bool swap) {
+    return swap ? make_uint4(v.z, v.w, v.x, v.y) : v;
+}
+
+// max(x, x of lane ^ 16) and max(x, x of lane ^ 32) with gfx950's row swaps (no
+// LDS round trip): each swap returns the two halves of a lane pair's values.
+__device__ __forceinline__ float xmax16(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float xmax32(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// LDS/record row of key k (0..31) of a tile: the inverse of sigma.
+__device__ __forceinline__ int key_row(int k) { return 16 * ((k >> 2) & 1) + 4 * (k >> 3) + (k & 3); }
+
+
+// Two 4-bit codes n (bits 0-3 and 16-19 of x) as the packed fp16 pair n - 8:
+// 0x6400 | n is exactly 1024 + n, and 1024 + n - 1032 is exact.
+__device__ __forceinline__ uint32_t codes_f16(uint32_t x) {
+    const uint32_t y = (x & 0x000F000Fu) | 0x64006400u;
+    half2v v;
+    __builtin_memcpy(&v, &y, 4);
+    const half2v d = v + half2v{(_Float16)-1032.0f, (_Float16)-1032.0f};
+    uint32_t r;
+    __builtin_memcpy(&r, &d, 4);
+    return r;
+}
+
+// 16 bytes per lane from sbase + voff into LDS at m0 + 16 * lane (asynchronous;
+// the caller waits with s_waitcnt vmcnt).
+__device__ __forceinline__ void dma16(uint32_t voff, const void *sbase, uint32_t m0v) {
+    // wave-uniform, in SGPRs whatever the compiler thinks of it; m0 as an operand: the
+    // compiler writes it and knows it holds the LDS base
+    const uint64_t b = (uint64_t)(uintptr_t)sbase;
+    const uint64_t bs = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32) |
+                        (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)b);
+    const uint32_t ms = (uint32_t)__builtin_amdgcn_readfirstlane((int)m0v);
+    asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(bs), "{m0}"(ms) : "memory");
+}
+
+// Two 8-byte LDS reads into one MFMA operand. volatile keeps them two single
+// ds_read_b64 straight into the operand's registers: merged into ds_read2 pairs
+// they would bring halves of different operands and need register moves.
+__device__ __forceinline__ half8 lds_half8(const uint8_t *base, int off_lo, int off_hi) {
+    typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+    typedef const volatile __attribute__((address_space(3))) u32x2 lds_u32x2;
+    const u32x2 a = *(lds_u32x2 *)(base + off_lo);
+    const u32x2 b = *(lds_u32x2 *)(base + off_hi);
+    const uint4 u = make_uint4(a.x, a.y, b.x, b.y);
+    half8 h;
+    __builtin_memcpy(&h, &u, 16);
+    return h;
+}
+
+
+// K codes and scales of tile t from its raw rows, by the 256 value lanes: lane vt
+// block vt & 7 of key vt >> 3. Row r = key_row(key) of the stage, 16-byte chunk 4b + m
+// (dims 32b + 4m + {0, 2, 1, 3, 16, 18, 17, 19}) at chunk (4b + m) ^ (r & 7), halves
+// swapped when r & 8.
+__device__ __forceinline__ void expand_k(uint8_t *smem, int t, int vt) {
+    const int key = vt >> 3, b = vt & 7, r = key_row(key);
+    const uint8_t *row = smem + kLdsRaw + (t & 1) * kRawTile + kHeadRowBytes * key;
+    uint8_t *stage = smem + (t & 1) * kKStage;
+    // the 16 bytes of codes start 2 bytes off a dword for even b
+    const uint32_t *src = reinterpret_cast<const uint32_t *>(row + ((18 * b + 2) & ~3));
+    const uint32_t sh = b & 1 ? 0u : 16u;
+    uint32_t w[5];
+#pragma unroll
+    for (int m = 0; m < 5; ++m) w[m] = src[m];
+    *reinterpret_cast<uint16_t *>(stage + kOffDk + (b * kPK + r) * 2) = *reinterpret_cast<const uint16_t *>(row + 18 * b);
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+        const uint32_t x = __builtin_amdgcn_alignbit(w[m + 1], w[m], sh);
+        const uint4 c = make_uint4(codes_f16(x), codes_f16(x >> 8), codes_f16(x >> 4), codes_f16(x >> 12));
+        *reinterpret_cast<uint4 *>(stage + r * 512 + 16 * ((4 * b + m) ^ (r & 7))) = swap_halves(c, r & 8);
+    }
+}
+
+// V codes and scales of tile t: lane vt takes bytes 4m + 2i, 4m + 2i + 1 of block b's
+// codes (m = vt & 3, b, i = vt >> 7) for the keys 8c .. 8c + 7 and writes those keys' 16-byte
+// chunk of the rows of the bytes' dims, chunk c of dim d at c ^ ((d >> 1) & 3), halves
+// swapped when d & 8. Scales of the first `left` keys whose page is there, the others
+// (and NaN or Inf, bytes that are no q4_0) as 0: their P is 0, and 0 * NaN would not be.
+// Returns the exponent that the scales are stored with: at most e, and such that the
+// largest is below 1.
+__device__ __forceinline__ int expand_v(uint8_t *smem, int t, int vt, int left, bool has_a, bool has_b, int e) {
+    const int lane = vt & 63, w = vt >> 6;
+    const uint8_t *raw = smem + kLdsRaw + (2 + (t & 1)) * kRawTile;
+    uint8_t *stage = smem + kLdsV + (t & 1) * kVStage;
+    // every wavefront reads all scales: block lane >> 3, keys 4 (lane & 7) ..
+    uint32_t d[4];
+    const int sb = lane >> 3, sk = 4 * (lane & 7);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        d[j] = *reinterpret_cast<const uint16_t *>(raw + kHeadRowBytes * (sk + j) + 18 * sb);
+        const bool ok = sk + j < left && (sk < 16 ? has_a : has_b) && (d[j] & 0x7C00u) != 0x7C00u;
+        d[j] = ok ? d[j] : 0u;
+    }
+    const int b = (vt >> 2) & 7, m = vt & 3, c = (vt >> 5) & 3, i = vt >> 7;
+    const uint8_t *src = raw + kHeadRowBytes * 8 * c + 18 * b + 2 + 4 * m + 2 * i;
+    uint32_t x[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        x[j] = (uint32_t)*reinterpret_cast<const uint16_t *>(src + kHeadRowBytes * 2 * j) |
+               ((uint32_t)*reinterpret_cast<const uint16_t *>(src + kHeadRowBytes * (2 * j + 1)) << 16);
+    const int mx = wave_max((int)(max(max(d[0] & 0x7fffu, d[1] & 0x7fffu), max(d[2] & 0x7fffu, d[3] & 0x7fffu))));
+    if (mx != 0) {
+        const int ex = mx >> 10;
+        const int lg = ex ? ex - 15 : (31 - __builtin_clz(mx)) - 24;  // floor(log2 max |d_v|)
+        e = min(e, -1 - lg);
+    }
+    if ((lane >> 4) == w) {
+        const float f = __builtin_amdgcn_ldexpf(1.0f, e);
+        uint16_t o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint16_t bits = (uint16_t)d[j];
+            _Float16 hv;
+            __builtin_memcpy(&hv, &bits, 2);
+            hv = (_Float16)((float)hv * f);
+            __builtin_memcpy(&o[j], &hv, 2);
+        }
+        uint2 u;
+        __builtin_memcpy(&u, o, 8);
+        *reinterpret_cast<uint2 *>(stage + kOffDv + 64 * sb + 2 * sk) = u;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {  // low nibbles of both bytes, high nibbles
+        const int sh = (k & 1) * 8 + (k >> 1) * 4;
+        const int dim = 32 * b + 4 * m + 2 * i + (k & 1) + 16 * (k >> 1);
+        const uint4 u = make_uint4(codes_f16(x[0] >> sh), codes_f16(x[1] >> sh), codes_f16(x[2] >> sh), codes_f16(x[3] >> sh));
+        *reinterpret_cast<uint4 *>(stage + 64 * dim + 16 * (c ^ ((dim >> 1) & 3))) = swap_halves(u, dim & 8);
+    }
+    return e;
+}
+
+// Q' of a row as B operands: the lane's 8 dims of every block (in the order of the K
+// chunks), q8_0 with ggml's x86 rounding (d = amax / 127 over the block, codes =
+// rint(x * 127 / amax)), times fp16(d) * scale * log2(e) in fp32, as fp16 hi and
+// lo = fp16(Q' - hi).
+__device__ __forceinline__ void quantize_q(const Call &p, int64_t row, int h, int g, bool ok, half8 (&hi)[8], half8 (&lo)[8]) {
+    const float *q = reinterpret_cast<const float *>(p.q + row * p.q_nb1 + (int64_t)h * p.q_nb2);
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+        const float4a a = *reinterpret_cast<const float4a *>(q + 32 * b + 4 * g);
+        const float4a c = *reinterpret_cast<const float4a *>(q + 32 * b + 16 + 4 * g);
+        float v[8] = {a.x, a.z, a.y, a.w, c.x, c.z, c.y, c.w};
+        float amax = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            v[j] = ok ? v[j] : 0.0f;
+            amax = fmaxf(amax, fabsf(v[j]));
+        }
+        amax = xmax32(xmax16(amax));
+        const float d = amax / 127.f;
+        const float id = amax != 0.0f ? 127.f / amax : 0.0f;
+        const float qd = (float)(_Float16)d * p.qscale;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            // x opaque: left visible, the compiler may round code * qd to fp16 twice
+            // (once from the fp32 product for hi, once from the exact product for the
+            // hi it subtracts), and a hi + lo off by one fp16 ulp of hi
+            float x = rintf(v[j] * id) * qd;
+            asm volatile("" : "+v"(x));
+            const _Float16 hh = (_Float16)x;
+            hi[b][j] = hh;
+            lo[b][j] = (_Float16)(x - (float)hh);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- work split
+
+// A workgroup's part of the call: query tile `tile` of request b's `tiles`, KV head kvh,
+// split `split` of `splits`, key tiles [t0, t1); slot: the request's first one (splits > 1).
+// b < 0: none.
+struct Item {
+    int b, kvh, tile, tiles, split, splits, t0, t1, slot;
+};
+
+constexpr int kMostSplits = 256;  // of a request (the merge's limit)
+constexpr int kChoices = 16;
+// splits of the longest request that are tried
+__device__ constexpr int kTried[kChoices] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64, 128};
+
+// Query tiles of a request (0: none of this kernel's) and its key tiles.
+__device__ __forceinline__ int tiles_of(const Call &c, int b, int qb, int *key_tiles) {
+    *key_tiles = 0;
+    if (b >= c.B) return 0;
+    const Request r = request(c, b);
+    if (r.n * c.G <= c.most_d) return 0;
+    *key_tiles = max((r.kv + kPK - 1) / kPK, 1);
+    return (r.n + qb - 1) / qb;
+}
+
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o);
+    return x;
+}
+
+// Every request is cut into splits of about `len` key tiles, the same for all, with the
+// len of the least estimated time (in tiles of one workgroup: kWg for a workgroup's
+// own start and end, kMerge for the merge and kMergeSlot for a slot's bytes). Where the
+// parts are about equal they run in rounds of one per CU; where they are not (ragged
+// batches, first chunks, whose tiles see from one to all of the keys) the time is the
+// work over the CUs and half a part.
+constexpr float kWg = 3.0f, kMerge = 3.0f, kMergeSlot = 0.016f;
+
+__device__ __forceinline__ Item many_item(const Call &c, int lin, int qb) {
+    const int lane = threadIdx.x & 63;
+    float work = 0.0f;
+    int longest = 0, wgs = 0;
+    for (int b0 = 0; b0 < c.B; b0 += 64) {
+        int kt;
+        const int T = tiles_of(c, b0 + lane, qb, &kt);
+        wgs += T;
+        longest = max(longest, kt);
+        // query tile i of T ends (T - 1 - i) * qb keys before the last one
+        if (T) work += fmaxf((float)T * (float)kt - 0.5f * (float)T * (float)(T - 1) * (float)qb / kPK, 0.5f * (float)T * (float)kt);
+    }
+    Item it{-1, 0, 0, 0, 0, 1, 0, 0, 0};
+    wgs = ::sqa::paged::wave_sum(wgs);
+    if (wgs == 0 || lin >= c.grid_c) return it;
+    work = wave_sum(work) * (float)c.Hkv;
+    longest = wave_max(longest);
+    int len = longest, total = wgs;  // wgs of one head and split; total of one head
+    bool even = true;
+    float best = INFINITY;
+    const float cus = (float)c.cus;
+#pragma unroll 1
+    for (int j = 0; j < kChoices; ++j) {
+        const int l = max((longest + kTried[j] - 1) / kTried[j], 2);
+        if (longest > l * kMostSplits) continue;
+        int n = 0, slots = 0;
+        for (int b0 = 0; b0 < c.B; b0 += 64) {
+            int kt;
+            const int T = tiles_of(c, b0 + lane, qb, &kt), S = (kt + l - 1) / l;
+            n += T * S;
+            slots += S > 1 ? T * S : 0;
+        }
+        n = ::sqa::paged::wave_sum(n);
+        slots = ::sqa::paged::wave_sum(slots);
+        if (j > 0 && ((int64_t)slots * c.Hkv > c.slots_c || (int64_t)n * c.Hkv > c.grid_c)) break;
+        const float N = (float)n * (float)c.Hkv, part = fminf((float)l, (float)longest);
+        const bool eq = work > 0.85f * N * part;
+        float t = eq ? ceilf(N / cus) * (part + kWg) : fmaxf((work + kWg * N) / cus + 0.5f * part, part + kWg);
+        t += slots ? kMerge + kMergeSlot * (float)slots * (float)c.Hkv : 0.0f;
+        if (t < best) best = t, len = l, total = n, even = eq;
+        if (l == 2) break;
+    }
+    // Workgroups go round-robin to the 8 XCDs. Equal parts are renumbered so that an
+    // XCD gets a run of ids, the query tiles of the same keys, which its L2 then serves
+    // to all of them; unequal ones go out as they come, the last query tiles first.
+    const int N = total * c.Hkv;
+    int id = lin;
+    if (even) {
+        const int x = lin & 7, per = N >> 3, rem = N & 7, k = lin >> 3;
+        if (k >= per + (x < rem ? 1 : 0)) return it;
+        id = x * per + (x < rem ? x : rem) + k;
+    }
+    if (id >= N) return it;
+    int first = 0, slot = 0;
+    for (int b0 = 0; b0 < c.B && first <= id; b0 += 64) {
+        int kt;
+        const int T = tiles_of(c, b0 + lane, qb, &kt), S = (kt + len - 1) / len;
+        const int n = T * S * c.Hkv, own = S > 1 ? n : 0;
+        const int upto = first + wave_scan(n), slots = slot + wave_scan(own);
+        const uint64_t hit = __ballot(id >= upto - n && id < upto);
+        if (hit) {
+            const int l = __builtin_ctzll(hit);
+            int r = id - __builtin_amdgcn_readlane(upto - n, l);
+            it.b = b0 + l;
+            it.tiles = __builtin_amdgcn_readlane(T, l);
+            it.splits = __builtin_amdgcn_readlane(S, l);
+            it.slot = __builtin_amdgcn_readlane(slots - own, l);
+            const int keys = __builtin_amdgcn_readlane(kt, l);
+            it.tile = r % it.tiles;
+            r /= it.tiles;
+            it.split = r % it.splits;
+            it.kvh = r / it.splits;
+            if (!even) it.tile = it.tiles - 1 - it.tile;
+            it.t0 = (int)((int64_t)it.split * keys / it.splits);
+            it.t1 = (int)((int64_t)(it.split + 1) * keys / it.splits);
+        }
+        first = __builtin_amdgcn_readlane(upto, 63);
+        slot = __builtin_amdgcn_readlane(slots, 63);
+    }
+    return it;
+}
+
+// kRG = 2: 128 query rows a workgroup; 1: 64 rows. OPT: the logits are capped or biased.
+template <int kRG, bool OPT>
+__global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    const int tid = threadIdx.x;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lane = tid & 63, g = lane >> 4, n = lane & 15;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)smem;
+
+    const Item it = many_item(p, (int)blockIdx.x, rows_per_wg(kRG) / p.G);
+    if (it.b < 0) return;
+    const Request rq = request(p, it.b);
+    const int qb = rows_per_wg(kRG) / p.G;  // tokens of a query tile
+    const int q_base = it.tile * qb;        // its first token in the request
+    const int q_top = min(q_base + qb, rq.n);
+    const bool whole = it.splits == 1;      // of the keys: the result goes out from here
+    const int slot = it.slot + (it.kvh * it.splits + it.split) * it.tiles + it.tile;
+    if (it.split == 0 && it.kvh == 0 && tid < q_top - q_base)
+        p.where[rq.q0 + q_base + tid] =
+            whole ? make_int4(0, 0, 0, kDone) : make_int4(it.slot + it.tile, it.splits, tid * p.G, 4 * it.tiles + kMany);
+
+    // Key range: the split, cut at the last key any token of the tile sees.
+    const int k_begin = it.t0 * kPK;
+    const int k_end = min(it.t1 * kPK, sees(rq, q_top - 1));
+    const int n_tiles = k_end > k_begin ? (k_end - k_begin + kPK - 1) / kPK : 0;
+    if (n_tiles == 0 && !whole) {
+        // a split past the tile's last visible key leaves its O unwritten: the
+        // merge takes no partial whose m is -inf
+        if (tid < rows_per_wg(kRG)) {
+            float *ml = p.ml_c + ((int64_t)slot * rows_per_wg(kRG) + tid) * 2;
+            store_through(ml, -INFINITY);
+            store_through(ml + 1, 0.0f);
+        }
+        return;
+    }
+    const int kvh = it.kvh;
+    const int see_all = sees(rq, q_base);  // keys that every token of the tile sees
+    const int32_t *table = p.table + (int64_t)it.b * p.table_stride;
+    const int last_group = max(rq.kv - 1, 0) & ~15;
+    // 16-key group gi of tile t; one behind the last key stands for the last one
+    auto group_key = [&](int t, int gi) {
+        return __builtin_amdgcn_readfirstlane(min(k_begin + t * kPK + 16 * gi, last_group));
+    };
+    auto id_of = [&](int t, int gi) { return t < n_tiles ? page_id(table, group_key(t, gi) >> p.lp) : 0; };
+    auto there = [&](int id) { return (uint32_t)id < (uint32_t)p.n_pages; };
+
+    const float lim_top = (float)(kSlack + kEp);  // the lazy test's bound on s'
+    const int nh = (n >> 3) & 1;
+
+    // The two kinds of wave run separate code with the same barrier count:
+    // one before the loop, n_tiles + 1 in it, then two for the hand-over of m and l.
+    if (wave < kScoreWaves) {
+        const int w = wave;
+        float *ml = reinterpret_cast<float *>(smem + kLdsP) + w * (kRG * 32);  // [rg][row][m, l]
+        // Q' hi and lo of rows r = 16 kRG w + 16rg + n (position q_base + r / G, head
+        // kvh*G + r % G) as B operands, dims 32b + 8g..+7
+        half8 bqh[kRG][8], bql[kRG][8];
+        int my_see[kRG], my_pos[kRG];
+        float my_slope[kRG];
+        float m_run[kRG], l_part[kRG];
+        // The logits are accumulated relative to the row's P reference mref =
+        // (m_run, or 0 before the first visible key) - ep: s' = s - mref, so that
+        // P = 2^s' needs no subtraction, and the lazy-maximum test s > m_run +
+        // ks reads s' > lim_s (ks + ep, or -inf before the first visible key).
+        // Both change only when the maximum moves.
+        float mref[kRG], lim_s[kRG];
+#pragma unroll
+        for (int rg = 0; rg < kRG; ++rg) {
+            const int r = 16 * kRG * w + 16 * rg + n;
+            const int i = r / p.G, h = kvh * p.G + r - i * p.G;
+            const bool ok = q_base + i < q_top;
+            my_see[rg] = ok ? sees(rq, q_base + i) : 0;
+            my_pos[rg] = rq.pos0 + q_base + i;
+            my_slope[rg] = OPT && p.bias != 0.0f ? slope2(p, h) : 0.0f;
+            quantize_q(p, ok ? rq.q0 + q_base + i : rq.q0, h, g, ok, bqh[rg], bql[rg]);
+            m_run[rg] = -INFINITY;
+            l_part[rg] = 0.0f;
+            mref[rg] = -(float)kEp;
+            lim_s[rg] = -INFINITY;
+        }
+        // K operand of key row 16kg + n, dims 32b + 8g..+7: chunk (4b + g) ^ (n & 7),
+        // halves swapped when n & 8; the XOR touches bit 2 of 4b + g, so even and odd
+        // b use two bases and b >> 1 adds 128 bytes.
+        int k_off[2][2];  // [b & 1][half]
+#pragma unroll
+        for (int bp = 0; bp < 2; ++bp)
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) k_off[bp][hf] = n * 512 + 16 * ((4 * bp + g) ^ (n & 7)) + 8 * (hf ^ nh);
+        const int p_off = w * (kRG * 2048) + 16 * lane;  // P slots [w][rg][half][lane]
+
+        int ida = id_of(0, 0), idb = id_of(0, 1);  // pages of the tile's two groups
+        if (n_tiles > 0) asm volatile("s_barrier" ::: "memory");  // raw rows of the first tile
+        for (int t = 0; t <= n_tiles && n_tiles > 0; ++t) {
+            // the value waves wait for their DMAs before this barrier, which makes them
+            // visible and retires the buffers the new ones overwrite
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (t == n_tiles) break;
+            const int kt = k_begin + t * kPK;
+            const bool has_a = there(ida), has_b = there(idb);
+            ida = id_of(t + 1, 0);
+            idb = id_of(t + 1, 1);
+            // this tile's four per-lane K bases, opaque to the compiler: every K read
+            // is then one of them plus an immediate offset (hoisting all 64
+            // base + offset sums out of the loop would need 64 more registers)
+            int kb[2][2];
+#pragma unroll
+            for (int bp = 0; bp < 2; ++bp)
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                    kb[bp][hf] = (t & 1) * kKStage + k_off[bp][hf];
+                    asm volatile("" : "+v"(kb[bp][hf]));
+                }
+            // ---- S^T: sa[rg][kg][i] = S[key kt + 8g + 4kg + i][row n of group rg] ----
+            floatx4 sa[kRG][2];
+#pragma unroll
+            for (int rg = 0; rg < kRG; ++rg) sa[rg][0] = sa[rg][1] = OPT ? 0.0f : -mref[rg];
+            // d_k of the lane's four C rows 16kg + 4g + i, block b: 8 bytes at
+            // Dk[b][16kg + 4g]
+            const uint8_t *dkb = smem + (t & 1) * kKStage + kOffDk + 8 * g;
+            // Software-pipelined by one step: step j = (block j >> 1, key group j & 1)
+            // issues its MFMAs, then the d_k scaling of step j - 1 runs while they
+            // execute. The scheduling barrier keeps the compiler from pulling the
+            // scaling back next to the MFMAs it reads (it did, leaving 4-12
+            // instructions between an MFMA and its consumer). The sum into sa keeps
+            // the block order of the plain loop.
+            floatx4 cp[kRG];
+            uint2 dkp;
+#pragma unroll
+            for (int j = 0; j <= 16; ++j) {
+                floatx4 cn[kRG];
+                uint2 dkn;
+                if (j < 16) {
+                    const int b = j >> 1, kg = j & 1;
+                    const int o = kg * 8192 + 128 * (b >> 1);
+                    const half8 ak = lds_half8(smem, kb[b & 1][0] + o, kb[b & 1][1] + o);
+                    dkn = *reinterpret_cast<const uint2 *>(dkb + 64 * b + 32 * kg);
+#pragma unroll
+                    for (int rg = 0; rg < kRG; ++rg) {
+                        const floatx4 c = __builtin_amdgcn_mfma_f32_16x16x32_f16(ak, bqh[rg][b],
+                                                                                 floatx4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                        cn[rg] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ak, bql[rg][b], c, 0, 0, 0);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                if (j > 0) {
+                    const int kg = (j - 1) & 1;
+                    _Float16 dk[4];
+                    __builtin_memcpy(dk, &dkp, 8);
+#pragma unroll
+                    for (int rg = 0; rg < kRG; ++rg)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) sa[rg][kg][i] = fmaf(cp[rg][i], (float)dk[i], sa[rg][kg][i]);
+                }
+                if (j < 16) {
+                    dkp = dkn;
+#pragma unroll
+                    for (int rg = 0; rg < kRG; ++rg) cp[rg] = cn[rg];
+                }
+            }
+            float s[kRG][8];  // keys 8g + jj, base-2 logits
+#pragma unroll
+            for (int rg = 0; rg < kRG; ++rg)
+#pragma unroll
+                for (int jj = 0; jj < 8; ++jj) s[rg][jj] = sa[rg][jj >> 2][jj & 3];
+            if (OPT) {
+#pragma unroll
+                for (int rg = 0; rg < kRG; ++rg) {
+                    if (p.cap2 != 0.0f) cap_logits(s[rg], p.cap2, p.cap_inv);
+                    const int far = my_pos[rg] - (kt + 8 * g);
+#pragma unroll
+                    for (int jj = 0; jj < 8; ++jj)
+                        s[rg][jj] = fmaf(-my_slope[rg], fabsf((float)(far - jj)), s[rg][jj]) - mref[rg];
+                }
+            }
+            // ---- causal limit, prefix, last key, pages that are not there: whatever the
+            // logit is, NaN of garbage bytes too
+            if (kt + kPK > see_all || !has_a || !has_b) {
+                const bool has = g < 2 ? has_a : has_b;  // lanes' keys 8g..8g+7
+#pragma unroll
+                for (int rg = 0; rg < kRG; ++rg) {
+                    const int see = has ? min(my_see[rg], k_end) - (kt + 8 * g) : 0;
+#pragma unroll
+                    for (int jj = 0; jj < 8; ++jj) s[rg][jj] = jj < see ? s[rg][jj] : -INFINITY;
+                }
+            }
+            // ---- online softmax (base 2); P and the rescale factors to LDS -----------
+            uint8_t *pb = smem + kLdsP + (t & 1) * kPBuf + p_off;
+            float *ab = reinterpret_cast<float *>(smem + kLdsA + (t & 1) * kABuf) + w * (kRG * 16);
+#pragma unroll
+            for (int rg = 0; rg < kRG; ++rg) {
+                // lazy maximum: the reference moves only when a logit passes it by more
+                // than ks, so P <= 2^ks and most tiles need no rescale of O
+                float alpha = 1.0f;
+                bool over = false;
+#pragma unroll
+                for (int jj = 0; jj < 8; ++jj) over |= s[rg][jj] > lim_s[rg];
+                if (__any(over)) {
+                    float mt = fmaxf(fmaxf(fmaxf(s[rg][0], s[rg][1]), fmaxf(s[rg][2], s[rg][3])),
+                                     fmaxf(fmaxf(s[rg][4], s[rg][5]), fmaxf(s[rg][6], s[rg][7])));
+                    mt = xmax16(mt);
+                    mt = xmax32(mt);
+                    const float m_new = fmaxf(m_run[rg], mt + mref[rg]);
+                    alpha = m_run[rg] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run[rg] - m_new);
+                    l_part[rg] *= alpha;
+                    m_run[rg] = m_new;
+                    // onto the new reference: s - mref_new = s' + (mref - mref_new)
+                    const float mref_new = (m_new == -INFINITY ? 0.0f : m_new) - (float)kEp;
+                    const float d = mref[rg] - mref_new;
+#pragma unroll
+                    for (int jj = 0; jj < 8; ++jj) s[rg][jj] += d;
+                    mref[rg] = mref_new;
+                    lim_s[rg] = m_new == -INFINITY ? -INFINITY : lim_top;
+                }
+                float pf[8], psum = 0.0f;
+#pragma unroll
+                for (int jj = 0; jj < 8; ++jj) {
+                    pf[jj] = __builtin_amdgcn_exp2f(s[rg][jj]);
+                    psum += pf[jj];
+                }
+                l_part[rg] += psum;
+                // P as an fp16 hi + lo pair (22 bits): the value waves form P d_v from it
+                half8 ph, pl;
+#pragma unroll
+                for (int jj = 0; jj < 8; ++jj) ph[jj] = (_Float16)pf[jj];
+                // the exact residual p - hi, with hi read from its packed fp16 half by
+                // v_fma_mix (no conversion of hi back to fp32)
+                uint32_t hw[4];
+                __builtin_memcpy(hw, &ph, 16);
+#pragma unroll
+                for (int jj = 0; jj < 8; ++jj) {
+                    float r;
+                    if (jj & 1)
+                        asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel:[0,0,1] op_sel_hi:[0,0,1]" : "=v"(r) : "v"(pf[jj]), "v"(hw[jj >> 1]));
+                    else
+                        asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel:[0,0,0] op_sel_hi:[0,0,1]" : "=v"(r) : "v"(pf[jj]), "v"(hw[jj >> 1]));
+                    pl[jj] = (_Float16)r;
+                }
+                *reinterpret_cast<half8 *>(pb + rg * 2048) = ph;
+                *reinterpret_cast<half8 *>(pb + rg * 2048 + 1024) = pl;
+                if (g == 0) ab[rg * 16 + n] = alpha;
+            }
+        }
+        // ---- hand m and l of the rows to the value waves ----------------------------
+        __syncthreads();
+        if (n_tiles > 0) {
+#pragma unroll
+            for (int rg = 0; rg < kRG; ++rg) {
+                float lp = l_part[rg];
+                lp += __shfl_xor(lp, 16);
+                lp += __shfl_xor(lp, 32);
+                if (g == 0) {
+                    ml[rg * 32 + 2 * n] = m_run[rg];
+                    ml[rg * 32 + 2 * n + 1] = lp;
+                }
+            }
+        }
+        __syncthreads();
+        return;
+    }
+
+    // ---- value waves: O[row 16 kRG w + 16rg + 4g + i][dim 16T + n] ----------------
+    const int w = wave - kScoreWaves;
+    const int vt = 64 * w + lane;
+    const float *ml = reinterpret_cast<const float *>(smem + kLdsP) + w * (kRG * 32);  // [rg][row][m, l]
+    // V operand of dim 16T + n, keys 8g..8g+7: chunk g ^ ((n >> 1) & 3), halves swapped when n & 8.
+    const int v_off0 = 64 * n + 16 * (g ^ ((n >> 1) & 3)) + 8 * nh;
+    const int v_off1 = v_off0 ^ 8;
+    const int p_off = w * (kRG * 2048) + 16 * lane;
+    floatx4 acc[kRG][16];
+#pragma unroll
+    for (int rg = 0; rg < kRG; ++rg)
+#pragma unroll
+        for (int T = 0; T < 16; ++T) acc[rg][T] = floatx4{0.f, 0.f, 0.f, 0.f};
+    // DMA: wave w moves 16 rows of a tile, group w & 1, of K (w < 2) or V. They lie on
+    // one page: 9 x 16 bytes a row as two instructions of 64 lanes and one of 16.
+    uint32_t off[3];
+#pragma unroll
+    for (int r = 0; r < 3; ++r) {
+        const int s = 64 * r + lane;
+        off[r] = (uint32_t)(s / 9) * (uint32_t)p.row_bytes + (uint32_t)(kvh * kHeadRowBytes + 16 * (s % 9));
+    }
+    const uint8_t *pool = w < 2 ? p.k : p.v;
+    const int64_t page_bytes = w < 2 ? p.k_page : p.v_page;
+    auto issue = [&](int t, int id) {
+        const int key = group_key(t, w & 1);
+        const uint8_t *from = pool + (int64_t)(there(id) ? id : 0) * page_bytes + (int64_t)(key & (p.page - 1)) * p.row_bytes;
+        const uint32_t to = lds0 + (uint32_t)(kLdsRaw + (2 * (w >> 1) + (t & 1)) * kRawTile + (w & 1) * (kRawTile / 2));
+        // rows behind the last key re-read the end of its row
+        const uint32_t lim = (uint32_t)(min(rq.kv - key, 16) * p.row_bytes - 16);
+        dma16(min(off[0], lim), from, to);
+        dma16(min(off[1], lim), from, to + 1024);
+        if (lane < 16) dma16(min(off[2], lim), from, to + 2048);
+    };
+    // ids of the groups of tiles t, t + 1, t + 2
+    int a0 = id_of(0, 0), b0 = id_of(0, 1), a1 = id_of(1, 0), b1 = id_of(1, 1), a2 = id_of(2, 0), b2 = id_of(2, 1);
+    auto mine = [&](int a, int b) { return w & 1 ? b : a; };
+    int e_new = kMaxE, e_acc = kMaxE;  // exponents of the V scales: of the next tile, of O
+    if (n_tiles > 0) {
+        issue(0, mine(a0, b0));
+        if (w < 2 && n_tiles > 1) issue(1, mine(a1, b1));
+        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+        expand_k(smem, 0, vt);
+    }
+    for (int t = 0; t <= n_tiles && n_tiles > 0; ++t) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        const int a3 = id_of(t + 3, 0), b3 = id_of(t + 3, 1);
+        if (w < 2) {
+            if (t + 2 < n_tiles) issue(t + 2, mine(a2, b2));
+        } else {
+            if (t + 1 < n_tiles) issue(t + 1, mine(a1, b1));
+        }
+        e_acc = e_new;
+        if (t < n_tiles) {
+            const int left = k_end - (k_begin + t * kPK);
+            e_new = expand_v(smem, t, vt, left, there(a0), there(b0), e_new);
+            if (t + 1 < n_tiles) expand_k(smem, t + 1, vt);
+        }
+        a0 = a1, b0 = b1, a1 = a2, b1 = b2, a2 = a3, b2 = b3;
+        if (t == 0) continue;  // O is still zero: it takes the first tile's exponent as it is
+        const int tp = t - 1;
+        const uint8_t *vs = smem + kLdsV + (tp & 1) * kVStage;
+        // this tile's two per-lane V bases, opaque to the compiler (see the K reads)
+        int vb0 = kLdsV + (tp & 1) * kVStage + v_off0, vb1 = kLdsV + (tp & 1) * kVStage + v_off1;
+        asm volatile("" : "+v"(vb0), "+v"(vb1));
+        const uint8_t *pb = smem + kLdsP + (tp & 1) * kPBuf + p_off;
+        const float *ab = reinterpret_cast<const float *>(smem + kLdsA + (tp & 1) * kABuf) + w * (kRG * 16);
+        half8 ph[kRG], pl[kRG];
+        bool resc = false;
+#pragma unroll
+        for (int rg = 0; rg < kRG; ++rg) {
+            // rescale factors of rows 4g..4g+3: exactly 1 unless a maximum moved
+            const floatx4 a4 = *reinterpret_cast<const floatx4 *>(ab + rg * 16 + 4 * g);
+            resc |= (a4[0] != 1.0f) | (a4[1] != 1.0f) | (a4[2] != 1.0f) | (a4[3] != 1.0f);
+            ph[rg] = *reinterpret_cast<const half8 *>(pb + rg * 2048);
+            pl[rg] = *reinterpret_cast<const half8 *>(pb + rg * 2048 + 1024);
+        }
+        if (__any(resc)) {  // rare with the lazy maximum: O = alpha O
+#pragma unroll
+            for (int rg = 0; rg < kRG; ++rg) {
+                const floatx4 a4 = *reinterpret_cast<const floatx4 *>(ab + rg * 16 + 4 * g);
+#pragma unroll
+                for (int T = 0; T < 16; ++T) acc[rg][T] *= a4;
+            }
+        }
+        // d_v of the 8 blocks and V of block 0 first, then V of block b + 1 while
+        // block b computes: the LDS latency stays off the MFMA chain
+        uint4 dvr[8];
+#pragma unroll
+        for (int b = 0; b < 8; ++b) dvr[b] = *reinterpret_cast<const uint4 *>(vs + kOffDv + 64 * b + 16 * g);
+        half8 bvn[2];
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) bvn[hf] = lds_half8(smem, vb0 + 1024 * hf, vb1 + 1024 * hf);
+#pragma unroll
+        for (int b = 0; b < 8; ++b) {
+            const half8 bv[2] = {bvn[0], bvn[1]};
+            if (b < 7) {
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf)
+                    bvn[hf] = lds_half8(smem, vb0 + 1024 * (2 * b + 2 + hf), vb1 + 1024 * (2 * b + 2 + hf));
+            }
+            half8 dvb;
+            __builtin_memcpy(&dvb, &dvr[b], 16);
+            // A = P 2^ep d_v as an fp16 hi + lo pair (22 bits): the products with the
+            // exact V codes are then exact in fp32, so a row that a few keys
+            // dominate carries no fp16 rounding of P d_v into its output. Ph d_v has
+            // at most 22 significant bits, so its residual after rounding to fp16
+            // (at most 11 bits) is exact in one fma; Pl d_v is 2^-11 of it and
+            // rounds once.
+            half8 ah[kRG], al[kRG];
+#pragma unroll
+            for (int rg = 0; rg < kRG; ++rg) {
+                ah[rg] = ph[rg] * dvb;
+                const half8 r = __builtin_elementwise_fma(ph[rg], dvb, -ah[rg]);
+                al[rg] = __builtin_elementwise_fma(pl[rg], dvb, r);
+            }
+#pragma unroll
+            for (int rg = 0; rg < kRG; ++rg)
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf)
+                    acc[rg][2 * b + hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[rg], bv[hf], acc[rg][2 * b + hf], 0, 0, 0);
+#pragma unroll
+            for (int rg = 0; rg < kRG; ++rg)
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf)
+                    acc[rg][2 * b + hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(al[rg], bv[hf], acc[rg][2 * b + hf], 0, 0, 0);
+        }
+        if (e_new != e_acc) {  // a larger V scale has come: O onto its exponent
+            const float f = __builtin_amdgcn_ldexpf(1.0f, e_new - e_acc);
+#pragma unroll
+            for (int rg = 0; rg < kRG; ++rg)
+#pragma unroll
+                for (int T = 0; T < 16; ++T) acc[rg][T] *= f;
+        }
+    }
+    __syncthreads();  // m and l of the rows ...
+    __syncthreads();  // ... are in LDS
+    const float o_scale = __builtin_amdgcn_ldexpf(1.0f, -e_new);
+#pragma unroll
+    for (int rg = 0; rg < kRG; ++rg) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = 16 * kRG * w + 16 * rg + 4 * g + i;
+            const int tok = r / p.G, h = kvh * p.G + r - tok * p.G;
+            if (q_base + tok >= q_top) continue;
+            const float mrow = n_tiles > 0 ? ml[rg * 32 + 2 * (4 * g + i)] : -INFINITY;
+            const float lrow = n_tiles > 0 ? ml[rg * 32 + 2 * (4 * g + i) + 1] : 0.0f;
+            if (whole) {
+                const int64_t row = rq.q0 + q_base + tok;
+                const float inv = lrow == 0.0f ? 0.0f : o_scale / lrow;
+#pragma unroll
+                for (int T = 0; T < 16; ++T) {
+                    float o = acc[rg][T][i] * inv;
+                    if (p.gate) {
+                        const float gv = reinterpret_cast<const float *>(p.gate + row * p.gate_nb2 + h * p.gate_nb1)[16 * T + n];
+                        o = o * (1.0f / (1.0f + expf(-gv)));
+                    }
+                    store_through(p.dst + (row * p.H + h) * kHeadDim + 16 * T + n, o);
+                }
+            } else {
+                const int64_t at = (int64_t)slot * rows_per_wg(kRG) + r;
+#pragma unroll
+                for (int T = 0; T < 16; ++T) store_through(p.acc_c + at * kHeadDim + 16 * T + n, acc[rg][T][i] * o_scale);
+                if (n == 0) {
+                    // the merge works in base e (acc and l of every split carry the same
+                    // 2^kEp, which cancels there)
+                    store_through(p.ml_c + at * 2, mrow == -INFINITY ? mrow : mrow * kLn2);
+                    store_through(p.ml_c + at * 2 + 1, lrow);
+                }
+            }
+        }
+    }
+}
+
+}  // namespace
+
+int launch_many(const Call &c, hipStream_t s) {
+    const bool opt = c.cap2 != 0.0f || c.bias != 0.0f;
+    static std::once_flag once;  // the LDS limit is raised once per process
+    static hipError_t err = hipSuccess;
+    std::call_once(once, [] {
+        for (const void *f : {(const void *)paged_many_kernel<1, false>, (const void *)paged_many_kernel<1, true>,
+                              (const void *)paged_many_kernel<2, false>, (const void *)paged_many_kernel<2, true>})
+            if (err == hipSuccess) err = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsBytes);
+    });
+    if (err != hipSuccess) return hip_status(err, "paged_attn LDS attribute");
+    const dim3 grid((unsigned)c.grid_c);
+    const int prof = profile_start("paged_chunk", s);
+    if (c.rows_c == 64 && opt) paged_many_kernel<1, true><<<grid, dim3(kThreads), kLdsBytes, s>>>(c);
+    else if (c.rows_c == 64) paged_many_kernel<1, false><<<grid, dim3(kThreads), kLdsBytes, s>>>(c);
+    else if (opt) paged_many_kernel<2, true><<<grid, dim3(kThreads), kLdsBytes, s>>>(c);
+    else paged_many_kernel<2, false><<<grid, dim3(kThreads), kLdsBytes, s>>>(c);
+    profile_stop(prof, s);
+    return hip_status(hipGetLastError(), "paged_attn launch");
+}
+
+}  // namespace paged
+}  // namespace sqa
