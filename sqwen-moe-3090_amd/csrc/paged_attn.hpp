@@ -101,6 +101,21 @@ __device__ __forceinline__ int page_id(const int32_t *row, int i) {
     return reinterpret_cast<constant_int *>((uintptr_t)row)[i];
 }
 
+// 16 bytes per lane from sbase + voff into LDS at m0v + 16 * lane (asynchronous; the
+// caller waits with s_waitcnt vmcnt). sbase and m0v are wave-uniform. The compiler
+// does not know what the asm holds, so the waits that it puts between a vector
+// instruction that writes a scalar register and a memory instruction that reads it
+// (5 states: sbase may come out of v_readfirstlane just before), and between a write of
+// m0 and a load into LDS (1), stand in the asm. Without them the load took a base half
+// old, half new.
+__device__ __forceinline__ void dma16(uint32_t voff, const void *sbase, uint32_t m0v) {
+    const uint64_t b = (uint64_t)(uintptr_t)sbase;
+    const uint64_t bs = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32) |
+                        (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)b);
+    const uint32_t ms = (uint32_t)__builtin_amdgcn_readfirstlane((int)m0v);
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(bs), "{m0}"(ms) : "memory");
+}
+
 // Distance slope of query head h times log2(e).
 __device__ __forceinline__ float slope2(const Call &c, int h) {
     const float e = h < c.nl2 ? (float)(h + 1) / (float)c.nl2 : 0.5f * (float)(2 * (h - c.nl2) + 1) / (float)c.nl2;

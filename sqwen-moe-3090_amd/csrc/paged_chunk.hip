@@ -20,11 +20,11 @@
 //   iteration t: rows of K tile t + 2 and V tile t + 1 are on their way; K tile t + 1
 //   and V tile t are expanded; P V of tile t - 1.
 // K codes leave a dword of nibbles by shifts and masks alone: the 8 values of a chunk
-// are its dims in the order 0 2 1 3 16 18 17 19, and Q' is laid out in the same order.
+// are its dims in the order 0 2 16 18 1 3 17 19, and Q' is laid out in the same order.
 // V needs the codes of 8 keys side by side: 16-bit reads of 8 rows, packed in pairs.
 //
-// d_v enters as d_v 2^E with E from the largest |d_v| of the keys so far (in [1/2, 1)
-// there; O is rescaled when it falls), and P as P 2^kEp, so that A = P d_v stays below
+// d_v enters as d_v 2^E with E, one for a pair of blocks, from the largest |d_v| of the
+// keys so far (in [1/2, 1) there; O is rescaled when it falls), and P as P 2^kEp, so that A = P d_v stays below
 // 2^14 and the parts that count stay clear of fp16's subnormals for V of any size.
 #include <mutex>
 
@@ -49,23 +49,20 @@ constexpr int kKStage = kOffDk + 8 * kPK * 2;
 constexpr int kOffDv = kHeadDim * kPK * 2;  // V stage: Vc, Dv
 constexpr int kVStage = kOffDv + 8 * kPK * 2;
 constexpr int kRawTile = kPK * kHeadRowBytes;  // q4_0 rows of a tile
-// LDS map: 2 K stages | 2 V stages | 2 P buffers | 2 rescale buffers | raw K, V tiles, 2 each
+// LDS map: 2 K stages | 2 V stages | 2 P buffers | 2 rescale buffers | 2 sets of exponents | raw K, V tiles, 2 each
 constexpr int kLdsV = 2 * kKStage;
 constexpr int kLdsP = kLdsV + 2 * kVStage;        // [4 waves][kRG][2 halves][64 lanes][16 B]
 constexpr int kPBuf = kScoreWaves * kMaxRG * 2 * 1024;
 constexpr int kLdsA = kLdsP + 2 * kPBuf;          // [4 waves][kRG][16 rows] f32
 constexpr int kABuf = kScoreWaves * kMaxRG * 16 * 4;
-constexpr int kLdsRaw = kLdsA + 2 * kABuf;        // [K, V][2][32 rows][144 B]
+constexpr int kLdsE = kLdsA + 2 * kABuf;          // [2][4] exponents of the V scales, one per pair of blocks
+constexpr int kLdsRaw = kLdsE + 32;               // [K, V][2][32 rows][144 B]
 constexpr int kLdsBytes = kLdsRaw + 4 * kRawTile + 16;
 static_assert(kLdsBytes <= 160 * 1024, "LDS budget");
 static_assert(kLdsRaw % 16 == 0 && kKStage % 16 == 0 && kVStage % 16 == 0, "alignment of the stages");
 constexpr int kSlack = 8;  // log2 of the largest P the lazy rescale admits
 constexpr int kEp = 6;     // P travels as P 2^kEp (at most 2^14)
 constexpr int kMaxE = 24;  // of the V scales: makes the smallest fp16 one
-
-__device__ __forceinline__ uint4 swap_halves(uint4 v, bool swap) {
-    return swap ? make_uint4(v.z, v.w, v.x, v.y) : v;
-}
 
 // max(x, x of lane ^ 16) and max(x, x of lane ^ 32) with gfx950's row swaps (no
 // LDS round trip): each swap returns the two halves of a lane pair's values.
@@ -82,28 +79,26 @@ __device__ __forceinline__ float xmax32(float x) {
 __device__ __forceinline__ int key_row(int k) { return 16 * ((k >> 2) & 1) + 4 * (k >> 3) + (k & 3); }
 
 
-// Two 4-bit codes n (bits 0-3 and 16-19 of x) as the packed fp16 pair n - 8:
-// 0x6400 | n is exactly 1024 + n, and 1024 + n - 1032 is exact.
-__device__ __forceinline__ uint32_t codes_f16(uint32_t x) {
+// Codes n of the low (bits 0-3, 16-19) or high nibbles (4-7, 20-23) of x as the packed
+// fp16 pair n - 8: 0x6400 | n is exactly 1024 + n and 0x6400 | 16 n is 1024 + 16 n; minus
+// 1032, or times 1/16 minus 72, is exact.
+__device__ __forceinline__ uint32_t codes_lo(uint32_t x) {
     const uint32_t y = (x & 0x000F000Fu) | 0x64006400u;
     half2v v;
     __builtin_memcpy(&v, &y, 4);
-    const half2v d = v + half2v{(_Float16)-1032.0f, (_Float16)-1032.0f};
+    v = v + half2v{(_Float16)-1032.0f, (_Float16)-1032.0f};
     uint32_t r;
-    __builtin_memcpy(&r, &d, 4);
+    __builtin_memcpy(&r, &v, 4);
     return r;
 }
-
-// 16 bytes per lane from sbase + voff into LDS at m0 + 16 * lane (asynchronous;
-// the caller waits with s_waitcnt vmcnt).
-__device__ __forceinline__ void dma16(uint32_t voff, const void *sbase, uint32_t m0v) {
-    // wave-uniform, in SGPRs whatever the compiler thinks of it; m0 as an operand: the
-    // compiler writes it and knows it holds the LDS base
-    const uint64_t b = (uint64_t)(uintptr_t)sbase;
-    const uint64_t bs = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32) |
-                        (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)b);
-    const uint32_t ms = (uint32_t)__builtin_amdgcn_readfirstlane((int)m0v);
-    asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(bs), "{m0}"(ms) : "memory");
+__device__ __forceinline__ uint32_t codes_hi(uint32_t x) {
+    const uint32_t y = (x & 0x00F000F0u) | 0x64006400u;
+    half2v v;
+    __builtin_memcpy(&v, &y, 4);
+    v = __builtin_elementwise_fma(v, half2v{(_Float16)0.0625f, (_Float16)0.0625f}, half2v{(_Float16)-72.0f, (_Float16)-72.0f});
+    uint32_t r;
+    __builtin_memcpy(&r, &v, 4);
+    return r;
 }
 
 // Two 8-byte LDS reads into one MFMA operand. volatile keeps them two single
@@ -121,86 +116,91 @@ __device__ __forceinline__ half8 lds_half8(const uint8_t *base, int off_lo, int 
 }
 
 
-// K codes and scales of tile t from its raw rows, by the 256 value lanes: lane vt
-// block vt & 7 of key vt >> 3. Row r = key_row(key) of the stage, 16-byte chunk 4b + m
-// (dims 32b + 4m + {0, 2, 1, 3, 16, 18, 17, 19}) at chunk (4b + m) ^ (r & 7), halves
-// swapped when r & 8.
-__device__ __forceinline__ void expand_k(uint8_t *smem, int t, int vt) {
-    const int key = vt >> 3, b = vt & 7, r = key_row(key);
-    const uint8_t *row = smem + kLdsRaw + (t & 1) * kRawTile + kHeadRowBytes * key;
-    uint8_t *stage = smem + (t & 1) * kKStage;
-    // the 16 bytes of codes start 2 bytes off a dword for even b
-    const uint32_t *src = reinterpret_cast<const uint32_t *>(row + ((18 * b + 2) & ~3));
-    const uint32_t sh = b & 1 ? 0u : 16u;
-    uint32_t w[5];
-#pragma unroll
-    for (int m = 0; m < 5; ++m) w[m] = src[m];
-    *reinterpret_cast<uint16_t *>(stage + kOffDk + (b * kPK + r) * 2) = *reinterpret_cast<const uint16_t *>(row + 18 * b);
-#pragma unroll
-    for (int m = 0; m < 4; ++m) {
-        const uint32_t x = __builtin_amdgcn_alignbit(w[m + 1], w[m], sh);
-        const uint4 c = make_uint4(codes_f16(x), codes_f16(x >> 8), codes_f16(x >> 4), codes_f16(x >> 12));
-        *reinterpret_cast<uint4 *>(stage + r * 512 + 16 * ((4 * b + m) ^ (r & 7))) = swap_halves(c, r & 8);
+// The expansion of a tile by the 256 value lanes, in 9 parts that the wavefronts place
+// between the MFMAs of P V. Stores are 8 bytes, the halves of a 16-byte chunk at
+// addresses that differ in bit 3 (which first is a matter of the row: no selects).
+//   K: lane vt takes block vt & 7 of key vt >> 3. Row r = key_row(key) of the stage,
+//      chunk 4b + m (dims 32b + 4m + {0, 2, 16, 18, 1, 3, 17, 19}) at (4b + m) ^ (r & 7),
+//      halves swapped when r & 8.
+//   V: lane takes bytes 4m + 2i, 4m + 2i + 1 of block b's codes for the keys 8c .. 8c + 7
+//      (c = lane >> 4, b = (lane >> 1) & 7, m = 2 (w >> 1) + (lane & 1), i = w & 1) and
+//      stores those keys' chunk of the bytes' 4 dims, chunk c of dim d at
+//      c ^ ((d >> 1) & 3), halves swapped when d & 8.
+//   V scales: lane takes key lane & 31 of block 2w + (lane >> 5).
+struct Expand {
+    int k_raw, k_sh, k_to, dk_raw, dk_to;   // LDS offsets in the first of two buffers
+    int v_raw, v_to, dv_raw, dv_to, dv_key;
+    uint32_t x[4], k[5];
+    __device__ __forceinline__ void init(int w, int lane) {
+        const int vt = 64 * w + lane, key = vt >> 3, kb = vt & 7, r = key_row(key);
+        dk_raw = kLdsRaw + kHeadRowBytes * key + 18 * kb;
+        k_raw = kLdsRaw + kHeadRowBytes * key + ((18 * kb + 2) & ~3);  // the codes start 2 bytes off a dword for even blocks
+        k_sh = kb & 1 ? 0 : 16;
+        k_to = r * 512 + 16 * ((4 * kb) ^ (r & 7)) + (r & 8);
+        dk_to = kOffDk + (kb * kPK + r) * 2;
+        const int c = lane >> 4, b = (lane >> 1) & 7, m = 2 * (w >> 1) + (lane & 1), i = w & 1;
+        v_raw = kLdsRaw + 2 * kRawTile + kHeadRowBytes * 8 * c + 18 * b + 2 + 4 * m + 2 * i;
+        const int dim = 32 * b + 4 * m + 2 * i;
+        v_to = kLdsV + 64 * dim + 16 * (c ^ ((dim >> 1) & 3)) + (dim & 8);
+        dv_key = lane & 31;
+        dv_raw = kLdsRaw + 2 * kRawTile + kHeadRowBytes * dv_key + 18 * (2 * w + (lane >> 5));
+        dv_to = kLdsV + kOffDv + 64 * (2 * w + (lane >> 5)) + 2 * dv_key;
     }
-}
-
-// V codes and scales of tile t: lane vt takes bytes 4m + 2i, 4m + 2i + 1 of block b's
-// codes (m = vt & 3, b, i = vt >> 7) for the keys 8c .. 8c + 7 and writes those keys' 16-byte
-// chunk of the rows of the bytes' dims, chunk c of dim d at c ^ ((d >> 1) & 3), halves
-// swapped when d & 8. Scales of the first `left` keys whose page is there, the others
-// (and NaN or Inf, bytes that are no q4_0) as 0: their P is 0, and 0 * NaN would not be.
-// Returns the exponent that the scales are stored with: at most e, and such that the
-// largest is below 1.
-__device__ __forceinline__ int expand_v(uint8_t *smem, int t, int vt, int left, bool has_a, bool has_b, int e) {
-    const int lane = vt & 63, w = vt >> 6;
-    const uint8_t *raw = smem + kLdsRaw + (2 + (t & 1)) * kRawTile;
-    uint8_t *stage = smem + kLdsV + (t & 1) * kVStage;
-    // every wavefront reads all scales: block lane >> 3, keys 4 (lane & 7) ..
-    uint32_t d[4];
-    const int sb = lane >> 3, sk = 4 * (lane & 7);
+    // reads of V tile t
+    __device__ __forceinline__ void read_v(const uint8_t *smem, int t) {
+        const uint8_t *src = smem + v_raw + (t & 1) * kRawTile;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        d[j] = *reinterpret_cast<const uint16_t *>(raw + kHeadRowBytes * (sk + j) + 18 * sb);
-        const bool ok = sk + j < left && (sk < 16 ? has_a : has_b) && (d[j] & 0x7C00u) != 0x7C00u;
-        d[j] = ok ? d[j] : 0u;
+        for (int j = 0; j < 4; ++j)
+            x[j] = (uint32_t)*reinterpret_cast<const uint16_t *>(src + kHeadRowBytes * 2 * j) |
+                   ((uint32_t)*reinterpret_cast<const uint16_t *>(src + kHeadRowBytes * (2 * j + 1)) << 16);
     }
-    const int b = (vt >> 2) & 7, m = vt & 3, c = (vt >> 5) & 3, i = vt >> 7;
-    const uint8_t *src = raw + kHeadRowBytes * 8 * c + 18 * b + 2 + 4 * m + 2 * i;
-    uint32_t x[4];
+    // reads of K tile t; its scales move on as they are
+    __device__ __forceinline__ void read_k(uint8_t *smem, int t) {
+        const uint32_t *src = reinterpret_cast<const uint32_t *>(smem + k_raw + (t & 1) * kRawTile);
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-        x[j] = (uint32_t)*reinterpret_cast<const uint16_t *>(src + kHeadRowBytes * 2 * j) |
-               ((uint32_t)*reinterpret_cast<const uint16_t *>(src + kHeadRowBytes * (2 * j + 1)) << 16);
-    const int mx = wave_max((int)(max(max(d[0] & 0x7fffu, d[1] & 0x7fffu), max(d[2] & 0x7fffu, d[3] & 0x7fffu))));
-    if (mx != 0) {
-        const int ex = mx >> 10;
-        const int lg = ex ? ex - 15 : (31 - __builtin_clz(mx)) - 24;  // floor(log2 max |d_v|)
-        e = min(e, -1 - lg);
+        for (int m = 0; m < 5; ++m) k[m] = src[m];
+        *reinterpret_cast<uint16_t *>(smem + dk_to + (t & 1) * kKStage) =
+            *reinterpret_cast<const uint16_t *>(smem + dk_raw + (t & 1) * kRawTile);
     }
-    if ((lane >> 4) == w) {
-        const float f = __builtin_amdgcn_ldexpf(1.0f, e);
-        uint16_t o[4];
+    // byte j of the lane's two, both nibbles
+    __device__ __forceinline__ void store_v(uint8_t *smem, int t, int j) {
+        const int to = v_to + (t & 1) * kVStage + 64 * j;
+        uint32_t y[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint16_t bits = (uint16_t)d[j];
-            _Float16 hv;
-            __builtin_memcpy(&hv, &bits, 2);
-            hv = (_Float16)((float)hv * f);
-            __builtin_memcpy(&o[j], &hv, 2);
+        for (int q = 0; q < 4; ++q) y[q] = j ? x[q] >> 8 : x[q];
+        *reinterpret_cast<uint2 *>(smem + to) = make_uint2(codes_lo(y[0]), codes_lo(y[1]));
+        *reinterpret_cast<uint2 *>(smem + (to ^ 8)) = make_uint2(codes_lo(y[2]), codes_lo(y[3]));
+        *reinterpret_cast<uint2 *>(smem + to + 1024) = make_uint2(codes_hi(y[0]), codes_hi(y[1]));
+        *reinterpret_cast<uint2 *>(smem + (to ^ 8) + 1024) = make_uint2(codes_hi(y[2]), codes_hi(y[3]));
+    }
+    // chunk m of the lane's block
+    __device__ __forceinline__ void store_k(uint8_t *smem, int t, int m) {
+        const int to = (k_to + (t & 1) * kKStage) ^ (16 * m);
+        const uint32_t y = __builtin_amdgcn_alignbit(k[m + 1], k[m], (uint32_t)k_sh), z = y >> 8;
+        *reinterpret_cast<uint2 *>(smem + to) = make_uint2(codes_lo(y), codes_hi(y));
+        *reinterpret_cast<uint2 *>(smem + (to ^ 8)) = make_uint2(codes_lo(z), codes_hi(z));
+    }
+    // V scales of tile t as d_v 2^e (two blocks of this wavefront), 0 for keys at or past
+    // `left`, on pages that are not there, and for NaN or Inf (bytes that are no q4_0):
+    // their P is 0, and 0 * NaN would not be. Returns e: at most the one given, and such
+    // that the largest is below 1.
+    __device__ __forceinline__ int scales_v(uint8_t *smem, int t, int left, bool has_a, bool has_b, int e) {
+        uint32_t d = *reinterpret_cast<const uint16_t *>(smem + dv_raw + (t & 1) * kRawTile);
+        const bool ok = dv_key < left && (dv_key < 16 ? has_a : has_b) && (d & 0x7C00u) != 0x7C00u;
+        d = ok ? d : 0u;
+        const int mx = wave_max((int)(d & 0x7fffu));
+        if (mx != 0) {
+            const int ex = mx >> 10;
+            const int lg = ex ? ex - 15 : (31 - __builtin_clz(mx)) - 24;  // floor(log2 max |d_v|)
+            e = min(e, -1 - lg);
         }
-        uint2 u;
-        __builtin_memcpy(&u, o, 8);
-        *reinterpret_cast<uint2 *>(stage + kOffDv + 64 * sb + 2 * sk) = u;
+        const uint16_t bits = (uint16_t)d;
+        _Float16 h;
+        __builtin_memcpy(&h, &bits, 2);
+        *reinterpret_cast<_Float16 *>(smem + dv_to + (t & 1) * kVStage) = (_Float16)__builtin_amdgcn_ldexpf((float)h, e);
+        return e;
     }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {  // low nibbles of both bytes, high nibbles
-        const int sh = (k & 1) * 8 + (k >> 1) * 4;
-        const int dim = 32 * b + 4 * m + 2 * i + (k & 1) + 16 * (k >> 1);
-        const uint4 u = make_uint4(codes_f16(x[0] >> sh), codes_f16(x[1] >> sh), codes_f16(x[2] >> sh), codes_f16(x[3] >> sh));
-        *reinterpret_cast<uint4 *>(stage + 64 * dim + 16 * (c ^ ((dim >> 1) & 3))) = swap_halves(u, dim & 8);
-    }
-    return e;
-}
+};
 
 // Q' of a row as B operands: the lane's 8 dims of every block (in the order of the K
 // chunks), q8_0 with ggml's x86 rounding (d = amax / 127 over the block, codes =
@@ -212,7 +212,7 @@ __device__ __forceinline__ void quantize_q(const Call &p, int64_t row, int h, in
     for (int b = 0; b < 8; ++b) {
         const float4a a = *reinterpret_cast<const float4a *>(q + 32 * b + 4 * g);
         const float4a c = *reinterpret_cast<const float4a *>(q + 32 * b + 16 + 4 * g);
-        float v[8] = {a.x, a.z, a.y, a.w, c.x, c.z, c.y, c.w};
+        float v[8] = {a.x, a.z, c.x, c.z, a.y, a.w, c.y, c.w};
         float amax = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -354,6 +354,9 @@ __device__ __forceinline__ Item many_item(const Call &c, int lin, int qb) {
         first = __builtin_amdgcn_readlane(upto, 63);
         slot = __builtin_amdgcn_readlane(slots, 63);
     }
+    // (divisions run on the vector unit: back into scalar registers)
+    for (int *x : {&it.b, &it.kvh, &it.tile, &it.tiles, &it.split, &it.splits, &it.t0, &it.t1, &it.slot})
+        *x = __builtin_amdgcn_readfirstlane(*x);
     return it;
 }
 
@@ -619,17 +622,11 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
 
     // ---- value waves: O[row 16 kRG w + 16rg + 4g + i][dim 16T + n] ----------------
     const int w = wave - kScoreWaves;
-    const int vt = 64 * w + lane;
     const float *ml = reinterpret_cast<const float *>(smem + kLdsP) + w * (kRG * 32);  // [rg][row][m, l]
     // V operand of dim 16T + n, keys 8g..8g+7: chunk g ^ ((n >> 1) & 3), halves swapped when n & 8.
     const int v_off0 = 64 * n + 16 * (g ^ ((n >> 1) & 3)) + 8 * nh;
     const int v_off1 = v_off0 ^ 8;
     const int p_off = w * (kRG * 2048) + 16 * lane;
-    floatx4 acc[kRG][16];
-#pragma unroll
-    for (int rg = 0; rg < kRG; ++rg)
-#pragma unroll
-        for (int T = 0; T < 16; ++T) acc[rg][T] = floatx4{0.f, 0.f, 0.f, 0.f};
     // DMA: wave w moves 16 rows of a tile, group w & 1, of K (w < 2) or V. They lie on
     // one page: 9 x 16 bytes a row as two instructions of 64 lanes and one of 16.
     uint32_t off[3];
@@ -653,13 +650,36 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
     // ids of the groups of tiles t, t + 1, t + 2
     int a0 = id_of(0, 0), b0 = id_of(0, 1), a1 = id_of(1, 0), b1 = id_of(1, 1), a2 = id_of(2, 0), b2 = id_of(2, 1);
     auto mine = [&](int a, int b) { return w & 1 ? b : a; };
-    int e_new = kMaxE, e_acc = kMaxE;  // exponents of the V scales: of the next tile, of O
+    Expand ex;
+    ex.init(w, lane);
+    int e_own = kMaxE;                            // of this wavefront's pair of blocks, up to the tile expanded last
+    int4 e_acc = make_int4(kMaxE, kMaxE, kMaxE, kMaxE);  // of O's pairs
+    auto scales = [&](int t, int a, int b) {
+        e_own = ex.scales_v(smem, t, k_end - (k_begin + t * kPK), there(a), there(b), e_own);
+        if (lane == 0) *reinterpret_cast<int *>(smem + kLdsE + 16 * (t & 1) + 4 * w) = e_own;
+    };
     if (n_tiles > 0) {
         issue(0, mine(a0, b0));
         if (w < 2 && n_tiles > 1) issue(1, mine(a1, b1));
         asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-        expand_k(smem, 0, vt);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            ex.read_k(smem, k);
+#pragma unroll
+            for (int m = 0; m < 4; ++m) ex.store_k(smem, k, m);
+        }
+        scales(0, a0, b0);
+        ex.read_v(smem, 0);
+        ex.store_v(smem, 0, 0);
+        ex.store_v(smem, 0, 1);
     }
+    floatx4 acc[kRG][16];
+#pragma unroll
+    for (int rg = 0; rg < kRG; ++rg)
+#pragma unroll
+        for (int T = 0; T < 16; ++T) acc[rg][T] = floatx4{0.f, 0.f, 0.f, 0.f};
+    // (behind the last tile the expansion works on bytes that are there, into stages that
+    // nobody reads any more)
     for (int t = 0; t <= n_tiles && n_tiles > 0; ++t) {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         const int a3 = id_of(t + 3, 0), b3 = id_of(t + 3, 1);
@@ -668,14 +688,9 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
         } else {
             if (t + 1 < n_tiles) issue(t + 1, mine(a1, b1));
         }
-        e_acc = e_new;
-        if (t < n_tiles) {
-            const int left = k_end - (k_begin + t * kPK);
-            e_new = expand_v(smem, t, vt, left, there(a0), there(b0), e_new);
-            if (t + 1 < n_tiles) expand_k(smem, t + 1, vt);
-        }
+        const int x0 = a0, y0 = b0;
         a0 = a1, b0 = b1, a1 = a2, b1 = b2, a2 = a3, b2 = b3;
-        if (t == 0) continue;  // O is still zero: it takes the first tile's exponent as it is
+        if (t == 0) continue;
         const int tp = t - 1;
         const uint8_t *vs = smem + kLdsV + (tp & 1) * kVStage;
         // this tile's two per-lane V bases, opaque to the compiler (see the K reads)
@@ -683,6 +698,11 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
         asm volatile("" : "+v"(vb0), "+v"(vb1));
         const uint8_t *pb = smem + kLdsP + (tp & 1) * kPBuf + p_off;
         const float *ab = reinterpret_cast<const float *>(smem + kLdsA + (tp & 1) * kABuf) + w * (kRG * 16);
+        // O onto the exponents of this tile's V scales where a larger one has come
+        int4 e_t = *reinterpret_cast<const int4 *>(smem + kLdsE + 16 * (tp & 1));
+        e_t.x = __builtin_amdgcn_readfirstlane(e_t.x), e_t.y = __builtin_amdgcn_readfirstlane(e_t.y);
+        e_t.z = __builtin_amdgcn_readfirstlane(e_t.z), e_t.w = __builtin_amdgcn_readfirstlane(e_t.w);
+        ex.read_v(smem, t);
         half8 ph[kRG], pl[kRG];
         bool resc = false;
 #pragma unroll
@@ -701,24 +721,36 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
                 for (int T = 0; T < 16; ++T) acc[rg][T] *= a4;
             }
         }
-        // d_v of the 8 blocks and V of block 0 first, then V of block b + 1 while
-        // block b computes: the LDS latency stays off the MFMA chain
-        uint4 dvr[8];
+        if ((e_t.x ^ e_acc.x) | (e_t.y ^ e_acc.y) | (e_t.z ^ e_acc.z) | (e_t.w ^ e_acc.w)) {
+            const int from[4] = {e_acc.x, e_acc.y, e_acc.z, e_acc.w}, to[4] = {e_t.x, e_t.y, e_t.z, e_t.w};
 #pragma unroll
-        for (int b = 0; b < 8; ++b) dvr[b] = *reinterpret_cast<const uint4 *>(vs + kOffDv + 64 * b + 16 * g);
+            for (int q = 0; q < 4; ++q) {
+                const float f = __builtin_amdgcn_ldexpf(1.0f, to[q] - from[q]);
+#pragma unroll
+                for (int rg = 0; rg < kRG; ++rg)
+#pragma unroll
+                    for (int T = 4 * q; T < 4 * q + 4; ++T) acc[rg][T] *= f;
+            }
+            e_acc = e_t;
+        }
+        // d_v and V of block b + 1 are read while block b computes: the LDS latency stays
+        // off the MFMA chain. Between the blocks, parts of the next tiles' expansion.
+        uint4 dvn = *reinterpret_cast<const uint4 *>(vs + kOffDv + 16 * g);
         half8 bvn[2];
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) bvn[hf] = lds_half8(smem, vb0 + 1024 * hf, vb1 + 1024 * hf);
 #pragma unroll
         for (int b = 0; b < 8; ++b) {
             const half8 bv[2] = {bvn[0], bvn[1]};
+            const uint4 dvr = dvn;
             if (b < 7) {
+                dvn = *reinterpret_cast<const uint4 *>(vs + kOffDv + 64 * (b + 1) + 16 * g);
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf)
                     bvn[hf] = lds_half8(smem, vb0 + 1024 * (2 * b + 2 + hf), vb1 + 1024 * (2 * b + 2 + hf));
             }
             half8 dvb;
-            __builtin_memcpy(&dvb, &dvr[b], 16);
+            __builtin_memcpy(&dvb, &dvr, 16);
             // A = P 2^ep d_v as an fp16 hi + lo pair (22 bits): the products with the
             // exact V codes are then exact in fp32, so a row that a few keys
             // dominate carries no fp16 rounding of P d_v into its output. Ph d_v has
@@ -742,18 +774,16 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf)
                     acc[rg][2 * b + hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(al[rg], bv[hf], acc[rg][2 * b + hf], 0, 0, 0);
-        }
-        if (e_new != e_acc) {  // a larger V scale has come: O onto its exponent
-            const float f = __builtin_amdgcn_ldexpf(1.0f, e_new - e_acc);
-#pragma unroll
-            for (int rg = 0; rg < kRG; ++rg)
-#pragma unroll
-                for (int T = 0; T < 16; ++T) acc[rg][T] *= f;
+            if (b == 0) scales(t, x0, y0);
+            if (b == 1) ex.store_v(smem, t, 0);
+            if (b == 2) ex.store_v(smem, t, 1);
+            if (b == 2) ex.read_k(smem, t + 1);
+            if (b >= 4) ex.store_k(smem, t + 1, b - 4);
         }
     }
     __syncthreads();  // m and l of the rows ...
     __syncthreads();  // ... are in LDS
-    const float o_scale = __builtin_amdgcn_ldexpf(1.0f, -e_new);
+    const int e_out[4] = {-e_acc.x, -e_acc.y, -e_acc.z, -e_acc.w};
 #pragma unroll
     for (int rg = 0; rg < kRG; ++rg) {
 #pragma unroll
@@ -765,10 +795,10 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
             const float lrow = n_tiles > 0 ? ml[rg * 32 + 2 * (4 * g + i) + 1] : 0.0f;
             if (whole) {
                 const int64_t row = rq.q0 + q_base + tok;
-                const float inv = lrow == 0.0f ? 0.0f : o_scale / lrow;
+                const float inv = lrow == 0.0f ? 0.0f : 1.0f / lrow;
 #pragma unroll
                 for (int T = 0; T < 16; ++T) {
-                    float o = acc[rg][T][i] * inv;
+                    float o = __builtin_amdgcn_ldexpf(acc[rg][T][i], e_out[T >> 2]) * inv;
                     if (p.gate) {
                         const float gv = reinterpret_cast<const float *>(p.gate + row * p.gate_nb2 + h * p.gate_nb1)[16 * T + n];
                         o = o * (1.0f / (1.0f + expf(-gv)));
@@ -778,7 +808,7 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
             } else {
                 const int64_t at = (int64_t)slot * rows_per_wg(kRG) + r;
 #pragma unroll
-                for (int T = 0; T < 16; ++T) store_through(p.acc_c + at * kHeadDim + 16 * T + n, acc[rg][T][i] * o_scale);
+                for (int T = 0; T < 16; ++T) store_through(p.acc_c + at * kHeadDim + 16 * T + n, __builtin_amdgcn_ldexpf(acc[rg][T][i], e_out[T >> 2]));
                 if (n == 0) {
                     // the merge works in base e (acc and l of every split carry the same
                     // 2^kEp, which cancels there)

@@ -72,19 +72,6 @@ constexpr int kMaxDvExp = 28;
 static_assert(2 * kLdsBytes <= 160 * 1024, "two workgroups per CU");
 static_assert(4 * 2 * 64 * 32 <= (kVStages - 1) * kTensorBytes, "Q operands must fit in V stages 1..2");
 
-// 16 bytes per lane from sbase + voff into LDS at m0 + 16 * lane. The data
-// arrives asynchronously; the caller waits with s_waitcnt vmcnt.
-// sbase and m0v are wave-uniform; readfirstlane keeps them in SGPRs even where
-// the compiler has placed them in VGPRs.
-__device__ __forceinline__ void dma16(uint32_t voff, const void *sbase, uint32_t m0v) {
-    const uint64_t b = (uint64_t)(uintptr_t)sbase;
-    const uint64_t bs = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32) |
-                        (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)b);
-    const uint32_t ms = (uint32_t)__builtin_amdgcn_readfirstlane((int)m0v);
-    // m0 as an operand: the compiler writes it and knows it holds the LDS base
-    asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(bs), "{m0}"(ms) : "memory");
-}
-
 typedef const __attribute__((address_space(3))) uint32_t lds_u32;  // LDS dword from a raw LDS address
 
 __device__ __forceinline__ uint32_t lds32(const uint8_t *p) { return *reinterpret_cast<const uint32_t *>(p); }
@@ -217,6 +204,8 @@ __device__ __forceinline__ Piece few_piece(const Call &c, int piece, int most) {
         }
         first = __builtin_amdgcn_readlane(upto, 63);
     }
+    // (divisions run on the vector unit: back into scalar registers)
+    for (int *x : {&pc.b, &pc.split, &pc.n, &pc.first, &pc.t0, &pc.t1}) *x = __builtin_amdgcn_readfirstlane(*x);
     return pc;
 }
 
