@@ -3,7 +3,7 @@
 //
 // Requests of few query rows (up to 16 per KV head; up to 8 where larger ones may be
 // in the call) go to paged_decode.hip, the others to paged_chunk.hip.
-#include "paged_attn.hpp"
+#include "paged_work.hpp"
 
 namespace sqa {
 namespace paged {
@@ -143,12 +143,12 @@ __global__ __launch_bounds__(kThreads) void merge_rows_kernel(Call c, int heads)
 
 size_t al256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-// What a call launches, and its workspace: the tokens' entries, then the slots of the
+// What a call launches, and its workspace: the tokens' entries, the many-row plan, the slots of the
 // few-row kernel, then those of the many-row kernel.
 struct Plan {
     int most_d, rows_d, rows_c;  // of Call
     int64_t slots_d, least_d, slots_c, grid_c;
-    size_t where, slot_d, slot_c;
+    size_t where, work, slot_d, slot_c;
 };
 
 Plan plan(int64_t n_tok, int64_t H, int64_t Hkv, int64_t B, int64_t max_q) {
@@ -168,6 +168,7 @@ Plan plan(int64_t n_tok, int64_t H, int64_t Hkv, int64_t B, int64_t max_q) {
         const int64_t wgs = (n_tok / (p.rows_c / G) + active) * Hkv;
         p.grid_c = (wgs + cus > 3 * cus ? wgs + cus : 3 * cus) + 7 & ~(int64_t)7;
         p.slots_c = 3 * cus;
+        p.work = al256(work_bytes(B));
         p.slot_c = (size_t)p.rows_c * (kHeadDim + 2) * 4;
     }
     return p;
@@ -181,7 +182,7 @@ int launch_combine(const Call &c, hipStream_t s) {
     if (rows <= 128) {
         merge_dims_kernel<<<dim3((unsigned)rows, 16), dim3(kThreads), 0, s>>>(c);
     } else {
-        const int heads = c.n_tok <= 1024 ? 1 : c.H;
+        const int heads = rows <= (1 << 16) ? 1 : 4;  // tokens without partials end at once
         const int64_t waves = (int64_t)c.n_tok * ((c.H + heads - 1) / heads);
         merge_rows_kernel<<<dim3((unsigned)((waves + 3) / 4)), dim3(kThreads), 0, s>>>(c, heads);
     }
@@ -196,7 +197,7 @@ using namespace paged;
 size_t paged_attn_workspace(int64_t n_tok, int64_t H, int64_t Hkv, int64_t B, int64_t max_q) {
     if (n_tok < 1) return 0;
     const Plan p = plan(n_tok, H, Hkv, B, max_q);
-    return p.where + (size_t)p.slots_d * p.slot_d + (size_t)p.slots_c * p.slot_c + 512;
+    return p.where + p.work + (size_t)p.slots_d * p.slot_d + (size_t)p.slots_c * p.slot_c + 512;
 }
 
 int launch_paged_attn(const PagedArgs &a, hipStream_t s) {
@@ -225,11 +226,11 @@ int launch_paged_attn(const PagedArgs &a, hipStream_t s) {
     c.cus = device_cu_count();
 
     const Plan p = plan(c.n_tok, c.H, c.Hkv, c.B, a.max_q);
-    const size_t need = p.where + (size_t)p.least_d * p.slot_d + 512;
+    const size_t need = p.where + p.work + (size_t)p.least_d * p.slot_d + 512;
     if (!a.ws || a.ws_bytes < need)
         return set_error(SQA_ERR_WORKSPACE, "paged_attn: workspace %zu bytes < %zu needed", a.ws ? a.ws_bytes : (size_t)0, need);
     if (p.grid_c > INT32_MAX) return set_error(SQA_ERR_UNSUPPORTED, "paged_attn: too many query tiles");
-    size_t left = a.ws_bytes - 512 - p.where;
+    size_t left = a.ws_bytes - 512 - p.where - p.work;
     c.most_d = p.most_d, c.rows_d = p.rows_d, c.rows_c = p.rows_c, c.grid_c = (int)p.grid_c;
     auto take = [&left](int64_t slots, size_t bytes) {
         if (!slots || (size_t)slots > left / bytes) slots = slots ? (int64_t)(left / bytes) : 0;
@@ -240,7 +241,8 @@ int launch_paged_attn(const PagedArgs &a, hipStream_t s) {
     c.slots_c = take(p.slots_c, p.slot_c);
     uint8_t *base = reinterpret_cast<uint8_t *>(((uintptr_t)a.ws + 255) & ~(uintptr_t)255);
     c.where = reinterpret_cast<int4 *>(base);
-    c.acc_d = reinterpret_cast<float *>(base + p.where);
+    c.work = reinterpret_cast<int *>(base + p.where);
+    c.acc_d = reinterpret_cast<float *>(base + p.where + p.work);
     c.acc_c = c.acc_d + (size_t)c.slots_d * c.rows_d * kHeadDim;
     c.ml_d = c.acc_c + (size_t)c.slots_c * c.rows_c * kHeadDim;
     c.ml_c = c.ml_d + (size_t)c.slots_d * c.rows_d * 2;

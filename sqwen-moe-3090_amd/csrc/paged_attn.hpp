@@ -44,7 +44,8 @@ struct Call {
     float *acc_c, *ml_c;         // [slot][rows_c][256], ...
     int rows_d, rows_c;          // rows of a slot
     int slots_d, slots_c;        // slots of the workspace
-    int grid_c;                  // workgroups of the many-row kernel
+    int *work;                   // the many-row kernel's plan (paged_work.hpp)
+    int grid_c;                  // its workgroups at most
     int most_d;                  // query rows per KV head that the few-row kernel takes (0: it does not run)
     int cus;
 };
@@ -94,12 +95,24 @@ __device__ __forceinline__ int wave_max(int x) {  // of values >= 0
     return __builtin_amdgcn_readlane(x, 63);
 }
 
-// Page id of entry i of a table row, by the scalar cache (i is wave-uniform; the
-// table is not written during the kernel).
-__device__ __forceinline__ int page_id(const int32_t *row, int i) {
-    typedef const __attribute__((address_space(4))) int32_t constant_int;
-    return reinterpret_cast<constant_int *>((uintptr_t)row)[i];
+// A wave-uniform value in a scalar register (what comes out of loads and divisions is in
+// vector registers, and the compiler would go on there: loops, addresses, page ids).
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// The request of a workgroup (b wave-uniform).
+__device__ __forceinline__ Request uniform_request(const Call &c, int b) {
+    const Request r = request(c, b);
+    return Request{uniform(r.q0), uniform(r.n), uniform(r.kv), uniform(r.pos0), uniform(r.prefix)};
 }
+
+// Row b of the table, and a page id of it, by the scalar cache (b and i wave-uniform; the
+// table is not written during the kernel).
+typedef const __attribute__((address_space(4))) int32_t *TableRow;
+__device__ __forceinline__ TableRow table_row(const Call &c, int b) {
+    const uint64_t at = (uint64_t)(uintptr_t)(c.table + (int64_t)b * c.table_stride);
+    return reinterpret_cast<TableRow>(((uint64_t)(uint32_t)uniform((int)(at >> 32)) << 32) | (uint32_t)uniform((int)(uint32_t)at));
+}
+__device__ __forceinline__ int page_id(TableRow row, int i) { return row[i]; }
 
 // 16 bytes per lane from sbase + voff into LDS at m0v + 16 * lane (asynchronous; the
 // caller waits with s_waitcnt vmcnt). sbase and m0v are wave-uniform. The compiler

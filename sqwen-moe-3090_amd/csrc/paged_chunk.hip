@@ -28,7 +28,7 @@
 // 2^14 and the parts that count stay clear of fp16's subnormals for V of any size.
 #include <mutex>
 
-#include "paged_attn.hpp"
+#include "paged_work.hpp"
 
 namespace sqa {
 namespace paged {
@@ -38,7 +38,7 @@ typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 
-constexpr int kPK = 32;                  // keys per tile
+constexpr int kPK = kChunkKeys;          // keys per tile
 constexpr int kScoreWaves = 4;
 constexpr int kValueWaves = 4;
 constexpr int kThreads = 64 * (kScoreWaves + kValueWaves);
@@ -82,8 +82,10 @@ __device__ __forceinline__ int key_row(int k) { return 16 * ((k >> 2) & 1) + 4 *
 // Codes n of the low (bits 0-3, 16-19) or high nibbles (4-7, 20-23) of x as the packed
 // fp16 pair n - 8: 0x6400 | n is exactly 1024 + n and 0x6400 | 16 n is 1024 + 16 n; minus
 // 1032, or times 1/16 minus 72, is exact.
-__device__ __forceinline__ uint32_t codes_lo(uint32_t x) {
-    const uint32_t y = (x & 0x000F000Fu) | 0x64006400u;
+// `magic` is 0x64006400 in a vector register: with the mask in a scalar one, and and or
+// are one instruction (two constants in scalar registers would make them two).
+__device__ __forceinline__ uint32_t codes_lo(uint32_t x, uint32_t magic) {
+    const uint32_t y = (x & 0x000F000Fu) | magic;
     half2v v;
     __builtin_memcpy(&v, &y, 4);
     v = v + half2v{(_Float16)-1032.0f, (_Float16)-1032.0f};
@@ -91,8 +93,8 @@ __device__ __forceinline__ uint32_t codes_lo(uint32_t x) {
     __builtin_memcpy(&r, &v, 4);
     return r;
 }
-__device__ __forceinline__ uint32_t codes_hi(uint32_t x) {
-    const uint32_t y = (x & 0x00F000F0u) | 0x64006400u;
+__device__ __forceinline__ uint32_t codes_hi(uint32_t x, uint32_t magic) {
+    const uint32_t y = (x & 0x00F000F0u) | magic;
     half2v v;
     __builtin_memcpy(&v, &y, 4);
     v = __builtin_elementwise_fma(v, half2v{(_Float16)0.0625f, (_Float16)0.0625f}, half2v{(_Float16)-72.0f, (_Float16)-72.0f});
@@ -119,32 +121,39 @@ __device__ __forceinline__ half8 lds_half8(const uint8_t *base, int off_lo, int 
 // The expansion of a tile by the 256 value lanes, in 9 parts that the wavefronts place
 // between the MFMAs of P V. Stores are 8 bytes, the halves of a 16-byte chunk at
 // addresses that differ in bit 3 (which first is a matter of the row: no selects).
-//   K: lane vt takes block vt & 7 of key vt >> 3. Row r = key_row(key) of the stage,
-//      chunk 4b + m (dims 32b + 4m + {0, 2, 16, 18, 1, 3, 17, 19}) at (4b + m) ^ (r & 7),
-//      halves swapped when r & 8.
+//   K: lane takes block b of key k: k & 3, b & 3, k >> 4, b >> 2 from the lane's bits 0-1,
+//      2-3, 4, 5, the middle bits of k from the wavefront. Row r = key_row(k) of the
+//      stage, chunk 4b + m (dims 32b + 4m + {0, 2, 16, 18, 1, 3, 17, 19}) at
+//      (4b + m) ^ (r & 7), halves swapped when r & 8.
 //   V: lane takes bytes 4m + 2i, 4m + 2i + 1 of block b's codes for the keys 8c .. 8c + 7
-//      (c = lane >> 4, b = (lane >> 1) & 7, m = 2 (w >> 1) + (lane & 1), i = w & 1) and
-//      stores those keys' chunk of the bytes' 4 dims, chunk c of dim d at
-//      c ^ ((d >> 1) & 3), halves swapped when d & 8.
+//      (c, i, m from the lane's bits 0-1, 2, 3-4, b = 2w + bit 5) and stores those keys'
+//      chunk of the bytes' 4 dims, chunk c of dim d at c ^ ((d >> 1) & 3), halves
+//      swapped when d & 8; odd m the second byte first.
 //   V scales: lane takes key lane & 31 of block 2w + (lane >> 5).
+// With these maps the 32 lanes that LDS serves at a time store to 32 different pairs of
+// banks (lanes over whole rows of K and over all blocks of V met in 16 of them 16 deep:
+// 3260 LDS cycles a tile, 56% of them conflicts).
 struct Expand {
     int k_raw, k_sh, k_to, dk_raw, dk_to;   // LDS offsets in the first of two buffers
-    int v_raw, v_to, dv_raw, dv_to, dv_key;
-    uint32_t x[4], k[5];
+    int v_raw, v_to, v_odd, dv_raw, dv_to, dv_key;
+    uint32_t x[4], k[5], magic;
     __device__ __forceinline__ void init(int w, int lane) {
-        const int vt = 64 * w + lane, key = vt >> 3, kb = vt & 7, r = key_row(key);
+        const int key = 16 * ((lane >> 4) & 1) + 4 * w + (lane & 3), kb = 4 * (lane >> 5) + ((lane >> 2) & 3), r = key_row(key);
         dk_raw = kLdsRaw + kHeadRowBytes * key + 18 * kb;
         k_raw = kLdsRaw + kHeadRowBytes * key + ((18 * kb + 2) & ~3);  // the codes start 2 bytes off a dword for even blocks
         k_sh = kb & 1 ? 0 : 16;
         k_to = r * 512 + 16 * ((4 * kb) ^ (r & 7)) + (r & 8);
         dk_to = kOffDk + (kb * kPK + r) * 2;
-        const int c = lane >> 4, b = (lane >> 1) & 7, m = 2 * (w >> 1) + (lane & 1), i = w & 1;
+        const int c = lane & 3, i = (lane >> 2) & 1, m = (lane >> 3) & 3, b = 2 * w + (lane >> 5);
         v_raw = kLdsRaw + 2 * kRawTile + kHeadRowBytes * 8 * c + 18 * b + 2 + 4 * m + 2 * i;
         const int dim = 32 * b + 4 * m + 2 * i;
         v_to = kLdsV + 64 * dim + 16 * (c ^ ((dim >> 1) & 3)) + (dim & 8);
+        v_odd = m & 1;
         dv_key = lane & 31;
-        dv_raw = kLdsRaw + 2 * kRawTile + kHeadRowBytes * dv_key + 18 * (2 * w + (lane >> 5));
-        dv_to = kLdsV + kOffDv + 64 * (2 * w + (lane >> 5)) + 2 * dv_key;
+        dv_raw = kLdsRaw + 2 * kRawTile + kHeadRowBytes * dv_key + 18 * b;
+        dv_to = kLdsV + kOffDv + 64 * b + 2 * dv_key;
+        magic = 0x64006400u;
+        asm volatile("" : "+v"(magic));
     }
     // reads of V tile t
     __device__ __forceinline__ void read_v(const uint8_t *smem, int t) {
@@ -162,23 +171,23 @@ struct Expand {
         *reinterpret_cast<uint16_t *>(smem + dk_to + (t & 1) * kKStage) =
             *reinterpret_cast<const uint16_t *>(smem + dk_raw + (t & 1) * kRawTile);
     }
-    // byte j of the lane's two, both nibbles
+    // byte j of the lane's two (odd m: the other one), both nibbles
     __device__ __forceinline__ void store_v(uint8_t *smem, int t, int j) {
-        const int to = v_to + (t & 1) * kVStage + 64 * j;
+        const int byte = v_odd ^ j, to = v_to + (t & 1) * kVStage + 64 * byte;
         uint32_t y[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) y[q] = j ? x[q] >> 8 : x[q];
-        *reinterpret_cast<uint2 *>(smem + to) = make_uint2(codes_lo(y[0]), codes_lo(y[1]));
-        *reinterpret_cast<uint2 *>(smem + (to ^ 8)) = make_uint2(codes_lo(y[2]), codes_lo(y[3]));
-        *reinterpret_cast<uint2 *>(smem + to + 1024) = make_uint2(codes_hi(y[0]), codes_hi(y[1]));
-        *reinterpret_cast<uint2 *>(smem + (to ^ 8) + 1024) = make_uint2(codes_hi(y[2]), codes_hi(y[3]));
+        for (int q = 0; q < 4; ++q) y[q] = x[q] >> (8 * byte);
+        *reinterpret_cast<uint2 *>(smem + to) = make_uint2(codes_lo(y[0], magic), codes_lo(y[1], magic));
+        *reinterpret_cast<uint2 *>(smem + (to ^ 8)) = make_uint2(codes_lo(y[2], magic), codes_lo(y[3], magic));
+        *reinterpret_cast<uint2 *>(smem + to + 1024) = make_uint2(codes_hi(y[0], magic), codes_hi(y[1], magic));
+        *reinterpret_cast<uint2 *>(smem + (to ^ 8) + 1024) = make_uint2(codes_hi(y[2], magic), codes_hi(y[3], magic));
     }
     // chunk m of the lane's block
     __device__ __forceinline__ void store_k(uint8_t *smem, int t, int m) {
         const int to = (k_to + (t & 1) * kKStage) ^ (16 * m);
         const uint32_t y = __builtin_amdgcn_alignbit(k[m + 1], k[m], (uint32_t)k_sh), z = y >> 8;
-        *reinterpret_cast<uint2 *>(smem + to) = make_uint2(codes_lo(y), codes_hi(y));
-        *reinterpret_cast<uint2 *>(smem + (to ^ 8)) = make_uint2(codes_lo(z), codes_hi(z));
+        *reinterpret_cast<uint2 *>(smem + to) = make_uint2(codes_lo(y, magic), codes_hi(y, magic));
+        *reinterpret_cast<uint2 *>(smem + (to ^ 8)) = make_uint2(codes_lo(z, magic), codes_hi(z, magic));
     }
     // V scales of tile t as d_v 2^e (two blocks of this wavefront), 0 for keys at or past
     // `left`, on pages that are not there, and for NaN or Inf (bytes that are no q4_0):
@@ -188,11 +197,15 @@ struct Expand {
         uint32_t d = *reinterpret_cast<const uint16_t *>(smem + dv_raw + (t & 1) * kRawTile);
         const bool ok = dv_key < left && (dv_key < 16 ? has_a : has_b) && (d & 0x7C00u) != 0x7C00u;
         d = ok ? d : 0u;
-        const int mx = wave_max((int)(d & 0x7fffu));
-        if (mx != 0) {
-            const int ex = mx >> 10;
-            const int lg = ex ? ex - 15 : (31 - __builtin_clz(mx)) - 24;  // floor(log2 max |d_v|)
-            e = min(e, -1 - lg);
+        // fp16 bits of 2^-e, the smallest scale that would reach 1 (e in [-17, 24])
+        const uint32_t over = e <= 14 ? (uint32_t)(15 - e) << 10 : 1u << (24 - e);
+        if (e == kMaxE || __any((d & 0x7fffu) >= over)) {
+            const int mx = wave_max((int)(d & 0x7fffu));
+            if (mx != 0) {
+                const int ex = mx >> 10;
+                const int lg = ex ? ex - 15 : (31 - __builtin_clz(mx)) - 24;  // floor(log2 max |d_v|)
+                e = min(e, -1 - lg);
+            }
         }
         const uint16_t bits = (uint16_t)d;
         _Float16 h;
@@ -246,117 +259,53 @@ struct Item {
     int b, kvh, tile, tiles, split, splits, t0, t1, slot;
 };
 
-constexpr int kMostSplits = 256;  // of a request (the merge's limit)
-constexpr int kChoices = 16;
-// splits of the longest request that are tried
-__device__ constexpr int kTried[kChoices] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64, 128};
-
-// Query tiles of a request (0: none of this kernel's) and its key tiles.
-__device__ __forceinline__ int tiles_of(const Call &c, int b, int qb, int *key_tiles) {
-    *key_tiles = 0;
-    if (b >= c.B) return 0;
-    const Request r = request(c, b);
-    if (r.n * c.G <= c.most_d) return 0;
-    *key_tiles = max((r.kv + kPK - 1) / kPK, 1);
-    return (r.n + qb - 1) / qb;
-}
-
-__device__ __forceinline__ float wave_sum(float x) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o);
-    return x;
-}
-
-// Every request is cut into splits of about `len` key tiles, the same for all, with the
-// len of the least estimated time (in tiles of one workgroup: kWg for a workgroup's
-// own start and end, kMerge for the merge and kMergeSlot for a slot's bytes). Where the
-// parts are about equal they run in rounds of one per CU; where they are not (ragged
-// batches, first chunks, whose tiles see from one to all of the keys) the time is the
-// work over the CUs and half a part.
-constexpr float kWg = 3.0f, kMerge = 3.0f, kMergeSlot = 0.016f;
-
 __device__ __forceinline__ Item many_item(const Call &c, int lin, int qb) {
-    const int lane = threadIdx.x & 63;
-    float work = 0.0f;
-    int longest = 0, wgs = 0;
-    for (int b0 = 0; b0 < c.B; b0 += 64) {
-        int kt;
-        const int T = tiles_of(c, b0 + lane, qb, &kt);
-        wgs += T;
-        longest = max(longest, kt);
-        // query tile i of T ends (T - 1 - i) * qb keys before the last one
-        if (T) work += fmaxf((float)T * (float)kt - 0.5f * (float)T * (float)(T - 1) * (float)qb / kPK, 0.5f * (float)T * (float)kt);
-    }
     Item it{-1, 0, 0, 0, 0, 1, 0, 0, 0};
-    wgs = ::sqa::paged::wave_sum(wgs);
-    if (wgs == 0 || lin >= c.grid_c) return it;
-    work = wave_sum(work) * (float)c.Hkv;
-    longest = wave_max(longest);
-    int len = longest, total = wgs;  // wgs of one head and split; total of one head
-    bool even = true;
-    float best = INFINITY;
-    const float cus = (float)c.cus;
-#pragma unroll 1
-    for (int j = 0; j < kChoices; ++j) {
-        const int l = max((longest + kTried[j] - 1) / kTried[j], 2);
-        if (longest > l * kMostSplits) continue;
-        int n = 0, slots = 0;
-        for (int b0 = 0; b0 < c.B; b0 += 64) {
-            int kt;
-            const int T = tiles_of(c, b0 + lane, qb, &kt), S = (kt + l - 1) / l;
-            n += T * S;
-            slots += S > 1 ? T * S : 0;
+    const Work w = *reinterpret_cast<const Work *>(c.work);
+    const int *first = c.work + kWorkWords, *slot = first + c.B + 1;
+    const int len = uniform(w.len), items = uniform(w.items);
+    if (uniform(w.listed)) {
+        if (lin >= items) return it;
+        const int4 e = reinterpret_cast<const int4 *>(c.work + (kWorkWords + 2 * c.B + 4) / 4 * 4)[lin];
+        it.b = uniform(e.x), it.tile = uniform(e.y), it.kvh = uniform(e.z), it.split = uniform(e.w);
+    } else {
+        // Workgroups go round-robin to the 8 XCDs. Equal parts are renumbered so that an
+        // XCD gets a run of ids, the query tiles of the same keys, which its L2 then
+        // serves to all of them; others go out as they come.
+        int id = lin;
+        if (uniform(w.even)) {
+            const int x = lin & 7, per = items >> 3, rem = items & 7, k = lin >> 3;
+            if (k >= per + (x < rem ? 1 : 0)) return it;
+            id = x * per + (x < rem ? x : rem) + k;
         }
-        n = ::sqa::paged::wave_sum(n);
-        slots = ::sqa::paged::wave_sum(slots);
-        if (j > 0 && ((int64_t)slots * c.Hkv > c.slots_c || (int64_t)n * c.Hkv > c.grid_c)) break;
-        const float N = (float)n * (float)c.Hkv, part = fminf((float)l, (float)longest);
-        const bool eq = work > 0.85f * N * part;
-        float t = eq ? ceilf(N / cus) * (part + kWg) : fmaxf((work + kWg * N) / cus + 0.5f * part, part + kWg);
-        t += slots ? kMerge + kMergeSlot * (float)slots * (float)c.Hkv : 0.0f;
-        if (t < best) best = t, len = l, total = n, even = eq;
-        if (l == 2) break;
-    }
-    // Workgroups go round-robin to the 8 XCDs. Equal parts are renumbered so that an
-    // XCD gets a run of ids, the query tiles of the same keys, which its L2 then serves
-    // to all of them; unequal ones go out as they come, the last query tiles first.
-    const int N = total * c.Hkv;
-    int id = lin;
-    if (even) {
-        const int x = lin & 7, per = N >> 3, rem = N & 7, k = lin >> 3;
-        if (k >= per + (x < rem ? 1 : 0)) return it;
-        id = x * per + (x < rem ? x : rem) + k;
-    }
-    if (id >= N) return it;
-    int first = 0, slot = 0;
-    for (int b0 = 0; b0 < c.B && first <= id; b0 += 64) {
-        int kt;
-        const int T = tiles_of(c, b0 + lane, qb, &kt), S = (kt + len - 1) / len;
-        const int n = T * S * c.Hkv, own = S > 1 ? n : 0;
-        const int upto = first + wave_scan(n), slots = slot + wave_scan(own);
-        const uint64_t hit = __ballot(id >= upto - n && id < upto);
-        if (hit) {
-            const int l = __builtin_ctzll(hit);
-            int r = id - __builtin_amdgcn_readlane(upto - n, l);
-            it.b = b0 + l;
-            it.tiles = __builtin_amdgcn_readlane(T, l);
-            it.splits = __builtin_amdgcn_readlane(S, l);
-            it.slot = __builtin_amdgcn_readlane(slots - own, l);
-            const int keys = __builtin_amdgcn_readlane(kt, l);
-            it.tile = r % it.tiles;
-            r /= it.tiles;
-            it.split = r % it.splits;
-            it.kvh = r / it.splits;
-            if (!even) it.tile = it.tiles - 1 - it.tile;
-            it.t0 = (int)((int64_t)it.split * keys / it.splits);
-            it.t1 = (int)((int64_t)(it.split + 1) * keys / it.splits);
+        if (id >= items) return it;
+        // the last request whose first item is at most id: 64 at a time
+        const int lane = threadIdx.x & 63;
+        int lo = 0, hi = c.B;
+        while (hi - lo > 1) {
+            const int step = (hi - lo + 63) / 64, at = lo + lane * step;
+            const uint64_t below = __ballot(at < hi && first[min(at, c.B)] <= id);
+            const int l = 63 - __builtin_clzll(below);  // lane 0 is always below
+            lo = uniform(lo + l * step);
+            hi = uniform(min(hi, lo + step));
         }
-        first = __builtin_amdgcn_readlane(upto, 63);
-        slot = __builtin_amdgcn_readlane(slots, 63);
+        it.b = lo;
+        it.tile = id - uniform(first[lo]);  // for now: item in the request
+        it.split = -1;
     }
-    // (divisions run on the vector unit: back into scalar registers)
-    for (int *x : {&it.b, &it.kvh, &it.tile, &it.tiles, &it.split, &it.splits, &it.t0, &it.t1, &it.slot})
-        *x = __builtin_amdgcn_readfirstlane(*x);
+    int kt;
+    const int T = chunk_tiles(c, uniform_request(c, it.b), qb, &kt), S = (kt + len - 1) / len;
+    it.tiles = uniform(T);
+    it.splits = uniform(S);
+    if (it.split < 0) {
+        const int r = it.tile / T;
+        it.tile = uniform(it.tile - r * T);
+        it.kvh = uniform(r / S);
+        it.split = uniform(r - it.kvh * S);
+    }
+    it.t0 = uniform((int)((int64_t)it.split * kt / S));
+    it.t1 = uniform((int)((int64_t)(it.split + 1) * kt / S));
+    it.slot = uniform(slot[it.b]);
     return it;
 }
 
@@ -371,7 +320,7 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
 
     const Item it = many_item(p, (int)blockIdx.x, rows_per_wg(kRG) / p.G);
     if (it.b < 0) return;
-    const Request rq = request(p, it.b);
+    const Request rq = uniform_request(p, it.b);
     const int qb = rows_per_wg(kRG) / p.G;  // tokens of a query tile
     const int q_base = it.tile * qb;        // its first token in the request
     const int q_top = min(q_base + qb, rq.n);
@@ -384,7 +333,7 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
     // Key range: the split, cut at the last key any token of the tile sees.
     const int k_begin = it.t0 * kPK;
     const int k_end = min(it.t1 * kPK, sees(rq, q_top - 1));
-    const int n_tiles = k_end > k_begin ? (k_end - k_begin + kPK - 1) / kPK : 0;
+    const int n_tiles = uniform(k_end > k_begin ? (k_end - k_begin + kPK - 1) / kPK : 0);
     if (n_tiles == 0 && !whole) {
         // a split past the tile's last visible key leaves its O unwritten: the
         // merge takes no partial whose m is -inf
@@ -397,7 +346,7 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
     }
     const int kvh = it.kvh;
     const int see_all = sees(rq, q_base);  // keys that every token of the tile sees
-    const int32_t *table = p.table + (int64_t)it.b * p.table_stride;
+    const TableRow table = table_row(p, it.b);
     const int last_group = max(rq.kv - 1, 0) & ~15;
     // 16-key group gi of tile t; one behind the last key stands for the last one
     auto group_key = [&](int t, int gi) {

@@ -30,7 +30,8 @@
 // contributes exactly 0 whatever its bytes.
 #include <mutex>
 
-#include "paged_attn.hpp"
+#define SQA_PLAN_CHUNKS
+#include "paged_work.hpp"
 
 namespace sqa {
 namespace paged {
@@ -70,6 +71,7 @@ constexpr float kPShift = 4.0f;
 // scales below 2^-20 lose low bits of A; 2^E stays two fp16 powers of two.
 constexpr int kMaxDvExp = 28;
 static_assert(2 * kLdsBytes <= 160 * 1024, "two workgroups per CU");
+static_assert((512 + 5 * 3000 + 8) * 4 <= kLdsBytes && (512 + kMaxRequests + 8) * 4 <= kLdsBytes, "the plan's LDS");
 static_assert(4 * 2 * 64 * 32 <= (kVStages - 1) * kTensorBytes, "Q operands must fit in V stages 1..2");
 
 typedef const __attribute__((address_space(3))) uint32_t lds_u32;  // LDS dword from a raw LDS address
@@ -141,8 +143,7 @@ struct Piece {
     int b, split, n, first, t0, t1;
 };
 
-constexpr int kMostSplits = 256;  // of a request (the merge's limit)
-constexpr int kChoices = 8;
+constexpr int kLengths = 8;
 
 // Tiles of a request; 0: none of this kernel's.
 __device__ __forceinline__ int tiles_of(const Call &c, int b, int most) {
@@ -152,14 +153,25 @@ __device__ __forceinline__ int tiles_of(const Call &c, int b, int most) {
     return max((r.kv + kTileKeys - 1) / kTileKeys, 1);
 }
 
+// ceil(t / len) for 0 <= t < 2^26: the float quotient is off by less than one.
+__device__ __forceinline__ int ceil_div(int t, int len, float inv) {
+    int q = (int)((float)t * inv);
+    q -= q * (int64_t)len > t;
+    q += (q + 1) * (int64_t)len <= t;
+    return q + (q * (int64_t)len < t);
+}
+
 // Piece length: of lengths from total / P up to nearly twice that, the shortest whose
 // pieces number at most P, the workgroups that run together; where no length does
 // (as many requests as that) total / P, and the rest follows as others end.
 __device__ __forceinline__ Piece few_piece(const Call &c, int piece, int most) {
     const int lane = threadIdx.x & 63;
+    const bool small = c.B <= 64;
+    const int own = tiles_of(c, lane, most);  // small batches: read once
+    auto tiles = [&](int b0) { return small ? own : tiles_of(c, b0 + lane, most); };
     int total = 0, longest = 0, active = 0;
     for (int b0 = 0; b0 < c.B; b0 += 64) {
-        const int t = tiles_of(c, b0 + lane, most);
+        const int t = tiles(b0);
         total += min(t, 1 << 18);  // 2^12 requests: below 2^31
         longest = max(longest, t);
         active += t > 0;
@@ -171,25 +183,25 @@ __device__ __forceinline__ Piece few_piece(const Call &c, int piece, int most) {
     int P = ((int64_t)total * c.Hkv >= 8 * c.cus ? 2 * c.cus : c.cus) / c.Hkv;
     P = max(min(P, room - active), 1);
     const int base = max(max((total + P - 1) / P, (longest + kMostSplits - 1) / kMostSplits), 1);
-    int n[kChoices] = {};
+    int n[kLengths] = {};
     for (int b0 = 0; b0 < c.B; b0 += 64) {
-        const int t = tiles_of(c, b0 + lane, most);
+        const int t = tiles(b0);
 #pragma unroll
-        for (int j = 0; j < kChoices; ++j) {
-            const int len = (base * (kChoices + j) + kChoices - 1) / kChoices;
-            n[j] += (t + len - 1) / len;
+        for (int j = 0; j < kLengths; ++j) {
+            const int len = (base * (kLengths + j) + kLengths - 1) / kLengths;
+            n[j] += ceil_div(t, len, 1.0f / (float)len);
         }
     }
     int len = 0;
 #pragma unroll
-    for (int j = 0; j < kChoices; ++j)
-        if (len == 0 && wave_sum(n[j]) <= P) len = (base * (kChoices + j) + kChoices - 1) / kChoices;
+    for (int j = 0; j < kLengths; ++j)
+        if (len == 0 && wave_sum(n[j]) <= P) len = (base * (kLengths + j) + kLengths - 1) / kLengths;
     if (len == 0) len = wave_sum(n[0]) <= room ? base : 1 << 26;  // 2^26 tiles: every request whole
     Piece pc{-1, 0, 1, 0, 0, 0};
     int first = 0;
     for (int b0 = 0; b0 < c.B && first <= piece; b0 += 64) {
-        const int t = tiles_of(c, b0 + lane, most);
-        const int k = (t + len - 1) / len;
+        const int t = tiles(b0);
+        const int k = ceil_div(t, len, 1.0f / (float)len);
         const int upto = first + wave_scan(k);
         const uint64_t hit = __ballot(piece >= upto - k && piece < upto);
         if (hit) {
@@ -245,8 +257,8 @@ __device__ __forceinline__ int lds_byte(int row, int c) {
 
 // TWO = false: requests of up to 8 query rows per KV head (one block-diagonal B set).
 // TWO = true : up to 16 rows (rows 0-7 and 8-15 as two B sets, one A operand).
-// OPT: the logits are capped or biased.
-template <bool TWO, bool OPT>
+// OPT: the logits are capped or biased. PLAN: a last workgroup plans the many-row kernel.
+template <bool TWO, bool OPT, bool PLAN>
 __global__ __launch_bounds__(kThreads, TWO || OPT ? 2 : 4) void paged_few_kernel(Call p) {
     extern __shared__ __align__(16) uint8_t smem[];
     const int tid = threadIdx.x;
@@ -262,6 +274,10 @@ __global__ __launch_bounds__(kThreads, TWO || OPT ? 2 : 4) void paged_few_kernel
     asm volatile("" : "+s"(lds0));
     constexpr int kRowMask = TWO ? 15 : 7;  // rows 8-15 mirror rows 0-7 when only 8 exist
 
+    if (PLAN && blockIdx.x == gridDim.x - 1) {
+        plan_chunks(p, reinterpret_cast<int *>(smem));
+        return;
+    }
     // ---------------- piece and KV head of this workgroup ---------------------
     // Workgroups go round-robin to the 8 XCDs: ids 8 Hkv a + 8h + x (x < 8) are
     // piece 8a + x, head h, so all heads of a piece share an XCD (and its L2).
@@ -269,17 +285,17 @@ __global__ __launch_bounds__(kThreads, TWO || OPT ? 2 : 4) void paged_few_kernel
     const int pa = hb / p.Hkv;
     const int kvh = hb - pa * p.Hkv;
     const Piece pc = few_piece(p, (pa << 3) | (int)(blockIdx.x & 7), p.most_d);
-    if (p.rows_c == 0 && blockIdx.x == 0) skip_large(p);
+    if (!PLAN && blockIdx.x == 0) skip_large(p);
     if (pc.b < 0) return;
-    const Request rq = request(p, pc.b);
+    const Request rq = uniform_request(p, pc.b);
     const int rows = rq.n * p.G;
     const int slot = (pc.first + pc.split) * p.Hkv + kvh;
     if (pc.split == 0 && kvh == 0 && tid < rq.n)
         p.where[rq.q0 + tid] = make_int4(pc.first * p.Hkv, pc.n, tid * p.G, p.Hkv * 4 + kFew);
     const int k0 = pc.t0 * kTileKeys;
     const int k1 = min(pc.t1 * kTileKeys, rq.kv);
-    const int n_tiles = k1 > k0 ? (k1 - k0 + kTileKeys - 1) / kTileKeys : 0;
-    const int32_t *table = p.table + (int64_t)pc.b * p.table_stride;
+    const int n_tiles = uniform(k1 > k0 ? (k1 - k0 + kTileKeys - 1) / kTileKeys : 0);
+    const TableRow table = table_row(p, pc.b);
     // page of 16-key group g16 of tile t; a group behind the last key stands for the last one
     const int last_key = max(rq.kv - 1, 0);
     auto group_key = [&](int t, int g16) {
@@ -979,21 +995,22 @@ __global__ __launch_bounds__(kThreads, TWO || OPT ? 2 : 4) void paged_few_kernel
 
 int launch_few(const Call &c, hipStream_t s) {
     const bool two = c.rows_d > 8, opt = c.cap2 != 0.0f || c.bias != 0.0f;
+    const int pieces = c.slots_d / c.Hkv;
+    const dim3 grid((unsigned)((pieces + 7) / 8 * 8 * c.Hkv + (c.rows_c ? 1 : 0)));
+    typedef void (*Kernel)(Call);
+    static const Kernel kernels[8] = {
+        paged_few_kernel<false, false, false>, paged_few_kernel<true, false, false>, paged_few_kernel<false, true, false>,
+        paged_few_kernel<true, true, false>,   paged_few_kernel<false, false, true>, paged_few_kernel<true, false, true>,
+        paged_few_kernel<false, true, true>,   paged_few_kernel<true, true, true>};
     static std::once_flag once;  // the LDS limit is raised once per process
     static hipError_t err = hipSuccess;
     std::call_once(once, [] {
-        for (const void *f : {(const void *)paged_few_kernel<false, false>, (const void *)paged_few_kernel<false, true>,
-                              (const void *)paged_few_kernel<true, false>, (const void *)paged_few_kernel<true, true>})
-            if (err == hipSuccess) err = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsBytes);
+        for (Kernel k : kernels)
+            if (err == hipSuccess) err = hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsBytes);
     });
     if (err != hipSuccess) return hip_status(err, "paged_attn LDS attribute");
-    const int pieces = c.slots_d / c.Hkv;
-    const dim3 grid((unsigned)((pieces + 7) / 8 * 8 * c.Hkv));
     const int prof = profile_start("paged_decode", s);
-    if (two && opt) paged_few_kernel<true, true><<<grid, dim3(kThreads), kLdsBytes, s>>>(c);
-    else if (two) paged_few_kernel<true, false><<<grid, dim3(kThreads), kLdsBytes, s>>>(c);
-    else if (opt) paged_few_kernel<false, true><<<grid, dim3(kThreads), kLdsBytes, s>>>(c);
-    else paged_few_kernel<false, false><<<grid, dim3(kThreads), kLdsBytes, s>>>(c);
+    kernels[two + 2 * opt + 4 * (c.rows_c != 0)]<<<grid, dim3(kThreads), kLdsBytes, s>>>(c);
     profile_stop(prof, s);
     return hip_status(hipGetLastError(), "paged_attn launch");
 }

@@ -1,0 +1,202 @@
+// paged_work.hpp - how the many-row kernel's work is cut up and ordered, for one
+// workgroup of 512 threads. Lengths are known on the GPU only; the plan is made by an
+// extra workgroup of the few-row kernel's launch, which runs before, so that the many
+// workgroups of the chunk kernel need a few loads to know their part (each making the
+// choice for itself took 5 us of every workgroup's time).
+#pragma once
+#include "paged_attn.hpp"
+
+namespace sqa {
+namespace paged {
+
+constexpr int kChunkKeys = 32;   // keys per tile of the chunk kernel
+constexpr int kMostSplits = 256; // of a request (the merge's limit)
+constexpr int kListed = 4096;    // items up to which the plan is a list in the order of dispatch
+
+// What the plan leaves in the workspace.
+struct Work {
+    int len;       // key tiles per split, at most
+    int items;     // workgroups with work
+    int listed;    // whether the list holds them, longest first
+    int even;      // else: equal parts, renumbered by XCD
+};
+// Words: Work | first item of every request [B + 1] | first slot [B] | list [kListed] of {b, tile, kvh, split}
+constexpr int kWorkWords = 16;
+__host__ __device__ inline size_t work_bytes(int64_t B) { return ((size_t)(kWorkWords + 2 * B + 4) / 4 * 4 + 4 * kListed) * 4; }
+
+// Query tiles of a request (0: none of the many-row kernel's) and its key tiles.
+__device__ __forceinline__ int chunk_tiles(const Call &c, const Request &r, int qb, int *key_tiles) {
+    *key_tiles = 0;
+    if (r.n * c.G <= c.most_d) return 0;
+    *key_tiles = max((r.kv + kChunkKeys - 1) / kChunkKeys, 1);
+    return (r.n + qb - 1) / qb;
+}
+
+#ifdef SQA_PLAN_CHUNKS
+
+constexpr int kChoices = 16;
+// splits of the longest request that are tried
+__device__ constexpr int kTried[kChoices] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64, 128};
+
+// Every request is cut into splits of at most `len` key tiles, the same for all, with
+// the len of the least estimated time, in tiles of one workgroup: kWg for a
+// workgroup's own start and end, kMerge for the merge, kMergeSlot for a slot's bytes.
+// Equal parts run in rounds of one per CU. Others (ragged batches, first chunks, whose
+// tiles see from one to all of the keys) go out longest first and take the work over
+// the CUs and a quarter of a part.
+constexpr float kWg = 2.0f, kMerge = 3.0f, kMergeSlot = 0.02f;
+
+// Run by all 512 threads of one workgroup; lds: 512 + 5 * 3000 + 4 words, or 512 +
+// B + 4. Lanes are requests
+// (a run of them above 512), then lengths that are tried, then items.
+__device__ __forceinline__ void plan_chunks(const Call &c, int *lds) {
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, qb = c.rows_c / c.G;
+    Work *out = reinterpret_cast<Work *>(c.work);
+    int *first = c.work + kWorkWords, *slot = first + c.B + 1;
+    int4 *list = reinterpret_cast<int4 *>(c.work + (kWorkWords + 2 * c.B + 4) / 4 * 4);
+    int *sums = lds, *start = lds + 512;                      // start: first item of every request
+    int4 *known = reinterpret_cast<int4 *>(start + (c.B + 4) / 4 * 4);  // {n, pos0, prefix, kv} of every request
+    const int per = (c.B + 511) / 512, b0 = min(tid * per, c.B), b1 = min(b0 + per, c.B);
+    const bool kept = c.B <= 3000;  // in LDS; larger batches read them again
+    auto load = [&](int b) {
+        if (!kept) return request(c, b);
+        const int4 k = known[b];
+        return Request{0, k.x, k.w, k.y, k.z};
+    };
+
+    int wgs = 0, longest = 0;
+    float work = 0.0f;  // key tiles that all query tiles see together
+    for (int b = b0; b < b1; ++b) {
+        const Request r = request(c, b);
+        if (kept) known[b] = make_int4(r.n, r.pos0, r.prefix, r.kv);
+        int kt;
+        const int T = chunk_tiles(c, r, qb, &kt);
+        // query tile i of T ends (T - 1 - i) * qb keys before the last one
+        const float all = (float)T * (float)kt;
+        work += fmaxf(all - 0.5f * (float)T * (float)(T - 1) * (float)qb / kChunkKeys, 0.5f * all);
+        wgs += T;
+        longest = max(longest, kt);
+    }
+    wgs = wave_sum(wgs);
+    longest = wave_max(longest);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) work += __shfl_xor(work, o);
+    if (lane == 0) sums[wave] = wgs, sums[8 + wave] = longest, sums[16 + wave] = __float_as_int(work);
+    __syncthreads();
+    wgs = longest = 0, work = 0.0f;
+    for (int w = 0; w < 8; ++w) wgs += sums[w], longest = max(longest, sums[8 + w]), work += __int_as_float(sums[16 + w]);
+    if (wgs == 0) {
+        if (tid == 0) *out = Work{1, 0, 0, 0};
+        return;
+    }
+    work *= (float)c.Hkv;
+    __syncthreads();
+    // query tiles times splits, of all requests (kChoices) and of split ones
+    int n[2 * kChoices] = {};
+    for (int b = b0; b < b1; ++b) {
+        int kt;
+        const int T = chunk_tiles(c, load(b), qb, &kt);
+        if (T == 0) continue;
+#pragma unroll
+        for (int j = 0; j < kChoices; ++j) {
+            const int l = max((longest + kTried[j] - 1) / kTried[j], 2), S = (kt + l - 1) / l;
+            n[j] += T * S;
+            n[kChoices + j] += S > 1 ? T * S : 0;
+        }
+    }
+    const bool some = __any(b0 < b1);
+#pragma unroll
+    for (int j = 0; j < 2 * kChoices; ++j) {
+        const int s = some ? wave_sum(n[j]) : 0;
+        if (lane == 0) sums[wave * 2 * kChoices + j] = s;
+    }
+    __syncthreads();
+    // lane j estimates length j
+    int v = 0;
+    for (int w = 0; w < 8; ++w) v += sums[w * 2 * kChoices + (lane & (2 * kChoices - 1))];
+    const int64_t N = (int64_t)v * c.Hkv, slots_j = (int64_t)__shfl_xor(v, kChoices) * c.Hkv;
+    const int j = lane & (kChoices - 1), l_j = max((longest + kTried[j] - 1) / kTried[j], 2);
+    const float part = (float)min(l_j, longest), cus = (float)c.cus;
+    const bool eq = work > 0.85f * (float)N * part;
+    float t = eq ? ceilf((float)N / cus) * (part + kWg) : fmaxf((work + kWg * (float)N) / cus + 0.25f * part, part + kWg);
+    t += slots_j ? kMerge + kMergeSlot * (float)slots_j : 0.0f;
+    // at most kMostSplits per request, slots and workgroups as there are
+    const bool fits = j == 0 || (slots_j <= c.slots_c && N <= c.grid_c && longest <= (int64_t)l_j * kMostSplits);
+    if (!fits || lane >= kChoices) t = INFINITY;
+    float best = t;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) best = fminf(best, __shfl_xor(best, o));
+    const int pick = __builtin_ctzll(__ballot(t == best));
+    const int len = __shfl(l_j, pick), total = min(__shfl((int)N, pick), c.grid_c);
+    const bool even = __shfl((int)eq, pick);
+    const int listed = !even && total <= kListed;
+    if (tid == 0) *out = Work{len, total, listed, even};
+    __syncthreads();
+
+    // first items and slots
+    int items = 0, slots = 0;
+    for (int b = b0; b < b1; ++b) {
+        int kt;
+        const int T = chunk_tiles(c, load(b), qb, &kt), S = (kt + len - 1) / len, k = T * S * c.Hkv;
+        start[b] = items;
+        items += k;
+        slots += S > 1 ? k : 0;
+    }
+    const int upto = wave_scan(items), slots_upto = wave_scan(slots);
+    if (lane == 63) sums[wave] = upto, sums[8 + wave] = slots_upto;
+    __syncthreads();
+    int before = upto - items, slots_before = slots_upto - slots;
+    for (int w = 0; w < wave; ++w) before += sums[w], slots_before += sums[8 + w];
+    for (int b = b0; b < b1; ++b) {
+        const int k = (b + 1 < b1 ? start[b + 1] : items) - start[b];
+        int kt;
+        (void)chunk_tiles(c, load(b), qb, &kt);
+        first[b] = start[b] + before;
+        slot[b] = slots_before;
+        slots_before += kt > len ? k : 0;
+    }
+    __syncthreads();
+    for (int b = b0; b < b1; ++b) start[b] += before;
+    if (tid == 511) start[c.B] = before + items, first[c.B] = before + items;
+    if (!listed) return;
+
+    // counting sort of the items by their length, longest first (the order inside a
+    // length is left to chance; no result depends on it)
+    constexpr int kBuckets = 64;
+    if (tid < kBuckets) sums[tid] = 0;
+    __syncthreads();
+    for (int pass = 0; pass < 2; ++pass) {
+        for (int id = tid; id < total; id += 512) {
+            int lo = 0, hi = c.B;  // last request whose first item is at most id
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (start[mid] <= id) lo = mid;
+                else hi = mid;
+            }
+            const Request r = load(lo);
+            int kt;
+            const int T = chunk_tiles(c, r, qb, &kt), S = (kt + len - 1) / len;
+            int k = id - start[lo];
+            const int tile = k % T;
+            k /= T;
+            const int split = k % S, kvh = k / S;
+            const int t0 = (int)((int64_t)split * kt / S), t1 = (int)((int64_t)(split + 1) * kt / S);
+            const int keys = sees(r, min((tile + 1) * qb, r.n) - 1);
+            const int own = max(min(t1, (keys + kChunkKeys - 1) / kChunkKeys) - t0, 0);
+            const int bucket = kBuckets - 1 - min((int)((float)own * (float)kBuckets / (float)(len + 1)), kBuckets - 1);
+            const int at = atomicAdd(&sums[bucket], 1);
+            if (pass) list[at] = make_int4(lo, tile, kvh, split);
+        }
+        __syncthreads();
+        if (pass == 0) {
+            const int k = sums[lane], e = wave_scan(k) - k;  // every wavefront for itself
+            __syncthreads();
+            if (wave == 0) sums[lane] = e;
+            __syncthreads();
+        }
+    }
+}
+#endif
+
+}  // namespace paged
+}  // namespace sqa
