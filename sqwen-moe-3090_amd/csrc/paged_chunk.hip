@@ -136,7 +136,7 @@ __device__ __forceinline__ half8 lds_half8(const uint8_t *base, int off_lo, int 
 struct Expand {
     int k_raw, k_sh, k_to, dk_raw, dk_to;   // LDS offsets in the first of two buffers
     int v_raw, v_to, v_odd, dv_raw, dv_to, dv_key;
-    uint32_t x[4], k[5], magic;
+    uint32_t x[4], k[5], d, dk, magic;
     __device__ __forceinline__ void init(int w, int lane) {
         const int key = 16 * ((lane >> 4) & 1) + 4 * w + (lane & 3), kb = 4 * (lane >> 5) + ((lane >> 2) & 3), r = key_row(key);
         dk_raw = kLdsRaw + kHeadRowBytes * key + 18 * kb;
@@ -162,14 +162,14 @@ struct Expand {
         for (int j = 0; j < 4; ++j)
             x[j] = (uint32_t)*reinterpret_cast<const uint16_t *>(src + kHeadRowBytes * 2 * j) |
                    ((uint32_t)*reinterpret_cast<const uint16_t *>(src + kHeadRowBytes * (2 * j + 1)) << 16);
+        d = *reinterpret_cast<const uint16_t *>(smem + dv_raw + (t & 1) * kRawTile);
     }
-    // reads of K tile t; its scales move on as they are
-    __device__ __forceinline__ void read_k(uint8_t *smem, int t) {
+    // reads of K tile t
+    __device__ __forceinline__ void read_k(const uint8_t *smem, int t) {
         const uint32_t *src = reinterpret_cast<const uint32_t *>(smem + k_raw + (t & 1) * kRawTile);
 #pragma unroll
         for (int m = 0; m < 5; ++m) k[m] = src[m];
-        *reinterpret_cast<uint16_t *>(smem + dk_to + (t & 1) * kKStage) =
-            *reinterpret_cast<const uint16_t *>(smem + dk_raw + (t & 1) * kRawTile);
+        dk = *reinterpret_cast<const uint16_t *>(smem + dk_raw + (t & 1) * kRawTile);
     }
     // byte j of the lane's two (odd m: the other one), both nibbles
     __device__ __forceinline__ void store_v(uint8_t *smem, int t, int j) {
@@ -186,6 +186,7 @@ struct Expand {
     __device__ __forceinline__ void store_k(uint8_t *smem, int t, int m) {
         const int to = (k_to + (t & 1) * kKStage) ^ (16 * m);
         const uint32_t y = __builtin_amdgcn_alignbit(k[m + 1], k[m], (uint32_t)k_sh), z = y >> 8;
+        if (m == 0) *reinterpret_cast<uint16_t *>(smem + dk_to + (t & 1) * kKStage) = (uint16_t)dk;
         *reinterpret_cast<uint2 *>(smem + to) = make_uint2(codes_lo(y, magic), codes_hi(y, magic));
         *reinterpret_cast<uint2 *>(smem + (to ^ 8)) = make_uint2(codes_lo(z, magic), codes_hi(z, magic));
     }
@@ -194,7 +195,6 @@ struct Expand {
     // their P is 0, and 0 * NaN would not be. Returns e: at most the one given, and such
     // that the largest is below 1.
     __device__ __forceinline__ int scales_v(uint8_t *smem, int t, int left, bool has_a, bool has_b, int e) {
-        uint32_t d = *reinterpret_cast<const uint16_t *>(smem + dv_raw + (t & 1) * kRawTile);
         const bool ok = dv_key < left && (dv_key < 16 ? has_a : has_b) && (d & 0x7C00u) != 0x7C00u;
         d = ok ? d : 0u;
         // fp16 bits of 2^-e, the smallest scale that would reach 1 (e in [-17, 24])
@@ -617,8 +617,8 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
 #pragma unroll
             for (int m = 0; m < 4; ++m) ex.store_k(smem, k, m);
         }
-        scales(0, a0, b0);
         ex.read_v(smem, 0);
+        scales(0, a0, b0);
         ex.store_v(smem, 0, 0);
         ex.store_v(smem, 0, 1);
     }
@@ -651,7 +651,6 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
         int4 e_t = *reinterpret_cast<const int4 *>(smem + kLdsE + 16 * (tp & 1));
         e_t.x = __builtin_amdgcn_readfirstlane(e_t.x), e_t.y = __builtin_amdgcn_readfirstlane(e_t.y);
         e_t.z = __builtin_amdgcn_readfirstlane(e_t.z), e_t.w = __builtin_amdgcn_readfirstlane(e_t.w);
-        ex.read_v(smem, t);
         half8 ph[kRG], pl[kRG];
         bool resc = false;
 #pragma unroll
@@ -688,6 +687,8 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
         half8 bvn[2];
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) bvn[hf] = lds_half8(smem, vb0 + 1024 * hf, vb1 + 1024 * hf);
+        ex.read_v(smem, t);
+        ex.read_k(smem, t + 1);
 #pragma unroll
         for (int b = 0; b < 8; ++b) {
             const half8 bv[2] = {bvn[0], bvn[1]};
@@ -723,10 +724,9 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf)
                     acc[rg][2 * b + hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(al[rg], bv[hf], acc[rg][2 * b + hf], 0, 0, 0);
-            if (b == 0) scales(t, x0, y0);
-            if (b == 1) ex.store_v(smem, t, 0);
-            if (b == 2) ex.store_v(smem, t, 1);
-            if (b == 2) ex.read_k(smem, t + 1);
+            if (b == 1) scales(t, x0, y0);
+            if (b == 2) ex.store_v(smem, t, 0);
+            if (b == 3) ex.store_v(smem, t, 1);
             if (b >= 4) ex.store_k(smem, t + 1, b - 4);
         }
     }
