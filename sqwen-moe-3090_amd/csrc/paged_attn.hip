@@ -24,7 +24,7 @@ __device__ __forceinline__ Row row_of(const Call &c, int t, int h) {
     Row r{nullptr, nullptr, 0, 0};
     const int4 w = c.where[t];
     if (t < c.q_start[0] || t >= c.q_start[c.B]) return r;  // of no request: w was not written
-    const int form = w.w & 3, step = w.w >> 2, kvh = h / c.G, row = w.z + h - kvh * c.G;
+    const int form = w.w & 3, step = w.w >> 2, kvh = group_of(c, h), row = w.z + h - kvh * c.G;
     const int heads = form == kFew ? 1 : w.y * step, rows = form == kFew ? c.rows_d : c.rows_c;
     const int64_t first = w.x + (int64_t)kvh * heads;
     // (arrays that are no plan's may leave an entry of an earlier call here)
@@ -215,6 +215,7 @@ int launch_paged_attn(const PagedArgs &a, hipStream_t s) {
     c.q_start = (const int32_t *)a.q_start->data, c.kv_len = (const int32_t *)a.kv_len->data;
     c.prefix = a.prefix ? (const int32_t *)a.prefix->data : nullptr;
     c.n_tok = (int)q.ne[1], c.H = (int)q.ne[2], c.Hkv = (int)k.ne[1], c.G = c.H / c.Hkv;
+    c.inv_g = 1.0f / (float)c.G;
     c.qscale = a.scale * kLog2e;
     c.cap2 = a.softcap * kLog2e, c.cap_inv = a.softcap > 0.0f ? 1.0f / c.cap2 : 0.0f;
     c.bias = a.max_bias;
@@ -239,6 +240,8 @@ int launch_paged_attn(const PagedArgs &a, hipStream_t s) {
     };
     c.slots_d = take(p.slots_d, p.slot_d);
     c.slots_c = take(p.slots_c, p.slot_c);
+    c.room = c.slots_d / c.Hkv;
+    c.few_pieces = c.cus / c.Hkv, c.all_pieces = 2 * c.cus / c.Hkv;
     uint8_t *base = reinterpret_cast<uint8_t *>(((uintptr_t)a.ws + 255) & ~(uintptr_t)255);
     c.where = reinterpret_cast<int4 *>(base);
     c.work = reinterpret_cast<int *>(base + p.where);

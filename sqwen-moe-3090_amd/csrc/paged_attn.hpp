@@ -31,6 +31,7 @@ struct Call {
     int64_t most_kv;             // keys that a table row can hold
     const int32_t *q_start, *kv_len, *prefix;
     int n_tok, B, H, Hkv, G;
+    float inv_g;                 // 1 / G, see group_of
     float qscale;                // softmax scale * log2(e)
     float cap2, cap_inv;         // logit cap * log2(e) and its inverse, 0: none
     float bias;                  // max_bias, 0: none
@@ -47,6 +48,8 @@ struct Call {
     int *work;                   // the many-row kernel's plan (paged_work.hpp)
     int grid_c;                  // its workgroups at most
     int most_d;                  // query rows per KV head that the few-row kernel takes (0: it does not run)
+    int room;                    // slots_d / Hkv: pieces that the workspace holds
+    int few_pieces, all_pieces;  // pieces that one, two workgroups per CU are
     int cus;
 };
 
@@ -72,6 +75,20 @@ __device__ __forceinline__ Request request(const Call &c, int b) {
 
 // Keys [0, sees) that token i sees.
 __device__ __forceinline__ int sees(const Request &r, int i) { return min(max(r.pos0 + i + 1, r.prefix), r.kv); }
+
+// r / G for 0 <= r < 2^20 (the float quotient is nowhere near a whole number but above it).
+__device__ __forceinline__ int group_of(const Call &c, int r) { return (int)(((float)r + 0.5f) * c.inv_g); }
+
+// t / n for 0 <= t < 2^30, n > 0: a float quotient, what it left out, and one step either way.
+__device__ __forceinline__ int div_floor(int t, int n) {
+    const float inv = __builtin_amdgcn_rcpf((float)n);
+    int q = (int)((float)t * inv), r = t - q * n;
+    const int more = (int)((float)r * inv);
+    q += more, r -= more * n;
+    if (r < 0) --q, r += n;
+    return q + (r >= n);
+}
+__device__ __forceinline__ int div_ceil(int t, int n) { return div_floor(t + n - 1, n); }  // t + n <= 2^30
 
 // Sum over the wavefront, and inclusive prefix sum, by DPP: row shifts sum each row
 // of 16, row broadcasts add the rows before.

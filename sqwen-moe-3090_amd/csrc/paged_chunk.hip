@@ -218,37 +218,44 @@ struct Expand {
 // Q' of a row as B operands: the lane's 8 dims of every block (in the order of the K
 // chunks), q8_0 with ggml's x86 rounding (d = amax / 127 over the block, codes =
 // rint(x * 127 / amax)), times fp16(d) * scale * log2(e) in fp32, as fp16 hi and
-// lo = fp16(Q' - hi).
-__device__ __forceinline__ void quantize_q(const Call &p, int64_t row, int h, int g, bool ok, half8 (&hi)[8], half8 (&lo)[8]) {
-    const float *q = reinterpret_cast<const float *>(p.q + row * p.q_nb1 + (int64_t)h * p.q_nb2);
+// lo = fp16(Q' - hi). The loads of a row are one batch (block by block they were 16
+// memory latencies at the start of every workgroup).
+struct QRow {
+    float4a v[16];
+    __device__ __forceinline__ void load(const Call &p, int64_t row, int h, int g) {
+        const float *q = reinterpret_cast<const float *>(p.q + row * p.q_nb1 + (int64_t)h * p.q_nb2) + 4 * g;
 #pragma unroll
-    for (int b = 0; b < 8; ++b) {
-        const float4a a = *reinterpret_cast<const float4a *>(q + 32 * b + 4 * g);
-        const float4a c = *reinterpret_cast<const float4a *>(q + 32 * b + 16 + 4 * g);
-        float v[8] = {a.x, a.z, c.x, c.z, a.y, a.w, c.y, c.w};
-        float amax = 0.0f;
+        for (int b = 0; b < 16; ++b) v[b] = *reinterpret_cast<const float4a *>(q + 16 * b);
+    }
+    __device__ __forceinline__ void quantize(float qscale, bool ok, half8 (&hi)[8], half8 (&lo)[8]) const {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            v[j] = ok ? v[j] : 0.0f;
-            amax = fmaxf(amax, fabsf(v[j]));
-        }
-        amax = xmax32(xmax16(amax));
-        const float d = amax / 127.f;
-        const float id = amax != 0.0f ? 127.f / amax : 0.0f;
-        const float qd = (float)(_Float16)d * p.qscale;
+        for (int b = 0; b < 8; ++b) {
+            const float4a a = v[2 * b], c = v[2 * b + 1];
+            float x[8] = {a.x, a.z, c.x, c.z, a.y, a.w, c.y, c.w};
+            float amax = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            // x opaque: left visible, the compiler may round code * qd to fp16 twice
-            // (once from the fp32 product for hi, once from the exact product for the
-            // hi it subtracts), and a hi + lo off by one fp16 ulp of hi
-            float x = rintf(v[j] * id) * qd;
-            asm volatile("" : "+v"(x));
-            const _Float16 hh = (_Float16)x;
-            hi[b][j] = hh;
-            lo[b][j] = (_Float16)(x - (float)hh);
+            for (int j = 0; j < 8; ++j) {
+                x[j] = ok ? x[j] : 0.0f;
+                amax = fmaxf(amax, fabsf(x[j]));
+            }
+            amax = xmax32(xmax16(amax));
+            const float d = amax / 127.f;
+            const float id = amax != 0.0f ? 127.f / amax : 0.0f;
+            const float qd = (float)(_Float16)d * qscale;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                // y opaque: left visible, the compiler may round code * qd to fp16 twice
+                // (once from the fp32 product for hi, once from the exact product for the
+                // hi it subtracts), and a hi + lo off by one fp16 ulp of hi
+                float y = rintf(x[j] * id) * qd;
+                asm volatile("" : "+v"(y));
+                const _Float16 hh = (_Float16)y;
+                hi[b][j] = hh;
+                lo[b][j] = (_Float16)(y - (float)hh);
+            }
         }
     }
-}
+};
 
 // ---------------------------------------------------------------- work split
 
@@ -294,17 +301,18 @@ __device__ __forceinline__ Item many_item(const Call &c, int lin, int qb) {
         it.split = -1;
     }
     int kt;
-    const int T = chunk_tiles(c, uniform_request(c, it.b), qb, &kt), S = (kt + len - 1) / len;
+    const int T = chunk_tiles(c, uniform_request(c, it.b), qb, &kt), S = div_ceil(kt, len);
     it.tiles = uniform(T);
     it.splits = uniform(S);
     if (it.split < 0) {
-        const int r = it.tile / T;
+        const int r = div_floor(it.tile, T);
         it.tile = uniform(it.tile - r * T);
-        it.kvh = uniform(r / S);
+        it.kvh = uniform(div_floor(r, S));
         it.split = uniform(r - it.kvh * S);
     }
-    it.t0 = uniform((int)((int64_t)it.split * kt / S));
-    it.t1 = uniform((int)((int64_t)(it.split + 1) * kt / S));
+    split_range(kt, S, it.split, &it.t0, &it.t1);
+    it.t0 = uniform(it.t0);
+    it.t1 = uniform(it.t1);
     it.slot = uniform(slot[it.b]);
     return it;
 }
@@ -318,10 +326,10 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
     const int lane = tid & 63, g = lane >> 4, n = lane & 15;
     const uint32_t lds0 = (uint32_t)(uintptr_t)smem;
 
-    const Item it = many_item(p, (int)blockIdx.x, rows_per_wg(kRG) / p.G);
+    const Item it = many_item(p, (int)blockIdx.x, group_of(p, rows_per_wg(kRG)));
     if (it.b < 0) return;
     const Request rq = uniform_request(p, it.b);
-    const int qb = rows_per_wg(kRG) / p.G;  // tokens of a query tile
+    const int qb = uniform(group_of(p, rows_per_wg(kRG)));  // tokens of a query tile
     const int q_base = it.tile * qb;        // its first token in the request
     const int q_top = min(q_base + qb, rq.n);
     const bool whole = it.splits == 1;      // of the keys: the result goes out from here
@@ -367,6 +375,8 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
         // kvh*G + r % G) as B operands, dims 32b + 8g..+7
         half8 bqh[kRG][8], bql[kRG][8];
         int my_see[kRG], my_pos[kRG];
+        QRow qrow[kRG];
+        bool row_ok[kRG];
         float my_slope[kRG];
         float m_run[kRG], l_part[kRG];
         // The logits are accumulated relative to the row's P reference mref =
@@ -378,17 +388,21 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
 #pragma unroll
         for (int rg = 0; rg < kRG; ++rg) {
             const int r = 16 * kRG * w + 16 * rg + n;
-            const int i = r / p.G, h = kvh * p.G + r - i * p.G;
+            const int i = group_of(p, r), h = kvh * p.G + r - i * p.G;
             const bool ok = q_base + i < q_top;
             my_see[rg] = ok ? sees(rq, q_base + i) : 0;
             my_pos[rg] = rq.pos0 + q_base + i;
             my_slope[rg] = OPT && p.bias != 0.0f ? slope2(p, h) : 0.0f;
-            quantize_q(p, ok ? rq.q0 + q_base + i : rq.q0, h, g, ok, bqh[rg], bql[rg]);
+            qrow[rg].load(p, ok ? rq.q0 + q_base + i : rq.q0, h, g);
+            row_ok[rg] = ok;
             m_run[rg] = -INFINITY;
             l_part[rg] = 0.0f;
             mref[rg] = -(float)kEp;
             lim_s[rg] = -INFINITY;
         }
+        __builtin_amdgcn_sched_barrier(0);  // the loads stay together
+#pragma unroll
+        for (int rg = 0; rg < kRG; ++rg) qrow[rg].quantize(p.qscale, row_ok[rg], bqh[rg], bql[rg]);
         // K operand of key row 16kg + n, dims 32b + 8g..+7: chunk (4b + g) ^ (n & 7),
         // halves swapped when n & 8; the XOR touches bit 2 of 4b + g, so even and odd
         // b use two bases and b >> 1 adds 128 bytes.
@@ -733,37 +747,52 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
     __syncthreads();  // m and l of the rows ...
     __syncthreads();  // ... are in LDS
     const int e_out[4] = {-e_acc.x, -e_acc.y, -e_acc.z, -e_acc.w};
+    // rows 16 kRG w + 16 rg + 4g + i, one after the other; the gate of the next one is on
+    // its way while a row goes out
+    auto token_of = [&](int k, int *h) {  // k = 4 rg + i
+        const int r = 16 * kRG * w + 16 * (k >> 2) + 4 * g + (k & 3), tok = group_of(p, r);
+        *h = kvh * p.G + r - tok * p.G;
+        return q_base + tok;
+    };
+    float gv[2][16];
+    auto load_gate = [&](int k, float (&x)[16]) {
+        int h;
+        const int tok = token_of(k, &h);
+        if (tok < q_top) {
+            const float *from = reinterpret_cast<const float *>(p.gate + (int64_t)(rq.q0 + tok) * p.gate_nb2 + h * p.gate_nb1) + n;
 #pragma unroll
-    for (int rg = 0; rg < kRG; ++rg) {
+            for (int T = 0; T < 16; ++T) x[T] = from[16 * T];
+        }
+    };
+    if (whole && p.gate) load_gate(0, gv[0]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = 16 * kRG * w + 16 * rg + 4 * g + i;
-            const int tok = r / p.G, h = kvh * p.G + r - tok * p.G;
-            if (q_base + tok >= q_top) continue;
-            const float mrow = n_tiles > 0 ? ml[rg * 32 + 2 * (4 * g + i)] : -INFINITY;
-            const float lrow = n_tiles > 0 ? ml[rg * 32 + 2 * (4 * g + i) + 1] : 0.0f;
-            if (whole) {
-                const int64_t row = rq.q0 + q_base + tok;
-                const float inv = lrow == 0.0f ? 0.0f : 1.0f / lrow;
+    for (int k = 0; k < 4 * kRG; ++k) {
+        const int rg = k >> 2, i = k & 3, r = 16 * kRG * w + 16 * rg + 4 * g + i;
+        if (whole && p.gate && k + 1 < 4 * kRG) load_gate(k + 1, gv[(k + 1) & 1]);
+        int h;
+        const int tok = token_of(k, &h);
+        if (tok >= q_top) continue;
+        const float mrow = n_tiles > 0 ? ml[rg * 32 + 2 * (4 * g + i)] : -INFINITY;
+        const float lrow = n_tiles > 0 ? ml[rg * 32 + 2 * (4 * g + i) + 1] : 0.0f;
+        if (whole) {
+            const float inv = lrow == 0.0f ? 0.0f : 1.0f / lrow;
+            float *to = p.dst + ((int64_t)(rq.q0 + tok) * p.H + h) * kHeadDim + n;
 #pragma unroll
-                for (int T = 0; T < 16; ++T) {
-                    float o = __builtin_amdgcn_ldexpf(acc[rg][T][i], e_out[T >> 2]) * inv;
-                    if (p.gate) {
-                        const float gv = reinterpret_cast<const float *>(p.gate + row * p.gate_nb2 + h * p.gate_nb1)[16 * T + n];
-                        o = o * (1.0f / (1.0f + expf(-gv)));
-                    }
-                    store_through(p.dst + (row * p.H + h) * kHeadDim + 16 * T + n, o);
-                }
-            } else {
-                const int64_t at = (int64_t)slot * rows_per_wg(kRG) + r;
+            for (int T = 0; T < 16; ++T) {
+                float o = __builtin_amdgcn_ldexpf(acc[rg][T][i], e_out[T >> 2]) * inv;
+                if (p.gate) o *= 1.0f / (1.0f + expf(-gv[k & 1][T]));
+                store_through(to + 16 * T, o);
+            }
+        } else {
+            const int64_t at = (int64_t)slot * rows_per_wg(kRG) + r;
 #pragma unroll
-                for (int T = 0; T < 16; ++T) store_through(p.acc_c + at * kHeadDim + 16 * T + n, __builtin_amdgcn_ldexpf(acc[rg][T][i], e_out[T >> 2]));
-                if (n == 0) {
-                    // the merge works in base e (acc and l of every split carry the same
-                    // 2^kEp, which cancels there)
-                    store_through(p.ml_c + at * 2, mrow == -INFINITY ? mrow : mrow * kLn2);
-                    store_through(p.ml_c + at * 2 + 1, lrow);
-                }
+            for (int T = 0; T < 16; ++T)
+                store_through(p.acc_c + at * kHeadDim + 16 * T + n, __builtin_amdgcn_ldexpf(acc[rg][T][i], e_out[T >> 2]));
+            if (n == 0) {
+                // the merge works in base e (acc and l of every split carry the same
+                // 2^kEp, which cancels there)
+                store_through(p.ml_c + at * 2, mrow == -INFINITY ? mrow : mrow * kLn2);
+                store_through(p.ml_c + at * 2 + 1, lrow);
             }
         }
     }

@@ -153,14 +153,6 @@ __device__ __forceinline__ int tiles_of(const Call &c, int b, int most) {
     return max((r.kv + kTileKeys - 1) / kTileKeys, 1);
 }
 
-// ceil(t / len) for 0 <= t < 2^26: the float quotient is off by less than one.
-__device__ __forceinline__ int ceil_div(int t, int len, float inv) {
-    int q = (int)((float)t * inv);
-    q -= q * (int64_t)len > t;
-    q += (q + 1) * (int64_t)len <= t;
-    return q + (q * (int64_t)len < t);
-}
-
 // Piece length: of lengths from total / P up to nearly twice that, the shortest whose
 // pieces number at most P, the workgroups that run together; where no length does
 // (as many requests as that) total / P, and the rest follows as others end.
@@ -179,29 +171,30 @@ __device__ __forceinline__ Piece few_piece(const Call &c, int piece, int most) {
     total = wave_sum(total);
     longest = wave_max(longest);
     active = wave_sum(active);
-    const int room = c.slots_d / c.Hkv;  // pieces that the workspace holds
-    int P = ((int64_t)total * c.Hkv >= 8 * c.cus ? 2 * c.cus : c.cus) / c.Hkv;
-    P = max(min(P, room - active), 1);
-    const int base = max(max((total + P - 1) / P, (longest + kMostSplits - 1) / kMostSplits), 1);
+    int P = (int64_t)total * c.Hkv >= 8 * c.cus ? c.all_pieces : c.few_pieces;
+    P = max(min(P, c.room - active), 1);
+    // (at or a little above total / P)
+    const int share = (int)ceilf((float)total * __builtin_amdgcn_rcpf((float)P) * 0.999999f);
+    const int base = max(max(share, (longest + kMostSplits - 1) / kMostSplits), 1);
     int n[kLengths] = {};
     for (int b0 = 0; b0 < c.B; b0 += 64) {
         const int t = tiles(b0);
 #pragma unroll
         for (int j = 0; j < kLengths; ++j) {
             const int len = (base * (kLengths + j) + kLengths - 1) / kLengths;
-            n[j] += ceil_div(t, len, 1.0f / (float)len);
+            n[j] += div_ceil(t, len);
         }
     }
     int len = 0;
 #pragma unroll
     for (int j = 0; j < kLengths; ++j)
         if (len == 0 && wave_sum(n[j]) <= P) len = (base * (kLengths + j) + kLengths - 1) / kLengths;
-    if (len == 0) len = wave_sum(n[0]) <= room ? base : 1 << 26;  // 2^26 tiles: every request whole
+    if (len == 0) len = wave_sum(n[0]) <= c.room ? base : 1 << 25;  // 2^25 tiles: every request whole
     Piece pc{-1, 0, 1, 0, 0, 0};
     int first = 0;
     for (int b0 = 0; b0 < c.B && first <= piece; b0 += 64) {
         const int t = tiles(b0);
-        const int k = ceil_div(t, len, 1.0f / (float)len);
+        const int k = div_ceil(t, len);
         const int upto = first + wave_scan(k);
         const uint64_t hit = __ballot(piece >= upto - k && piece < upto);
         if (hit) {
@@ -211,8 +204,9 @@ __device__ __forceinline__ Piece few_piece(const Call &c, int piece, int most) {
             pc.first = __builtin_amdgcn_readlane(upto - k, l);
             pc.split = piece - pc.first;
             const int tiles = __builtin_amdgcn_readlane(t, l);
-            pc.t0 = (int)((int64_t)pc.split * tiles / pc.n);
-            pc.t1 = (int)((int64_t)(pc.split + 1) * tiles / pc.n);
+            const int q = div_floor(tiles, pc.n), rest = tiles - q * pc.n;  // the first `rest` splits are one longer
+            pc.t0 = pc.split * q + min(pc.split, rest);
+            pc.t1 = pc.t0 + q + (pc.split < rest);
         }
         first = __builtin_amdgcn_readlane(upto, 63);
     }
@@ -259,7 +253,7 @@ __device__ __forceinline__ int lds_byte(int row, int c) {
 // TWO = true : up to 16 rows (rows 0-7 and 8-15 as two B sets, one A operand).
 // OPT: the logits are capped or biased. PLAN: a last workgroup plans the many-row kernel.
 template <bool TWO, bool OPT, bool PLAN>
-__global__ __launch_bounds__(kThreads, TWO || OPT ? 2 : 4) void paged_few_kernel(Call p) {
+__global__ __launch_bounds__(kThreads, 4) void paged_few_kernel(Call p) {
     extern __shared__ __align__(16) uint8_t smem[];
     const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // wave-uniform, in an SGPR
@@ -274,18 +268,16 @@ __global__ __launch_bounds__(kThreads, TWO || OPT ? 2 : 4) void paged_few_kernel
     asm volatile("" : "+s"(lds0));
     constexpr int kRowMask = TWO ? 15 : 7;  // rows 8-15 mirror rows 0-7 when only 8 exist
 
-    if (PLAN && blockIdx.x == gridDim.x - 1) {
-        plan_chunks(p, reinterpret_cast<int *>(smem));
+    if (PLAN && blockIdx.z == gridDim.z - 1) {
+        if (blockIdx.x == 0 && blockIdx.y == 0) plan_chunks(p, reinterpret_cast<int *>(smem));
         return;
     }
     // ---------------- piece and KV head of this workgroup ---------------------
-    // Workgroups go round-robin to the 8 XCDs: ids 8 Hkv a + 8h + x (x < 8) are
-    // piece 8a + x, head h, so all heads of a piece share an XCD (and its L2).
-    const int hb = (int)blockIdx.x >> 3;
-    const int pa = hb / p.Hkv;
-    const int kvh = hb - pa * p.Hkv;
-    const Piece pc = few_piece(p, (pa << 3) | (int)(blockIdx.x & 7), p.most_d);
-    if (!PLAN && blockIdx.x == 0) skip_large(p);
+    // Workgroups go round-robin to the 8 XCDs, x (of 8) first, then the KV heads (y), then
+    // z: the heads of piece 8z + x share an XCD (and its L2).
+    const int kvh = (int)blockIdx.y;
+    const Piece pc = few_piece(p, (int)(8 * blockIdx.z + blockIdx.x), p.most_d);
+    if (!PLAN && blockIdx.x + blockIdx.y + blockIdx.z == 0) skip_large(p);
     if (pc.b < 0) return;
     const Request rq = uniform_request(p, pc.b);
     const int rows = rq.n * p.G;
@@ -332,7 +324,7 @@ __global__ __launch_bounds__(kThreads, TWO || OPT ? 2 : 4) void paged_few_kernel
             for (int set = 0; set < kSets; ++set) {
                 const int r = 8 * set + (n & 7);
                 const bool row_ok = r < rows;
-                const int t = r / p.G;
+                const int t = group_of(p, r);
                 const int hq = kvh * p.G + (r - t * p.G);
                 const float *qrow = reinterpret_cast<const float *>(
                     p.q + (row_ok ? (int64_t)(rq.q0 + t) * p.q_nb1 + (int64_t)hq * p.q_nb2 : 0));
@@ -399,7 +391,7 @@ __global__ __launch_bounds__(kThreads, TWO || OPT ? 2 : 4) void paged_few_kernel
         // This lane's logit row (column n of the combined C): query position and validity.
         const int my_r = TWO ? n : (n & 7);
         const bool my_ok = my_r < rows;
-        const int my_t = my_ok ? my_r / p.G : 0;
+        const int my_t = my_ok ? group_of(p, my_r) : 0;
         const int my_see = sees(rq, my_t);  // keys that the row sees
         const int my_pos = rq.pos0 + my_t;
         float my_slope = 0.0f;
@@ -995,8 +987,7 @@ __global__ __launch_bounds__(kThreads, TWO || OPT ? 2 : 4) void paged_few_kernel
 
 int launch_few(const Call &c, hipStream_t s) {
     const bool two = c.rows_d > 8, opt = c.cap2 != 0.0f || c.bias != 0.0f;
-    const int pieces = c.slots_d / c.Hkv;
-    const dim3 grid((unsigned)((pieces + 7) / 8 * 8 * c.Hkv + (c.rows_c ? 1 : 0)));
+    const dim3 grid(8, (unsigned)c.Hkv, (unsigned)((c.room + 7) / 8 + (c.rows_c ? 1 : 0)));
     typedef void (*Kernel)(Call);
     static const Kernel kernels[8] = {
         paged_few_kernel<false, false, false>, paged_few_kernel<true, false, false>, paged_few_kernel<false, true, false>,

@@ -29,7 +29,14 @@ __device__ __forceinline__ int chunk_tiles(const Call &c, const Request &r, int 
     *key_tiles = 0;
     if (r.n * c.G <= c.most_d) return 0;
     *key_tiles = max((r.kv + kChunkKeys - 1) / kChunkKeys, 1);
-    return (r.n + qb - 1) / qb;
+    return div_ceil(r.n, qb);
+}
+
+// Split `split` of S of kt key tiles.
+__device__ __forceinline__ void split_range(int kt, int S, int split, int *t0, int *t1) {
+    const int q = div_floor(kt, S), rest = kt - q * S;  // the first `rest` are one longer
+    *t0 = split * q + min(split, rest);
+    *t1 = *t0 + q + (split < rest);
 }
 
 #ifdef SQA_PLAN_CHUNKS
@@ -99,7 +106,7 @@ __device__ __forceinline__ void plan_chunks(const Call &c, int *lds) {
         if (T == 0) continue;
 #pragma unroll
         for (int j = 0; j < kChoices; ++j) {
-            const int l = max((longest + kTried[j] - 1) / kTried[j], 2), S = (kt + l - 1) / l;
+            const int l = max(div_ceil(longest, kTried[j]), 2), S = div_ceil(kt, l);
             n[j] += T * S;
             n[kChoices + j] += S > 1 ? T * S : 0;
         }
@@ -115,7 +122,7 @@ __device__ __forceinline__ void plan_chunks(const Call &c, int *lds) {
     int v = 0;
     for (int w = 0; w < 8; ++w) v += sums[w * 2 * kChoices + (lane & (2 * kChoices - 1))];
     const int64_t N = (int64_t)v * c.Hkv, slots_j = (int64_t)__shfl_xor(v, kChoices) * c.Hkv;
-    const int j = lane & (kChoices - 1), l_j = max((longest + kTried[j] - 1) / kTried[j], 2);
+    const int j = lane & (kChoices - 1), l_j = max(div_ceil(longest, kTried[j]), 2);
     const float part = (float)min(l_j, longest), cus = (float)c.cus;
     const bool eq = work > 0.85f * (float)N * part;
     float t = eq ? ceilf((float)N / cus) * (part + kWg) : fmaxf((work + kWg * (float)N) / cus + 0.25f * part, part + kWg);
@@ -137,7 +144,7 @@ __device__ __forceinline__ void plan_chunks(const Call &c, int *lds) {
     int items = 0, slots = 0;
     for (int b = b0; b < b1; ++b) {
         int kt;
-        const int T = chunk_tiles(c, load(b), qb, &kt), S = (kt + len - 1) / len, k = T * S * c.Hkv;
+        const int T = chunk_tiles(c, load(b), qb, &kt), S = div_ceil(kt, len), k = T * S * c.Hkv;
         start[b] = items;
         items += k;
         slots += S > 1 ? k : 0;
@@ -175,12 +182,10 @@ __device__ __forceinline__ void plan_chunks(const Call &c, int *lds) {
             }
             const Request r = load(lo);
             int kt;
-            const int T = chunk_tiles(c, r, qb, &kt), S = (kt + len - 1) / len;
-            int k = id - start[lo];
-            const int tile = k % T;
-            k /= T;
-            const int split = k % S, kvh = k / S;
-            const int t0 = (int)((int64_t)split * kt / S), t1 = (int)((int64_t)(split + 1) * kt / S);
+            const int T = chunk_tiles(c, r, qb, &kt), S = div_ceil(kt, len);
+            const int k = id - start[lo], q = div_floor(k, T), tile = k - q * T, kvh = div_floor(q, S), split = q - kvh * S;
+            int t0, t1;
+            split_range(kt, S, split, &t0, &t1);
             const int keys = sees(r, min((tile + 1) * qb, r.n) - 1);
             const int own = max(min(t1, (keys + kChunkKeys - 1) / kChunkKeys) - t0, 0);
             const int bucket = kBuckets - 1 - min((int)((float)own * (float)kBuckets / (float)(len + 1)), kBuckets - 1);
