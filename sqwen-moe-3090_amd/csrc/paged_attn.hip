@@ -39,10 +39,8 @@ __device__ __forceinline__ Row row_of(const Call &c, int t, int h) {
     return r;
 }
 
-__device__ __forceinline__ float gated(const Call &c, int t, int h, int d, float r) {
-    if (!c.gate) return r;
-    const float g = reinterpret_cast<const float *>(c.gate + t * c.gate_nb2 + h * c.gate_nb1)[d];
-    return r * (1.0f / (1.0f + expf(-g)));
+__device__ __forceinline__ const float *gate_row(const Call &c, int t, int h) {
+    return reinterpret_cast<const float *>(c.gate + t * c.gate_nb2 + h * c.gate_nb1);
 }
 
 // Few rows of many splits: 16 workgroups per row, 16 dims each; a thread holds one dim
@@ -87,57 +85,80 @@ __global__ __launch_bounds__(kThreads) void merge_dims_kernel(Call c) {
     __syncthreads();
     if (tid < 16) {
         const float L = (xl[0] + xl[1]) + (xl[2] + xl[3]), O = (xo[0][dl] + xo[1][dl]) + (xo[2][dl] + xo[3][dl]);
-        c.dst[((int64_t)t * c.H + h) * kHeadDim + d] = gated(c, t, h, d, L == 0.0f ? 0.0f : O / L);
+        const float o = L == 0.0f ? 0.0f : O / L;
+        c.dst[((int64_t)t * c.H + h) * kHeadDim + d] = c.gate ? gate_by(o, gate_row(c, t, h)[d]) : o;
     }
 }
 
-// Many rows: a wavefront per row, 4 dims a lane; the heads of a token in turn.
-__global__ __launch_bounds__(kThreads) void merge_rows_kernel(Call c, int heads) {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int groups = (c.H + heads - 1) / heads;  // of a token
-    const int id = (int)blockIdx.x * 4 + wave;
-    const int t = id / groups, h0 = (id - t * groups) * heads;
-    if (t >= c.n_tok) return;
-    for (int h = h0; h < min(h0 + heads, c.H); ++h) {
-        const Row r = row_of(c, t, h);
-        if (r.n == 0) return;
-        constexpr int kBatch = 8;
-        float M = -INFINITY, L = 0.0f;
-        floatx4 o = {0.f, 0.f, 0.f, 0.f};
-        for (int s0 = 0; s0 < r.n; s0 += 64) {  // 64 splits' weights at a time
-            const int s = s0 + lane;
-            const float2 ml = s < r.n ? *reinterpret_cast<const float2 *>(r.ml + s * (r.step / 128)) : make_float2(-INFINITY, 0.0f);
-            float m = ml.x;
+// Many rows: a wavefront takes R heads of a token together, 4 dims a lane, so that their
+// loads share one memory latency after the other (row entry, (m, l), partials). 64 / R
+// splits at a time: lane r * 64 / R + i holds split i's weight for head r.
+template <int R>
+__global__ __launch_bounds__(kThreads) void merge_rows_kernel(Call c) {
+    constexpr int kS = 64 / R, kBatch = R >= 4 ? 2 : 8;
+    const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int t = (int)blockIdx.y + (int)(blockIdx.z << 15), h0 = ((int)blockIdx.x * 4 + wave) * R;
+    if (t >= c.n_tok || h0 >= c.H) return;
+    Row r[R];
 #pragma unroll
-            for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
-            if (m == -INFINITY) continue;
-            const float Mn = fmaxf(M, m), al = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((M - Mn) * kLog2e);
-            const float w = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((ml.x - Mn) * kLog2e);
-            float l = ml.x == -INFINITY ? 0.0f : ml.y * w;
+    for (int k = 0; k < R; ++k) r[k] = row_of(c, t, min(h0 + k, c.H - 1));
+    if (r[0].n == 0) return;  // of the token: all heads alike
+    const int n = r[0].n, k_own = lane / kS, i_own = lane % kS;
+    const float *ml_own = r[0].ml;
 #pragma unroll
-            for (int x = 1; x < 64; x <<= 1) l += __shfl_xor(l, x);
-            L = L * al + l;
-            o *= al;
-            M = Mn;
-            const int end = min(r.n - s0, 64);
-            for (int s1 = 0; s1 < end; s1 += kBatch) {
-                floatx4 a[kBatch];
-                float wt[kBatch];
+    for (int k = 1; k < R; ++k) ml_own = k_own == k ? r[k].ml : ml_own;
+    floatx4 o[R], g[R];
+    float M = -INFINITY, L = 0.0f;  // of head k_own
 #pragma unroll
-                for (int j = 0; j < kBatch; ++j) {
-                    wt[j] = s1 + j < end ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), s1 + j)) : 0.0f;
-                    if (wt[j] != 0.0f) a[j] = *reinterpret_cast<const floatx4 *>(r.acc + (s0 + s1 + j) * r.step + 4 * lane);
+    for (int k = 0; k < R; ++k) {
+        o[k] = floatx4{0.f, 0.f, 0.f, 0.f};
+        if (c.gate) g[k] = *reinterpret_cast<const float4a *>(gate_row(c, t, min(h0 + k, c.H - 1)) + 4 * lane);
+    }
+    for (int s0 = 0; s0 < n; s0 += kS) {
+        const int s = s0 + i_own;
+        const float2 ml = s < n ? *reinterpret_cast<const float2 *>(ml_own + s * (r[0].step / 128)) : make_float2(-INFINITY, 0.0f);
+        float m = ml.x;
+#pragma unroll
+        for (int x = 1; x < kS; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
+        const float Mn = fmaxf(M, m), al = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((M - Mn) * kLog2e);
+        const float w = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((ml.x - Mn) * kLog2e);
+        float l = ml.x == -INFINITY ? 0.0f : ml.y * w;
+#pragma unroll
+        for (int x = 1; x < kS; x <<= 1) l += __shfl_xor(l, x);
+        L = L * al + l;
+        M = Mn;
+#pragma unroll
+        for (int k = 0; k < R; ++k) o[k] *= __int_as_float(__builtin_amdgcn_readlane(__float_as_int(al), k * kS));
+        const int end = min(n - s0, kS);
+        for (int s1 = 0; s1 < end; s1 += kBatch) {
+            floatx4 a[kBatch][R];
+            float wt[kBatch][R];
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j)
+#pragma unroll
+                for (int k = 0; k < R; ++k) {
+                    wt[j][k] = s1 + j < end ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), k * kS + min(s1 + j, kS - 1))) : 0.0f;
+                    if (wt[j][k] != 0.0f)
+                        a[j][k] = *reinterpret_cast<const floatx4 *>(r[k].acc + (s0 + s1 + j) * r[k].step + 4 * lane);
                 }
 #pragma unroll
-                for (int j = 0; j < kBatch; ++j)
-                    if (wt[j] != 0.0f) o += a[j] * wt[j];
-            }
-        }
-        float *out = c.dst + ((int64_t)t * c.H + h) * kHeadDim + 4 * lane;
-        floatx4 x;
+            for (int j = 0; j < kBatch; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = gated(c, t, h, 4 * lane + i, L == 0.0f ? 0.0f : o[i] / L);
-        *reinterpret_cast<floatx4 *>(out) = x;
+                for (int k = 0; k < R; ++k)
+                    if (wt[j][k] != 0.0f) o[k] += a[j][k] * wt[j][k];
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+        if (h0 + k >= c.H) break;
+        const float Lk = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(L), k * kS));
+        const float inv = Lk == 0.0f ? 0.0f : 1.0f / Lk;
+        floatx4 x = o[k] * inv;
+        if (c.gate) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = gate_by(x[i], g[k][i]);
+        }
+        *reinterpret_cast<floatx4 *>(c.dst + ((int64_t)t * c.H + h0 + k) * kHeadDim + 4 * lane) = x;
     }
 }
 
@@ -182,9 +203,12 @@ int launch_combine(const Call &c, hipStream_t s) {
     if (rows <= 128) {
         merge_dims_kernel<<<dim3((unsigned)rows, 16), dim3(kThreads), 0, s>>>(c);
     } else {
-        const int heads = rows <= (1 << 16) ? 1 : 4;  // tokens without partials end at once
-        const int64_t waves = (int64_t)c.n_tok * ((c.H + heads - 1) / heads);
-        merge_rows_kernel<<<dim3((unsigned)((waves + 3) / 4)), dim3(kThreads), 0, s>>>(c, heads);
+        // four heads a wavefront where that leaves wavefronts enough for the chip
+        const bool four = rows > 8192 && c.H >= 16;
+        const dim3 grid((unsigned)((c.H + (four ? 16 : 4) - 1) / (four ? 16 : 4)),
+                        (unsigned)(c.n_tok < (1 << 15) ? c.n_tok : 1 << 15), (unsigned)((c.n_tok + (1 << 15) - 1) >> 15));
+        if (four) merge_rows_kernel<4><<<grid, dim3(kThreads), 0, s>>>(c);
+        else merge_rows_kernel<1><<<grid, dim3(kThreads), 0, s>>>(c);
     }
     profile_stop(prof, s);
     return hip_status(hipGetLastError(), "paged_attn merge launch");

@@ -152,35 +152,37 @@ __device__ __forceinline__ float slope2(const Call &c, int h) {
     return exp2f(-c.bias * e) * kLog2e;
 }
 
-// cap2 * tanh(s / cap2) of N base-2 logits. Below 0.4, where most logits of a capped
-// model lie, by the odd Taylor polynomial to x^13 (the rest is below 2^-24 of x
-// there); above it as (e - 1) / (e + 1) with e = exp(2x), whose subtraction loses
-// nothing any more. A step of tanh's own 2^-24 times a cap of 50 would be 3e-6 in
-// a weight, so small x must not come out of 1 - 2 / (e + 1).
+// cap2 * tanh(s / cap2) + off of N base-2 logits. Below a quarter, where most logits of
+// a capped model lie, by the odd Taylor polynomial to x^9 (the rest is below 2^-26 of x
+// there); above it as (e - 1) / (e + 1) with e = exp(2x), whose subtraction loses little
+// any more. A step of tanh's own 2^-24 times a cap of 50 would be 3e-6 in a weight, so
+// small x must not come out of 1 - 2 / (e + 1).
 template <int N>
-__device__ __forceinline__ void cap_logits(float (&s)[N], float cap2, float cap_inv) {
-    float x[N];
-    bool far = false;
+__device__ __forceinline__ void cap_logits(float (&s)[N], float cap2, float cap_inv, float off) {
+    float x[N], top = 0.0f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         x[i] = s[i] * cap_inv;
-        far |= !(fabsf(x[i]) < 0.4f);
+        top = fmaxf(top, fabsf(x[i]));  // (a NaN belongs to a key that is not seen)
         const float y = x[i] * x[i];
-        float t = fmaf(y, 0.0035921280f, -0.0088632355f);
-        t = fmaf(y, t, 0.021869488f);
-        t = fmaf(y, t, -0.053968254f);
+        float t = fmaf(y, 0.021869488f, -0.053968254f);
         t = fmaf(y, t, 0.13333333f);
         t = fmaf(y, t, -0.33333333f);
-        s[i] = cap2 * fmaf(x[i] * y, t, x[i]);
+        s[i] = fmaf(cap2, fmaf(x[i] * y, t, x[i]), off);
     }
-    if (!__any(far)) return;
+    if (!__any(top >= 0.25f)) return;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         const float z = fminf(fmaxf(x[i], -12.0f), 12.0f);
         const float e = __builtin_amdgcn_exp2f(2.0f * kLog2e * z);
         const float t = (e - 1.0f) * __builtin_amdgcn_rcpf(e + 1.0f);
-        s[i] = fabsf(x[i]) < 0.4f ? s[i] : cap2 * t;
+        s[i] = fabsf(x[i]) < 0.25f ? s[i] : fmaf(cap2, t, off);
     }
+}
+
+// x * sigmoid(g), by the hardware's exp2 and reciprocal (about 1 ulp each)
+__device__ __forceinline__ float gate_by(float x, float g) {
+    return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * g));
 }
 
 int launch_few(const Call &c, hipStream_t s);      // paged_decode.hip

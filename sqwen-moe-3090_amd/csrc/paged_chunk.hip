@@ -438,7 +438,7 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
             // ---- S^T: sa[rg][kg][i] = S[key kt + 8g + 4kg + i][row n of group rg] ----
             floatx4 sa[kRG][2];
 #pragma unroll
-            for (int rg = 0; rg < kRG; ++rg) sa[rg][0] = sa[rg][1] = OPT ? 0.0f : -mref[rg];
+            for (int rg = 0; rg < kRG; ++rg) sa[rg][0] = sa[rg][1] = OPT && p.cap2 != 0.0f ? 0.0f : -mref[rg];
             // d_k of the lane's four C rows 16kg + 4g + i, block b: 8 bytes at
             // Dk[b][16kg + 4g]
             const uint8_t *dkb = smem + (t & 1) * kKStage + kOffDk + 8 * g;
@@ -488,14 +488,18 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
 #pragma unroll
                 for (int jj = 0; jj < 8; ++jj) s[rg][jj] = sa[rg][jj >> 2][jj & 3];
             if (OPT) {
+                // one row group after the other (both at once need more registers than there are)
 #pragma unroll
                 for (int rg = 0; rg < kRG; ++rg) {
-                    if (p.cap2 != 0.0f) cap_logits(s[rg], p.cap2, p.cap_inv);
-                    const int far = my_pos[rg] - (kt + 8 * g);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (p.cap2 != 0.0f) cap_logits(s[rg], p.cap2, p.cap_inv, -mref[rg]);
+                    if (p.bias != 0.0f) {
+                        const float far = (float)(my_pos[rg] - (kt + 8 * g));
 #pragma unroll
-                    for (int jj = 0; jj < 8; ++jj)
-                        s[rg][jj] = fmaf(-my_slope[rg], fabsf((float)(far - jj)), s[rg][jj]) - mref[rg];
+                        for (int jj = 0; jj < 8; ++jj) s[rg][jj] = fmaf(-my_slope[rg], fabsf(far - (float)jj), s[rg][jj]);
+                    }
                 }
+                __builtin_amdgcn_sched_barrier(0);
             }
             // ---- causal limit, prefix, last key, pages that are not there: whatever the
             // logit is, NaN of garbage bytes too
@@ -777,12 +781,15 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
         if (whole) {
             const float inv = lrow == 0.0f ? 0.0f : 1.0f / lrow;
             float *to = p.dst + ((int64_t)(rq.q0 + tok) * p.H + h) * kHeadDim + n;
+            float o[16];
 #pragma unroll
-            for (int T = 0; T < 16; ++T) {
-                float o = __builtin_amdgcn_ldexpf(acc[rg][T][i], e_out[T >> 2]) * inv;
-                if (p.gate) o *= 1.0f / (1.0f + expf(-gv[k & 1][T]));
-                store_through(to + 16 * T, o);
+            for (int T = 0; T < 16; ++T) o[T] = __builtin_amdgcn_ldexpf(acc[rg][T][i], e_out[T >> 2]) * inv;
+            if (p.gate) {
+#pragma unroll
+                for (int T = 0; T < 16; ++T) o[T] = gate_by(o[T], gv[k & 1][T]);
             }
+#pragma unroll
+            for (int T = 0; T < 16; ++T) store_through(to + 16 * T, o[T]);
         } else {
             const int64_t at = (int64_t)slot * rows_per_wg(kRG) + r;
 #pragma unroll

@@ -508,7 +508,7 @@ __global__ __launch_bounds__(kThreads, 4) void paged_few_kernel(Call p) {
                 }
             }
             if (OPT) {
-                if (p.cap2 != 0.0f) cap_logits(s, p.cap2, p.cap_inv);
+                if (p.cap2 != 0.0f) cap_logits(s, p.cap2, p.cap_inv, 0.0f);
                 if (p.bias != 0.0f) {
                     const int far = my_pos - (kt + key0 + 4 * g);
 #pragma unroll
