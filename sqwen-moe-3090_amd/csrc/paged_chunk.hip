@@ -231,27 +231,34 @@ struct QRow {
 #pragma unroll
         for (int b = 0; b < 8; ++b) {
             const float4a a = v[2 * b], c = v[2 * b + 1];
-            float x[8] = {a.x, a.z, c.x, c.z, a.y, a.w, c.y, c.w};
+            const float x[8] = {a.x, a.z, c.x, c.z, a.y, a.w, c.y, c.w};
             float amax = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                x[j] = ok ? x[j] : 0.0f;
-                amax = fmaxf(amax, fabsf(x[j]));
-            }
+            for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[j]));
             amax = xmax32(xmax16(amax));
             const float d = amax / 127.f;
             const float id = amax != 0.0f ? 127.f / amax : 0.0f;
-            const float qd = (float)(_Float16)d * qscale;
+            const float qd = ok ? (float)(_Float16)d * qscale : 0.0f;
+            float y[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 // y opaque: left visible, the compiler may round code * qd to fp16 twice
                 // (once from the fp32 product for hi, once from the exact product for the
                 // hi it subtracts), and a hi + lo off by one fp16 ulp of hi
-                float y = rintf(x[j] * id) * qd;
-                asm volatile("" : "+v"(y));
-                const _Float16 hh = (_Float16)y;
-                hi[b][j] = hh;
-                lo[b][j] = (_Float16)(y - (float)hh);
+                y[j] = rintf(x[j] * id) * qd;
+                asm volatile("" : "+v"(y[j]));
+                hi[b][j] = (_Float16)y[j];
+            }
+            uint32_t hw[4];
+            __builtin_memcpy(hw, &hi[b], 16);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {  // the exact residual, hi read from its packed half
+                float r;
+                if (j & 1)
+                    asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel:[0,0,1] op_sel_hi:[0,0,1]" : "=v"(r) : "v"(y[j]), "v"(hw[j >> 1]));
+                else
+                    asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel:[0,0,0] op_sel_hi:[0,0,1]" : "=v"(r) : "v"(y[j]), "v"(hw[j >> 1]));
+                lo[b][j] = (_Float16)r;
             }
         }
     }
@@ -259,61 +266,37 @@ struct QRow {
 
 // ---------------------------------------------------------------- work split
 
-// A workgroup's part of the call: query tile `tile` of request b's `tiles`, KV head kvh,
-// split `split` of `splits`, key tiles [t0, t1); slot: the request's first one (splits > 1).
-// b < 0: none.
-struct Item {
-    int b, kvh, tile, tiles, split, splits, t0, t1, slot;
-};
-
 __device__ __forceinline__ Item many_item(const Call &c, int lin, int qb) {
-    Item it{-1, 0, 0, 0, 0, 1, 0, 0, 0};
+    Item it{};
     const Work w = *reinterpret_cast<const Work *>(c.work);
-    const int *first = c.work + kWorkWords, *slot = first + c.B + 1;
+    it = reinterpret_cast<const Item *>(c.work + kListAt)[min(lin, kListed - 1)];  // beside it, used if there is a list
     const int len = uniform(w.len), items = uniform(w.items);
-    if (uniform(w.listed)) {
-        if (lin >= items) return it;
-        const int4 e = reinterpret_cast<const int4 *>(c.work + (kWorkWords + 2 * c.B + 4) / 4 * 4)[lin];
-        it.b = uniform(e.x), it.tile = uniform(e.y), it.kvh = uniform(e.z), it.split = uniform(e.w);
-    } else {
-        // Workgroups go round-robin to the 8 XCDs. Equal parts are renumbered so that an
-        // XCD gets a run of ids, the query tiles of the same keys, which its L2 then
-        // serves to all of them; others go out as they come.
-        int id = lin;
-        if (uniform(w.even)) {
-            const int x = lin & 7, per = items >> 3, rem = items & 7, k = lin >> 3;
-            if (k >= per + (x < rem ? 1 : 0)) return it;
-            id = x * per + (x < rem ? x : rem) + k;
-        }
-        if (id >= items) return it;
-        // the last request whose first item is at most id: 64 at a time
-        const int lane = threadIdx.x & 63;
-        int lo = 0, hi = c.B;
-        while (hi - lo > 1) {
-            const int step = (hi - lo + 63) / 64, at = lo + lane * step;
-            const uint64_t below = __ballot(at < hi && first[min(at, c.B)] <= id);
-            const int l = 63 - __builtin_clzll(below);  // lane 0 is always below
-            lo = uniform(lo + l * step);
-            hi = uniform(min(hi, lo + step));
-        }
-        it.b = lo;
-        it.tile = id - uniform(first[lo]);  // for now: item in the request
-        it.split = -1;
+    const int id = uniform(w.even) ? id_of_workgroup(lin, items) : lin < items ? lin : -1;
+    if (id < 0 || uniform(w.listed)) {
+        if (id < 0) it.b = -1;
+        return it;
     }
+    // the last request whose first item is at most id: 64 at a time
+    const int *first = c.work + kFirstAt, *slot = first + c.B + 1, lane = threadIdx.x & 63;
+    int lo = 0, hi = c.B;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 63) / 64, at = lo + lane * step;
+        const uint64_t below = __ballot(at < hi && first[min(at, c.B)] <= id);
+        const int l = 63 - __builtin_clzll(below);  // lane 0 is always below
+        lo = uniform(lo + l * step);
+        hi = uniform(min(hi, lo + step));
+    }
+    it.b = lo;
+    it.rq = uniform_request(c, lo);
     int kt;
-    const int T = chunk_tiles(c, uniform_request(c, it.b), qb, &kt), S = div_ceil(kt, len);
-    it.tiles = uniform(T);
-    it.splits = uniform(S);
-    if (it.split < 0) {
-        const int r = div_floor(it.tile, T);
-        it.tile = uniform(it.tile - r * T);
-        it.kvh = uniform(div_floor(r, S));
-        it.split = uniform(r - it.kvh * S);
-    }
-    split_range(kt, S, it.split, &it.t0, &it.t1);
-    it.t0 = uniform(it.t0);
-    it.t1 = uniform(it.t1);
-    it.slot = uniform(slot[it.b]);
+    it.tiles = uniform(chunk_tiles(c, it.rq, qb, &kt));
+    it.splits = uniform(div_ceil(kt, len));
+    const int k = id - uniform(first[lo]), q = uniform(div_floor(k, it.tiles));
+    it.tile = k - q * it.tiles;
+    it.kvh = uniform(div_floor(q, it.splits));
+    it.split = q - it.kvh * it.splits;
+    split_range(kt, it.splits, it.split, &it.t0, &it.t1);
+    it.slot = slot[lo];
     return it;
 }
 
@@ -326,10 +309,11 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
     const int lane = tid & 63, g = lane >> 4, n = lane & 15;
     const uint32_t lds0 = (uint32_t)(uintptr_t)smem;
 
-    const Item it = many_item(p, (int)blockIdx.x, group_of(p, rows_per_wg(kRG)));
-    if (it.b < 0) return;
-    const Request rq = uniform_request(p, it.b);
     const int qb = uniform(group_of(p, rows_per_wg(kRG)));  // tokens of a query tile
+    Item it = many_item(p, (int)blockIdx.x, qb);
+    if (uniform(it.b) < 0) return;
+    for (int *x : {&it.b, &it.kvh, &it.tile, &it.tiles, &it.split, &it.splits, &it.t0, &it.t1, &it.slot}) *x = uniform(*x);
+    const Request rq{uniform(it.rq.q0), uniform(it.rq.n), uniform(it.rq.kv), uniform(it.rq.pos0), uniform(it.rq.prefix)};
     const int q_base = it.tile * qb;        // its first token in the request
     const int q_top = min(q_base + qb, rq.n);
     const bool whole = it.splits == 1;      // of the keys: the result goes out from here
@@ -488,7 +472,13 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
 #pragma unroll
                 for (int jj = 0; jj < 8; ++jj) s[rg][jj] = sa[rg][jj >> 2][jj & 3];
             if (OPT) {
-                // one row group after the other (both at once need more registers than there are)
+                // one row group after the other (both at once need more registers than there
+                // are), and the scaled sums before (the compiler moved those of the second
+                // group behind the first one's cap, and kept 64 products alive till there)
+#pragma unroll
+                for (int rg = 0; rg < kRG; ++rg)
+#pragma unroll
+                    for (int jj = 0; jj < 8; ++jj) asm volatile("" : "+v"(s[rg][jj]));
 #pragma unroll
                 for (int rg = 0; rg < kRG; ++rg) {
                     __builtin_amdgcn_sched_barrier(0);

@@ -71,7 +71,7 @@ constexpr float kPShift = 4.0f;
 // scales below 2^-20 lose low bits of A; 2^E stays two fp16 powers of two.
 constexpr int kMaxDvExp = 28;
 static_assert(2 * kLdsBytes <= 160 * 1024, "two workgroups per CU");
-static_assert((512 + 5 * 3000 + 8) * 4 <= kLdsBytes && (512 + kMaxRequests + 8) * 4 <= kLdsBytes, "the plan's LDS");
+static_assert((512 + 6 * 2600 + 8) * 4 <= kLdsBytes && (512 + kMaxRequests + 8) * 4 <= kLdsBytes, "the plan's LDS");
 static_assert(4 * 2 * 64 * 32 <= (kVStages - 1) * kTensorBytes, "Q operands must fit in V stages 1..2");
 
 typedef const __attribute__((address_space(3))) uint32_t lds_u32;  // LDS dword from a raw LDS address

@@ -11,18 +11,37 @@ namespace paged {
 
 constexpr int kChunkKeys = 32;   // keys per tile of the chunk kernel
 constexpr int kMostSplits = 256; // of a request (the merge's limit)
-constexpr int kListed = 4096;    // items up to which the plan is a list in the order of dispatch
+constexpr int kListed = 4088;    // items up to which the plan is a list in the order of dispatch
 
 // What the plan leaves in the workspace.
 struct Work {
     int len;       // key tiles per split, at most
     int items;     // workgroups with work
-    int listed;    // whether the list holds them, longest first
+    int listed;    // whether the list holds them, in the order of dispatch
     int even;      // else: equal parts, renumbered by XCD
 };
-// Words: Work | first item of every request [B + 1] | first slot [B] | list [kListed] of {b, tile, kvh, split}
-constexpr int kWorkWords = 16;
-__host__ __device__ inline size_t work_bytes(int64_t B) { return ((size_t)(kWorkWords + 2 * B + 4) / 4 * 4 + 4 * kListed) * 4; }
+
+// A workgroup's part of the call: query tile `tile` of request b's `tiles`, KV head kvh,
+// split `split` of `splits`, key tiles [t0, t1); slot: the request's first one (splits > 1).
+// b < 0: none.
+struct Item {
+    int b, kvh, tile, tiles, split, splits, t0, t1, slot;
+    Request rq;
+    int spare[2];
+};
+static_assert(sizeof(Item) == 64, "one scalar load");
+
+// Words: Work | list [kListed] of Item | first item of every request [B + 1] | first slot [B]
+constexpr int kListAt = 16, kFirstAt = kListAt + 16 * kListed;
+__host__ __device__ inline size_t work_bytes(int64_t B) { return (size_t)(kFirstAt + 2 * B + 4) * 4; }
+
+// Where item `id` of `items` equal parts stands in the order of dispatch: workgroups go
+// round-robin to the 8 XCDs, and an XCD gets a run of ids, the query tiles of the same
+// keys, which its L2 then serves to all of them.
+__device__ __forceinline__ int id_of_workgroup(int lin, int items) {  // -1: none
+    const int x = lin & 7, per = items >> 3, rem = items & 7, k = lin >> 3;
+    return k >= per + (x < rem ? 1 : 0) ? -1 : x * per + min(x, rem) + k;
+}
 
 // Query tiles of a request (0: none of the many-row kernel's) and its key tiles.
 __device__ __forceinline__ int chunk_tiles(const Call &c, const Request &r, int qb, int *key_tiles) {
@@ -53,29 +72,27 @@ __device__ constexpr int kTried[kChoices] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20
 // the CUs and a quarter of a part.
 constexpr float kWg = 2.0f, kMerge = 3.0f, kMergeSlot = 0.02f;
 
-// Run by all 512 threads of one workgroup; lds: 512 + 5 * 3000 + 4 words, or 512 +
-// B + 4. Lanes are requests
+// Run by all 512 threads of one workgroup; lds: 512 + 6 * 2600 + 1 words, or 512 +
+// B + 1. Lanes are requests
 // (a run of them above 512), then lengths that are tried, then items.
 __device__ __forceinline__ void plan_chunks(const Call &c, int *lds) {
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, qb = c.rows_c / c.G;
     Work *out = reinterpret_cast<Work *>(c.work);
-    int *first = c.work + kWorkWords, *slot = first + c.B + 1;
-    int4 *list = reinterpret_cast<int4 *>(c.work + (kWorkWords + 2 * c.B + 4) / 4 * 4);
+    int *first = c.work + kFirstAt, *slot = first + c.B + 1;
+    Item *list = reinterpret_cast<Item *>(c.work + kListAt);
     int *sums = lds, *start = lds + 512;                      // start: first item of every request
-    int4 *known = reinterpret_cast<int4 *>(start + (c.B + 4) / 4 * 4);  // {n, pos0, prefix, kv} of every request
+    Request *known = reinterpret_cast<Request *>(start + c.B + 1);
     const int per = (c.B + 511) / 512, b0 = min(tid * per, c.B), b1 = min(b0 + per, c.B);
-    const bool kept = c.B <= 3000;  // in LDS; larger batches read them again
+    const bool kept = c.B <= 2600;  // in LDS; larger batches read them again
     auto load = [&](int b) {
-        if (!kept) return request(c, b);
-        const int4 k = known[b];
-        return Request{0, k.x, k.w, k.y, k.z};
+        return kept ? known[b] : request(c, b);
     };
 
     int wgs = 0, longest = 0;
     float work = 0.0f;  // key tiles that all query tiles see together
     for (int b = b0; b < b1; ++b) {
         const Request r = request(c, b);
-        if (kept) known[b] = make_int4(r.n, r.pos0, r.prefix, r.kv);
+        if (kept) known[b] = r;
         int kt;
         const int T = chunk_tiles(c, r, qb, &kt);
         // query tile i of T ends (T - 1 - i) * qb keys before the last one
@@ -136,7 +153,7 @@ __device__ __forceinline__ void plan_chunks(const Call &c, int *lds) {
     const int pick = __builtin_ctzll(__ballot(t == best));
     const int len = __shfl(l_j, pick), total = min(__shfl((int)N, pick), c.grid_c);
     const bool even = __shfl((int)eq, pick);
-    const int listed = !even && total <= kListed;
+    const int listed = total <= kListed;
     if (tid == 0) *out = Work{len, total, listed, even};
     __syncthreads();
 
@@ -167,6 +184,39 @@ __device__ __forceinline__ void plan_chunks(const Call &c, int *lds) {
     if (tid == 511) start[c.B] = before + items, first[c.B] = before + items;
     if (!listed) return;
 
+    auto item_of = [&](int id, int *own) {
+        int lo = 0, hi = c.B;  // last request whose first item is at most id
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (start[mid] <= id) lo = mid;
+            else hi = mid;
+        }
+        Item it;
+        it.b = lo;
+        it.rq = load(lo);
+        int kt;
+        it.tiles = chunk_tiles(c, it.rq, qb, &kt);
+        it.splits = div_ceil(kt, len);
+        const int k = id - start[lo], q = div_floor(k, it.tiles);
+        it.tile = k - q * it.tiles;
+        it.kvh = div_floor(q, it.splits);
+        it.split = q - it.kvh * it.splits;
+        split_range(kt, it.splits, it.split, &it.t0, &it.t1);
+        it.slot = slot[lo];
+        it.spare[0] = it.spare[1] = 0;
+        const int keys = sees(it.rq, min((it.tile + 1) * qb, it.rq.n) - 1);
+        *own = max(min(it.t1, (keys + kChunkKeys - 1) / kChunkKeys) - it.t0, 0);
+        return it;
+    };
+    __syncthreads();  // start and slot are complete
+    int own;
+    if (even) {
+        for (int lin = tid; lin < c.grid_c && (lin >> 3) <= (total >> 3); lin += 512) {
+            const int id = id_of_workgroup(lin, total);
+            if (id >= 0 && lin < kListed) list[lin] = item_of(id, &own);
+        }
+        return;
+    }
     // counting sort of the items by their length, longest first (the order inside a
     // length is left to chance; no result depends on it)
     constexpr int kBuckets = 64;
@@ -174,23 +224,10 @@ __device__ __forceinline__ void plan_chunks(const Call &c, int *lds) {
     __syncthreads();
     for (int pass = 0; pass < 2; ++pass) {
         for (int id = tid; id < total; id += 512) {
-            int lo = 0, hi = c.B;  // last request whose first item is at most id
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (start[mid] <= id) lo = mid;
-                else hi = mid;
-            }
-            const Request r = load(lo);
-            int kt;
-            const int T = chunk_tiles(c, r, qb, &kt), S = div_ceil(kt, len);
-            const int k = id - start[lo], q = div_floor(k, T), tile = k - q * T, kvh = div_floor(q, S), split = q - kvh * S;
-            int t0, t1;
-            split_range(kt, S, split, &t0, &t1);
-            const int keys = sees(r, min((tile + 1) * qb, r.n) - 1);
-            const int own = max(min(t1, (keys + kChunkKeys - 1) / kChunkKeys) - t0, 0);
+            const Item it = item_of(id, &own);
             const int bucket = kBuckets - 1 - min((int)((float)own * (float)kBuckets / (float)(len + 1)), kBuckets - 1);
             const int at = atomicAdd(&sums[bucket], 1);
-            if (pass) list[at] = make_int4(lo, tile, kvh, split);
+            if (pass) list[at] = it;
         }
         __syncthreads();
         if (pass == 0) {
