@@ -9,15 +9,17 @@
 // the token needs is asked for at the start (A rows, B rows, base beside x), so one
 // memory latency stands before the sums; fp32 throughout.
 //
-// More: a workgroup takes 16 tokens. Its 8 wavefronts split K, each with all ranks:
-// t^T = A x^T on v_mfma_f32_16x16x32_f16, A as it is, x as an fp16 pair: hi = fp16(x),
-// lo = fp16((x - hi) 2^11), in sums of their own (the shift keeps lo clear of
-// subnormals: 22 bits down to |x| = 2^-13, an absolute 2^-36 below). The eight partial
-// t are added in LDS; then they split the columns, out^T = B t^T with t as a pair in
-// the same way. The transposed forms leave a lane with 4 consecutive columns of one
-// token: 16-byte accesses of base and out. Tokens of a tile with other adapters are
-// served in further passes over the tile; a pass takes effect by a select per token,
-// so no adapter's values reach another one's tokens, not even its NaN.
+// More: a workgroup takes 16 tokens. x, gate and A come in as runs of whole rows, 256
+// values of K at a time, and are laid out in LDS (rows are a power of two apart in
+// memory: loads in the shape of MFMA operands, 16 rows of 64 bytes, fell into one set of
+// L1 and took 137 cycles each, 100 us for 4096 tokens at rank 64). The 8 wavefronts share
+// a chunk's steps of K: t^T = A x^T on v_mfma_f32_16x16x32_f16, A as it is, x as an fp16
+// pair: hi = fp16(x), lo = fp16((x - hi) 2^11), in sums of their own (the shift keeps lo
+// clear of subnormals: 22 bits down to |x| = 2^-13, an absolute 2^-36 below). The partial
+// t are added in LDS; then the wavefronts share the columns, out^T = B t^T with t as a
+// pair in the same way, turned in LDS into rows of 64 columns for base and out. The
+// adapters of a tile are taken by kPasses workgroups in turn, each writing its tokens
+// alone; no adapter's values reach another one's tokens, not even its NaN.
 #include <mutex>
 
 #include "paged.hpp"
@@ -139,147 +141,236 @@ __global__ __launch_bounds__(kThreads) void lora_token_kernel(Params p) {
 
 // ----------------------------------------------------------------- tiles
 
-constexpr int kTile = 16;  // tokens of a workgroup
+constexpr int kTile = 16;   // tokens of a workgroup
+constexpr int kPasses = 4;  // workgroups that share a tile's adapters
+constexpr int kCols = 64;   // columns that a wavefront takes at a time
 
-// hi = fp16(x) and lo = fp16((x - hi) 2^11) of 8 values
-__device__ __forceinline__ void split(const float (&x)[8], half8 &hi, half8 &lo) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const _Float16 h = (_Float16)x[i];
-        hi[i] = h;
-        lo[i] = (_Float16)((x[i] - (float)h) * 2048.0f);
-    }
+// Sizes of a form: RT tiles of 16 ranks, r <= 16 RT.
+template <int RT>
+struct Form {
+    static constexpr int kR = 16 * RT;
+    static constexpr int kChunk = RT == 8 ? 128 : 256;  // values of K between two barriers
+    static constexpr int kStepWaves = kChunk / 32, kRankWaves = kWaves / kStepWaves;  // of a chunk: steps of 32, groups of ranks
+    static constexpr int kTiles = RT / kRankWaves;      // rank tiles of a wavefront
+    static constexpr int kRow = kChunk * 2 + 16;        // bytes of a staged row (16 more: its rows on other banks)
+    static constexpr int kX = 2 * kTile * kRow, kStage = kX + kR * kRow;  // x hi, x lo, A
+    static constexpr int kT = kTile * (kR + 4) * 4;     // t: [token][rank]
+    static constexpr int kOutRow = kCols * 4 + 16, kOut = kWaves * kTile * kOutRow;
+    static constexpr int kPart = kWaves * kTiles * 16 * kTile * 4;
+    static constexpr int kBytes = kT + (2 * kStage > kOut ? 2 * kStage : kOut);
+    static_assert(kPart <= 2 * kStage && kBytes <= 160 * 1024, "LDS");
+};
+
+// hi = fp16(x) and lo = fp16((x - hi) 2^11)
+__device__ __forceinline__ void split(float x, _Float16 &hi, _Float16 &lo) {
+    hi = (_Float16)x;
+    lo = (_Float16)((x - (float)hi) * 2048.0f);
 }
 
-// RT: tiles of 16 ranks, r <= 16 RT.
 // MFMA operands (lane = 16 g + n): A[n][8g..8g+7], B[8g..8g+7][n], C[4g..4g+3][n].
-template <int RT>
+template <int RT, bool GATE>
 __global__ __launch_bounds__(kThreads, 2) void lora_tile_kernel(Params p) {
-    extern __shared__ float part[];  // [8 waves][RT * 16 ranks][16 tokens], then t [16 tokens][RT * 16 + 4]
-    constexpr int kR = 16 * RT, kTRow = kR + 4;
-    float *t = part + kWaves * kR * kTile;
+    typedef Form<RT> F;
+    typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ int ids[kTile];
+    float *t = reinterpret_cast<float *>(smem);  // [token][kR + 4]
+    uint8_t *stage = smem + F::kT;
+    constexpr int kTRow = F::kR + 4;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, n = lane & 15;
-    const int m = (int)blockIdx.x * kTile + n;  // the lane's token
-    const bool in = m < p.M;
-    const int64_t row = in ? m : p.M - 1;
-    int id = p.ids[row];
-    id = in && id >= 0 && id < p.n ? id : -1;
-    const float *x = reinterpret_cast<const float *>(p.x + row * p.x_nb1);
-    const float *gt = p.gate ? reinterpret_cast<const float *>(p.gate + row * p.gate_nb1) : nullptr;
-    const float *base = reinterpret_cast<const float *>(p.base + row * p.base_nb1);
-    float *dst = reinterpret_cast<float *>(p.dst + row * p.dst_nb1);
-    // K in steps of 32, N in tiles of 16: this wavefront's share
-    const int k_steps = p.K / 32, k0 = k_steps * wave / kWaves, k1 = k_steps * (wave + 1) / kWaves;
-    const int n_tiles = p.N / 16, c0 = n_tiles * wave / kWaves, c1 = n_tiles * (wave + 1) / kWaves;
-
+    // Workgroups go round-robin to the 8 XCDs: an XCD gets a run of tiles, which share
+    // adapters (in its L2) more often than not.
+    const int tiles = (int)gridDim.x, xcd = (int)blockIdx.x & 7, per = tiles >> 3, rem = tiles & 7;
+    const int m0 = (xcd * per + min(xcd, rem) + ((int)blockIdx.x >> 3)) * kTile;
+    const int tokens = min(p.M - m0, kTile);
+    int id = p.ids[m0 + min(n, tokens - 1)];
+    id = n < tokens && id >= 0 && id < p.n ? id : -1;
+    if (tid < kTile) ids[tid] = tid < tokens ? id : -2;
+    __syncthreads();
     uint64_t todo = __ballot(id >= 0 && g == 0);
-    bool done = false;  // whether dst holds base already (a later pass)
+    bool rest = blockIdx.y == 0;  // tokens without adapter go with the first pass of the first workgroup
     if (!todo) {
-        for (int c = c0; c < c1; ++c)
-            if (in) *reinterpret_cast<floatx4 *>(dst + 16 * c + 4 * g) = *reinterpret_cast<const floatx4 *>(base + 16 * c + 4 * g);
+        if (!rest) return;
+        for (int e = tid; e < tokens * (p.N / 4); e += kThreads) {
+            const int m = e / (p.N / 4), c = e - m * (p.N / 4);
+            reinterpret_cast<floatx4 *>(p.dst + (m0 + m) * p.dst_nb1)[c] =
+                reinterpret_cast<const floatx4 *>(p.base + (m0 + m) * p.base_nb1)[c];
+        }
         return;
     }
-    while (todo) {
+    // this thread's values of a chunk: kNX times 4 of a token, kNA times 8 of a rank
+    constexpr int kNX = kTile * F::kChunk / 4 / kThreads, kNA = (F::kR * F::kChunk / 8 + kThreads - 1) / kThreads;
+    constexpr int kQuads = F::kChunk / 4, kOcts = F::kChunk / 8;
+    const float *xr[kNX], *gr[kNX];
+    int x_at[kNX];
+#pragma unroll
+    for (int i = 0; i < kNX; ++i) {
+        const int e = tid + kThreads * i, m = e / kQuads, k = 4 * (e - m * kQuads);
+        const int64_t row = m0 + min(m, tokens - 1);
+        xr[i] = reinterpret_cast<const float *>(p.x + row * p.x_nb1) + k;
+        gr[i] = GATE ? reinterpret_cast<const float *>(p.gate + row * p.gate_nb1) + k : nullptr;
+        x_at[i] = m * F::kRow + 2 * k;
+    }
+    const int chunks = p.K / F::kChunk, turn = (m0 / kTile) % chunks;  // tiles begin elsewhere in K: other channels of memory
+    for (int pass = 0; todo; ++pass) {
         const int cur = __builtin_amdgcn_readlane(id, __builtin_ctzll(todo));
-        const bool mine = id == cur;
-        todo &= ~__ballot(mine && g == 0);
+        todo &= ~__ballot(id == cur && g == 0);
+        if ((pass & (kPasses - 1)) != (int)blockIdx.y) continue;
         const _Float16 *a = p.a + (int64_t)cur * p.r * p.K, *b = p.b + (int64_t)cur * p.N * p.r;
         const float sc = p.scale ? p.scale[cur] : 1.0f;
-        floatx4 hi[RT], lo[RT];
+        const _Float16 *ar[kNA];
+        int a_at[kNA];
 #pragma unroll
-        for (int q = 0; q < RT; ++q) hi[q] = lo[q] = floatx4{0.f, 0.f, 0.f, 0.f};
-        // rows of A past r re-read its last one: their t is never used
-        const _Float16 *ar[RT];
+        for (int i = 0; i < kNA; ++i) {
+            const int e = tid + kThreads * i, j = min(e / kOcts, F::kR - 1), k = 8 * (e % kOcts);
+            ar[i] = a + (int64_t)min(j, p.r - 1) * p.K + k;  // rows past r: the last one again, their t is not used
+            a_at[i] = F::kX + j * F::kRow + 2 * k;
+        }
+        floatx4 xv[2][kNX], gv[2][kNX];
+        half8 av[2][kNA];
+        auto load = [&](int s, int c) {  // chunk c into register set s
+            c = min(c, chunks - 1) + turn;
+            const int k = (c >= chunks ? c - chunks : c) * F::kChunk;
 #pragma unroll
-        for (int q = 0; q < RT; ++q) ar[q] = a + (int64_t)min(16 * q + n, p.r - 1) * p.K + 8 * g;
-        constexpr int kU = 2;
-        for (int s0 = k0; s0 < k1; s0 += kU) {
-            floatx4 xv[kU][2], gv[kU][2];
-            half8 av[kU][RT];
-#pragma unroll
-            for (int u = 0; u < kU; ++u) {
-                const int k = 32 * min(s0 + u, k1 - 1) + 8 * g;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    xv[u][h] = *reinterpret_cast<const float4a *>(x + k + 4 * h);
-                    if (gt) gv[u][h] = *reinterpret_cast<const float4a *>(gt + k + 4 * h);
-                }
-#pragma unroll
-                for (int q = 0; q < RT; ++q) av[u][q] = *reinterpret_cast<const half8 *>(ar[q] + 32 * min(s0 + u, k1 - 1));
+            for (int i = 0; i < kNX; ++i) {
+                xv[s][i] = *reinterpret_cast<const float4a *>(xr[i] + k);
+                if (GATE) gv[s][i] = *reinterpret_cast<const float4a *>(gr[i] + k);
             }
 #pragma unroll
-            for (int u = 0; u < kU; ++u) {
-                if (s0 + u >= k1) break;
-                float v[8];
+            for (int i = 0; i < kNA; ++i) av[s][i] = *reinterpret_cast<const half8 *>(ar[i] + k);
+        };
+        auto put = [&](int s, int buf) {  // register set s into LDS
+            uint8_t *to = stage + buf * F::kStage;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const floatx4 w = gt ? gated(xv[u][h], gv[u][h]) : xv[u][h];
+            for (int i = 0; i < kNX; ++i) {
+                const floatx4 v = GATE ? gated(xv[s][i], gv[s][i]) : xv[s][i];
+                half4 h, l;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) v[4 * h + i] = w[i];
+                for (int q = 0; q < 4; ++q) {
+                    _Float16 a, b;
+                    split(v[q], a, b);
+                    h[q] = a, l[q] = b;
                 }
-                half8 xh, xl;
-                split(v, xh, xl);
+                *reinterpret_cast<half4 *>(to + x_at[i]) = h;
+                *reinterpret_cast<half4 *>(to + F::kX / 2 + x_at[i]) = l;
+            }
 #pragma unroll
-                for (int q = 0; q < RT; ++q) {
-                    hi[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av[u][q], xh, hi[q], 0, 0, 0);
-                    lo[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av[u][q], xl, lo[q], 0, 0, 0);
+            for (int i = 0; i < kNA; ++i) *reinterpret_cast<half8 *>(to + a_at[i]) = av[s][i];
+        };
+        floatx4 hi[F::kTiles], lo[F::kTiles];
+#pragma unroll
+        for (int q = 0; q < F::kTiles; ++q) hi[q] = lo[q] = floatx4{0.f, 0.f, 0.f, 0.f};
+        const int step = wave % F::kStepWaves, rank0 = 16 * F::kTiles * (wave / F::kStepWaves);
+        const int op = n * F::kRow + 64 * step + 16 * g;  // of an operand's row n in the stage
+        load(0, 0);
+        load(1, 1);
+        __syncthreads();  // (a pass before: its output staging is read)
+        put(0, 0);
+        load(0, 2);
+        // chunk c from LDS, chunk c + 1 into the other buffer, chunk c + 3 on its way
+        for (int c0 = 0; c0 < chunks; c0 += 2) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                __syncthreads();
+                if (c0 + u < chunks) {
+                    const uint8_t *from = stage + u * F::kStage;
+                    const half8 xh = *reinterpret_cast<const half8 *>(from + op), xl = *reinterpret_cast<const half8 *>(from + F::kX / 2 + op);
+#pragma unroll
+                    for (int q = 0; q < F::kTiles; ++q) {
+                        const half8 aq = *reinterpret_cast<const half8 *>(from + F::kX + (rank0 + 16 * q) * F::kRow + op);
+                        hi[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(aq, xh, hi[q], 0, 0, 0);
+                        lo[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(aq, xl, lo[q], 0, 0, 0);
+                    }
                 }
+                put(u ^ 1, u ^ 1);
+                load(u ^ 1, c0 + u + 3);
             }
         }
+        __syncthreads();
+        // the first columns' base and B, before the barriers of the sum
+        constexpr int kS = (F::kR + 31) / 32, kCT = kCols / 16, kNB = kTile * kCols / 4 / 64;
+        const int groups = (p.N + kCols - 1) / kCols;
+        floatx4 old[2][kNB];
+        half8 bv[2][kCT][kS];
+        auto load_cols = [&](int s, int grp) {
+            grp = min(grp, groups - 1);
 #pragma unroll
-        for (int q = 0; q < RT; ++q)
+            for (int i = 0; i < kNB; ++i) {
+                const int e = lane + 64 * i, m = e / (kCols / 4), c = min(grp * kCols + 4 * (e % (kCols / 4)), p.N - 4);
+                old[s][i] = *reinterpret_cast<const floatx4 *>(p.base + (m0 + min(m, tokens - 1)) * p.base_nb1 + 4 * c);
+            }
+#pragma unroll
+            for (int u = 0; u < kCT; ++u)
+#pragma unroll
+                for (int q = 0; q < kS; ++q) {
+                    const int c = min(grp * kCols + 16 * u, p.N - 16) + n, k = 32 * q + 8 * g;
+                    bv[s][u][q] = *reinterpret_cast<const half8 *>(b + (int64_t)c * p.r + min(k, p.r - 8));
+                    bv[s][u][q] = k < p.r ? bv[s][u][q] : half8{};  // past r: 0 (times t, 0 there)
+                }
+        };
+        load_cols(0, wave);
+        float *part = reinterpret_cast<float *>(stage);  // [step wave][rank][token]
+#pragma unroll
+        for (int q = 0; q < F::kTiles; ++q)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                part[(wave * kR + 16 * q + 4 * g + i) * kTile + n] = fmaf(lo[q][i], 1.0f / 2048.0f, hi[q][i]);
+                part[(step * F::kR + rank0 + 16 * q + 4 * g + i) * kTile + n] = fmaf(lo[q][i], 1.0f / 2048.0f, hi[q][i]);
         __syncthreads();
-        for (int e = tid; e < kR * kTile; e += kThreads) {
+        for (int e = tid; e < F::kR * kTile; e += kThreads) {
             float s = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) s += part[w * kR * kTile + e];
+            for (int w = 0; w < F::kStepWaves; ++w) s += part[w * F::kR * kTile + e];
             t[(e & 15) * kTRow + (e >> 4)] = e >> 4 < p.r ? s * sc : 0.0f;
         }
         __syncthreads();
-        // t of the lane's token, ranks 32s + 8g ..
-        constexpr int kS = (kR + 31) / 32;
+        // t of the lane's token, ranks 32q + 8g ..
         half8 th[kS], tl[kS];
 #pragma unroll
-        for (int s = 0; s < kS; ++s) {
-            float v[8];
+        for (int q = 0; q < kS; ++q)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = 32 * s + 8 * g < kR ? t[n * kTRow + 32 * s + 8 * g + i] : 0.0f;
-            split(v, th[s], tl[s]);
-        }
-        // kC tiles of 16 columns at a time, all their loads before the first use
-        constexpr int kC = RT == 8 ? 2 : 4;
-        const float *from = done ? dst : base;
-        for (int cc = c0; cc < c1; cc += kC) {
-            floatx4 old[kC];
-            half8 bv[kC][kS];
-#pragma unroll
-            for (int u = 0; u < kC; ++u) {
-                const int c = min(cc + u, c1 - 1);
-                old[u] = *reinterpret_cast<const floatx4 *>(from + 16 * c + 4 * g);
-#pragma unroll
-                for (int s = 0; s < kS; ++s) {
-                    bv[u][s] = half8{};
-                    if (32 * s + 8 * g < p.r) bv[u][s] = *reinterpret_cast<const half8 *>(b + (int64_t)(16 * c + n) * p.r + 32 * s + 8 * g);
-                }
+            for (int i = 0; i < 8; ++i) {
+                _Float16 a, b;
+                split(32 * q + 8 * g < F::kR ? t[n * kTRow + 32 * q + 8 * g + i] : 0.0f, a, b);
+                th[q][i] = a, tl[q][i] = b;
             }
+        // out^T = B t^T of kCols columns, turned in LDS so that base and out are whole rows of them
+        uint8_t *turned = stage + wave * kTile * F::kOutRow;
+        for (int g0 = wave; g0 < groups; g0 += 2 * kWaves) {
 #pragma unroll
-            for (int u = 0; u < kC; ++u) {
-                floatx4 h = {0.f, 0.f, 0.f, 0.f}, l = h;
+            for (int s = 0; s < 2; ++s) {
+                const int grp = g0 + s * kWaves;
+                load_cols(s ^ 1, grp + kWaves);
+                if (grp >= groups) continue;
 #pragma unroll
-                for (int s = 0; s < kS; ++s) {
-                    h = __builtin_amdgcn_mfma_f32_16x16x32_f16(bv[u][s], th[s], h, 0, 0, 0);
-                    l = __builtin_amdgcn_mfma_f32_16x16x32_f16(bv[u][s], tl[s], l, 0, 0, 0);
+                for (int u = 0; u < kCT; ++u) {
+                    floatx4 h = {0.f, 0.f, 0.f, 0.f}, l = h;
+#pragma unroll
+                    for (int q = 0; q < kS; ++q) {
+                        h = __builtin_amdgcn_mfma_f32_16x16x32_f16(bv[s][u][q], th[q], h, 0, 0, 0);
+                        l = __builtin_amdgcn_mfma_f32_16x16x32_f16(bv[s][u][q], tl[q], l, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) h[i] = fmaf(l[i], 1.0f / 2048.0f, h[i]);
+                    *reinterpret_cast<floatx4 *>(turned + n * F::kOutRow + 4 * (16 * u + 4 * g)) = h;
                 }
-                floatx4 o;
+                // (a wavefront's own staging: its LDS operations are in order)
+                __builtin_amdgcn_wave_barrier();
 #pragma unroll
-                for (int i = 0; i < 4; ++i) o[i] = mine ? old[u][i] + fmaf(l[i], 1.0f / 2048.0f, h[i]) : old[u][i];
-                if (in && (mine || !done) && cc + u < c1) *reinterpret_cast<floatx4 *>(dst + 16 * (cc + u) + 4 * g) = o;
+                for (int i = 0; i < kNB; ++i) {
+                    const int e = lane + 64 * i, m = e / (kCols / 4), c = grp * kCols + 4 * (e % (kCols / 4));
+                    const floatx4 add = *reinterpret_cast<const floatx4 *>(turned + m * F::kOutRow + 16 * (e % (kCols / 4)));
+                    const int own = ids[m];
+                    floatx4 o;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) o[q] = own == cur ? old[s][i][q] + add[q] : old[s][i][q];
+                    // (dst may be base: a value is read before it is written, by this wavefront alone)
+                    if (c < p.N && (own == cur || (own == -1 && rest)))
+                        *reinterpret_cast<floatx4 *>(p.dst + (m0 + m) * p.dst_nb1 + 4 * c) = o;
+                }
+                __builtin_amdgcn_wave_barrier();
             }
         }
-        done = true;
+        rest = false;
     }
 }
 
@@ -299,18 +390,23 @@ int launch_lora_add(const sqa_tensor &base, const sqa_tensor &x, const sqa_tenso
         const int parts = p.M <= 32 ? 4 : p.M <= 96 ? 2 : 1;
         lora_token_kernel<<<dim3((unsigned)p.M, (unsigned)parts), dim3(kThreads), (size_t)p.K * 4, s>>>(p);
     } else {
-        const dim3 grid((unsigned)((p.M + kTile - 1) / kTile));
-        auto lds = [](int rt) { return (size_t)(kWaves * 16 * rt * kTile + kTile * (16 * rt + 4)) * 4; };
-        static std::once_flag once;  // the one form above the 64 KB that need no asking
+        const dim3 grid((unsigned)((p.M + kTile - 1) / kTile), kPasses);
+        typedef void (*Kernel)(Params);
+        static const Kernel kernels[2][4] = {
+            {lora_tile_kernel<1, false>, lora_tile_kernel<2, false>, lora_tile_kernel<4, false>, lora_tile_kernel<8, false>},
+            {lora_tile_kernel<1, true>, lora_tile_kernel<2, true>, lora_tile_kernel<4, true>, lora_tile_kernel<8, true>}};
+        static const int lds[4] = {Form<1>::kBytes, Form<2>::kBytes, Form<4>::kBytes, Form<8>::kBytes};
+        static std::once_flag once;  // the LDS limit is raised once per process
         static hipError_t err = hipSuccess;
-        std::call_once(once, [&] {
-            err = hipFuncSetAttribute((const void *)lora_tile_kernel<8>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds(8));
+        std::call_once(once, [] {
+            for (int g = 0; g < 2; ++g)
+                for (int i = 0; i < 4; ++i)
+                    if (err == hipSuccess)
+                        err = hipFuncSetAttribute((const void *)kernels[g][i], hipFuncAttributeMaxDynamicSharedMemorySize, lds[i]);
         });
         if (err != hipSuccess) return hip_status(err, "lora_add LDS attribute");
-        if (p.r <= 16) lora_tile_kernel<1><<<grid, dim3(kThreads), lds(1), s>>>(p);
-        else if (p.r <= 32) lora_tile_kernel<2><<<grid, dim3(kThreads), lds(2), s>>>(p);
-        else if (p.r <= 64) lora_tile_kernel<4><<<grid, dim3(kThreads), lds(4), s>>>(p);
-        else lora_tile_kernel<8><<<grid, dim3(kThreads), lds(8), s>>>(p);
+        const int rt = p.r <= 16 ? 0 : p.r <= 32 ? 1 : p.r <= 64 ? 2 : 3;
+        kernels[p.gate != nullptr][rt]<<<grid, dim3(kThreads), lds[rt], s>>>(p);
     }
     profile_stop(prof, s);
     return hip_status(hipGetLastError(), "lora_add launch");

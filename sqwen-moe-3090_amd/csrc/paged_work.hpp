@@ -115,31 +115,23 @@ __device__ __forceinline__ void plan_chunks(const Call &c, int *lds) {
     }
     work *= (float)c.Hkv;
     __syncthreads();
-    // query tiles times splits, of all requests (kChoices) and of split ones
-    int n[2 * kChoices] = {};
-    for (int b = b0; b < b1; ++b) {
-        int kt;
-        const int T = chunk_tiles(c, load(b), qb, &kt);
-        if (T == 0) continue;
-#pragma unroll
-        for (int j = 0; j < kChoices; ++j) {
-            const int l = max(div_ceil(longest, kTried[j]), 2), S = div_ceil(kt, l);
-            n[j] += T * S;
-            n[kChoices + j] += S > 1 ? T * S : 0;
-        }
-    }
-    const bool some = __any(b0 < b1);
-#pragma unroll
-    for (int j = 0; j < 2 * kChoices; ++j) {
-        const int s = some ? wave_sum(n[j]) : 0;
-        if (lane == 0) sums[wave * 2 * kChoices + j] = s;
-    }
-    __syncthreads();
-    // lane j estimates length j
-    int v = 0;
-    for (int w = 0; w < 8; ++w) v += sums[w * 2 * kChoices + (lane & (2 * kChoices - 1))];
-    const int64_t N = (int64_t)v * c.Hkv, slots_j = (int64_t)__shfl_xor(v, kChoices) * c.Hkv;
+    // lane j (of 16) estimates length j: query tiles times splits, of all requests and of
+    // split ones; 32 requests at a time
     const int j = lane & (kChoices - 1), l_j = max(div_ceil(longest, kTried[j]), 2);
+    int n_j = 0, split_j = 0;
+    for (int b = 4 * wave + (lane >> 4); b < c.B; b += 32) {
+        int kt;
+        const int T = chunk_tiles(c, load(b), qb, &kt), n = T * div_ceil(kt, l_j);
+        n_j += n;
+        split_j += kt > l_j ? n : 0;
+    }
+    n_j += __shfl_xor(n_j, 16), split_j += __shfl_xor(split_j, 16);
+    n_j += __shfl_xor(n_j, 32), split_j += __shfl_xor(split_j, 32);
+    if (lane < kChoices) sums[wave * 32 + lane] = n_j, sums[wave * 32 + 16 + lane] = split_j;
+    __syncthreads();
+    n_j = split_j = 0;
+    for (int w = 0; w < 8; ++w) n_j += sums[w * 32 + j], split_j += sums[w * 32 + 16 + j];
+    const int64_t N = (int64_t)n_j * c.Hkv, slots_j = (int64_t)split_j * c.Hkv;
     const float part = (float)min(l_j, longest), cus = (float)c.cus;
     const bool eq = work > 0.85f * (float)N * part;
     float t = eq ? ceilf((float)N / cus) * (part + kWg) : fmaxf((work + kWg * (float)N) / cus + 0.25f * part, part + kWg);
