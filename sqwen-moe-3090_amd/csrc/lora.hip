@@ -17,9 +17,9 @@
 // pair: hi = fp16(x), lo = fp16((x - hi) 2^11), in sums of their own (the shift keeps lo
 // clear of subnormals: 22 bits down to |x| = 2^-13, an absolute 2^-36 below). The partial
 // t are added in LDS; then the wavefronts share the columns, out^T = B t^T with t as a
-// pair in the same way, turned in LDS into rows of 64 columns for base and out. The
-// adapters of a tile are taken by kPasses workgroups in turn, each writing its tokens
-// alone; no adapter's values reach another one's tokens, not even its NaN.
+// pair in the same way, turned in LDS into rows of 64 columns (32 above rank 64, for want
+// of registers) for base and out. The adapters of a tile are taken by kPasses workgroups in
+// turn, each writing its tokens alone; no adapter's values reach another one's tokens, not even its NaN.
 #include <mutex>
 
 #include "paged.hpp"
@@ -143,7 +143,6 @@ __global__ __launch_bounds__(kThreads) void lora_token_kernel(Params p) {
 
 constexpr int kTile = 16;   // tokens of a workgroup
 constexpr int kPasses = 4;  // workgroups that share a tile's adapters
-constexpr int kCols = 64;   // columns that a wavefront takes at a time
 
 // Sizes of a form: RT tiles of 16 ranks, r <= 16 RT.
 template <int RT>
@@ -155,6 +154,7 @@ struct Form {
     static constexpr int kRow = kChunk * 2 + 16;        // bytes of a staged row (16 more: its rows on other banks)
     static constexpr int kX = 2 * kTile * kRow, kStage = kX + kR * kRow;  // x hi, x lo, A
     static constexpr int kT = kTile * (kR + 4) * 4;     // t: [token][rank]
+    static constexpr int kCols = RT == 8 ? 32 : 64;     // columns that a wavefront takes at a time
     static constexpr int kOutRow = kCols * 4 + 16, kOut = kWaves * kTile * kOutRow;
     static constexpr int kPart = kWaves * kTiles * 16 * kTile * 4;
     static constexpr int kBytes = kT + (2 * kStage > kOut ? 2 * kStage : kOut);
@@ -211,7 +211,9 @@ __global__ __launch_bounds__(kThreads, 2) void lora_tile_kernel(Params p) {
         gr[i] = GATE ? reinterpret_cast<const float *>(p.gate + row * p.gate_nb1) + k : nullptr;
         x_at[i] = m * F::kRow + 2 * k;
     }
-    const int chunks = p.K / F::kChunk, turn = (m0 / kTile) % chunks;  // tiles begin elsewhere in K: other channels of memory
+    // (tiles that begin elsewhere in K, on other channels of memory, lose more to A, which
+    // neighbours then no longer read together: 80 us against 74 at 4096 tokens)
+    const int chunks = p.K / F::kChunk;
     for (int pass = 0; todo; ++pass) {
         const int cur = __builtin_amdgcn_readlane(id, __builtin_ctzll(todo));
         todo &= ~__ballot(id == cur && g == 0);
@@ -229,8 +231,7 @@ __global__ __launch_bounds__(kThreads, 2) void lora_tile_kernel(Params p) {
         floatx4 xv[2][kNX], gv[2][kNX];
         half8 av[2][kNA];
         auto load = [&](int s, int c) {  // chunk c into register set s
-            c = min(c, chunks - 1) + turn;
-            const int k = (c >= chunks ? c - chunks : c) * F::kChunk;
+            const int k = min(c, chunks - 1) * F::kChunk;
 #pragma unroll
             for (int i = 0; i < kNX; ++i) {
                 xv[s][i] = *reinterpret_cast<const float4a *>(xr[i] + k);
@@ -288,7 +289,7 @@ __global__ __launch_bounds__(kThreads, 2) void lora_tile_kernel(Params p) {
         }
         __syncthreads();
         // the first columns' base and B, before the barriers of the sum
-        constexpr int kS = (F::kR + 31) / 32, kCT = kCols / 16, kNB = kTile * kCols / 4 / 64;
+        constexpr int kS = (F::kR + 31) / 32, kCols = F::kCols, kCT = kCols / 16, kNB = kTile * kCols / 4 / 64;
         const int groups = (p.N + kCols - 1) / kCols;
         floatx4 old[2][kNB];
         half8 bv[2][kCT][kS];
@@ -363,9 +364,10 @@ __global__ __launch_bounds__(kThreads, 2) void lora_tile_kernel(Params p) {
                     floatx4 o;
 #pragma unroll
                     for (int q = 0; q < 4; ++q) o[q] = own == cur ? old[s][i][q] + add[q] : old[s][i][q];
-                    // (dst may be base: a value is read before it is written, by this wavefront alone)
+                    // (dst may be base: a value is read before it is written, by this wavefront alone;
+                    // past L2, which the adapters need: 71 us against 74 at 4096 tokens)
                     if (c < p.N && (own == cur || (own == -1 && rest)))
-                        *reinterpret_cast<floatx4 *>(p.dst + (m0 + m) * p.dst_nb1 + 4 * c) = o;
+                        __builtin_nontemporal_store(o, reinterpret_cast<floatx4 *>(p.dst + (m0 + m) * p.dst_nb1 + 4 * c));
                 }
                 __builtin_amdgcn_wave_barrier();
             }
