@@ -149,8 +149,10 @@ __device__ __forceinline__ void dma16(uint32_t voff, const void *sbase, uint32_t
     const uint64_t bs = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32) |
                         (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)b);
     const uint32_t ms = (uint32_t)__builtin_amdgcn_readfirstlane((int)m0v);
-    // m0 as an operand: the compiler writes it and knows it holds the LDS base
-    asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(bs), "{m0}"(ms) : "memory");
+    // m0 as an operand: the compiler writes it and knows it holds the LDS base. It does not
+    // know what the asm holds: the wait states that a load into LDS needs after a write of
+    // m0 (1), and a memory instruction after v_readfirstlane wrote its base (5), stand in it.
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(bs), "{m0}"(ms) : "memory");
 }
 
 typedef const __attribute__((address_space(3))) uint32_t lds_u32;  // LDS dword from a raw LDS address
