@@ -78,20 +78,46 @@ __global__ __launch_bounds__(kThreads) void lora_token_kernel(Params p) {
         return;
     }
     const _Float16 *a = p.a + (int64_t)id * p.r * p.K, *b = p.b + (int64_t)id * p.N * p.r;
-    const float sc = p.scale ? p.scale[id] : 1.0f;
-    // the first rank's row and the first column's are on their way while x is gated
-    constexpr int kAhead = 8;
-    half8 an[kAhead];
-    const bool first = wave < p.r;
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j)
-        if (first && 512 * j + 8 * lane < p.K) an[j] = *reinterpret_cast<const half8 *>(a + (int64_t)wave * p.K + 512 * j + 8 * lane);
+    // x, the first rank's row and the first column's are on their way together (addresses
+    // clamped, not branched around: a load in a branch waits for the ones before it)
     const float *x = reinterpret_cast<const float *>(p.x + m * p.x_nb1);
     const float *g = p.gate ? reinterpret_cast<const float *>(p.gate + m * p.gate_nb1) : nullptr;
-    for (int k = 4 * tid; k < p.K; k += 4 * kThreads) {
-        floatx4 v = *reinterpret_cast<const float4a *>(x + k);
-        if (g) v = gated(v, *reinterpret_cast<const float4a *>(g + k));
-        *reinterpret_cast<floatx4 *>(xs + k) = v;
+    constexpr int kX = 2, kAhead = 8, kB = 4;  // runs of 2048, 512 values of K, 8 ranks
+    floatx4 xv[kX], gv[kX];
+    auto load_x = [&](int k0) {
+#pragma unroll
+        for (int q = 0; q < kX; ++q) {
+            const int k = min(k0 + 4 * kThreads * q + 4 * tid, p.K - 4);
+            xv[q] = *reinterpret_cast<const float4a *>(x + k);
+            if (g) gv[q] = *reinterpret_cast<const float4a *>(g + k);
+        }
+    };
+    half8 an[kAhead];
+    auto load_a = [&](int j, int k0) {
+        const _Float16 *row = a + (int64_t)min(j, p.r - 1) * p.K;
+#pragma unroll
+        for (int q = 0; q < kAhead; ++q) an[q] = *reinterpret_cast<const half8 *>(row + min(k0 + 512 * q + 8 * lane, p.K - 8));
+    };
+    half8 bn[kB];
+    float old = 0.0f;
+    auto load_b = [&](int c) {
+        c = min(c, 4 * q1 - 1);
+#pragma unroll
+        for (int q = 0; q < kB; ++q) bn[q] = *reinterpret_cast<const half8 *>(b + (int64_t)c * p.r + min(8 * q, p.r - 8));
+        old = base[c];
+    };
+    load_x(0);
+    load_a(wave, 0);
+    const float sc = p.scale ? p.scale[id] : 1.0f;
+    const bool columns = q0 < q1;  // (fewer quads than parts: some have none)
+    if (columns) load_b(4 * q0 + tid);
+    for (int k0 = 0; k0 < p.K; k0 += 4 * kThreads * kX) {
+        if (k0) load_x(k0);
+#pragma unroll
+        for (int q = 0; q < kX; ++q) {
+            const int k = k0 + 4 * kThreads * q + 4 * tid;
+            if (k < p.K) *reinterpret_cast<floatx4 *>(xs + k) = g ? gated(xv[q], gv[q]) : xv[q];
+        }
     }
     __syncthreads();
     for (int j = wave; j < p.r; j += kWaves) {
@@ -101,11 +127,8 @@ __global__ __launch_bounds__(kThreads) void lora_token_kernel(Params p) {
 #pragma unroll
             for (int q = 0; q < kAhead; ++q) av[q] = an[q];
             // the next stretch: of this rank, or the start of the next one
-            const int kn = k0 + 512 * kAhead, jn = kn < p.K ? j : j + kWaves, k1 = kn < p.K ? kn : 0;
-#pragma unroll
-            for (int q = 0; q < kAhead; ++q)
-                if (jn < p.r && k1 + 512 * q + 8 * lane < p.K)
-                    an[q] = *reinterpret_cast<const half8 *>(a + (int64_t)jn * p.K + k1 + 512 * q + 8 * lane);
+            const int kn = k0 + 512 * kAhead;
+            load_a(kn < p.K ? j : j + kWaves, kn < p.K ? kn : 0);
 #pragma unroll
             for (int q = 0; q < kAhead; ++q) {
                 const int k = k0 + 512 * q + 8 * lane;
@@ -125,14 +148,23 @@ __global__ __launch_bounds__(kThreads) void lora_token_kernel(Params p) {
     __syncthreads();
     for (int c = 4 * q0 + tid; c < 4 * q1; c += kThreads) {
         const half8 *row = reinterpret_cast<const half8 *>(b + (int64_t)c * p.r);
-        float s = base[c];
-        for (int j = 0; j < p.r / 8; ++j) {
-            const half8 bv = row[j];
-            const floatx4 u = *reinterpret_cast<const floatx4 *>(t + 8 * j), v = *reinterpret_cast<const floatx4 *>(t + 8 * j + 4);
+        half8 bv[kB];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                s = fmaf(u[i], (float)bv[i], s);
-                s = fmaf(v[i], (float)bv[4 + i], s);
+        for (int q = 0; q < kB; ++q) bv[q] = bn[q];
+        float s = old;
+        load_b(c + kThreads);
+        for (int j0 = 0; j0 < p.r; j0 += 8 * kB) {
+#pragma unroll
+            for (int q = 0; q < kB; ++q) {
+                const int j = j0 + 8 * q;
+                if (j >= p.r) continue;
+                const half8 w = j0 ? row[j / 8] : bv[q];
+                const floatx4 u = *reinterpret_cast<const floatx4 *>(t + j), v = *reinterpret_cast<const floatx4 *>(t + j + 4);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s = fmaf(u[i], (float)w[i], s);
+                    s = fmaf(v[i], (float)w[4 + i], s);
+                }
             }
         }
         dst[c] = s;
