@@ -53,20 +53,40 @@ __device__ __forceinline__ floatx4 gated(floatx4 x, floatx4 g) {
     return x;
 }
 
-__device__ __forceinline__ float wave_sum(float x) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o);
-    return x;
-}
-
 // ------------------------------------------------------------- few tokens
 
-// Grid (tokens, parts of the columns). Wavefront w sums ranks w, w + 8, ...: a lane 8
-// values of every 512.
+__device__ __forceinline__ float bits(uint32_t x) { return __uint_as_float(x); }
+
+template <int kCtrl>
+__device__ __forceinline__ float add_dpp(float x) {
+    return x + bits((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), kCtrl, 0xf, 0xf, true));
+}
+constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kHalfMirror = 0x141, kMirror = 0x140;  // lane ^ 1, ^ 2, 7 - i, 15 - i
+
+// Sums of 8 values over the wavefront: s[0], s[1] hold those of value 0 or 1, + 2 in odd
+// rows of 16 lanes, + 4 in the upper half. A swap folds two values at once.
+__device__ __forceinline__ void fold(float (&s)[8]) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(s[q]), __float_as_uint(s[q + 4]), false, false);
+        s[q] = bits(r[0]) + bits(r[1]);
+    }
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(s[q]), __float_as_uint(s[q + 2]), false, false);
+        s[q] = bits(r[0]) + bits(r[1]);
+        s[q] = add_dpp<kMirror>(add_dpp<kHalfMirror>(add_dpp<kXor2>(add_dpp<kXor1>(s[q]))));
+    }
+}
+
+// Grid (tokens, parts of the columns); K <= 4096 kRuns. A wavefront keeps its values of x,
+// runs of 512, 8 a lane, in registers and takes 8 ranks at a time; where K has fewer runs
+// than there are wavefronts, groups of them share the ranks. Then 1 to 16 lanes take a
+// column, 8 ranks each.
+template <int kRuns>
 __global__ __launch_bounds__(kThreads) void lora_token_kernel(Params p) {
-    extern __shared__ float xs[];  // K values of x sigmoid(gate)
-    __shared__ __align__(16) float t[kMaxRank];
-    const int m = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    __shared__ __align__(16) float part[kWaves][kMaxRank];
+    const int m = blockIdx.x, tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
     const int id = p.ids[m];
     const float *base = reinterpret_cast<const float *>(p.base + m * p.base_nb1);
     float *dst = reinterpret_cast<float *>(p.dst + m * p.dst_nb1);
@@ -77,97 +97,122 @@ __global__ __launch_bounds__(kThreads) void lora_token_kernel(Params p) {
             reinterpret_cast<floatx4 *>(dst)[q] = reinterpret_cast<const floatx4 *>(base)[q];
         return;
     }
+    if (q0 == q1) return;  // fewer quads than parts
     const _Float16 *a = p.a + (int64_t)id * p.r * p.K, *b = p.b + (int64_t)id * p.N * p.r;
-    // x, the first rank's row and the first column's are on their way together (addresses
-    // clamped, not branched around: a load in a branch waits for the ones before it)
+    // Everything that the first sums need is on its way together (addresses clamped, not
+    // branched around: a load in a branch waits for the ones before it).
+    const int runs = (p.K + 511) / 512, lw = runs > 4 ? 3 : runs > 2 ? 2 : runs - 1;  // log2 of the wavefronts along K
+    const int wk = wave & ((1 << lw) - 1), group = wave >> lw, groups = kWaves >> lw, batches = p.r / 8;
     const float *x = reinterpret_cast<const float *>(p.x + m * p.x_nb1);
     const float *g = p.gate ? reinterpret_cast<const float *>(p.gate + m * p.gate_nb1) : nullptr;
-    constexpr int kX = 2, kAhead = 8, kB = 4;  // runs of 2048, 512 values of K, 8 ranks
-    floatx4 xv[kX], gv[kX];
-    auto load_x = [&](int k0) {
+    auto at = [&](int i) { return 512 * (wk + kWaves * i) + 8 * lane; };  // (lw < 3 has one run a wavefront)
+    floatx4 xv[kRuns][2], gv[kRuns][2];
 #pragma unroll
-        for (int q = 0; q < kX; ++q) {
-            const int k = min(k0 + 4 * kThreads * q + 4 * tid, p.K - 4);
-            xv[q] = *reinterpret_cast<const float4a *>(x + k);
-            if (g) gv[q] = *reinterpret_cast<const float4a *>(g + k);
+    for (int i = 0; i < kRuns; ++i)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const int k = min(at(i), p.K - 8) + 4 * q;
+            xv[i][q] = *reinterpret_cast<const float4a *>(x + k);
+            if (g) gv[i][q] = *reinterpret_cast<const float4a *>(g + k);
+        }
+    half8 av[2][8];
+    auto load_a = [&](int s, int batch, int i) {
+        const _Float16 *row = a + (int64_t)min(batch, batches - 1) * 8 * p.K + min(at(i), p.K - 8);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) av[s][j] = *reinterpret_cast<const half8 *>(row + (int64_t)j * p.K);
+    };
+    load_a(0, group, 0);
+    // columns: 2^ll lanes of a column, chunk `ch` of 8 ranks
+    constexpr int kB = 4;
+    const int ll = batches > 8 ? 4 : batches > 4 ? 3 : batches > 2 ? 2 : batches - 1;
+    const int ch = lane & ((1 << ll) - 1), c_own = 4 * q0 + (64 >> ll) * wave + (lane >> ll), c_step = kThreads >> ll;
+    half8 bv[2][kB];
+    float old[2][kB];
+    auto load_b = [&](int s, int c) {
+#pragma unroll
+        for (int q = 0; q < kB; ++q) {
+            const int cc = min(c + q * c_step, 4 * q1 - 1);
+            bv[s][q] = *reinterpret_cast<const half8 *>(b + (int64_t)cc * p.r + 8 * min(ch, batches - 1));
+            old[s][q] = base[cc];
         }
     };
-    half8 an[kAhead];
-    auto load_a = [&](int j, int k0) {
-        const _Float16 *row = a + (int64_t)min(j, p.r - 1) * p.K;
-#pragma unroll
-        for (int q = 0; q < kAhead; ++q) an[q] = *reinterpret_cast<const half8 *>(row + min(k0 + 512 * q + 8 * lane, p.K - 8));
-    };
-    half8 bn[kB];
-    float old = 0.0f;
-    auto load_b = [&](int c) {
-        c = min(c, 4 * q1 - 1);
-#pragma unroll
-        for (int q = 0; q < kB; ++q) bn[q] = *reinterpret_cast<const half8 *>(b + (int64_t)c * p.r + min(8 * q, p.r - 8));
-        old = base[c];
-    };
-    load_x(0);
-    load_a(wave, 0);
     const float sc = p.scale ? p.scale[id] : 1.0f;
-    const bool columns = q0 < q1;  // (fewer quads than parts: some have none)
-    if (columns) load_b(4 * q0 + tid);
-    for (int k0 = 0; k0 < p.K; k0 += 4 * kThreads * kX) {
-        if (k0) load_x(k0);
+    load_b(0, c_own);
 #pragma unroll
-        for (int q = 0; q < kX; ++q) {
-            const int k = k0 + 4 * kThreads * q + 4 * tid;
-            if (k < p.K) *reinterpret_cast<floatx4 *>(xs + k) = g ? gated(xv[q], gv[q]) : xv[q];
+    for (int i = 0; i < kRuns; ++i)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            if (g) xv[i][q] = gated(xv[i][q], gv[i][q]);
+            if (at(i) >= p.K) xv[i][q] = floatx4{0.f, 0.f, 0.f, 0.f};
+        }
+    auto sum = [&](int s, int i, float (&to)[8]) {
+        const bool inside = at(i) < p.K;
+        const bool whole = 512 * (wk + kWaves * i + 1) <= p.K;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            half8 v = av[s][j];
+            if (!whole) v = inside ? v : half8{};  // (its x is 0, but 0 times Inf is not)
+#pragma unroll
+            for (int q = 0; q < 8; ++q) to[j] = fmaf(xv[i][q >> 2][q & 3], (float)v[q], to[j]);
+        }
+    };
+    auto put = [&](int batch, float (&s)[8]) {
+        fold(s);
+        if ((lane & 15) == 0) {
+            float *to = &part[wk][8 * batch + 2 * ((lane >> 4) & 1) + 4 * (lane >> 5)];
+            to[0] = s[0], to[1] = s[1];
+        }
+    };
+    for (int batch = group; batch < batches; batch += (kRuns == 1 ? 2 : 1) * groups) {
+        if (kRuns == 1) {
+            float s[8] = {}, u[8] = {};
+            load_a(1, batch + groups, 0);
+            sum(0, 0, s);
+            put(batch, s);
+            load_a(0, batch + 2 * groups, 0);
+            sum(1, 0, u);
+            if (batch + groups < batches) put(batch + groups, u);
+        } else {
+            float s[8] = {};
+#pragma unroll
+            for (int i = 0; i < kRuns; ++i) {
+                load_a((i + 1) & 1, i + 1 < kRuns ? batch : batch + groups, (i + 1) % kRuns);
+                sum(i & 1, i, s);
+            }
+            put(batch, s);
         }
     }
     __syncthreads();
-    for (int j = wave; j < p.r; j += kWaves) {
-        float s0 = 0.0f, s1 = 0.0f;
-        for (int k0 = 0; k0 < p.K; k0 += 512 * kAhead) {
-            half8 av[kAhead];
+    float t[8];
 #pragma unroll
-            for (int q = 0; q < kAhead; ++q) av[q] = an[q];
-            // the next stretch: of this rank, or the start of the next one
-            const int kn = k0 + 512 * kAhead;
-            load_a(kn < p.K ? j : j + kWaves, kn < p.K ? kn : 0);
+    for (int q = 0; q < 8; ++q) t[q] = 0.0f;
+    for (int w = 0; w < 1 << lw; ++w) {
+        const floatx4 *from = reinterpret_cast<const floatx4 *>(&part[w][8 * min(ch, batches - 1)]);
+        const floatx4 u = from[0], v = from[1];
 #pragma unroll
-            for (int q = 0; q < kAhead; ++q) {
-                const int k = k0 + 512 * q + 8 * lane;
-                if (k < p.K) {
-                    const floatx4 u = *reinterpret_cast<const floatx4 *>(xs + k), v = *reinterpret_cast<const floatx4 *>(xs + k + 4);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        s0 = fmaf(u[i], (float)av[q][i], s0);
-                        s1 = fmaf(v[i], (float)av[q][4 + i], s1);
-                    }
-                }
-            }
-        }
-        const float s = wave_sum(s0 + s1);
-        if (lane == 0) t[j] = s * sc;
+        for (int q = 0; q < 4; ++q) t[q] += u[q], t[4 + q] += v[q];
     }
-    __syncthreads();
-    for (int c = 4 * q0 + tid; c < 4 * q1; c += kThreads) {
-        const half8 *row = reinterpret_cast<const half8 *>(b + (int64_t)c * p.r);
-        half8 bv[kB];
 #pragma unroll
-        for (int q = 0; q < kB; ++q) bv[q] = bn[q];
-        float s = old;
-        load_b(c + kThreads);
-        for (int j0 = 0; j0 < p.r; j0 += 8 * kB) {
+    for (int q = 0; q < 8; ++q) t[q] *= sc;
+    auto columns = [&](int s, int c) {
 #pragma unroll
-            for (int q = 0; q < kB; ++q) {
-                const int j = j0 + 8 * q;
-                if (j >= p.r) continue;
-                const half8 w = j0 ? row[j / 8] : bv[q];
-                const floatx4 u = *reinterpret_cast<const floatx4 *>(t + j), v = *reinterpret_cast<const floatx4 *>(t + j + 4);
+        for (int q = 0; q < kB; ++q) {
+            float o = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    s = fmaf(u[i], (float)w[i], s);
-                    s = fmaf(v[i], (float)w[4 + i], s);
-                }
-            }
+            for (int i = 0; i < 8; ++i) o = fmaf(t[i], (float)bv[s][q][i], o);
+            if (ch >= batches) o = 0.0f;
+            if (ll > 0) o = add_dpp<kXor1>(o);
+            if (ll > 1) o = add_dpp<kXor2>(o);
+            if (ll > 2) o = add_dpp<kHalfMirror>(o);
+            if (ll > 3) o = add_dpp<kMirror>(o);
+            if (ch == 0 && c + q * c_step < 4 * q1) dst[c + q * c_step] = old[s][q] + o;
         }
-        dst[c] = s;
+    };
+    for (int c = c_own; c < 4 * q1; c += 2 * kB * c_step) {
+        load_b(1, c + kB * c_step);
+        columns(0, c);
+        load_b(0, c + 2 * kB * c_step);
+        columns(1, c + kB * c_step);
     }
 }
 
@@ -419,10 +464,10 @@ int launch_lora_add(const sqa_tensor &base, const sqa_tensor &x, const sqa_tenso
                    scale ? (const float *)scale->data : nullptr, (char *)dst.data, (int)x.ne[0], (int)base.ne[0],
                    (int)a.ne[1], (int)a.ne[2], (int)x.ne[1]};
     const int prof = profile_start("lora_add", s);
-    // x of a token has to fit in LDS beside its ranks
-    if (p.M <= 256 && p.K <= 15 * 1024) {
-        const int parts = p.M <= 32 ? 4 : p.M <= 96 ? 2 : 1;
-        lora_token_kernel<<<dim3((unsigned)p.M, (unsigned)parts), dim3(kThreads), (size_t)p.K * 4, s>>>(p);
+    if (p.M <= 256 && p.K <= 16 * 1024) {
+        const dim3 grid((unsigned)p.M, p.M <= 32 ? 4 : p.M <= 96 ? 2 : 1);
+        if (p.K <= 4096) lora_token_kernel<1><<<grid, dim3(kThreads), 0, s>>>(p);
+        else lora_token_kernel<4><<<grid, dim3(kThreads), 0, s>>>(p);
     } else {
         const dim3 grid((unsigned)((p.M + kTile - 1) / kTile), kPasses);
         typedef void (*Kernel)(Params);

@@ -112,3 +112,15 @@ def test_lora_unused_adapters_hold_anything(sqa, dev):
         d["a"][3], d["b"][3], d["scale"][3] = float("nan"), float("inf"), float("nan")
         d["x"][d["ids"] < 0] = float("nan")
         close(sqa.lora_add(**d), want)
+
+
+@pytest.mark.parametrize("M", [1, 5, 40, 130])
+@pytest.mark.parametrize("K,N,r", [(1280, 64, 120), (2304, 208, 8), (4352, 64, 32), (5120, 2048, 64), (12288, 80, 56),
+                                   (16384, 16, 128), (16640, 64, 16)])
+def test_lora_widths(sqa, dev, M, K, N, r):
+    """Numbers of runs of K and of ranks that leave wavefronts and lanes without work, and K past
+    what the form for few tokens keeps (sums of up to 16640 terms, 2e-8 more than above)."""
+    d = inputs(dev, M + K, M, K, N, r, 5, gate=K % 512 == 0)
+    out = torch.empty_like(d["base"])
+    sqa.lora_add(**d, out=out)
+    close(out, paged_ref.lora(**d))
