@@ -1,13 +1,15 @@
 // lora.hip - low-rank adapters of many requests beside a shared projection:
 // out = base + scale[id] B[id] (A[id] (x sigmoid(gate))), an id per token.
 //
-// Bound by memory: x, gate, base and out once each (64 to 100 KB a token group of 16 per
-// 4096 + 2048 columns), the adapters in use out of L2; by latency for few tokens. Both
-// kernels therefore do the two products in one launch, with A x in LDS between them.
+// Bound by memory: x, gate, base and out once each (48 KB a token at 4096 + 2048 columns),
+// the adapters in use out of L2; by latency for few tokens. Both kernels therefore do the
+// two products in one launch, with A x in LDS between them.
 //
-// Few tokens (decode): a workgroup per token and part of the columns. Every byte that
-// the token needs is asked for at the start (A rows, B rows, base beside x), so one
-// memory latency stands before the sums; fp32 throughout.
+// Few tokens (decode): a workgroup per token and part of the columns. Every byte that the
+// first sums need is asked for at the start (A and B rows, base beside x), so one memory
+// latency stands before them; x stays in registers, 8 ranks are summed at a time and folded
+// over the lanes two by two; fp32 throughout. 48 tokens of 32 adapters at rank 16: 6.0 us
+// (an empty launch: 3.6).
 //
 // More: a workgroup takes 16 tokens. x, gate and A come in as runs of whole rows, 256
 // values of K at a time, and are laid out in LDS (rows are a power of two apart in
@@ -19,7 +21,10 @@
 // t are added in LDS; then the wavefronts share the columns, out^T = B t^T with t as a
 // pair in the same way, turned in LDS into rows of 64 columns (32 above rank 64, for want
 // of registers) for base and out. The adapters of a tile are taken by kPasses workgroups in
-// turn, each writing its tokens alone; no adapter's values reach another one's tokens, not even its NaN.
+// turn, each writing its tokens alone; no adapter's values reach another one's tokens, not
+// even its NaN. 4096 tokens in runs of 512 at rank 64: 71 us, 205 MB at 2.9 TB/s (a copy:
+// 4.98); the rest is the chain of barriers in a tile's walk along K and its second half,
+// which no other tile's loads fill.
 #include <mutex>
 
 #include "paged.hpp"
@@ -30,7 +35,6 @@ namespace {
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef float float4a __attribute__((ext_vector_type(4), aligned(4)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kWaves = 8;
@@ -464,7 +468,12 @@ int launch_lora_add(const sqa_tensor &base, const sqa_tensor &x, const sqa_tenso
                    scale ? (const float *)scale->data : nullptr, (char *)dst.data, (int)x.ne[0], (int)base.ne[0],
                    (int)a.ne[1], (int)a.ne[2], (int)x.ne[1]};
     const int prof = profile_start("lora_add", s);
-    if (p.M <= 256 && p.K <= 16 * 1024) {
+    // A workgroup per token up to two a CU: with K 4096 and N 2048, 512 tokens of as many
+    // adapters take 10.8 us at rank 16, 27 at 64, 46 at 128, where tiles take 31, 56, 83;
+    // tokens that share adapters by 128 11.5, 25, 43 against 17, 29, 44. 768 tokens that share
+    // take 16, 35, 61 against 18, 30, 44.
+    if (p.M <= 512 && p.K <= 16 * 1024) {
+        // (below 97 tokens parts of the columns fill the other CUs)
         const dim3 grid((unsigned)p.M, p.M <= 32 ? 4 : p.M <= 96 ? 2 : 1);
         if (p.K <= 4096) lora_token_kernel<1><<<grid, dim3(kThreads), 0, s>>>(p);
         else lora_token_kernel<4><<<grid, dim3(kThreads), 0, s>>>(p);

@@ -124,3 +124,14 @@ def test_lora_widths(sqa, dev, M, K, N, r):
     out = torch.empty_like(d["base"])
     sqa.lora_add(**d, out=out)
     close(out, paged_ref.lora(**d))
+
+
+@pytest.mark.parametrize("M", [513, 530, 1037])
+@pytest.mark.parametrize("K,N,r", [(256, 16, 8), (512, 80, 24), (4096, 2048, 64), (768, 32, 128), (256, 48, 40), (1280, 144, 120)])
+def test_lora_tiles(sqa, dev, M, K, N, r):
+    """Tiles whose tokens have one adapter each, or share a few."""
+    for seed, n in ((0, 3), (1, 40)):
+        d = inputs(dev, M + seed, M, K, N, r, n, gate=seed == 1)
+        out = torch.empty_like(d["base"])
+        sqa.lora_add(**d, out=out)
+        close(out, paged_ref.lora(**d))
