@@ -341,8 +341,12 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
     const TableRow table = table_row(p, it.b);
     const int last_group = max(rq.kv - 1, 0) & ~15;
     // 16-key group gi of tile t; one behind the last key stands for the last one
+    // Tiles in order, with a bias the last first: the logits grow towards the token, and
+    // every tile in order would move the maximum.
+    const bool back = OPT && p.bias != 0.0f;
+    auto tile_at = [&](int t) { return back ? n_tiles - 1 - t : t; };
     auto group_key = [&](int t, int gi) {
-        return __builtin_amdgcn_readfirstlane(min(k_begin + t * kPK + 16 * gi, last_group));
+        return __builtin_amdgcn_readfirstlane(min(k_begin + tile_at(t) * kPK + 16 * gi, last_group));
     };
     auto id_of = [&](int t, int gi) { return t < n_tiles ? page_id(table, group_key(t, gi) >> p.lp) : 0; };
     auto there = [&](int id) { return (uint32_t)id < (uint32_t)p.n_pages; };
@@ -404,7 +408,7 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
             // visible and retires the buffers the new ones overwrite
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
             if (t == n_tiles) break;
-            const int kt = k_begin + t * kPK;
+            const int kt = k_begin + tile_at(t) * kPK;
             const bool has_a = there(ida), has_b = there(idb);
             ida = id_of(t + 1, 0);
             idb = id_of(t + 1, 1);
@@ -612,7 +616,7 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
     int e_own = kMaxE;                            // of this wavefront's pair of blocks, up to the tile expanded last
     int4 e_acc = make_int4(kMaxE, kMaxE, kMaxE, kMaxE);  // of O's pairs
     auto scales = [&](int t, int a, int b) {
-        e_own = ex.scales_v(smem, t, k_end - (k_begin + t * kPK), there(a), there(b), e_own);
+        e_own = ex.scales_v(smem, t, k_end - (k_begin + tile_at(t) * kPK), there(a), there(b), e_own);
         if (lane == 0) *reinterpret_cast<int *>(smem + kLdsE + 16 * (t & 1) + 4 * w) = e_own;
     };
     if (n_tiles > 0) {
