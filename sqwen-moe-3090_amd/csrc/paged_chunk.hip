@@ -389,6 +389,8 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
             lim_s[rg] = -INFINITY;
         }
         __builtin_amdgcn_sched_barrier(0);  // the loads stay together
+        // raw rows of the first tile: the value waves expand them while Q is quantized
+        if (n_tiles > 0) asm volatile("s_barrier" ::: "memory");
 #pragma unroll
         for (int rg = 0; rg < kRG; ++rg) qrow[rg].quantize(p.qscale, row_ok[rg], bqh[rg], bql[rg]);
         // K operand of key row 16kg + n, dims 32b + 8g..+7: chunk (4b + g) ^ (n & 7),
@@ -402,7 +404,6 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
         const int p_off = w * (kRG * 2048) + 16 * lane;  // P slots [w][rg][half][lane]
 
         int ida = id_of(0, 0), idb = id_of(0, 1);  // pages of the tile's two groups
-        if (n_tiles > 0) asm volatile("s_barrier" ::: "memory");  // raw rows of the first tile
         for (int t = 0; t <= n_tiles && n_tiles > 0; ++t) {
             // the value waves wait for their DMAs before this barrier, which makes them
             // visible and retires the buffers the new ones overwrite
