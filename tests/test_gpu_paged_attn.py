@@ -285,3 +285,46 @@ def test_many_requests(sqa, orc, dev):
     new[5], new[700] = 60, 33
     b = Batch(orc, 5, new, past, 4, 2, 16)
     close(call(sqa, dev, b), b.ref(orc))
+
+
+def test_more_chunks_than_the_plan_lists(sqa, orc, dev):
+    """1100 requests of 20 tokens and 4 KV heads are 4400 parts of the many-row kernel."""
+    r = np.random.default_rng(6)
+    new, past = [20] * 1100, [int(x) for x in r.integers(0, 40, 1100)]
+    new[3], new[500], past[500] = 0, 150, 300
+    b = Batch(orc, 6, new, past, 4, 4, 16)
+    close(call(sqa, dev, b), b.ref(orc))
+
+
+def test_chunks_among_thousands_of_requests(sqa, orc, dev):
+    r = np.random.default_rng(7)
+    new = [int(x) for x in r.choice([0, 1, 1, 1, 2, 30], 2700)]
+    past = [int(x) for x in r.integers(0, 40, 2700)]
+    b = Batch(orc, 7, new, past, 4, 4, 16)
+    close(call(sqa, dev, b), b.ref(orc))
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [150, 1, 90]])
+def test_two_calls_at_once(sqa, orc, dev, new):
+    """On two streams, each with its own workspace."""
+    pair = [Batch(orc, 40 + i, new, [700 - 300 * i, 2000, 65], gate=i == 1) for i in (0, 1)]
+    made = [(b.args(dev), torch.zeros(b.q.shape, device=dev)) for b in pair]
+    size = sqa.paged_attn_workspace_size(made[0][0][0][0], made[0][0][0][1], made[0][0][0][3], max(new))
+    works = [torch.full((size,), 0xFF, dtype=torch.uint8, device=dev) for _ in pair]
+    streams = [torch.cuda.Stream() for _ in pair]
+    torch.cuda.synchronize()
+    for _ in range(8):
+        for ((a, kw), out), work, s in zip(made, works, streams):
+            with torch.cuda.stream(s):
+                sqa.paged_attn(*a, **kw, out=out, workspace=work)
+    torch.cuda.synchronize()
+    for b, (_, out) in zip(pair, made):
+        close(out.cpu().numpy().astype(np.float64), b.ref(orc))
+
+
+@pytest.mark.parametrize("n,H,Hkv", [(1, 16, 2), (2, 16, 2), (4, 4, 2), (40, 16, 2)])
+def test_bias_over_many_tiles(sqa, orc, dev, n, H, Hkv):
+    """Slopes that leave only the last keys, and slopes that leave all, over whole and cut tiles."""
+    b = Batch(orc, n + H, [n, n, n], [2000, 65, 0], H, Hkv, 64, gate=n == 2)
+    for bias in (1.0, 8.0, 30.0):
+        close(call(sqa, dev, b, max_bias=bias), b.ref(orc, bias=bias))
