@@ -330,8 +330,8 @@ int sqa_paged_plan(const sqa_tensor *n_past, const sqa_tensor *n_new, const sqa_
  * sees enters the result. The results of a call repeat bit for bit.
  * D == 256, H / Hkv <= 16, page, B and W as for the plan. Requests with more than
  * max_q tokens may be left as they were.
- * workspace: sqa_paged_attn_workspace_size bytes; a smaller one (at least
- * sqa_paged_attn_workspace_least) takes fewer splits of the keys.
+ * workspace: sqa_paged_attn_workspace_size bytes. A smaller one takes fewer splits of
+ * the keys, down to one per request and KV head; below that SQA_ERR_WORKSPACE.
  */
 int sqa_paged_attn(const sqa_tensor *q, const sqa_tensor *k, const sqa_tensor *v,
                    const sqa_tensor *table, const sqa_tensor *q_start, const sqa_tensor *kv_len,
@@ -347,14 +347,17 @@ int sqa_supports_paged_attn(const sqa_tensor *q, const sqa_tensor *k, const sqa_
 /*
  * Low-rank adapters of many requests beside a shared projection:
  *   dst[:, m] = base[:, m] + scale[i] * B_i (A_i (x[:, m] * sigmoid(gate[:, m]))),  i = ids[m]
- *   base  F32 [N, M]  the shared projection's output; may be dst itself (no other overlap with dst)
+ *   base  F32 [N, M]  the shared projection's output; may be dst itself (nothing else may
+ *                     overlap dst: not x or gate, nor base in part)
  *   x     F32 [K, M], gate F32 [K, M] or NULL (unit element stride)
  *   a     F16 [K, r, n_adapters], b F16 [r, N, n_adapters]  contiguous, 16-byte aligned
  *   ids   I32 [M]; an id outside [0, n_adapters) is a token without adapter
  *   scale F32 [n_adapters] or NULL (1)
  *   dst   F32 [N, M]
- * Products are exact and sums fp32 where a token's own few rows are summed, and an
- * fp16 hi + lo pair of x and of A x elsewhere (22 bits; |x|, |A x| < 65504).
+ * Up to 512 tokens and K <= 16384: fp32 throughout, any finite size. Otherwise
+ * x * sigmoid(gate) and scale * A x enter as fp16 hi + lo pairs: 22 bits where their size
+ * is 2^-13 or more, an absolute 2^-36 below, both below 65504; products are exact and
+ * sums fp32.
  * K % 256 == 0, N % 16 == 0, r % 8 == 0, r <= 128; base and dst rows 16-byte aligned.
  */
 int sqa_lora_add(const sqa_tensor *base, const sqa_tensor *x, const sqa_tensor *gate, const sqa_tensor *a,
@@ -414,7 +417,8 @@ int sqa_kv_cache_append(sqa_kv_cache *kv, int32_t slot, const sqa_tensor *k_cur,
 int sqa_profile_begin(int32_t max_records);
 int sqa_profile_end(void);
 /* Synchronise and sum the recorded durations of one kernel: "fa_decode",
- * "fa_combine", "fa_prefill", "set_rows_q4_0", "sigmoid_mul". */
+ * "fa_combine", "fa_prefill", "set_rows_q4_0", "sigmoid_mul", "paged_plan",
+ * "paged_decode", "paged_chunk", "paged_merge", "lora_add". */
 int sqa_profile_get(const char *kernel, double *total_ms, int64_t *count);
 
 #ifdef __cplusplus

@@ -153,9 +153,10 @@ __device__ __forceinline__ int tiles_of(const Call &c, int b, int most) {
     return max((r.kv + kTileKeys - 1) / kTileKeys, 1);
 }
 
-// Piece length: of lengths from total / P up to nearly twice that, the shortest whose
-// pieces number at most P, the workgroups that run together; where no length does
-// (as many requests as that) total / P, and the rest follows as others end.
+// Piece length: from total / P up to nearly twice that, the shortest whose pieces number
+// at most P, the workgroups that run together (of up to 64 requests; of more, the shortest
+// of 8 lengths); where no length does (as many requests as that) total / P, and the rest
+// follows as others end.
 __device__ __forceinline__ Piece few_piece(const Call &c, int piece, int most) {
     const int lane = threadIdx.x & 63;
     const bool small = c.B <= 64;
@@ -176,8 +177,18 @@ __device__ __forceinline__ Piece few_piece(const Call &c, int piece, int most) {
     // (at or a little above total / P)
     const int share = (int)ceilf((float)total * __builtin_amdgcn_rcpf((float)P) * 0.999999f);
     const int base = max(max(share, (longest + kMostSplits - 1) / kMostSplits), 1);
+    int len = 0;
+    if (small) {
+        int lo = base, hi = 2 * base;  // the first length that will do, if it is below hi
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (wave_sum(div_ceil(own, mid)) <= P) hi = mid;
+            else lo = mid + 1;
+        }
+        len = lo < 2 * base ? lo : 0;
+    }
     int n[kLengths] = {};
-    for (int b0 = 0; b0 < c.B; b0 += 64) {
+    for (int b0 = 0; b0 < c.B && len == 0; b0 += 64) {
         const int t = tiles(b0);
 #pragma unroll
         for (int j = 0; j < kLengths; ++j) {
@@ -185,7 +196,6 @@ __device__ __forceinline__ Piece few_piece(const Call &c, int piece, int most) {
             n[j] += div_ceil(t, len);
         }
     }
-    int len = 0;
 #pragma unroll
     for (int j = 0; j < kLengths; ++j)
         if (len == 0 && wave_sum(n[j]) <= P) len = (base * (kLengths + j) + kLengths - 1) / kLengths;
@@ -297,6 +307,16 @@ __global__ __launch_bounds__(kThreads, 4) void paged_few_kernel(Call p) {
     auto tile_at = [&](int t) { return back ? n_tiles - 1 - t : t; };
     auto group_key = [&](int t, int g16) {
         return __builtin_amdgcn_readfirstlane(min(k0 + tile_at(t) * kTileKeys + 16 * g16, last_key & ~15));
+    };
+
+    // Of two workgroups on a CU the first one gets ahead (1.30 us a tile against 1.82) and
+    // leaves the CU to the other, at 1.2, for the last quarter of the time. The second one's
+    // wavefronts go first in three tiles of four: 16 requests of 120000 keys 246 -> 243 us,
+    // 12 of 10500 with two tokens 32.2 -> 31.0.
+    const bool second = (int)(blockIdx.x + 8 * (blockIdx.y + gridDim.y * blockIdx.z)) >= p.cus;
+    auto take_turns = [&](int t) {
+        if (((t & 3) == 3) != second) __builtin_amdgcn_s_setprio(1);
+        else __builtin_amdgcn_s_setprio(0);
     };
 
     uint8_t *qs_lds = smem + kOffV + kTensorBytes;  // Q operands (V stages 1-2, free until V(1) is issued)
@@ -439,6 +459,7 @@ __global__ __launch_bounds__(kThreads, 4) void paged_few_kernel(Call p) {
             const int t = TWO ? __builtin_amdgcn_readfirstlane(tt) : tt;
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // K(t) and P(t-1) readable
 
+            take_turns(t);
             // -- fold the last tile's sum into l under the workgroup's common max --
             if (t > 0) {
                 const int pb = (t - 1) & 1;
@@ -736,6 +757,7 @@ __global__ __launch_bounds__(kThreads, 4) void paged_few_kernel(Call p) {
         for (int tt = 0; tt <= n_tiles; ++tt) {
             const int t = TWO ? __builtin_amdgcn_readfirstlane(tt) : tt;  // wave-uniform tile index
             const int c1 = c == 2 ? 0 : c + 1, c2 = c == 0 ? 2 : c - 1;  // (t + 1) mod 3, (t + 2) mod 3
+            take_turns(t);
             wait_interval(t);
             const int id3 = id_of(t + 3);
             if (t + 2 < n_tiles) issue_k(t + 2, c2, id2);
