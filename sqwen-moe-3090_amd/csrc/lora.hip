@@ -242,8 +242,11 @@ struct Form {
     static_assert(kPart <= 2 * kStage && kBytes <= 160 * 1024, "LDS");
 };
 
-// hi = fp16(x) and lo = fp16((x - hi) 2^11)
+// hi = fp16(x) and lo = fp16((x - hi) 2^11). x opaque: where it is a product, the compiler
+// took hi from the fp32 product and the hi that it subtracts from the exact one, and hi + lo
+// was an fp16 ulp of hi off where the two differ.
 __device__ __forceinline__ void split(float x, _Float16 &hi, _Float16 &lo) {
+    asm volatile("" : "+v"(x));
     hi = (_Float16)x;
     lo = (_Float16)((x - (float)hi) * 2048.0f);
 }

@@ -24,10 +24,12 @@
 // block dots on v_mfma_i32_16x16x64_i8 (block-diagonal B operand: 8 rows x 2 blocks),
 // d_k d_q in fp32; softmax base 2 in fp32 with a reference maximum that moves only
 // when a logit passes it by kSlack; A = P d_v 2^E as an fp16 hi + lo pair, B = the
-// nibbles, v_mfma_f32_16x16x32_f16, exact products, fp32 sums; the codes' offset of 8
-// enters by one more MFMA against ones. E follows the largest |d_v| seen. A key that no
-// row sees (behind the last, behind the causal limit, on a page that is not there)
-// contributes exactly 0 whatever its bytes.
+// codes, v_mfma_f32_16x16x32_f16, exact products, fp32 sums. E follows the largest
+// |d_v| seen. A key that no row sees (behind the last, behind the causal limit, on a
+// page that is not there) contributes exactly 0 whatever its bytes.
+// Bound: the issue of its vector, LDS and matrix instructions (two workgroups a CU make
+// 1.2 tiles of 18 KB a us, 5.7 TB/s on the chip) and about 8 us at a launch's start
+// and end: 16 requests of 100000 to 131071 keys 231 us, 4.6 TB/s (a copy: 4.98).
 #include <mutex>
 
 #define SQA_PLAN_CHUNKS
@@ -64,12 +66,14 @@ constexpr int kOffFlag = kOffM + 2 * 4 * 16 * 4;               // [2 tiles][4 wa
 constexpr int kOffL = kOffFlag + 2 * 4 * 4;                    // [4 waves][16 rows] f32
 constexpr int kLdsBytes = kOffL + 4 * 16 * 4;
 constexpr float kSlack = 8.0f;  // log2 of the largest P the lazy rescale admits
-// P is stored as P 2^-kPShift (<= 2^(kSlack - kPShift) = 16) and l summed from the
-// same values; with |d_v 2^E| < 2^11, A = P d_v 2^E stays below 2^15.
-constexpr float kPShift = 4.0f;
+// P is stored as P 2^-kPShift (<= 2^(kSlack - kPShift) = 2^14) and l summed from the
+// same values; with |d_v 2^E| < 2, A = P d_v 2^E stays below 2^15. (The range goes to P:
+// at P 2^-4 its lo part lay so deep in fp16's subnormals that the output was 1.4e-6 off
+// for 4096 keys, now 2e-7.)
+constexpr float kPShift = -6.0f;
 // Largest d_v exponent E of the value wavefronts (d_v enters A as d_v 2^E): V
 // scales below 2^-20 lose low bits of A; 2^E stays two fp16 powers of two.
-constexpr int kMaxDvExp = 28;
+constexpr int kMaxDvExp = 18;
 static_assert(2 * kLdsBytes <= 160 * 1024, "two workgroups per CU");
 static_assert((512 + 6 * 2600 + 8) * 4 <= kLdsBytes && (512 + kMaxRequests + 8) * 4 <= kLdsBytes, "the plan's LDS");
 static_assert(4 * 2 * 64 * 32 <= (kVStages - 1) * kTensorBytes, "Q operands must fit in V stages 1..2");
@@ -693,12 +697,11 @@ __global__ __launch_bounds__(kThreads, 4) void paged_few_kernel(Call p) {
         }
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // Q operands published
         const int dq = wq;  // dims 64dq..64dq+63: blocks 2dq, 2dq+1
-        // B operand from the nibbles: a nibble in the low bits of an fp16 is the
-        // subnormal nib * 2^-24 (low nibble), which one packed multiply by 2^14
-        // makes nib * 2^-10, exact and normal; left in bits 4-7, the high nibble
-        // is nib * 2^-20 and enters as it is.
-        const half8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
-        const half8 kLoToNormal = {16384, 16384, 16384, 16384, 16384, 16384, 16384, 16384};  // 2^14
+        // B operand from the nibbles: in the low bits of an fp16 a nibble is the subnormal
+        // nib 2^-24, in bits 4-7 nib 2^-20; one packed fma makes either (nib - 8) 2^-10, exact
+        // and normal. (The offset as one more MFMA against ones, sum A, cost 243 us instead of
+        // 237 for 16 requests of 120000 keys.)
+        const half8 kLo = (half8)(_Float16)16384.0f, kHi = (half8)(_Float16)1024.0f, kOffset = (half8)(_Float16)-0.0078125f;
         uint8_t *dv_comp = smem + kOffDv + vw * 256;  // [bl][half][g][j] fp16
         const int ra = n & kRowMask;  // P row of this lane's A operand
         // d_v compaction: lane -> block bl, half h, key group gg, pair jj: keys
@@ -720,24 +723,21 @@ __global__ __launch_bounds__(kThreads, 4) void paged_few_kernel(Call p) {
             vsel[bl] = b | (0x0cu << 8) | ((4u + b) << 16) | (0x0cu << 24);
         }
 
-        // acc[2bl] = 2^-10 sum_k A nib_lo, acc[2bl + 1] = 2^-20 sum_k A nib_hi, and
-        // cor[bl] = sum_k A, with A = P d_v of block 2dq + bl, so that
-        // O[row 4g+i][dim 64dq + 32bl + n] = 2^10 acc - 8 cor (2^20 acc for the
-        // high nibble, dim + 16).
-        floatx4 acc[4], cor[2];
+        // acc[2bl] = 2^-10 sum_k A (nib_lo - 8), acc[2bl + 1] the same of the high nibble, with
+        // A = P d_v of block 2dq + bl: 2^10 acc[2bl + hi] = O[row 4g+i][dim 64dq + 32bl + 16hi + n].
+        floatx4 acc[4];
 #pragma unroll
         for (int T = 0; T < 4; ++T) acc[T] = floatx4{0.f, 0.f, 0.f, 0.f};
-        cor[0] = cor[1] = floatx4{0.f, 0.f, 0.f, 0.f};
-        // d_v enters A as d_v 2^E (E per wavefront, only ever lowered): P 2^-4 <= 16
-        // times |d_v 2^E| < 2^11 keeps A below 2^15, and the largest d_v near 2^8
+        // d_v enters A as d_v 2^E (E per wavefront, only ever lowered): P 2^6 <= 2^14
+        // times |d_v 2^E| < 2 keeps A below 2^15, and the largest d_v near 2^-2
         // keeps A clear of fp16 subnormals, whatever the size of V. The partial O
         // is scaled back by 2^-E; l does not carry E.
         int e_dv = kMaxDvExp;
-        uint32_t dv_thr = 0;  // fp16 magnitude bits of 2^(11 - E)
+        uint32_t dv_thr = 0;  // fp16 magnitude bits of 2^(1 - E)
         half2v dv_s1, dv_s2;  // 2^floor(E/2), 2^(E - floor(E/2))
         auto set_dv_scale = [&](int e) {
             e_dv = e;
-            const int x = 11 - e;
+            const int x = 1 - e;
             dv_thr = x >= 16 ? 0x7C00u : (x >= -14 ? (uint32_t)(x + 15) << 10 : 1u << (x + 24));
             const int e1 = e >> 1, e2 = e - e1;
             const uint16_t b1 = (uint16_t)((e1 + 15) << 10), b2 = (uint16_t)((e2 + 15) << 10);
@@ -815,8 +815,8 @@ __global__ __launch_bounds__(kThreads, 4) void paged_few_kernel(Call p) {
                     __builtin_memcpy(&w, &wh, 4);
                     *reinterpret_cast<uint32_t *>(dv_comp + cdst) = w;
                 };
-                // a d_v at or above 2^(11 - E) lowers E so that the largest |d_v| of
-                // the tile lands in [2^8, 2^9); O is rescaled by the exact power of
+                // a d_v at or above 2^(1 - E) lowers E so that the largest |d_v| of
+                // the tile lands in [2^-2, 2^-1); O is rescaled by the exact power of
                 // two and the tile's d_v are stored again. On the split's first tile
                 // O is still zero: E comes straight from the tile's largest |d_v|.
                 const uint32_t mag = max(da & 0x7FFFu, db & 0x7FFFu);
@@ -825,7 +825,7 @@ __global__ __launch_bounds__(kThreads, 4) void paged_few_kernel(Call p) {
                     if (mx != 0) {
                         const int ex = mx >> 10;
                         const int lg = ex ? ex - 15 : (31 - __clz(mx)) - 24;  // floor(log2 max |d_v|)
-                        set_dv_scale(min(8 - lg, kMaxDvExp));
+                        set_dv_scale(min(-2 - lg, kMaxDvExp));
                     }
                     store_scaled();
                 } else {
@@ -834,13 +834,11 @@ __global__ __launch_bounds__(kThreads, 4) void paged_few_kernel(Call p) {
                     const int mx = wave_max((int)mag);
                     const int ex = mx >> 10;
                     const int lg = ex ? ex - 15 : (31 - __clz(mx)) - 24;  // floor(log2 max |d_v|)
-                    const int e_new = 8 - lg;
+                    const int e_new = -2 - lg;
                     if (e_new < e_dv) {
                         const float f = __builtin_amdgcn_ldexpf(1.0f, e_new - e_dv);
 #pragma unroll
                         for (int T = 0; T < 4; ++T) acc[T] *= f;
-                        cor[0] *= f;
-                        cor[1] *= f;
                         set_dv_scale(e_new);
                         store_scaled();
                     }
@@ -868,8 +866,6 @@ __global__ __launch_bounds__(kThreads, 4) void paged_few_kernel(Call p) {
                 const floatx4 f4 = {fac[0], fac[1], fac[2], fac[3]};
 #pragma unroll
                 for (int T = 0; T < 4; ++T) acc[T] *= f4;
-                cor[0] *= f4;
-                cor[1] *= f4;
                 // P of score wavefront w (keys 16w..16w+15: this lane's half-h slots 8g..8g+7
                 // come from wavefront 2h + (g >> 1)) onto the new max
                 float mw[4];
@@ -906,7 +902,7 @@ __global__ __launch_bounds__(kThreads, 4) void paged_few_kernel(Call p) {
             // A = P d_v exactly as Ah + Al in packed fp16: Ph d_v has at most 22
             // significant bits, so its residual after rounding to fp16 (at most 11) is
             // exact in one fma; Pl d_v is 2^-11 of it and rounds once. Every MFMA
-            // product is then exact in fp32, and V's -8 offset comes in as -8 sum A.
+            // product is then exact in fp32.
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 // the slice's V bytes for the 32 keys of this half, two keys per register:
@@ -940,21 +936,17 @@ __global__ __launch_bounds__(kThreads, 4) void paged_few_kernel(Call p) {
                     half8 blo, bhi;
                     __builtin_memcpy(&blo, wlo, 16);
                     __builtin_memcpy(&bhi, whi, 16);
-                    // nib 2^-24 times 2^14: nib 2^-10 exactly, in the normal range (with
-                    // the low nibbles as subnormals 2^-24 deep, the MFMA's sums lost up
-                    // to ~2^-12 of the output at long contexts; the high nibbles' nib
-                    // 2^-20 cost nothing measurable)
-                    blo = blo * kLoToNormal;
+                    // (nib 2^-24) 2^14 - 8 2^-10 and (nib 2^-20) 2^10 - 8 2^-10, exact
+                    blo = __builtin_elementwise_fma(blo, kLo, kOffset);
+                    bhi = __builtin_elementwise_fma(bhi, kHi, kOffset);
                     if (TWO) {
                         const half8 ah = pa[h] * dv8;
                         const half8 ar = __builtin_elementwise_fma(pa[h], dv8, -ah);
                         const half8 al = __builtin_elementwise_fma(pl[h], dv8, ar);
                         acc[2 * bl] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, blo, acc[2 * bl], 0, 0, 0);
                         acc[2 * bl + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bhi, acc[2 * bl + 1], 0, 0, 0);
-                        cor[bl] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, ones, cor[bl], 0, 0, 0);
                         acc[2 * bl] = __builtin_amdgcn_mfma_f32_16x16x32_f16(al, blo, acc[2 * bl], 0, 0, 0);
                         acc[2 * bl + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(al, bhi, acc[2 * bl + 1], 0, 0, 0);
-                        cor[bl] = __builtin_amdgcn_mfma_f32_16x16x32_f16(al, ones, cor[bl], 0, 0, 0);
                     } else {
                         // hi lanes: pl = 0, so a = round(pa d_v); lo lanes: a = pl_lo d_v plus the
                         // exact residual of the hi part, rounded once
@@ -963,7 +955,6 @@ __global__ __launch_bounds__(kThreads, 4) void paged_few_kernel(Call p) {
                         const half8 a = __builtin_elementwise_fma(pa[h], dv8, tr);
                         acc[2 * bl] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, blo, acc[2 * bl], 0, 0, 0);
                         acc[2 * bl + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bhi, acc[2 * bl + 1], 0, 0, 0);
-                        cor[bl] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ones, cor[bl], 0, 0, 0);
                     }
                 }
             }
@@ -971,13 +962,13 @@ __global__ __launch_bounds__(kThreads, 4) void paged_few_kernel(Call p) {
 
         // ---------------- this split's partial O (un-normalised) -----------------
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // pairs the statistics barrier
-        const float o_scale = __builtin_amdgcn_ldexpf(1.0f, -e_dv);
+        const float o_scale = __builtin_amdgcn_ldexpf(1024.0f, -e_dv);
         auto store_row = [&](int row, int i) {
             float *dst = p.acc_d + ((int64_t)slot * p.rows_d + row) * 256 + 64 * dq + n;
 #pragma unroll
             for (int bl = 0; bl < 2; ++bl) {
-                store_through(dst + 32 * bl, fmaf(acc[2 * bl][i], 1024.0f, -8.0f * cor[bl][i]) * o_scale);
-                store_through(dst + 32 * bl + 16, fmaf(acc[2 * bl + 1][i], 1048576.0f, -8.0f * cor[bl][i]) * o_scale);
+                store_through(dst + 32 * bl, acc[2 * bl][i] * o_scale);
+                store_through(dst + 32 * bl + 16, acc[2 * bl + 1][i] * o_scale);
             }
         };
         if (!TWO) {
@@ -995,8 +986,6 @@ __global__ __launch_bounds__(kThreads, 4) void paged_few_kernel(Call p) {
                 };
 #pragma unroll
                 for (int T = 0; T < 4; ++T) fold(acc[T]);
-                fold(cor[0]);
-                fold(cor[1]);
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {

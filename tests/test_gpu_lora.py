@@ -135,3 +135,13 @@ def test_lora_tiles(sqa, dev, M, K, N, r):
         out = torch.empty_like(d["base"])
         sqa.lora_add(**d, out=out)
         close(out, paged_ref.lora(**d))
+
+
+@pytest.mark.parametrize("M", [40, 600])
+def test_lora_gated_values_keep_their_bits(sqa, dev, M):
+    """x sigmoid(gate) and A x at 22 bits or more (2^-22 each, uniform) and sums of some 40
+    roundings of 2^-24: below 1e-6 of the adapter's part, here the whole output."""
+    d = inputs(dev, 9, M, 4096, 512, 64, 2, gate=True, ids=[m % 2 for m in range(M)])
+    d["base"].zero_()
+    got, want = sqa.lora_add(**d).double().cpu(), paged_ref.lora(**d)
+    assert float((got - want).norm() / want.norm()) <= 1e-6

@@ -328,3 +328,12 @@ def test_bias_over_many_tiles(sqa, orc, dev, n, H, Hkv):
     b = Batch(orc, n + H, [n, n, n], [2000, 65, 0], H, Hkv, 64, gate=n == 2)
     for bias in (1.0, 8.0, 30.0):
         close(call(sqa, dev, b, max_bias=bias), b.ref(orc, bias=bias))
+
+
+@pytest.mark.parametrize("new", [[1], [2], [40]])
+def test_weights_keep_their_bits(sqa, orc, dev, new):
+    """Logits within some 3 roundings of 2^-24 of their block terms (about 1 here), P and P d_v at
+    22 bits: below 1e-6 of the output together, where thousands of keys share the weight."""
+    b = Batch(orc, 3, new, [4096], page=64)
+    got, want = call(sqa, dev, b), b.ref(orc)
+    assert np.linalg.norm(got - want) <= 1e-6 * np.linalg.norm(want)
