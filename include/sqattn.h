@@ -297,8 +297,9 @@ int sqa_out_proj(const sqa_tensor *w, const sqa_tensor *x, const sqa_tensor *gat
  * The pages of ended requests join the ring first (in the order of requests and
  * table entries), then pages leave it in the order of requests. A request whose
  * new pages are not all there, whose tokens pass the table's W pages or the T rows
- * is refused: it gets no page, its slots are -1, its length stays. state_out and
- * n_past_out must not overlap state and n_past (the caller swaps them or copies).
+ * is refused: it gets no page, its slots are -1, its length stays. What the plan writes
+ * (outputs, table and ring) must not overlap any other array of the call (the caller
+ * swaps state and n_past with their outputs, or copies).
  * All arrays contiguous but table. B <= 4096, W <= 2^18, W * page < 2^31, T <= 2^29.
  */
 int sqa_paged_plan(const sqa_tensor *n_past, const sqa_tensor *n_new, const sqa_tensor *table,

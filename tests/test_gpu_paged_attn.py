@@ -337,3 +337,9 @@ def test_weights_keep_their_bits(sqa, orc, dev, new):
     b = Batch(orc, 3, new, [4096], page=64)
     got, want = call(sqa, dev, b), b.ref(orc)
     assert np.linalg.norm(got - want) <= 1e-6 * np.linalg.norm(want)
+
+
+def test_more_kv_heads_than_workgroups_run_together(sqa, orc, dev):
+    for new in ([1, 1], [30, 1]):
+        b = Batch(orc, 8, new, [50, 70], 600, 600, 16)
+        close(call(sqa, dev, b), b.ref(orc))

@@ -95,6 +95,21 @@ def test_paged_plan_refusals(sqa):
         assert call(**kw) == status, (kw, sqa.last_error())
 
 
+@pytest.mark.parametrize("a,b", [("kv_len", "n_past"), ("n_past_out", "n_new"), ("q_start", "kv_len"), ("slots", "table"),
+                                 ("ring", "table"), ("pos", "slots"), ("state_out", "ring"), ("table", "n_new")])
+def test_paged_plan_refuses_arrays_that_overlap_what_it_writes(sqa, a, b):
+    size = {"n_past": 4, "n_new": 4, "state": 4, "state_out": 4, "n_past_out": 4, "q_start": 5, "kv_len": 4, "ring": 64,
+            "pos": 80, "slots": 20}
+    names = ["n_past", "n_new", "table", "ring", "state", "state_out", "n_past_out", "q_start", "kv_len", "slots", "pos"]
+    t = {k: T(sqa, 26, [10, 4], [4, 48], 4096 * (i + 1)) if k == "table" else ivec(sqa, size[k], 4096 * (i + 1), 27 if k == "slots" else 26)
+         for i, k in enumerate(names)}
+    end = t[b].data + (3 * 48 + 40 if b == "table" else size[b] * (8 if b == "slots" else 4))
+    t[a].data = end - 8
+    args = [ref(t[k]) for k in names]
+    assert sqa.lib().sqa_paged_plan(*args[:5], 16, *args[5:], None) == 1, sqa.last_error()
+    assert "overlap" in sqa.last_error()
+
+
 def test_lora_refusals(sqa):
     M, K, N, r, n = 6, 512, 64, 16, 3
     f = lambda ne0, ne1, typ=0, nb0=4, pad=0, ptr=4096: T(sqa, typ, [ne0, ne1], [nb0, 4 * (ne0 + pad)], ptr)  # noqa: E731
