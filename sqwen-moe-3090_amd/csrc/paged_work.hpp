@@ -143,10 +143,11 @@ __device__ __forceinline__ void plan_chunks(const Call &c, int *lds) {
         int n_x = 0;
         for (int b = lane >> 4; b < c.B && N > c.cus && N <= kRounds * c.cus; b += 4) {
             const Request r = load(b);
+            if (r.n * c.G <= c.most_d) continue;
             int kt;
             const int T = chunk_tiles(c, r, qb, &kt), S = div_ceil(kt, l_j), past = r.kv - r.n;
             const int most = div_ceil(kt, max(S, 1)), prefix = (min(r.prefix, r.kv) + kChunkKeys - 1) / kChunkKeys;
-            if (T == 0 || most < x) continue;
+            if (most < x) continue;
             // splits that the first query tile sees whole, and the others
             const int whole = min(div_floor(max(past, 0) / kChunkKeys, most), S);
             n_x += whole * T;
@@ -253,23 +254,38 @@ __device__ __forceinline__ void plan_chunks(const Call &c, int *lds) {
     }
     // counting sort of the items by their length, longest first (the order inside a
     // length is left to chance; no result depends on it)
-    constexpr int kBuckets = 64;
+    constexpr int kBuckets = 64, kKept = 2;  // items that a thread makes once (of more, twice)
+    auto bucket_of = [&](int own) {
+        return kBuckets - 1 - min((int)((float)own * (float)kBuckets / (float)(len + 1)), kBuckets - 1);
+    };
     if (tid < kBuckets) sums[tid] = 0;
+    Item it[kKept];
+    int bucket[kKept];
+#pragma unroll
+    for (int u = 0; u < kKept; ++u)
+        if (tid + 512 * u < total) {
+            it[u] = item_of(tid + 512 * u, &own);
+            bucket[u] = bucket_of(own);
+        }
     __syncthreads();
-    for (int pass = 0; pass < 2; ++pass) {
-        for (int id = tid; id < total; id += 512) {
-            const Item it = item_of(id, &own);
-            const int bucket = kBuckets - 1 - min((int)((float)own * (float)kBuckets / (float)(len + 1)), kBuckets - 1);
-            const int at = atomicAdd(&sums[bucket], 1);
-            if (pass) list[at] = it;
-        }
-        __syncthreads();
-        if (pass == 0) {
-            const int k = sums[lane], e = wave_scan(k) - k;  // every wavefront for itself
-            __syncthreads();
-            if (wave == 0) sums[lane] = e;
-            __syncthreads();
-        }
+#pragma unroll
+    for (int u = 0; u < kKept; ++u)
+        if (tid + 512 * u < total) atomicAdd(&sums[bucket[u]], 1);
+    for (int id = tid + 512 * kKept; id < total; id += 512) {
+        (void)item_of(id, &own);
+        atomicAdd(&sums[bucket_of(own)], 1);
+    }
+    __syncthreads();
+    const int k = sums[lane], at = wave_scan(k) - k;  // every wavefront for itself
+    __syncthreads();
+    if (wave == 0) sums[lane] = at;
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kKept; ++u)
+        if (tid + 512 * u < total) list[atomicAdd(&sums[bucket[u]], 1)] = it[u];
+    for (int id = tid + 512 * kKept; id < total; id += 512) {
+        const Item more = item_of(id, &own);
+        list[atomicAdd(&sums[bucket_of(own)], 1)] = more;
     }
 }
 #endif
