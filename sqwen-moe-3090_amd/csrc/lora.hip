@@ -11,8 +11,8 @@
 // over the lanes two by two; fp32 throughout. 48 tokens of 32 adapters at rank 16: 6.0 us
 // (an empty launch: 3.6).
 //
-// More: a workgroup takes 16 tokens. x, gate and A come in as runs of whole rows, 256
-// values of K at a time, and are laid out in LDS (rows are a power of two apart in
+// More: a workgroup takes 16 tokens. x, gate and A come in as runs of whole rows, 128
+// values of K at a time (256 up to rank 16), and are laid out in LDS (rows are a power of two apart in
 // memory: loads in the shape of MFMA operands, 16 rows of 64 bytes, fell into one set of
 // L1 and took 137 cycles each, 100 us for 4096 tokens at rank 64). The 8 wavefronts share
 // a chunk's steps of K: t^T = A x^T on v_mfma_f32_16x16x32_f16, A as it is, x as an fp16
@@ -22,9 +22,8 @@
 // pair in the same way, turned in LDS into rows of 64 columns (32 above rank 64, for want
 // of registers) for base and out. The adapters of a tile are taken by kPasses workgroups in
 // turn, each writing its tokens alone; no adapter's values reach another one's tokens, not
-// even its NaN. 4096 tokens in runs of 512 at rank 64: 71 us, 205 MB at 2.9 TB/s (a copy:
-// 4.98); the rest is the chain of barriers in a tile's walk along K and its second half,
-// which no other tile's loads fill.
+// even its NaN. 4096 tokens in runs of 512: rank 16 45 us, 4.5 TB/s (a copy: 4.98), rank 64
+// 60 (67 from call to call), where A and B out of L2 are as many bytes as x and gate.
 #include <mutex>
 
 #include "paged.hpp"
@@ -229,7 +228,8 @@ constexpr int kPasses = 4;  // workgroups that share a tile's adapters
 template <int RT>
 struct Form {
     static constexpr int kR = 16 * RT;
-    static constexpr int kChunk = RT == 8 ? 128 : 256;  // values of K between two barriers
+    // values of K between two barriers (256 at rank 64: 72 us against 67.5 for 4096 tokens)
+    static constexpr int kChunk = RT == 1 ? 256 : 128;
     static constexpr int kStepWaves = kChunk / 32, kRankWaves = kWaves / kStepWaves;  // of a chunk: steps of 32, groups of ranks
     static constexpr int kTiles = RT / kRankWaves;      // rank tiles of a wavefront
     static constexpr int kRow = kChunk * 2 + 16;        // bytes of a staged row (16 more: its rows on other banks)
