@@ -471,10 +471,10 @@ int launch_lora_add(const sqa_tensor &base, const sqa_tensor &x, const sqa_tenso
                    scale ? (const float *)scale->data : nullptr, (char *)dst.data, (int)x.ne[0], (int)base.ne[0],
                    (int)a.ne[1], (int)a.ne[2], (int)x.ne[1]};
     const int prof = profile_start("lora_add", s);
-    // A workgroup per token up to two a CU: with K 4096 and N 2048, 512 tokens of as many
-    // adapters take 10.8 us at rank 16, 27 at 64, 46 at 128, where tiles take 31, 56, 83;
-    // tokens that share adapters by 128 11.5, 25, 43 against 17, 29, 44. 768 tokens that share
-    // take 16, 35, 61 against 18, 30, 44.
+    // A workgroup per token up to two a CU: with K 4096 and N 2048, 512 tokens that change
+    // between 8 adapters take 11 us at rank 16, 27 at 64, 49 at 128, where tiles take 35, 53,
+    // 85; that share them by 128 11, 27, 45 against 18, 28, 43. 768 that share take 16, 35, 61
+    // against 19, 29, 43.
     if (p.M <= 512 && p.K <= 16 * 1024) {
         // (below 97 tokens parts of the columns fill the other CUs)
         const dim3 grid((unsigned)p.M, p.M <= 32 ? 4 : p.M <= 96 ? 2 : 1);
