@@ -156,6 +156,7 @@ int sqa_paged_plan(const sqa_tensor *n_past, const sqa_tensor *n_new, const sqa_
         !dense1(state, SQA_TYPE_I32, 4, 4) || !dense1(state_out, SQA_TYPE_I32, 4, 4) || !dense1(slots, SQA_TYPE_I64, T, 8) ||
         !dense1(pos, SQA_TYPE_I32, 4 * T, 4))
         return set_error(SQA_ERR_INVALID, "%s: arrays must be contiguous, I32 (slots I64), of B, B + 1, 4, T and 4 T entries", what);
+    if (B > 1 && table->nb[1] < (uint64_t)(4 * W)) return set_error(SQA_ERR_INVALID, "%s: table rows overlap", what);
     // every workgroup reads the inputs while others write
     const sqa_tensor *all[] = {state_out, n_past_out, q_start, kv_len, slots, pos, table, ring, n_past, n_new, state};
     for (int i = 0; i < 8; ++i)

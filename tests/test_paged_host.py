@@ -91,6 +91,7 @@ def test_paged_plan_refusals(sqa):
         (1, {"n_past": T(sqa, 26, [B], [8])}), (1, {"n_past": ivec(sqa, B, 0)}), (1, {"kv_len": ivec(sqa, B, 4098)}),
         (1, {"state_out": ivec(sqa, 4, good["state"].data + 8)}), (1, {"n_past_out": ivec(sqa, B, good["n_past"].data)}),
         (2, {"table": T(sqa, 26, [1 << 18, B], [4, 4 << 18]), "page": 1 << 14}),
+        (1, {"table": T(sqa, 26, [W, B], [4, 0], 1 << 20)}), (1, {"table": T(sqa, 26, [W, B], [4, W * 4 - 4], 1 << 20)}),
     ]:
         assert call(**kw) == status, (kw, sqa.last_error())
 
