@@ -145,16 +145,14 @@ __device__ __forceinline__ float exp2_or_zero(float a, float b) {  // 2^(a-b), 0
 // at piece `first`. b < 0: no such piece.
 struct Piece {
     int b, split, n, first, t0, t1;
+    Request rq;
 };
 
 constexpr int kLengths = 8;
 
-// Tiles of a request; 0: none of this kernel's.
-__device__ __forceinline__ int tiles_of(const Call &c, int b, int most) {
-    if (b >= c.B) return 0;
-    const Request r = request(c, b);
-    if (r.n == 0 || r.n * c.G > most) return 0;
-    return max((r.kv + kTileKeys - 1) / kTileKeys, 1);
+// Tiles of request b, r; 0: none of this kernel's.
+__device__ __forceinline__ int tiles_of(const Call &c, int b, const Request &r, int most) {
+    return b >= c.B || r.n == 0 || r.n * c.G > most ? 0 : max((r.kv + kTileKeys - 1) / kTileKeys, 1);
 }
 
 // Piece length: from total / P up to nearly twice that, the shortest whose pieces number
@@ -164,8 +162,11 @@ __device__ __forceinline__ int tiles_of(const Call &c, int b, int most) {
 __device__ __forceinline__ Piece few_piece(const Call &c, int piece, int most) {
     const int lane = threadIdx.x & 63;
     const bool small = c.B <= 64;
-    const int own = tiles_of(c, lane, most);  // small batches: read once
-    auto tiles = [&](int b0) { return small ? own : tiles_of(c, b0 + lane, most); };
+    const Request mine = request(c, min(lane, c.B - 1));  // small batches: read once
+    const int own = tiles_of(c, lane, mine, most);
+    auto tiles = [&](int b0) {
+        return small ? own : tiles_of(c, b0 + lane, request(c, min(b0 + lane, c.B - 1)), most);
+    };
     int total = 0, longest = 0, active = 0;
     for (int b0 = 0; b0 < c.B; b0 += 64) {
         const int t = tiles(b0);
@@ -204,7 +205,7 @@ __device__ __forceinline__ Piece few_piece(const Call &c, int piece, int most) {
     for (int j = 0; j < kLengths; ++j)
         if (len == 0 && wave_sum(n[j]) <= P) len = (base * (kLengths + j) + kLengths - 1) / kLengths;
     if (len == 0) len = wave_sum(n[0]) <= c.room ? base : 1 << 25;  // 2^25 tiles: every request whole
-    Piece pc{-1, 0, 1, 0, 0, 0};
+    Piece pc{-1, 0, 1, 0, 0, 0, {}};
     int first = 0;
     for (int b0 = 0; b0 < c.B && first <= piece; b0 += 64) {
         const int t = tiles(b0);
@@ -221,11 +222,16 @@ __device__ __forceinline__ Piece few_piece(const Call &c, int piece, int most) {
             const int q = div_floor(tiles, pc.n), rest = tiles - q * pc.n;  // the first `rest` splits are one longer
             pc.t0 = pc.split * q + min(pc.split, rest);
             pc.t1 = pc.t0 + q + (pc.split < rest);
+            const int *from[5] = {&mine.q0, &mine.n, &mine.kv, &mine.pos0, &mine.prefix};
+            int *to[5] = {&pc.rq.q0, &pc.rq.n, &pc.rq.kv, &pc.rq.pos0, &pc.rq.prefix};
+#pragma unroll
+            for (int i = 0; i < 5; ++i) *to[i] = __builtin_amdgcn_readlane(*from[i], l);
         }
         first = __builtin_amdgcn_readlane(upto, 63);
     }
     // (divisions run on the vector unit: back into scalar registers)
     for (int *x : {&pc.b, &pc.split, &pc.n, &pc.first, &pc.t0, &pc.t1}) *x = __builtin_amdgcn_readfirstlane(*x);
+    if (!small && pc.b >= 0) pc.rq = uniform_request(c, pc.b);
     return pc;
 }
 
@@ -293,7 +299,7 @@ __global__ __launch_bounds__(kThreads, 4) void paged_few_kernel(Call p) {
     const Piece pc = few_piece(p, (int)(8 * blockIdx.z + blockIdx.x), p.most_d);
     if (!PLAN && blockIdx.x + blockIdx.y + blockIdx.z == 0) skip_large(p);
     if (pc.b < 0) return;
-    const Request rq = uniform_request(p, pc.b);
+    const Request rq = pc.rq;
     const int rows = rq.n * p.G;
     const int slot = (pc.first + pc.split) * p.Hkv + kvh;
     if (pc.split == 0 && kvh == 0 && tid < rq.n)
