@@ -12,15 +12,6 @@ bool dense1(const sqa_tensor *t, int type, int64_t n, int64_t esize) {
            (n <= 1 || t->nb[0] == (uint64_t)esize) && (n == 0 || (t->data && (uintptr_t)t->data % esize == 0));
 }
 
-// Of contiguous arrays, or a table (its rows with what lies between them).
-bool overlap(const sqa_tensor *a, const sqa_tensor *b) {
-    auto bytes = [](const sqa_tensor *t) {
-        return (uint64_t)t->ne[0] * (t->type == SQA_TYPE_I64 ? 8 : 4) + (uint64_t)(t->ne[1] - 1) * t->nb[1];
-    };
-    const uintptr_t a0 = (uintptr_t)a->data, b0 = (uintptr_t)b->data;
-    return bytes(a) && bytes(b) && a0 < b0 + bytes(b) && b0 < a0 + bytes(a);
-}
-
 bool power_of_two(int64_t x) { return x > 0 && (x & (x - 1)) == 0; }
 
 int check_table(const sqa_tensor *t, const char *what) {
@@ -157,12 +148,20 @@ int sqa_paged_plan(const sqa_tensor *n_past, const sqa_tensor *n_new, const sqa_
         !dense1(pos, SQA_TYPE_I32, 4 * T, 4))
         return set_error(SQA_ERR_INVALID, "%s: arrays must be contiguous, I32 (slots I64), of B, B + 1, 4, T and 4 T entries", what);
     if (B > 1 && table->nb[1] < (uint64_t)(4 * W)) return set_error(SQA_ERR_INVALID, "%s: table rows overlap", what);
-    // every workgroup reads the inputs while others write
+    // Every workgroup reads the inputs while others write. (A table's rows with what lies
+    // between them; what is written stands first.)
     const sqa_tensor *all[] = {state_out, n_past_out, q_start, kv_len, slots, pos, table, ring, n_past, n_new, state};
+    uintptr_t from[11], to[11];
+    for (int i = 0; i < 11; ++i) {
+        const uint64_t bytes = (uint64_t)all[i]->ne[0] * (i == 4 ? 8 : 4) + (i == 6 ? (uint64_t)(B - 1) * table->nb[1] : 0);
+        from[i] = (uintptr_t)all[i]->data;
+        to[i] = from[i] + bytes;
+    }
+    bool clash = false;
     for (int i = 0; i < 8; ++i)
         for (int j = i + 1; j < 11; ++j)
-            if (overlap(all[i], all[j]))
-                return set_error(SQA_ERR_INVALID, "%s: what the plan writes must not overlap its other arrays", what);
+            clash |= (from[i] < to[j]) & (from[j] < to[i]) & (from[i] < to[i]) & (from[j] < to[j]);
+    if (clash) return set_error(SQA_ERR_INVALID, "%s: what the plan writes must not overlap its other arrays", what);
     const PlanArgs a{(const int32_t *)n_past->data, (const int32_t *)n_new->data, (int32_t *)table->data,
                      (int64_t)(table->nb[1] / 4), (int32_t *)ring->data, (const int32_t *)state->data,
                      (int32_t *)state_out->data, (int32_t *)n_past_out->data, (int32_t *)q_start->data,
