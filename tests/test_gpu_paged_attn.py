@@ -343,3 +343,25 @@ def test_more_kv_heads_than_workgroups_run_together(sqa, orc, dev):
     for new in ([1, 1], [30, 1]):
         b = Batch(orc, 8, new, [50, 70], 600, 600, 16)
         close(call(sqa, dev, b), b.ref(orc))
+
+
+@pytest.mark.parametrize("new", [[1, 1], [2, 2, 1], [4, 60, 1]])
+@pytest.mark.parametrize("opt", [{}, {"softcap": 20.0, "max_bias": 8.0}])
+def test_a_row_that_is_not_finite_stays_alone(sqa, orc, dev, new, opt):
+    b = Batch(orc, 12, new, [300, 90, 40][:len(new)], page=32)
+    want = b.ref(orc, cap=opt.get("softcap", 0.0), bias=opt.get("max_bias", 0.0))
+    bad = [(0, 3, np.nan), (1, 9, np.inf), (b.q_start[-1] - 1, 15, -np.inf)]
+    for t, h, x in bad:
+        b.q[t, h, 7] = x
+    got = call(sqa, dev, b, **opt)
+    ok = np.ones(want.shape[:2], dtype=bool)
+    for t, h, _ in bad:
+        ok[t, h] = False
+    close(got[ok], want[ok])
+
+
+@pytest.mark.parametrize("new", [[1, 2], [40, 1]])
+def test_rows_before_and_behind_the_requests_stay(sqa, orc, dev, new):
+    b = Batch(orc, 13, new, [100, 30], pad=8)
+    b.q_start = [t + 5 for t in b.q_start]
+    close(call(sqa, dev, b, fill=7.0), b.ref(orc, fill=7.0))
