@@ -156,16 +156,24 @@ __device__ __forceinline__ int tiles_of(const Call &c, int b, const Request &r, 
 }
 
 // Piece length: from total / P up to nearly twice that, the shortest whose pieces number
-// at most P, the workgroups that run together (of up to 64 requests; of more, the shortest
-// of 8 lengths); where no length does (as many requests as that) total / P, and the rest
+// at most P, the workgroups that run together (of up to 256 requests, which a wavefront
+// holds; of more, the shortest of 8 lengths); where no length does (as many requests as that) total / P, and the rest
 // follows as others end.
 __device__ __forceinline__ Piece few_piece(const Call &c, int piece, int most) {
     const int lane = threadIdx.x & 63;
-    const bool small = c.B <= 64;
-    const Request mine = request(c, min(lane, c.B - 1));  // small batches: read once
-    const int own = tiles_of(c, lane, mine, most);
+    constexpr int kHeld = 4;
+    const bool held = c.B <= 64 * kHeld;
+    const Request mine = request(c, min(lane, c.B - 1));
+    int own[kHeld] = {tiles_of(c, lane, mine, most)};
+#pragma unroll
+    for (int i = 1; i < kHeld; ++i)
+        if (held && 64 * i < c.B) own[i] = tiles_of(c, 64 * i + lane, request(c, min(64 * i + lane, c.B - 1)), most);
     auto tiles = [&](int b0) {
-        return small ? own : tiles_of(c, b0 + lane, request(c, min(b0 + lane, c.B - 1)), most);
+        if (!held) return tiles_of(c, b0 + lane, request(c, min(b0 + lane, c.B - 1)), most);
+        int t = own[0];
+#pragma unroll
+        for (int i = 1; i < kHeld; ++i) t = b0 == 64 * i ? own[i] : t;
+        return t;
     };
     int total = 0, longest = 0, active = 0;
     for (int b0 = 0; b0 < c.B; b0 += 64) {
@@ -183,11 +191,15 @@ __device__ __forceinline__ Piece few_piece(const Call &c, int piece, int most) {
     const int share = (int)ceilf((float)total * __builtin_amdgcn_rcpf((float)P) * 0.999999f);
     const int base = max(max(share, (longest + kMostSplits - 1) / kMostSplits), 1);
     int len = 0;
-    if (small) {
+    if (held) {
         int lo = base, hi = 2 * base;  // the first length that will do, if it is below hi
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
-            if (wave_sum(div_ceil(own, mid)) <= P) hi = mid;
+            int k = div_ceil(own[0], mid);
+#pragma unroll
+            for (int i = 1; i < kHeld; ++i)
+                if (64 * i < c.B) k += div_ceil(own[i], mid);
+            if (wave_sum(k) <= P) hi = mid;
             else lo = mid + 1;
         }
         len = lo < 2 * base ? lo : 0;
@@ -231,7 +243,7 @@ __device__ __forceinline__ Piece few_piece(const Call &c, int piece, int most) {
     }
     // (divisions run on the vector unit: back into scalar registers)
     for (int *x : {&pc.b, &pc.split, &pc.n, &pc.first, &pc.t0, &pc.t1}) *x = __builtin_amdgcn_readfirstlane(*x);
-    if (!small && pc.b >= 0) pc.rq = uniform_request(c, pc.b);
+    if (pc.b >= 64) pc.rq = uniform_request(c, pc.b);
     return pc;
 }
 
