@@ -74,6 +74,7 @@ constexpr float kPShift = -6.0f;
 // Largest d_v exponent E of the value wavefronts (d_v enters A as d_v 2^E): V
 // scales below 2^-20 lose low bits of A; 2^E stays two fp16 powers of two.
 constexpr int kMaxDvExp = 18;
+static_assert(kMaxRequests * 4 <= kLdsBytes, "tiles of every request");
 static_assert(2 * kLdsBytes <= 160 * 1024, "two workgroups per CU");
 static_assert((512 + 6 * 2600 + 8) * 4 <= kLdsBytes && (512 + kMaxRequests + 8) * 4 <= kLdsBytes, "the plan's LDS");
 static_assert(4 * 2 * 64 * 32 <= (kVStages - 1) * kTensorBytes, "Q operands must fit in V stages 1..2");
@@ -156,25 +157,21 @@ __device__ __forceinline__ int tiles_of(const Call &c, int b, const Request &r, 
 }
 
 // Piece length: from total / P up to nearly twice that, the shortest whose pieces number
-// at most P, the workgroups that run together (of up to 256 requests, which a wavefront
-// holds; of more, the shortest of 8 lengths); where no length does (as many requests as that) total / P, and the rest
-// follows as others end.
-__device__ __forceinline__ Piece few_piece(const Call &c, int piece, int most) {
+// at most P, the workgroups that run together (of up to 256 requests; of more, the shortest
+// of 8 lengths); where no length does (as many requests as that) total / P, and the rest
+// follows as others end. Up to 64 requests are in a wavefront's lanes, more in LDS (read
+// again from memory for each of the sums, 1000 requests of up to 500 keys took 181 us
+// instead of 140; 16 a lane, the code for it cost every call 1.3 us).
+__device__ __forceinline__ Piece few_piece(const Call &c, int *lds, int piece, int most) {
     const int lane = threadIdx.x & 63;
-    constexpr int kHeld = 4;
-    const bool held = c.B <= 64 * kHeld;
+    const bool small = c.B <= 64;
     const Request mine = request(c, min(lane, c.B - 1));
-    int own[kHeld] = {tiles_of(c, lane, mine, most)};
-#pragma unroll
-    for (int i = 1; i < kHeld; ++i)
-        if (held && 64 * i < c.B) own[i] = tiles_of(c, 64 * i + lane, request(c, min(64 * i + lane, c.B - 1)), most);
-    auto tiles = [&](int b0) {
-        if (!held) return tiles_of(c, b0 + lane, request(c, min(b0 + lane, c.B - 1)), most);
-        int t = own[0];
-#pragma unroll
-        for (int i = 1; i < kHeld; ++i) t = b0 == 64 * i ? own[i] : t;
-        return t;
-    };
+    const int own = tiles_of(c, lane, mine, most);
+    if (!small) {
+        for (int b = threadIdx.x; b < c.B; b += kThreads) lds[b] = tiles_of(c, b, request(c, b), most);
+        __syncthreads();
+    }
+    auto tiles = [&](int b0) { return small ? own : b0 + lane < c.B ? lds[b0 + lane] : 0; };
     int total = 0, longest = 0, active = 0;
     for (int b0 = 0; b0 < c.B; b0 += 64) {
         const int t = tiles(b0);
@@ -191,14 +188,12 @@ __device__ __forceinline__ Piece few_piece(const Call &c, int piece, int most) {
     const int share = (int)ceilf((float)total * __builtin_amdgcn_rcpf((float)P) * 0.999999f);
     const int base = max(max(share, (longest + kMostSplits - 1) / kMostSplits), 1);
     int len = 0;
-    if (held) {
+    if (c.B <= 256) {
         int lo = base, hi = 2 * base;  // the first length that will do, if it is below hi
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
-            int k = div_ceil(own[0], mid);
-#pragma unroll
-            for (int i = 1; i < kHeld; ++i)
-                if (64 * i < c.B) k += div_ceil(own[i], mid);
+            int k = 0;
+            for (int b0 = 0; b0 < c.B; b0 += 64) k += div_ceil(tiles(b0), mid);
             if (wave_sum(k) <= P) hi = mid;
             else lo = mid + 1;
         }
@@ -244,6 +239,7 @@ __device__ __forceinline__ Piece few_piece(const Call &c, int piece, int most) {
     // (divisions run on the vector unit: back into scalar registers)
     for (int *x : {&pc.b, &pc.split, &pc.n, &pc.first, &pc.t0, &pc.t1}) *x = __builtin_amdgcn_readfirstlane(*x);
     if (pc.b >= 64) pc.rq = uniform_request(c, pc.b);
+    if (!small) __syncthreads();  // lds is free again
     return pc;
 }
 
@@ -308,7 +304,7 @@ __global__ __launch_bounds__(kThreads, 4) void paged_few_kernel(Call p) {
     // Workgroups go round-robin to the 8 XCDs, x (of 8) first, then the KV heads (y), then
     // z: the heads of piece 8z + x share an XCD (and its L2).
     const int kvh = (int)blockIdx.y;
-    const Piece pc = few_piece(p, (int)(8 * blockIdx.z + blockIdx.x), p.most_d);
+    const Piece pc = few_piece(p, reinterpret_cast<int *>(smem), (int)(8 * blockIdx.z + blockIdx.x), p.most_d);
     if (!PLAN && blockIdx.x + blockIdx.y + blockIdx.z == 0) skip_large(p);
     if (pc.b < 0) return;
     const Request rq = pc.rq;
