@@ -528,13 +528,17 @@ def paged_plan(state, ring, table, n_past, n_new, page, slots, pos=None, state_o
     (n_pages,); table: int32 (B, W); n_past, n_new: int32 (B,); slots: int64 (T,);
     pos: int32 (4 * T,). A request that finds too few pages, too little room in its
     table row or in slots is refused whole: state_out[2] counts them."""
-    def new(t, n):
-        return t if t is not None else torch.empty(n, dtype=torch.int32, device=slots.device)
+    if state_out is None or n_past_out is None or q_start is None or kv_len is None or pos is None:
+        def new(t, n):
+            return t if t is not None else torch.empty(n, dtype=torch.int32, device=slots.device)
 
-    B, T = table.shape[0], slots.shape[0]
-    step = PagedStep(new(state_out, 4), new(n_past_out, B), new(q_start, B + 1), new(kv_len, B), slots, new(pos, 4 * T))
+        B, T = table.shape[0], slots.shape[0]
+        state_out, n_past_out, q_start = new(state_out, 4), new(n_past_out, B), new(q_start, B + 1)
+        kv_len, pos = new(kv_len, B), new(pos, 4 * T)
+    step = PagedStep(state_out, n_past_out, q_start, kv_len, slots, pos)
     if stream is None:
-        rc = (_host or _load_host()).plan(state, ring, table, n_past, n_new, page, *step)
+        rc = (_host or _load_host()).plan(state, ring, table, n_past, n_new, page, state_out, n_past_out, q_start, kv_len,
+                                          slots, pos)
         if rc is not None:
             if rc:
                 _check(rc)
