@@ -304,9 +304,12 @@ __global__ __launch_bounds__(kThreads, 4) void paged_few_kernel(Call p) {
     // Workgroups go round-robin to the 8 XCDs, x (of 8) first, then the KV heads (y), then
     // z: the heads of piece 8z + x share an XCD (and its L2).
     const int kvh = (int)blockIdx.y;
-    const Piece pc = few_piece(p, reinterpret_cast<int *>(smem), (int)(8 * blockIdx.z + blockIdx.x), p.most_d);
+    const int piece = (int)(8 * blockIdx.z + blockIdx.x);
+    const Piece pc = few_piece(p, reinterpret_cast<int *>(smem), piece, p.most_d);
     if (!PLAN && blockIdx.x + blockIdx.y + blockIdx.z == 0) skip_large(p);
-    if (pc.b < 0) return;
+    // The workspace has slots for `room` pieces. Requests whose ranges of q_start overlap may be
+    // more than there are tokens, which room counts on, and the grid is a multiple of 8 of them.
+    if (pc.b < 0 || piece >= p.room) return;
     const Request rq = pc.rq;
     const int rows = rq.n * p.G;
     const int slot = (pc.first + pc.split) * p.Hkv + kvh;
