@@ -25,9 +25,9 @@ __device__ __forceinline__ Row row_of(const Call &c, int t, int h) {
     const int4 w = c.where[t];
     if (t < c.q_start[0] || t >= c.q_start[c.B]) return r;  // of no request: w was not written
     const int form = w.w & 3, step = w.w >> 2, kvh = group_of(c, h), row = w.z + h - kvh * c.G;
-    const int heads = form == kFew ? 1 : w.y * step, rows = form == kFew ? c.rows_d : c.rows_c;
-    const int64_t first = w.x + (int64_t)kvh * heads;
-    // (arrays that are no plan's may leave an entry of an earlier call here)
+    const int rows = form == kFew ? c.rows_d : c.rows_c;
+    const int64_t heads = form == kFew ? 1 : (int64_t)w.y * step, first = w.x + kvh * heads;
+    // (arrays that are no plan's may leave here what the workspace held: any four numbers)
     if (form == kDone || w.x < 0 || step < 1 || w.y < 1 || w.y > 256 || row < 0 || row >= rows ||
         first + (int64_t)(w.y - 1) * step >= (form == kFew ? c.slots_d : c.slots_c))
         return r;
