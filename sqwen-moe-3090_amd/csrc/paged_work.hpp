@@ -91,11 +91,12 @@ __device__ __forceinline__ void plan_chunks(const Call &c, int *lds) {
         return kept ? known[b] : request(c, b);
     };
 
-    int wgs = 0, longest = 0;
+    int wgs = 0, longest = 0, tokens = 0;
     float work = 0.0f;  // key tiles that all query tiles see together
     for (int b = b0; b < b1; ++b) {
         const Request r = request(c, b);
         if (kept) known[b] = r;
+        tokens = min(tokens + r.n, c.n_tok + 1);
         int kt;
         const int T = chunk_tiles(c, r, qb, &kt);
         // query tile i of T ends (T - 1 - i) * qb keys before the last one
@@ -108,11 +109,15 @@ __device__ __forceinline__ void plan_chunks(const Call &c, int *lds) {
     longest = wave_max(longest);
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) work += __shfl_xor(work, o);
-    if (lane == 0) sums[wave] = wgs, sums[8 + wave] = longest, sums[16 + wave] = __float_as_int(work);
+    tokens = min(wave_sum(tokens), c.n_tok + 1);  // (64 (2^24 + 1) at most)
+    if (lane == 0) sums[wave] = wgs, sums[8 + wave] = longest, sums[16 + wave] = __float_as_int(work), sums[24 + wave] = tokens;
     __syncthreads();
-    wgs = longest = 0, work = 0.0f;
-    for (int w = 0; w < 8; ++w) wgs += sums[w], longest = max(longest, sums[8 + w]), work += __int_as_float(sums[16 + w]);
-    if (wgs == 0) {
+    wgs = longest = tokens = 0, work = 0.0f;
+    for (int w = 0; w < 8; ++w)
+        wgs += sums[w], longest = max(longest, sums[8 + w]), work += __int_as_float(sums[16 + w]), tokens += sums[24 + w];
+    // More tokens than there are: ranges of q_start overlap. The sums of tiles below, and the
+    // workgroups and slots that the host provided, are for disjoint ones.
+    if (wgs == 0 || tokens > c.n_tok) {
         if (tid == 0) *out = Work{1, 0, 0, 0};
         return;
     }

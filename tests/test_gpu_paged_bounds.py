@@ -48,3 +48,15 @@ def test_tokens_that_no_piece_writes(sqa, dev, H, Hkv, held):
     q_start = [b & 1 for b in range(600)] + [3]
     out = call(sqa, dev, 3, H, Hkv, q_start, [9] * 600, 2, held=held)
     assert (out[2] == 7).all()
+
+
+@pytest.mark.parametrize("n_tok,H,Hkv,B", [(40, 4, 4, 600), (129, 16, 2, 3000), (1 << 24, 1, 1, 4096)])
+def test_chunks_whose_ranges_overlap(sqa, dev, n_tok, H, Hkv, B):
+    """Half of the requests have all the rows: at 2^24 tokens their query tiles and splits pass 32 bits."""
+    call(sqa, dev, n_tok, H, Hkv, [n_tok * (b & 1) for b in range(B + 1)], [3000] * B, n_tok, page=1024)
+
+
+def test_chunks_whose_ranges_cross(sqa, dev):
+    """q_start that does not ascend, of ranges that together have no more tokens than there are."""
+    out = call(sqa, dev, 200, 16, 2, [0, 90, 60, 100, 100, 99, 110], [500, 7, 40, 0, 9, 60], 90)
+    assert (out[110:] == 7).all() and not (out[:60] == 7).any()
