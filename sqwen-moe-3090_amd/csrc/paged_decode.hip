@@ -186,7 +186,8 @@ __device__ __forceinline__ Piece few_piece(const Call &c, int *lds, int piece, i
     P = max(min(P, c.room - active), 1);
     // (at or a little above total / P)
     const int share = (int)ceilf((float)total * __builtin_amdgcn_rcpf((float)P) * 0.999999f);
-    const int base = max(max(share, (longest + kMostSplits - 1) / kMostSplits), 1);
+    // (no request has more than 2^25 tiles; lengths of up to 15 times this have to fit an int)
+    const int base = min(max(max(share, (longest + kMostSplits - 1) / kMostSplits), 1), 1 << 25);
     int len = 0;
     if (c.B <= 256) {
         int lo = base, hi = 2 * base;  // the first length that will do, if it is below hi
