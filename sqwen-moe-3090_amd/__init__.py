@@ -204,6 +204,22 @@ def _stream(stream):
     return getattr(stream, "cuda_stream", stream)
 
 
+def _make(stream, device, make):
+    """make() on the stream that a call runs on, for the tensors that it makes itself: what fills one is
+    then in order with the kernels, and freed memory goes to tensors of that stream, behind them."""
+    if stream is None:
+        return make()
+    if not isinstance(stream, torch.cuda.Stream):
+        handle = _stream(stream)
+        handle = getattr(handle, "value", handle)
+        stream = torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
+    with torch.cuda.stream(stream):
+        t = make()
+    if t is not None:  # the caller's own stream may read it until it is freed
+        t.record_stream(torch.cuda.current_stream(t.device))
+    return t
+
+
 def _ref(t):
     return ctypes.byref(t) if t is not None else None
 
@@ -530,7 +546,11 @@ def paged_plan(state, ring, table, n_past, n_new, page, slots, pos=None, state_o
     table row or in slots is refused whole: state_out[2] counts them."""
     if state_out is None or n_past_out is None or q_start is None or kv_len is None or pos is None:
         def new(t, n):
-            return t if t is not None else torch.empty(n, dtype=torch.int32, device=slots.device)
+            if t is not None:
+                return t
+            return _make(stream, slots.device, lambda: torch.empty(n, dtype=torch.int32, device=slots.device))
+
+        _need(stream is None or slots.is_cuda, "tensors must be on the GPU")
 
         B, T = table.shape[0], slots.shape[0]
         state_out, n_past_out, q_start = new(state_out, 4), new(n_past_out, B), new(q_start, B + 1)
@@ -600,7 +620,7 @@ def paged_attn(q, k_pool, v_pool, table, q_start, kv_len, max_q, scale=None, max
         n_tok, H, D = q.shape
         scale = D ** -0.5 if scale is None else scale
         if out is None:
-            out = torch.zeros((n_tok, H, D), dtype=torch.float32, device=q.device)
+            out = _make(stream, q.device, lambda: torch.zeros((n_tok, H, D), dtype=torch.float32, device=q.device))
         _need(out.dtype == torch.float32 and out.dim() == 3 and out.is_contiguous(), "out must be contiguous float32 (n_tok, H, D)")
         tt, to = _table_desc(table), out_desc(out)
         ts, tl = _vec(q_start, torch.int32, "q_start"), _vec(kv_len, torch.int32, "kv_len")
@@ -613,7 +633,7 @@ def paged_attn(q, k_pool, v_pool, table, q_start, kv_len, max_q, scale=None, max
         _need(q.shape[2] <= 1 or q.stride(2) == 1, "q rows must have unit element stride")
         if workspace is None:
             need = int(lib().sqa_paged_attn_workspace_size(ctypes.byref(tq), ctypes.byref(tk), ctypes.byref(tt), int(max_q)))
-            workspace, _ = _workspace(need, q.device)
+            workspace = _make(stream, q.device, lambda: _workspace(need, q.device)[0])
         _need(workspace is None or workspace.is_contiguous(), "workspace must be contiguous")
         _check(lib().sqa_paged_attn(ctypes.byref(tq), ctypes.byref(tk), ctypes.byref(tv), ctypes.byref(tt), ctypes.byref(ts),
                                     ctypes.byref(tl), _ref(tp), int(max_q), scale, max_bias, softcap, _ref(tg),
@@ -658,7 +678,7 @@ def lora_add(base, x, a, b, ids, scale=None, gate=None, out=None, stream=None):
             return out
     with _on(x.device, base=base, a=a, b=b, ids=ids, scale=scale, gate=gate, out=out):
         if out is None:
-            out = torch.empty_like(base, memory_format=torch.contiguous_format)
+            out = _make(stream, x.device, lambda: torch.empty_like(base, memory_format=torch.contiguous_format))
         td, tx, tg, ta, tb, to = _lora_descs(base, x, a, b, gate, out)
         ti = _vec(ids, torch.int32, "ids")
         ts = None if scale is None else _vec(scale, torch.float32, "scale")
