@@ -368,13 +368,13 @@ def flash_attn_ext(q, k_cache, v_cache, n_kv, mask=None, scale=None, max_bias=0.
     n_q, H, D = q.shape
     scale = D ** -0.5 if scale is None else scale
     if out is None:
-        out = torch.empty((n_q, H, D), dtype=torch.float32, device=q.device)
+        out = _make(stream, q.device, lambda: torch.empty((n_q, H, D), dtype=torch.float32, device=q.device))
     tq, tk, tv = q_desc(q), cache_view(k_cache, n_kv), cache_view(v_cache, n_kv)
     to, tm = out_desc(out), mask_desc(mask)
     if workspace is None:  # a given workspace is checked by the library
         need = int(lib().sqa_flash_attn_ext_workspace_size(ctypes.byref(tq), ctypes.byref(tk), ctypes.byref(tv),
                                                            ctypes.byref(to)))
-        workspace, _ = _workspace(need, q.device)
+        workspace = _make(stream, q.device, lambda: _workspace(need, q.device)[0])
     wptr = workspace.data_ptr() if workspace is not None else None
     wbytes = workspace.numel() if workspace is not None else 0
     _check(lib().sqa_flash_attn_ext(ctypes.byref(tq), ctypes.byref(tk), ctypes.byref(tv), _ref(tm), scale,
@@ -389,7 +389,7 @@ def flash_attn_ext_static(q, k_cache, v_cache, n_kv, mask=None, scale=None, max_
     n_q, H, D = q.shape
     scale = D ** -0.5 if scale is None else scale
     if out is None:
-        out = torch.empty((n_q, H, D), dtype=torch.float32, device=q.device)
+        out = _make(stream, q.device, lambda: torch.empty((n_q, H, D), dtype=torch.float32, device=q.device))
     tq, tk, tv = q_desc(q), cache_view(k_cache, n_kv), cache_view(v_cache, n_kv)
     to, tm = out_desc(out), mask_desc(mask)
     _check(lib().sqa_flash_attn_ext_static(ctypes.byref(tq), ctypes.byref(tk), ctypes.byref(tv), _ref(tm), scale,
@@ -409,7 +409,7 @@ def flash_attn_ext_causal(q, k_cache, v_cache, n_kv, q_pos0, gate=None, scale=No
     n_q, H, D = q.shape
     scale = D ** -0.5 if scale is None else scale
     if out is None:
-        out = torch.empty((n_q, H, D), dtype=torch.float32, device=q.device)
+        out = _make(stream, q.device, lambda: torch.empty((n_q, H, D), dtype=torch.float32, device=q.device))
     tq, tk, tv = q_desc(q), cache_view(k_cache, n_kv), cache_view(v_cache, n_kv)
     to = out_desc(out)
     tg = None
@@ -419,7 +419,7 @@ def flash_attn_ext_causal(q, k_cache, v_cache, n_kv, q_pos0, gate=None, scale=No
     if workspace is None:  # a given workspace is checked by the library
         need = int(lib().sqa_flash_attn_ext_workspace_size(ctypes.byref(tq), ctypes.byref(tk), ctypes.byref(tv),
                                                            ctypes.byref(to)))
-        workspace, _ = _workspace(need, q.device)
+        workspace = _make(stream, q.device, lambda: _workspace(need, q.device)[0])
     wptr = workspace.data_ptr() if workspace is not None else None
     wbytes = workspace.numel() if workspace is not None else 0
     _check(lib().sqa_flash_attn_ext_causal(ctypes.byref(tq), ctypes.byref(tk), ctypes.byref(tv), q_pos0,
@@ -430,7 +430,7 @@ def flash_attn_ext_causal(q, k_cache, v_cache, n_kv, q_pos0, gate=None, scale=No
 def sigmoid_mul(x, gate, out=None, stream=None):
     """out = x * sigmoid(gate) over 2-D float32 [n_tok, n] (attn.rs:282-283)."""
     if out is None:
-        out = torch.empty_like(x)
+        out = _make(stream, x.device, lambda: torch.empty_like(x))
     n1, n0 = x.shape
     d = [Tensor.make(TYPE_F32, [n0, n1], [4, t.stride(0) * 4], t.data_ptr()) for t in (out, x, gate)]
     _check(lib().sqa_sigmoid_mul(ctypes.byref(d[0]), ctypes.byref(d[1]), ctypes.byref(d[2]), _stream(stream)))
@@ -464,11 +464,11 @@ def out_proj(w, x, gate=None, out=None, workspace=None, stream=None):
             return out
     M, K = x.shape
     if out is None:
-        out = torch.empty((M, w.shape[0]), dtype=torch.float32, device=x.device)
+        out = _make(stream, x.device, lambda: torch.empty((M, w.shape[0]), dtype=torch.float32, device=x.device))
     tw, tx, tg, to = _out_proj_descs(w, x, gate, out)
     need = int(lib().sqa_out_proj_workspace_size(ctypes.byref(tw), ctypes.byref(tx)))
     if workspace is None:
-        workspace, _ = _workspace(need, x.device)
+        workspace = _make(stream, x.device, lambda: _workspace(need, x.device)[0])
     _check(lib().sqa_out_proj(ctypes.byref(tw), ctypes.byref(tx), _ref(tg), ctypes.byref(to),
                               workspace.data_ptr() if workspace is not None else None,
                               workspace.numel() if workspace is not None else 0, _stream(stream)))
@@ -795,11 +795,12 @@ class KvCache:
         n_q, H, D = q.shape
         scale = D ** -0.5 if scale is None else scale
         if out is None:
-            out = torch.empty((n_q, H, D), dtype=torch.float32, device=q.device)
+            out = _make(stream, q.device, lambda: torch.empty((n_q, H, D), dtype=torch.float32, device=q.device))
         tq, tk, tv = q_desc(q), self.view(slot, "k"), self.view(slot, "v")
         to, tm = out_desc(out), mask_desc(mask)
         if workspace is None:
-            workspace, _ = _workspace(self.workspace_size(slot, q), q.device)
+            need = self.workspace_size(slot, q)
+            workspace = _make(stream, q.device, lambda: _workspace(need, q.device)[0])
         wptr = workspace.data_ptr() if workspace is not None else None
         wbytes = workspace.numel() if workspace is not None else 0
         _check(lib().sqa_flash_attn_ext(ctypes.byref(tq), ctypes.byref(tk), ctypes.byref(tv), _ref(tm), scale,
