@@ -204,16 +204,23 @@ def _stream(stream):
     return getattr(stream, "cuda_stream", stream)
 
 
+def _stream_of(stream, device):
+    """Makes a call's stream (None: the device's current one) and its device the current ones."""
+    if stream is None:
+        return torch.cuda.device(device)
+    if not isinstance(stream, torch.cuda.Stream):
+        handle = _stream(stream)
+        handle = getattr(handle, "value", handle)
+        stream = torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
+    return torch.cuda.stream(stream)
+
+
 def _make(stream, device, make):
     """make() on the stream that a call runs on, for the tensors that it makes itself: what fills one is
     then in order with the kernels, and freed memory goes to tensors of that stream, behind them."""
     if stream is None:
         return make()
-    if not isinstance(stream, torch.cuda.Stream):
-        handle = _stream(stream)
-        handle = getattr(handle, "value", handle)
-        stream = torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
-    with torch.cuda.stream(stream):
+    with _stream_of(stream, device):
         t = make()
     if t is not None:  # the caller's own stream may read it until it is freed
         t.record_stream(torch.cuda.current_stream(t.device))
@@ -863,8 +870,9 @@ class PagedKvCache:
 
     def append(self, layer, k_cur, v_cur, step, stream=None):
         """Quantize the step's K and V rows, float32 (n_rows, Hkv*D), into the layer's pages."""
-        set_rows_q4_0(self.rows(layer, "k"), k_cur, step.slots, stream)
-        set_rows_q4_0(self.rows(layer, "v"), v_cur, step.slots, stream)
+        with _stream_of(stream, self.table.device):
+            set_rows_q4_0(self.rows(layer, "k"), k_cur, step.slots)
+            set_rows_q4_0(self.rows(layer, "v"), v_cur, step.slots)
 
     def workspace_size(self, q, max_q):
         return paged_attn_workspace_size(q, self.k[0], self.table, max_q)
