@@ -856,9 +856,9 @@ class PagedKvCache:
                          torch.zeros(B, dtype=i32, device=dev), torch.zeros(n_rows, dtype=torch.int64, device=dev),
                          torch.zeros(4 * n_rows, dtype=i32, device=dev))
 
-    def plan(self, n_new, step):
+    def plan(self, n_new, step, stream=None):
         """Gives the step's new tokens (n_new: int32 (max_requests,), < 0 ends a request) their pages."""
-        with torch.cuda.device(self.table.device):
+        with _stream_of(stream, self.table.device):
             paged_plan(self.state, self.ring, self.table, self.n_past, n_new, self.page, step.slots, step.pos,
                        step.state, step.n_past, step.q_start, step.kv_len)
             self._now.copy_(self._next)

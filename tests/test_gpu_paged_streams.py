@@ -104,3 +104,32 @@ def test_plan_and_adapters(sqa, dev):
         got = sqa.lora_add(base, x, a, b, ids, stream=handle)
         torch.cuda.synchronize()
         assert torch.equal(got, added)
+
+
+def test_a_step_on_another_stream(sqa, dev):
+    """plan, append and attend of PagedKvCache all take the stream: in order with each other, whatever
+    the current stream does."""
+    gen = torch.Generator(device=dev).manual_seed(8)
+    kv, vv = torch.randn((2, 40, HKV * D), generator=gen, device=dev)
+    q = torch.randn((40, H, D), generator=gen, device=dev)
+    n_new = torch.tensor([30, 1, 0, 9], dtype=torch.int32, device=dev)
+    s = torch.cuda.Stream()
+    got = []
+    for handle in (None, *handles(s)):
+        cache = sqa.PagedKvCache(1, D, HKV, 12, 16, 4, 4, device=dev)
+        for t in cache.k + cache.v:
+            t.zero_()
+        step = cache.new_step(40)
+        torch.cuda.synchronize()
+        if handle is not None:
+            busy(torch.cuda.current_stream())
+        for _ in range(2):
+            cache.plan(n_new, step, stream=handle)
+            cache.append(0, kv, vv, step, stream=handle)
+            out = cache.attend(0, q, step, 30, stream=handle)
+        (torch.cuda.current_stream() if handle is None else s).synchronize()
+        torch.cuda.synchronize()
+        got.append([out, cache.n_past.clone(), cache.state.clone(), cache.table, cache.ring, step.slots, *cache.k, *cache.v])
+    for other in got[1:]:
+        assert all(torch.equal(x, y) for x, y in zip(got[0], other))
+    assert got[0][1].tolist() == [60, 2, 0, 18]
