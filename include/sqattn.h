@@ -349,8 +349,9 @@ int sqa_supports_paged_attn(const sqa_tensor *q, const sqa_tensor *k, const sqa_
 /*
  * Low-rank adapters of many requests beside a shared projection:
  *   dst[:, m] = base[:, m] + scale[i] * B_i (A_i (x[:, m] * sigmoid(gate[:, m]))),  i = ids[m]
- *   base  F32 [N, M]  the shared projection's output; may be dst itself (nothing else may
- *                     overlap dst: not x or gate, nor base in part)
+ *   base  F32 [N, M]  the shared projection's output; may be dst itself (dst that overlaps
+ *                     anything else, or base in part, is refused; other columns of rows
+ *                     that are as far apart are no overlap)
  *   x     F32 [K, M], gate F32 [K, M] or NULL (unit element stride)
  *   a     F16 [K, r, n_adapters], b F16 [r, N, n_adapters]  contiguous, 16-byte aligned
  *   ids   I32 [M]; an id outside [0, n_adapters) is a token without adapter

@@ -12,6 +12,29 @@ bool dense1(const sqa_tensor *t, int type, int64_t n, int64_t esize) {
            (n <= 1 || t->nb[0] == (uint64_t)esize) && (n == 0 || (t->data && (uintptr_t)t->data % esize == 0));
 }
 
+// n rows of `len` bytes, `step` bytes apart
+struct Rows {
+    uintptr_t at;
+    uint64_t len, step;
+    int64_t n;
+    uintptr_t end() const { return at + (uint64_t)(n - 1) * step + len; }
+};
+
+Rows rows_of(const sqa_tensor *t) {  // ne[1] rows of ne[0] 4-byte values
+    return Rows{(uintptr_t)t->data, 4 * (uint64_t)t->ne[0], t->nb[1], t->ne[1]};
+}
+Rows run_of(const sqa_tensor *t, uint64_t bytes) { return Rows{(uintptr_t)t->data, bytes, 0, bytes ? 1 : 0}; }
+
+// Whether two sets of rows share a byte. Rows of one step, such as parts of a wider buffer's
+// columns, may lie between each other; of different steps, all that lies between is taken as theirs.
+bool meet(const Rows &a, const Rows &b) {
+    if (a.n < 1 || b.n < 1 || a.end() <= b.at || b.end() <= a.at) return false;
+    const uint64_t step = a.n == 1 ? b.step : a.step;
+    if ((a.n > 1 && b.n > 1 && a.step != b.step) || (a.n == 1 && b.n == 1) || a.len > step || b.len > step) return true;
+    const uint64_t r = b.at >= a.at ? (b.at - a.at) % step : (step - (a.at - b.at) % step) % step;  // b's start in a's row
+    return r < a.len || step - r < b.len;
+}
+
 bool power_of_two(int64_t x) { return x > 0 && (x & (x - 1)) == 0; }
 
 int check_table(const sqa_tensor *t, const char *what) {
@@ -219,6 +242,14 @@ int sqa_lora_add(const sqa_tensor *base, const sqa_tensor *x, const sqa_tensor *
     if (scale && !dense1(scale, SQA_TYPE_F32, a->ne[2], 4))
         return set_error(SQA_ERR_INVALID, "lora_add: scale must be contiguous F32 [n_adapters]");
     if (x->ne[1] == 0) return SQA_OK;
+    // Several workgroups read a token's row, or a tile's, while others write their part of it.
+    const Rows out = rows_of(dst);
+    const bool in_place = base->data == dst->data && (dst->ne[1] == 1 || base->nb[1] == dst->nb[1]);
+    const uint64_t r = (uint64_t)a->ne[1], n = (uint64_t)a->ne[2];
+    if (meet(out, rows_of(x)) || (gate && meet(out, rows_of(gate))) || (!in_place && meet(out, rows_of(base))) ||
+        meet(out, run_of(a, 2 * r * n * (uint64_t)a->ne[0])) || meet(out, run_of(b, 2 * r * n * (uint64_t)b->ne[1])) ||
+        meet(out, run_of(ids, 4 * (uint64_t)ids->ne[0])) || (scale && meet(out, run_of(scale, 4 * n))))
+        return set_error(SQA_ERR_INVALID, "lora_add: dst must not overlap another array, but for a base that is dst itself");
     return launch_lora_add(*base, *x, gate, *a, *b, *ids, scale, *dst, (hipStream_t)stream);
 }
 
