@@ -332,6 +332,7 @@ int sqa_paged_plan(const sqa_tensor *n_past, const sqa_tensor *n_new, const sqa_
  * results of a call repeat bit for bit.
  * D == 256, H / Hkv <= 16, page, B and W as for the plan. Requests with more than
  * max_q tokens may be left as they were.
+ * q or gate may be dst itself; dst or a workspace that overlaps anything else is refused.
  * workspace: sqa_paged_attn_workspace_size bytes. A smaller one takes fewer splits of
  * the keys, down to one per request and KV head; below that SQA_ERR_WORKSPACE.
  */

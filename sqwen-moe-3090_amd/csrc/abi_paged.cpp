@@ -222,6 +222,33 @@ int sqa_paged_attn(const sqa_tensor *q, const sqa_tensor *k, const sqa_tensor *v
                  (uintptr_t)gate->data % 4 || (q->ne[1] > 0 && !gate->data)))
         return set_error(SQA_ERR_INVALID, "%s: gate must be F32 [D, H, n_tok]", what);
     if (q->ne[1] == 0) return SQA_OK;
+    // Some rows of dst, and the workspace, are written while others are computed. A row of q or
+    // gate is read for no row of dst but its own.
+    const int64_t n_tok = q->ne[1], H = q->ne[2];
+    auto heads = [&](const sqa_tensor *t, uint64_t token, uint64_t head) {  // its rows, by token or by head
+        const uint64_t row = 4 * (uint64_t)kHeadDim, by_token = row + (uint64_t)(H - 1) * head;
+        return token >= by_token || n_tok == 1 ? Rows{(uintptr_t)t->data, by_token, token, n_tok}
+                                               : Rows{(uintptr_t)t->data, row + (uint64_t)(n_tok - 1) * token, head, H};
+    };
+    auto same = [&](const sqa_tensor *t, uint64_t token, uint64_t head) {  // dst itself
+        return t->data == dst->data && (n_tok == 1 || token == dst->nb[2]) && (H == 1 || head == dst->nb[1]);
+    };
+    auto pages = [&](const sqa_tensor *t) { return Rows{(uintptr_t)t->data, t->nb[2] * (uint64_t)t->ne[2], t->nb[3], t->ne[3]}; };
+    const Rows out = run_of(dst, 4ull * kHeadDim * (uint64_t)(H * n_tok)), tab{(uintptr_t)table->data, 4 * (uint64_t)table->ne[0], table->nb[1], B};
+    const Rows rows_q = heads(q, q->nb[1], q->nb[2]);
+    const size_t most = paged_attn_workspace(n_tok, H, k->ne[1], B, max_q);
+    const Rows ws{(uintptr_t)workspace, workspace_bytes < most ? workspace_bytes : most, 0, workspace ? 1 : 0};
+    bool clash = meet(out, ws) || meet(ws, rows_q) || (!same(q, q->nb[1], q->nb[2]) && meet(out, rows_q));
+    if (gate) {
+        const Rows rows_g = heads(gate, gate->nb[2], gate->nb[1]);
+        clash |= meet(ws, rows_g) || (!same(gate, gate->nb[2], gate->nb[1]) && meet(out, rows_g));
+    }
+    for (const Rows &r : {pages(k), pages(v), tab, run_of(q_start, 4 * (uint64_t)(B + 1)), run_of(kv_len, 4 * (uint64_t)B),
+                          prefix ? run_of(prefix, 4 * (uint64_t)B) : Rows{}})
+        clash |= meet(out, r) || meet(ws, r);
+    if (clash)
+        return set_error(SQA_ERR_INVALID, "%s: dst and the workspace must not overlap another array, but for a q or gate that is dst itself",
+                         what);
     const PagedArgs a{q, k, v, table, q_start, kv_len, prefix, gate, dst, max_q, scale, max_bias, logit_softcap,
                       workspace, workspace_bytes};
     return launch_paged_attn(a, (hipStream_t)stream);
