@@ -328,7 +328,8 @@ int sqa_paged_plan(const sqa_tensor *n_past, const sqa_tensor *n_new, const sqa_
  * sqa_flash_attn_ext_causal. A token that sees no key gets zeros; rows of dst
  * outside [q_start[0], q_start[B]) are left as they were. Keys of a page whose
  * table entry is outside [0, n_pages) are not seen; no byte of keys that no token
- * sees enters the result. The scales of keys that are seen have to be finite. The
+ * sees enters the result. The scales of keys that are seen have to be finite. A row of
+ * q that holds NaN or Inf gives a row of NaN (if it sees a key), other rows stay. The
  * results of a call repeat bit for bit.
  * D == 256, H / Hkv <= 16, page, B and W as for the plan. Requests with more than
  * max_q tokens may be left as they were.

@@ -163,7 +163,7 @@ __device__ __forceinline__ void cap_logits(float (&s)[N], float cap2, float cap_
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         x[i] = s[i] * cap_inv;
-        top = fmaxf(top, fabsf(x[i]));  // (a NaN belongs to a key that is not seen)
+        top = fmaxf(top, fabsf(x[i]));  // (passes over a NaN)
         const float y = x[i] * x[i];
         float t = fmaf(y, 0.021869488f, -0.053968254f);
         t = fmaf(y, t, 0.13333333f);
@@ -176,7 +176,7 @@ __device__ __forceinline__ void cap_logits(float (&s)[N], float cap2, float cap_
         const float z = fminf(fmaxf(x[i], -12.0f), 12.0f);
         const float e = __builtin_amdgcn_exp2f(2.0f * kLog2e * z);
         const float t = (e - 1.0f) * __builtin_amdgcn_rcpf(e + 1.0f);
-        s[i] = fabsf(x[i]) < 0.25f ? s[i] : fmaf(cap2, t, off);
+        s[i] = fabsf(x[i]) >= 0.25f ? fmaf(cap2, t, off) : s[i];  // (NaN stays NaN)
     }
 }
 

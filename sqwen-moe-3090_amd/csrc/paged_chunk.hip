@@ -799,8 +799,9 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
                 store_through(p.acc_c + at * kHeadDim + 16 * T + n, __builtin_amdgcn_ldexpf(acc[rg][T][i], e_out[T >> 2]));
             if (n == 0) {
                 // the merge works in base e (acc and l of every split carry the same
-                // 2^kEp, which cancels there)
-                store_through(p.ml_c + at * 2, mrow == -INFINITY ? mrow : mrow * kLn2);
+                // 2^kEp, which cancels there); a row of NaN has seen keys, though none of
+                // them moved its maximum
+                store_through(p.ml_c + at * 2, lrow != lrow ? lrow : mrow == -INFINITY ? mrow : mrow * kLn2);
                 store_through(p.ml_c + at * 2 + 1, lrow);
             }
         }

@@ -386,14 +386,17 @@ __global__ __launch_bounds__(kThreads, 4) void paged_few_kernel(Call p) {
                     x[4 * j + 3] = v4.w;
                 }
                 const bool use = row_ok && q_active;
-                float amax = 0.0f;
+                // (0 times NaN or Inf is NaN: the block's scale then is NaN, and so is every logit of the
+                // row; fmaxf and the codes would pass over a NaN)
+                float amax = 0.0f, odd = 0.0f;
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
                     x[j] = use ? x[j] : 0.0f;
                     amax = fmaxf(amax, fabsf(x[j]));
+                    odd = fmaf(x[j], 0.0f, odd);
                 }
                 amax = xmax16(amax);  // the other 16 values of the block
-                const float d = amax / 127.f;
+                const float d = amax / 127.f + xsum16(odd);
                 const float id = amax != 0.0f ? 127.f / amax : 0.0f;
                 int sumq = 0;
                 uint32_t w4[4];
@@ -643,7 +646,8 @@ __global__ __launch_bounds__(kThreads, 4) void paged_few_kernel(Call p) {
         if (wq == 0 && g == 0 && row_writer && my_ok) {
             const float L = (lbuf[my_r] + lbuf[16 + my_r]) + (lbuf[32 + my_r] + lbuf[48 + my_r]);
             float *ml = p.ml_d + ((int64_t)slot * p.rows_d + my_r) * 2;
-            store_through(ml, m_ref == -INFINITY ? m_ref : m_ref * kLn2);  // the merge works in base e
+            // the merge works in base e; a row of NaN has seen keys, though none of them moved its maximum
+            store_through(ml, L != L ? L : m_ref == -INFINITY ? m_ref : m_ref * kLn2);
             store_through(ml + 1, L);
         }
     } else {
