@@ -12,8 +12,9 @@ namespace {
 constexpr int kThreads = 256;
 
 typedef float floatx4 __attribute__((ext_vector_type(4)));
-// Merge of a row's partials: out = sum_s acc_s e^(m_s - M) / sum_s l_s e^(m_s - M), M = max m_s,
-// then the gate. A partial whose m is -inf (no key seen) may hold anything.
+// Merge of a row's partials: out = sum_s acc_s 2^(m_s - M) / sum_s l_s 2^(m_s - M), M = max m_s,
+// then the gate. m is in base 2 as the kernels hold it: through base e and back, 50 nats lost 2e-6
+// of a split's weight. A partial whose m is -inf (no key seen) may hold anything.
 struct Row {
     const float *acc, *ml;  // of the row in its first slot
     int64_t step;           // floats of acc between its splits (ml: step / 128)
@@ -72,7 +73,7 @@ __global__ __launch_bounds__(kThreads) void merge_dims_kernel(Call c) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
         const bool dead = ml[j].x == -INFINITY;
-        const float w = dead ? 0.0f : __builtin_amdgcn_exp2f((ml[j].x - M) * kLog2e);
+        const float w = dead ? 0.0f : __builtin_amdgcn_exp2f(ml[j].x - M);
         o = dead ? o : fmaf(acc[j], w, o);
         l = dead ? l : fmaf(ml[j].y, w, l);
     }
@@ -122,8 +123,8 @@ __global__ __launch_bounds__(kThreads) void merge_rows_kernel(Call c) {
         float m = ml.x;
 #pragma unroll
         for (int x = 1; x < kS; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
-        const float Mn = fmaxf(M, m), al = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((M - Mn) * kLog2e);
-        const float w = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((ml.x - Mn) * kLog2e);
+        const float Mn = fmaxf(M, m), al = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - Mn);
+        const float w = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - Mn);
         float l = ml.x == -INFINITY ? 0.0f : ml.y * w;
 #pragma unroll
         for (int x = 1; x < kS; x <<= 1) l += __shfl_xor(l, x);

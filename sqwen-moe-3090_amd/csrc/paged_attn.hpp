@@ -7,7 +7,6 @@ namespace sqa {
 namespace paged {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 
 // 16 bytes at any 4-byte address (the hardware's loads ask for no more)
 typedef float float4a __attribute__((ext_vector_type(4), aligned(4)));

@@ -798,10 +798,9 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
             for (int T = 0; T < 16; ++T)
                 store_through(p.acc_c + at * kHeadDim + 16 * T + n, __builtin_amdgcn_ldexpf(acc[rg][T][i], e_out[T >> 2]));
             if (n == 0) {
-                // the merge works in base e (acc and l of every split carry the same
-                // 2^kEp, which cancels there); a row of NaN has seen keys, though none of
-                // them moved its maximum
-                store_through(p.ml_c + at * 2, lrow != lrow ? lrow : mrow == -INFINITY ? mrow : mrow * kLn2);
+                // (acc and l of every split carry the same 2^kEp, which cancels in the merge; a
+                // row of NaN has seen keys, though none of them moved its maximum)
+                store_through(p.ml_c + at * 2, lrow != lrow ? lrow : mrow);
                 store_through(p.ml_c + at * 2 + 1, lrow);
             }
         }

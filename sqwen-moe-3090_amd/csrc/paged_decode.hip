@@ -646,8 +646,8 @@ __global__ __launch_bounds__(kThreads, 4) void paged_few_kernel(Call p) {
         if (wq == 0 && g == 0 && row_writer && my_ok) {
             const float L = (lbuf[my_r] + lbuf[16 + my_r]) + (lbuf[32 + my_r] + lbuf[48 + my_r]);
             float *ml = p.ml_d + ((int64_t)slot * p.rows_d + my_r) * 2;
-            // the merge works in base e; a row of NaN has seen keys, though none of them moved its maximum
-            store_through(ml, L != L ? L : m_ref == -INFINITY ? m_ref : m_ref * kLn2);
+            // (a row of NaN has seen keys, though none of them moved its maximum)
+            store_through(ml, L != L ? L : m_ref);
             store_through(ml + 1, L);
         }
     } else {
