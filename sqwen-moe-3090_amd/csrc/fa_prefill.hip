@@ -466,9 +466,9 @@ __global__ __launch_bounds__(256) void pf_mask_pack_kernel(const char *__restric
 // the caller waits with s_waitcnt vmcnt).
 __device__ __forceinline__ void dma16(uint32_t voff, const void *sbase, uint32_t m0v) {
     // m0 as an operand: the compiler writes it and knows it holds the LDS base. It does not
-    // know what the asm holds: the wait state that a load into LDS needs after a write of m0
-    // stands in it.
-    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "{m0}"(m0v) : "memory");
+    // know what the asm holds: the wait states that a load into LDS needs after a write of m0
+    // (1), and a memory instruction after v_readfirstlane wrote its base (5), stand in it.
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "{m0}"(m0v) : "memory");
 }
 
 // Two 8-byte LDS reads into one MFMA operand. volatile keeps them two single

@@ -402,9 +402,9 @@ __device__ __forceinline__ void dma16(uint32_t voff, const void *sbase, uint32_t
                         (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)b);
     const uint32_t ms = (uint32_t)__builtin_amdgcn_readfirstlane((int)m0v);
     // m0 as an operand: the compiler writes it and knows it holds the LDS base. It does not
-    // know what the asm holds: the wait state that a load into LDS needs after a write of m0
-    // stands in it.
-    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(bs), "{m0}"(ms) : "memory");
+    // know what the asm holds: the wait states that a load into LDS needs after a write of m0
+    // (1), and a memory instruction after v_readfirstlane wrote its base (5), stand in it.
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(bs), "{m0}"(ms) : "memory");
 }
 
 __global__ __launch_bounds__(64 * kG2Waves) void op_gemm2_kernel(GemmParams p) {
