@@ -359,10 +359,11 @@ int sqa_supports_paged_attn(const sqa_tensor *q, const sqa_tensor *k, const sqa_
  *   ids   I32 [M]; an id outside [0, n_adapters) is a token without adapter
  *   scale F32 [n_adapters] or NULL (1)
  *   dst   F32 [N, M]
- * Up to 512 tokens and K <= 16384: fp32 throughout, any finite size. Otherwise
+ * Values of any finite size. Up to 512 tokens and K <= 16384: fp32 throughout. Otherwise
  * x * sigmoid(gate) and scale * A x enter as fp16 hi + lo pairs: 22 bits where their size
- * is 2^-13 or more, an absolute 2^-36 below, both below 65504; products are exact and
- * sums fp32.
+ * is 2^-13 or more, an absolute 2^-36 below; products are exact and sums fp32. 16
+ * neighbouring tokens with one of 65504 or more among these take A x in fp32 instead, and
+ * scale * A x to 22 bits of the token's largest (slower).
  * K % 256 == 0, N % 16 == 0, r % 8 == 0, r <= 128; base and dst rows 16-byte aligned.
  */
 int sqa_lora_add(const sqa_tensor *base, const sqa_tensor *x, const sqa_tensor *gate, const sqa_tensor *a,

@@ -676,7 +676,9 @@ def lora_add(base, x, a, b, ids, scale=None, gate=None, out=None, stream=None):
 
     base: float32 (M, N), may be out; x, gate: float32 (M, K); a: float16 (n, r, K);
     b: float16 (n, N, r); ids: int32 (M,), an id outside [0, n) is a token without
-    adapter; scale: float32 (n,) or None."""
+    adapter; scale: float32 (n,) or None. out may be base, and overlaps nothing else.
+    Up to 512 tokens (and K of 16384) all is float32; more tokens take x * sigmoid(gate)
+    and scale * A x at 22 bits, an absolute 2^-36 below 2^-13."""
     if stream is None and out is not None:
         rc = (_host or _load_host()).lora(base, x, a, b, ids, scale, gate, out)
         if rc is not None:

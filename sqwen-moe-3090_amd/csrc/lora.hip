@@ -18,7 +18,8 @@
 // a chunk's steps of K: t^T = A x^T on v_mfma_f32_16x16x32_f16, A as it is, x as an fp16
 // pair: hi = fp16(x), lo = fp16((x - hi) 2^11), in sums of their own (the shift keeps lo
 // clear of subnormals: 22 bits down to |x| = 2^-13, an absolute 2^-36 below). The partial
-// t are added in LDS; then the wavefronts share the columns, out^T = B t^T with t as a
+// t are added in LDS (where one is too large for fp16, or Inf or NaN of an x that is, the
+// tile's t are taken again in fp32); then the wavefronts share the columns, out^T = B t^T with t as a
 // pair in the same way, turned in LDS into rows of 64 columns (32 above rank 64, for want
 // of registers) for base and out. The adapters of a tile are taken by kPasses workgroups in
 // turn, each writing its tokens alone; no adapter's values reach another one's tokens, not
@@ -251,13 +252,35 @@ __device__ __forceinline__ void split(float x, _Float16 &hi, _Float16 &lo) {
     lo = (_Float16)((x - (float)hi) * 2048.0f);
 }
 
+// t of a tile's tokens of adapter cur in plain fp32, a wavefront to a value: for values that fp16 does not hold.
+__device__ __forceinline__ void rank_sums(const Params &p, int cur, float sc, int m0, const int *ids, float *t, int t_row) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    for (int e = wave; e < kTile * p.r; e += kWaves) {
+        const int m = e & (kTile - 1), j = e / kTile;
+        if (ids[m] != cur) continue;
+        const float *x = reinterpret_cast<const float *>(p.x + (m0 + m) * p.x_nb1);
+        const float *g = p.gate ? reinterpret_cast<const float *>(p.gate + (m0 + m) * p.gate_nb1) : nullptr;
+        const _Float16 *a = p.a + ((int64_t)cur * p.r + j) * p.K;
+        float s = 0.0f;
+        for (int k = 4 * lane; k < p.K; k += 256) {
+            floatx4 v = *reinterpret_cast<const float4a *>(x + k);
+            if (g) v = gated(v, *reinterpret_cast<const float4a *>(g + k));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s = fmaf(v[i], (float)a[k + i], s);
+        }
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o);
+        if (lane == 0) t[m * t_row + j] = s * sc;
+    }
+}
+
 // MFMA operands (lane = 16 g + n): A[n][8g..8g+7], B[8g..8g+7][n], C[4g..4g+3][n].
 template <int RT, bool GATE>
 __global__ __launch_bounds__(kThreads, 2) void lora_tile_kernel(Params p) {
     typedef Form<RT> F;
     typedef _Float16 half4 __attribute__((ext_vector_type(4)));
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ int ids[kTile];
+    __shared__ int ids[kTile], over;
     float *t = reinterpret_cast<float *>(smem);  // [token][kR + 4]
     uint8_t *stage = smem + F::kT;
     constexpr int kTRow = F::kR + 4;
@@ -394,6 +417,7 @@ __global__ __launch_bounds__(kThreads, 2) void lora_tile_kernel(Params p) {
                 }
         };
         load_cols(0, wave);
+        if (tid == 0) over = 0;
         float *part = reinterpret_cast<float *>(stage);  // [step wave][rank][token]
 #pragma unroll
         for (int q = 0; q < F::kTiles; ++q)
@@ -405,9 +429,22 @@ __global__ __launch_bounds__(kThreads, 2) void lora_tile_kernel(Params p) {
             float s = 0.0f;
 #pragma unroll
             for (int w = 0; w < F::kStepWaves; ++w) s += part[w * F::kR * kTile + e];
-            t[(e & 15) * kTRow + (e >> 4)] = e >> 4 < p.r ? s * sc : 0.0f;
+            s = e >> 4 < p.r ? s * sc : 0.0f;
+            t[(e & 15) * kTRow + (e >> 4)] = s;
+            // too large for fp16, or Inf or NaN of an x that is
+            if (!(fabsf(s) < 65504.0f) && ids[e & 15] == cur) over = 1;
         }
         __syncthreads();
+        // then t again in fp32, and 2^-e t of a token's own e in the columns
+        float up = 1.0f, down = 1.0f;
+        if (__builtin_expect(__builtin_amdgcn_readfirstlane(over) != 0, 0)) {
+            rank_sums(p, cur, sc, m0, ids, t, kTRow);
+            __syncthreads();
+            float top = 0.0f;
+            for (int j = 0; j < p.r; ++j) top = fmaxf(top, fabsf(t[n * kTRow + j]));
+            const int e = max((int)(__float_as_uint(top) >> 23) - 127 - 14, 0);  // top 2^-e < 2^15
+            down = __builtin_amdgcn_ldexpf(1.0f, -e), up = __builtin_amdgcn_ldexpf(1.0f, e);
+        }
         // t of the lane's token, ranks 32q + 8g ..
         half8 th[kS], tl[kS];
 #pragma unroll
@@ -415,7 +452,7 @@ __global__ __launch_bounds__(kThreads, 2) void lora_tile_kernel(Params p) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 _Float16 a, b;
-                split(32 * q + 8 * g < F::kR ? t[n * kTRow + 32 * q + 8 * g + i] : 0.0f, a, b);
+                split(32 * q + 8 * g < F::kR ? t[n * kTRow + 32 * q + 8 * g + i] * down : 0.0f, a, b);
                 th[q][i] = a, tl[q][i] = b;
             }
         // out^T = B t^T of kCols columns, turned in LDS so that base and out are whole rows of them
@@ -435,7 +472,7 @@ __global__ __launch_bounds__(kThreads, 2) void lora_tile_kernel(Params p) {
                         l = __builtin_amdgcn_mfma_f32_16x16x32_f16(bv[s][u][q], tl[q], l, 0, 0, 0);
                     }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) h[i] = fmaf(l[i], 1.0f / 2048.0f, h[i]);
+                    for (int i = 0; i < 4; ++i) h[i] = fmaf(l[i], 1.0f / 2048.0f, h[i]) * up;
                     *reinterpret_cast<floatx4 *>(turned + n * F::kOutRow + 4 * (16 * u + 4 * g)) = h;
                 }
                 // (a wavefront's own staging: its LDS operations are in order)
