@@ -295,9 +295,17 @@ int sqa_out_proj(const sqa_tensor *w, const sqa_tensor *x, const sqa_tensor *gat
  *   slots      I64 [T]     pool row of every token, -1 for a refused one and behind the last
  *   pos        I32 [4 * T] rotary positions t, h, w, e of every token (text: all equal)
  * The pages of ended requests join the ring first (in the order of requests and
- * table entries), then pages leave it in the order of requests. A request whose
- * new pages are not all there, whose tokens pass the table's W pages or the T rows
- * is refused: it gets no page, its slots are -1, its length stays. What the plan writes
+ * table entries), then pages leave it in the order of requests. A request is refused if
+ * its tokens pass the table's W pages, if the n_new of the places up to it (ended ones
+ * aside) pass T, or if it needs new pages and those wanted up to it pass the free ones,
+ * where every place that its table and T have room for counts with all that it wants. A
+ * refused request gets no page, its slots are -1, its length stays; it holds its rows of
+ * q_start. So places are served in order: behind one that wants more pages than are free,
+ * those that want any are refused too (those that want none are served), and behind one
+ * that passes T all are, also one without new tokens. What is refused stays so while it is
+ * asked for again and no request ends: the caller plans it with n_new = 0 until state_out[1]
+ * covers what it wants, ceil((n_past + n_new) / page) - ceil(n_past / page) pages, or with
+ * fewer tokens, and the places behind it go on. What the plan writes
  * (outputs, table and ring) must not overlap any other array of the call (the caller
  * swaps state and n_past with their outputs, or copies).
  * All arrays contiguous but table. B <= 4096, W <= 2^18, W * page < 2^31, T <= 2^29.

@@ -549,8 +549,10 @@ def paged_plan(state, ring, table, n_past, n_new, page, slots, pos=None, state_o
 
     state: int32 (4,) {first free place of the ring, free pages, ., .}; ring: int32
     (n_pages,); table: int32 (B, W); n_past, n_new: int32 (B,); slots: int64 (T,);
-    pos: int32 (4 * T,). A request that finds too few pages, too little room in its
-    table row or in slots is refused whole: state_out[2] counts them."""
+    pos: int32 (4 * T,). A request that finds too few pages, too little room in its table row or in
+    slots is refused whole: state_out[2] counts them. Places are served in order and a
+    refused one's wants stay counted, so those behind it that need a page are refused too:
+    plan it with n_new = 0 until state_out[1], the free pages, covers it."""
     if state_out is None or n_past_out is None or q_start is None or kv_len is None or pos is None:
         def new(t, n):
             if t is not None:

@@ -5,7 +5,8 @@
 //   rel_b  = sum of have over ended requests    (pages that come back)
 //   need_b = ceil((past_b + new_b) / page) - have_b, 0 where b's tokens fit nowhere
 //   upto_b = sum of need up to and with b
-// A request is served where it fits and upto_b <= count + rel (or it needs none).
+// A request is served where it fits and upto_b <= count + rel (or it needs none): in order,
+// what a refused one needs stays in the sums of those behind it.
 // Three prefix sums over the batch and then work of its own for every token: its
 // request by a search in end, its page from the table, or, on a fresh page, from
 // the ring at head + upto_b - need_b + i (behind the ring's old pages: from the
