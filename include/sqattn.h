@@ -293,7 +293,9 @@ int sqa_out_proj(const sqa_tensor *w, const sqa_tensor *x, const sqa_tensor *gat
  *   q_start    I32 [B + 1] request b's tokens are rows q_start[b] .. q_start[b + 1] - 1
  *   kv_len     I32 [B]     cached plus new tokens; 0 for refused and ended requests
  *   slots      I64 [T]     pool row of every token, -1 for a refused one and behind the last
- *   pos        I32 [4 * T] rotary positions t, h, w, e of every token (text: all equal)
+ *   pos        I32 [4 * T] rotary positions t, h, w, e of every token: its place in the request
+ *                          four times, as text has them (a caller with image tokens writes theirs
+ *                          over it before the producers read it)
  * The pages of ended requests join the ring first (in the order of requests and
  * table entries), then pages leave it in the order of requests. A request is refused if
  * its tokens pass the table's W pages, if the n_new of the places up to it (ended ones

@@ -549,7 +549,8 @@ def paged_plan(state, ring, table, n_past, n_new, page, slots, pos=None, state_o
 
     state: int32 (4,) {first free place of the ring, free pages, ., .}; ring: int32
     (n_pages,); table: int32 (B, W); n_past, n_new: int32 (B,); slots: int64 (T,);
-    pos: int32 (4 * T,). A request that finds too few pages, too little room in its table row or in
+    pos: int32 (4 * T,), a token's place in its request four times (text; write over it for
+    images). A request that finds too few pages, too little room in its table row or in
     slots is refused whole: state_out[2] counts them. Places are served in order and a
     refused one's wants stay counted, so those behind it that need a page are refused too:
     plan it with n_new = 0 until state_out[1], the free pages, covers it."""
