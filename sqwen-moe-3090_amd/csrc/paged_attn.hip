@@ -203,7 +203,10 @@ Plan plan(int64_t n_tok, int64_t H, int64_t Hkv, int64_t B, int64_t max_q) {
 int launch_combine(const Call &c, hipStream_t s) {
     const int prof = profile_start("paged_merge", s);
     const int64_t rows = (int64_t)c.n_tok * c.H;
-    if (rows <= 128) {
+    // 16 workgroups a row below 128 rows: requests of 8000 keys with 16 rows each, the whole call
+    // with these and with a wavefront a row: 16 rows 11.5 and 23.9 us, 64 15.3 and 17.4, 112 20.9
+    // and 20.7, 128 22.8 and 21.8, 192 26.9 and 24.8.
+    if (rows < 128) {
         merge_dims_kernel<<<dim3((unsigned)rows, 16), dim3(kThreads), 0, s>>>(c);
     } else {
         // four heads a wavefront where that leaves wavefronts enough for the chip

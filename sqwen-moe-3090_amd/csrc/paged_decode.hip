@@ -6,8 +6,9 @@
 //   length inside a request, as many as workgroups are resident together (two per
 //   CU), or one per CU where that leaves a piece fewer than four tiles. Lengths are
 //   known on the GPU only: every wavefront takes the sums over the batch for itself,
-//   64 requests at a time (few_piece), and finds its piece, so no launch and no
-//   barrier stands before the work.
+//   64 requests at a time, and finds its piece (few_piece), so no launch stands before
+//   the work. Up to 64 requests are in its lanes, without a barrier; more go into LDS
+//   once, by all wavefronts, between two barriers.
 //   The KV heads of a piece run on one XCD, whose L2 serves the lines that the heads
 //   share in a row of Hkv x 144 bytes.
 //
@@ -157,11 +158,14 @@ __device__ __forceinline__ int tiles_of(const Call &c, int b, const Request &r, 
 }
 
 // Piece length: from total / P up to nearly twice that, the shortest whose pieces number
-// at most P, the workgroups that run together (of up to 256 requests; of more, the shortest
-// of 8 lengths); where no length does (as many requests as that) total / P, and the rest
-// follows as others end. Up to 64 requests are in a wavefront's lanes, more in LDS (read
-// again from memory for each of the sums, 1000 requests of up to 500 keys took 181 us
-// instead of 140; 16 a lane, the code for it cost every call 1.3 us).
+// at most P, the workgroups that run together: by bisection of up to 256 requests, of more
+// the shortest of 8 lengths. (Up to 64 in lanes the steps cost nothing; 128 requests of 2000
+// to 8000 keys 102.5 us with bisection and 105.3 with 8 lengths, 200 183.5 and 184.5, 300
+// 273.2 and 263.3, 1000 of 500 to 2000 316.9 and 264.1.) Where no length does (as many
+// requests as that) total / P, and the rest follows as others end. Up to 64 requests are in
+// a wavefront's lanes, more in LDS (read again from memory for each of the sums, 1000
+// requests of up to 500 keys took 181 us instead of 140; 16 a lane, the code for it cost
+// every call 1.3 us).
 __device__ __forceinline__ Piece few_piece(const Call &c, int *lds, int piece, int most) {
     const int lane = threadIdx.x & 63;
     const bool small = c.B <= 64;
