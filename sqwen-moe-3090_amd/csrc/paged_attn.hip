@@ -3,6 +3,8 @@
 //
 // Requests of few query rows (up to 16 per KV head; up to 8 where larger ones may be
 // in the call) go to paged_decode.hip, the others to paged_chunk.hip.
+#include <float.h>
+
 #include "paged_work.hpp"
 
 namespace sqa {
@@ -247,7 +249,10 @@ int launch_paged_attn(const PagedArgs &a, hipStream_t s) {
     c.n_tok = (int)q.ne[1], c.H = (int)q.ne[2], c.Hkv = (int)k.ne[1], c.G = c.H / c.Hkv;
     c.inv_g = 1.0f / (float)c.G;
     c.qscale = a.scale * kLog2e;
-    c.cap2 = a.softcap * kLog2e, c.cap_inv = a.softcap > 0.0f ? 1.0f / c.cap2 : 0.0f;
+    // (a cap beyond the range is none; the inverse of one below it stays finite, so that 0 stays 0)
+    c.cap2 = a.softcap * kLog2e;
+    if (c.cap2 > FLT_MAX) c.cap2 = 0.0f;
+    c.cap_inv = c.cap2 > 0.0f ? fminf(1.0f / c.cap2, FLT_MAX) : 0.0f;
     c.bias = a.max_bias;
     c.nl2 = 1;
     while (2 * c.nl2 <= c.H) c.nl2 *= 2;

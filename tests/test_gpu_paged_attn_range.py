@@ -32,3 +32,14 @@ def test_long_requests_that_share_a_page_in_the_smallest_workspace(sqa, dev):
         sqa.paged_attn(q, *pools, table, start, torch.full((B,), kv, dtype=torch.int32, device=dev), 1, out=o, workspace=ws)
     torch.cuda.synchronize()
     assert float((out[1] - out[0]).norm() / out[0].norm()) <= 3e-3
+
+
+@pytest.mark.parametrize("new,past", [([1, 2], [0, 300]), ([60, 1], [90, 700])])
+@pytest.mark.parametrize("cap", [1e-45, 1e-40, 1e-30, 1e30, 2.3e38, 2.5e38, 3.4e38])
+def test_caps_of_any_size(sqa, orc, dev, new, past, cap):
+    """A cap far below the logits leaves equal weights, one far above them leaves them as they are."""
+    from test_gpu_paged_attn import Batch, call, close
+
+    b = Batch(orc, 5, new, past, page=32, scale_q=3.0)
+    b.q[-1, :3] = 0  # logits of 0 exactly
+    close(call(sqa, dev, b, softcap=cap), b.ref(orc, cap=float(torch.tensor(cap, dtype=torch.float32))))
