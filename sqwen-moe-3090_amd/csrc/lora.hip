@@ -23,8 +23,9 @@
 // pair in the same way, turned in LDS into rows of 64 columns (32 above rank 64, for want
 // of registers) for base and out. The adapters of a tile are taken by kPasses workgroups in
 // turn, each writing its tokens alone; no adapter's values reach another one's tokens, not
-// even its NaN. 4096 tokens in runs of 512: rank 16 45 us, 4.5 TB/s (a copy: 4.98), rank 64
-// 60 (67 from call to call), where A and B out of L2 are as many bytes as x and gate.
+// even its NaN. 4096 tokens in runs of 512: rank 16 43 us, 4.7 TB/s (a copy: 4.98), rank 64
+// 46, where A and B out of L2 are as many bytes as x and gate; in runs of 342 to 512, with
+// tokens without adapter between them and others in the next call, 67.
 #include <mutex>
 
 #include "paged.hpp"
@@ -509,9 +510,11 @@ int launch_lora_add(const sqa_tensor &base, const sqa_tensor &x, const sqa_tenso
                    (int)a.ne[1], (int)a.ne[2], (int)x.ne[1]};
     const int prof = profile_start("lora_add", s);
     // A workgroup per token up to two a CU: with K 4096 and N 2048, 512 tokens that change
-    // between 8 adapters take 11 us at rank 16, 27 at 64, 49 at 128, where tiles take 35, 53,
-    // 85; that share them by 128 11, 27, 45 against 18, 28, 43. 768 that share take 16, 35, 61
-    // against 19, 29, 43.
+    // between 8 adapters take 12.8 us at rank 16, 26.7 at 64, 43.1 at 128, where tiles take
+    // 32.3, 53.2, 83.4; that share them by 128 12.8, 26.7, 43.8 against 19.5, 30.7, 45.9. 768
+    // that share take 18.7, 39.0, 62.8 against 22.8, 33.9, 50.1; that change 18.5, 38.7, 62.1
+    // against 34.9, 55.4, 85.4. A token's workgroup reads its adapter whole out of L2: at rank 64
+    // the 512 read 400 MB, 15 TB/s.
     if (p.M <= 512 && p.K <= 16 * 1024) {
         // (below 97 tokens parts of the columns fill the other CUs)
         const dim3 grid((unsigned)p.M, p.M <= 32 ? 4 : p.M <= 96 ? 2 : 1);

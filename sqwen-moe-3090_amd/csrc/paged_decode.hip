@@ -285,6 +285,7 @@ __device__ __forceinline__ int lds_byte(int row, int c) {
 // TWO = false: requests of up to 8 query rows per KV head (one block-diagonal B set).
 // TWO = true : up to 16 rows (rows 0-7 and 8-15 as two B sets, one A operand).
 // OPT: the logits are capped or biased. PLAN: a last workgroup plans the many-row kernel.
+// (128 registers a lane; TWO with OPT and PLAN keeps one more in scratch, the others none.)
 template <bool TWO, bool OPT, bool PLAN>
 __global__ __launch_bounds__(kThreads, 4) void paged_few_kernel(Call p) {
     extern __shared__ __align__(16) uint8_t smem[];

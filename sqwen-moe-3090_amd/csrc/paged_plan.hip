@@ -13,8 +13,9 @@
 // ended request that gives it).
 //
 // Bound by latency: a dependent chain of loads (lengths, table or ring entry), two scans
-// and the launch; a step's arrays are some 10 to 300 KB: 8 requests 4.4 us, 1024 requests
-// with 8192 tokens 8.8 (an empty launch: 3.6). Every workgroup takes the
+// and the launch; a step's arrays are some 10 to 300 KB: 8 requests 3.8 us (4.6 from call to
+// call, the host's time), 1024 requests with 8192 tokens 8.5 (8.6); an empty launch takes
+// 3.6. 256 threads, so four of 1024 requests each in the scans. Every workgroup takes the
 // prefix sums again for itself (B lengths, in LDS) instead of waiting for another
 // one's, so one launch does all; tokens, table entries and returned pages are then
 // spread over the workgroups, none of which reads what another one writes: a token
@@ -87,7 +88,7 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PlanArgs a) {
     count = min(max(count, 0), n_pages);
 
     // the lengths, read once and 4 at a time (by the thread of their run, a latency after the
-    // other, 1024 requests took 10.1 us, with the sums by shuffles; now 8.8)
+    // other, 1024 requests took 10.1 us, with the sums by shuffles; now 8.6)
     constexpr int kBatch = 4;
     for (int b = tid; b < a.B; b += kBatch * kThreads) {
         int32_t p[kBatch], n[kBatch];
