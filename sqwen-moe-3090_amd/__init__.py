@@ -855,7 +855,8 @@ class PagedKvCache:
         return self._now[4:]
 
     def new_step(self, n_rows):
-        """Buffers of a step of up to n_rows tokens (kept by the caller, reused step after step)."""
+        """Buffers of a step of up to n_rows tokens (kept by the caller, reused step after step). state and
+        n_past are the cache's own: every step's show what plan() made last."""
         i32, B, dev = torch.int32, self.table.shape[0], self.table.device
         return PagedStep(self._next[:4], self._next[4:], torch.zeros(B + 1, dtype=i32, device=dev),
                          torch.zeros(B, dtype=i32, device=dev), torch.zeros(n_rows, dtype=torch.int64, device=dev),
