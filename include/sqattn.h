@@ -93,6 +93,18 @@ int sqa_set_rows_q4_0(const sqa_tensor *dst, const sqa_tensor *src, const sqa_te
  * (reference: src/backend/ffi.rs:361-362). Returns 1 if supported. */
 int sqa_supports_set_rows(const sqa_tensor *dst, const sqa_tensor *src, const sqa_tensor *idx);
 
+/*
+ * Cached rows read back: dst[i, :] = the values of row idx[i] of src, (code - 8) * d exactly,
+ * rounded once where dst is F16. The counterpart of set_rows (ggml's GGML_OP_GET_ROWS).
+ *   src: Q4_0 [ne0, src_rows] (row stride src->nb[1], even)
+ *   idx: I64 [n_rows] (element stride idx->nb[0]); rows may come more than once
+ *   dst: F32 or F16 [ne0, n_rows] (row stride dst->nb[1], elements contiguous)
+ * ne0 % 32 == 0. An index outside [0, src->ne[1]) reads as a row of zeros (the slots of -1 that a
+ * page plan gives). dst must not overlap src or idx.
+ */
+int sqa_get_rows_q4_0(const sqa_tensor *dst, const sqa_tensor *src, const sqa_tensor *idx, void *stream);
+int sqa_supports_get_rows(const sqa_tensor *dst, const sqa_tensor *src, const sqa_tensor *idx);
+
 /* ------------------------------------------------------------------------ */
 /* K/Q producer: per-head RMSNorm, IMROPE, q4_0 quantize-on-write            */
 /* ------------------------------------------------------------------------ */
@@ -142,6 +154,28 @@ int sqa_rope_norm_f32(const sqa_tensor *dst, const sqa_tensor *src, const sqa_te
  * 361-362). Returns 1 if the call with these operands would run. */
 int sqa_supports_rope_norm(const sqa_tensor *dst, const sqa_tensor *src, const sqa_tensor *norm_w,
                            const sqa_tensor *pos, const sqa_rope *rope, const sqa_tensor *idx);
+
+/*
+ * Cached rows moved, keys to other positions: row to[i] of dst = row from[i] of src, whose heads'
+ * first n_rot dims are rotated on by delta (a conversation that drops its oldest part, a cached
+ * passage behind another prompt).
+ *   src   Q4_0 [D, n_head, src_rows]  nb = 18, D / 32 * 18, row stride nb[2] (even)
+ *   dst   Q4_0 [D, n_head, dst_rows]  the same; may be src itself
+ *   to, from I64 [n]; a row with either outside its cache is skipped
+ *   delta I32 [4 * n] contiguous: how far each of the positions t, h, w, e moves, any sign; with
+ *         rope NULL both are NULL and rows are copied as they are (V; any D % 32 == 0)
+ * Pairs, sections and directions as in sqa_rope_norm_set_rows_q4_0, angle delta * freq_scale *
+ * freq_base^(-2 ic / n_rot) in 64 bits, cos and sin of it rounded to fp32; attn_factor, which the
+ * cached values have already, plays no part. Blocks that hold a rotated dim are quantized again
+ * (quantize_row_q4_0), the others' bytes stay. D of 64, 128 or 256 with a rope.
+ * In place (dst is src) a row that one entry reads must be no other entry's to[]: from == to is
+ * fine, as are ranges that do not meet; otherwise, and where to[] names a row twice, that row is
+ * unspecified. dst overlaps nothing else.
+ */
+int sqa_move_rows_q4_0(const sqa_tensor *dst, const sqa_tensor *src, const sqa_tensor *to, const sqa_tensor *from,
+                       const sqa_tensor *delta, const sqa_rope *rope, void *stream);
+int sqa_supports_move_rows(const sqa_tensor *dst, const sqa_tensor *src, const sqa_tensor *to, const sqa_tensor *from,
+                           const sqa_tensor *delta, const sqa_rope *rope);
 
 /* ------------------------------------------------------------------------ */
 /* flash_attn_ext                                                            */
@@ -359,6 +393,56 @@ int sqa_supports_paged_attn(const sqa_tensor *q, const sqa_tensor *k, const sqa_
                             float logit_softcap, const sqa_tensor *dst);
 
 /*
+ * Requests that share cached keys. A group is a row of a page table (shared_table) and a
+ * length; a request of group g continues its first shared_len[g] keys: they come before the
+ * request's own, which its own row of the batch's table holds (the plan knows only those). The
+ * shared table may be the batch's own table and the group a place of it, a request that holds a
+ * prompt for the others. One level: of that request, only its own pages are continued.
+ *
+ * Once per step, who shares what:
+ *   q_start I32 [B + 1], kv_len I32 [B]   as sqa_paged_plan writes them
+ *   group       I32 [B]      group of every request; outside [0, G): none
+ *   shared_len  I32 [G]      keys of every group
+ *   members     I32 [T]      token rows of the members (a group of no keys and a request with
+ *                            kv_len <= 0 have none), by group, request and token; -1 behind the last
+ *   m_start     I32 [G + 1]  group g's are members[m_start[g]] .. members[m_start[g + 1] - 1]
+ *   m_pos       I32 [T]      their positions, shared_len[g] + kv_len[b] - n + i; -1 behind the last
+ *   token_group I32 [T]      group of every token row, -1 for none and for rows of no request
+ *   pos         I32 [4 * T]  or NULL: m_pos goes to the members' rotary positions, four times (as
+ *                            sqa_paged_plan lays them out); those of other tokens stay
+ * All contiguous; what is written overlaps nothing. B, G <= 4096, T <= 2^24.
+ */
+int sqa_paged_share(const sqa_tensor *q_start, const sqa_tensor *kv_len, const sqa_tensor *group,
+                    const sqa_tensor *shared_len, const sqa_tensor *members, const sqa_tensor *m_start,
+                    const sqa_tensor *m_pos, const sqa_tensor *token_group, const sqa_tensor *pos, void *stream);
+
+/*
+ * sqa_paged_attn of requests that share keys: every token of group g sees the group's first
+ * shared_len[g] keys, and its own as in sqa_paged_attn, under one softmax; a group's keys are read
+ * and multiplied once for all its tokens. The distance |p - j| of max_bias is from m_pos to the
+ * shared key's place, and between own keys as there.
+ *   shared_table I32 [W', G]  row stride nb[1]; shared_len I32 [G]
+ *   members, m_pos, token_group I32 [n_tok], m_start I32 [G + 1]   as sqa_paged_share writes them
+ * Everything else, and what is refused, as in sqa_paged_attn; shared keys on pages outside the pool
+ * are not seen. With members, m_start, m_pos and token_group of another call results are
+ * unspecified, memory stays safe.
+ * workspace: sqa_paged_attn_shared_workspace_size bytes; a smaller one takes fewer splits of
+ * the keys, down to one per request, group tile and KV head; below that SQA_ERR_WORKSPACE.
+ */
+int sqa_paged_attn_shared(const sqa_tensor *q, const sqa_tensor *k, const sqa_tensor *v,
+                          const sqa_tensor *table, const sqa_tensor *q_start, const sqa_tensor *kv_len,
+                          const sqa_tensor *prefix, const sqa_tensor *shared_table, const sqa_tensor *shared_len,
+                          const sqa_tensor *members, const sqa_tensor *m_start, const sqa_tensor *m_pos,
+                          const sqa_tensor *token_group, int64_t max_q, float scale, float max_bias,
+                          float logit_softcap, const sqa_tensor *gate, const sqa_tensor *dst,
+                          void *workspace, size_t workspace_bytes, void *stream);
+size_t sqa_paged_attn_shared_workspace_size(const sqa_tensor *q, const sqa_tensor *k, const sqa_tensor *table,
+                                            const sqa_tensor *shared_table, int64_t max_q);
+int sqa_supports_paged_attn_shared(const sqa_tensor *q, const sqa_tensor *k, const sqa_tensor *v,
+                                   const sqa_tensor *table, const sqa_tensor *shared_table, int64_t max_q,
+                                   float scale, float max_bias, float logit_softcap, const sqa_tensor *dst);
+
+/*
  * Low-rank adapters of many requests beside a shared projection:
  *   dst[:, m] = base[:, m] + scale[i] * B_i (A_i (x[:, m] * sigmoid(gate[:, m]))),  i = ids[m]
  *   base  F32 [N, M]  the shared projection's output; may be dst itself (dst that overlaps
@@ -434,7 +518,8 @@ int sqa_profile_begin(int32_t max_records);
 int sqa_profile_end(void);
 /* Synchronise and sum the recorded durations of one kernel: "fa_decode",
  * "fa_combine", "fa_prefill", "set_rows_q4_0", "sigmoid_mul", "paged_plan",
- * "paged_decode", "paged_chunk", "paged_merge", "lora_add". */
+ * "paged_decode", "paged_chunk", "paged_merge", "lora_add", "get_rows_q4_0", "move_rows_q4_0",
+ * "paged_share", "paged_shared", "paged_shared_merge". */
 int sqa_profile_get(const char *kernel, double *total_ms, int64_t *count);
 
 #ifdef __cplusplus

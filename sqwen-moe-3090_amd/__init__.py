@@ -20,6 +20,7 @@ import collections
 import ctypes
 import importlib.machinery
 import importlib.util
+import math
 import struct
 import os
 
@@ -31,7 +32,8 @@ __all__ = [
     "flash_attn_workspace_size", "out_proj", "out_proj_workspace_size", "KvCache", "cache_view", "row_bytes", "profile_begin", "profile_end",
     "profile_get", "Rope", "rope_params", "rope_norm_set_rows_q4_0", "rope_norm_f32",
     "paged_plan", "paged_attn", "paged_attn_workspace_size", "supports_paged_attn", "PagedStep", "PagedKvCache",
-    "lora_add", "supports_lora_add",
+    "lora_add", "supports_lora_add", "get_rows_q4_0", "move_rows_q4_0",
+    "paged_share", "paged_attn_shared", "paged_attn_shared_workspace_size", "supports_paged_attn_shared", "PagedShare",
 ]
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -148,6 +150,14 @@ def lib():
             "sqa_paged_attn": (ctypes.c_int, [P, P, P, P, P, P, P, i64, f32, f32, f32, P, P, vp, sz, vp]),
             "sqa_paged_attn_workspace_size": (sz, [P, P, P, i64]),
             "sqa_supports_paged_attn": (ctypes.c_int, [P, P, P, P, i64, f32, f32, f32, P]),
+            "sqa_get_rows_q4_0": (ctypes.c_int, [P, P, P, vp]),
+            "sqa_supports_get_rows": (ctypes.c_int, [P, P, P]),
+            "sqa_move_rows_q4_0": (ctypes.c_int, [P, P, P, P, P, ctypes.POINTER(Rope), vp]),
+            "sqa_supports_move_rows": (ctypes.c_int, [P, P, P, P, P, ctypes.POINTER(Rope)]),
+            "sqa_paged_share": (ctypes.c_int, [P] * 9 + [vp]),
+            "sqa_paged_attn_shared": (ctypes.c_int, [P] * 13 + [i64, f32, f32, f32, P, P, vp, sz, vp]),
+            "sqa_paged_attn_shared_workspace_size": (sz, [P, P, P, P, i64]),
+            "sqa_supports_paged_attn_shared": (ctypes.c_int, [P, P, P, P, P, i64, f32, f32, f32, P]),
             "sqa_lora_add": (ctypes.c_int, [P, P, P, P, P, P, P, P, vp]),
             "sqa_supports_lora_add": (ctypes.c_int, [P, P, P, P, P, P]),
             "sqa_profile_begin": (ctypes.c_int, [i32]),
@@ -163,6 +173,7 @@ def lib():
     return _lib
 
 
+_FLOATS = {torch.float32: (TYPE_F32, 4), torch.float16: (TYPE_F16, 2)}
 _host = None
 
 
@@ -287,6 +298,66 @@ def set_rows_q4_0(cache, src, idx, stream=None):
     ti = Tensor.make(TYPE_I64, [idx.shape[0]], [idx.stride(0) * 8], idx.data_ptr())
     _check(lib().sqa_set_rows_q4_0(ctypes.byref(td), ctypes.byref(ts), ctypes.byref(ti), _stream(stream)))
     return cache
+
+
+def get_rows_q4_0(cache, idx, out=None, dtype=torch.float32, stream=None):
+    """out[i] = the values of cache row idx[i] (GGML_OP_GET_ROWS of a q4_0 cache): set_rows_q4_0's counterpart.
+
+    cache: uint8 (rows, ..., row_bytes) contiguous; idx: int64 (n,), an index outside the cache reads as zeros;
+    out: float32 or float16 (n, ne0) with contiguous elements, made here of dtype where it is not given."""
+    if stream is None and out is not None:
+        rc = (_host or _load_host()).get_rows(cache, idx, out)
+        if rc is not None:
+            if rc:
+                _check(rc)
+            return out
+    with _on(cache.device, idx=idx, out=out):
+        _need(cache.dim() >= 2 and cache.dtype == torch.uint8 and cache.is_contiguous(), "cache must be contiguous uint8 (rows, ...)")
+        _need(idx.dim() == 1 and idx.dtype == torch.int64, "idx must be int64 (n,)")
+        rb, n = math.prod(cache.shape[1:]), idx.shape[0]
+        ne0 = rb // Q4_0_BLOCK * QK4_0
+        if out is None:
+            _need(dtype in _FLOATS, "dtype must be float32 or float16")
+            out = _make(stream, cache.device, lambda: torch.empty((n, ne0), dtype=dtype, device=cache.device))
+        _need(out.dim() == 2 and out.dtype in _FLOATS and (out.shape[1] <= 1 or out.stride(1) == 1),
+              "out must be float32 or float16 (n, ne0) with contiguous elements")
+        code, size = _FLOATS[out.dtype]
+        to = Tensor.make(code, [out.shape[1], out.shape[0]], [size, out.stride(0) * size], out.data_ptr())
+        ts = Tensor.make(TYPE_Q4_0, [ne0, cache.shape[0]], [Q4_0_BLOCK, rb], cache.data_ptr())
+        ti = Tensor.make(TYPE_I64, [n], [idx.stride(0) * 8], idx.data_ptr())
+        _check(lib().sqa_get_rows_q4_0(ctypes.byref(to), ctypes.byref(ts), ctypes.byref(ti), _stream(stream)))
+    return out
+
+
+def _heads_desc(cache, name):
+    _need(cache.dim() == 3 and cache.dtype == torch.uint8 and cache.is_contiguous() and cache.shape[2] % Q4_0_BLOCK == 0,
+          f"{name} must be contiguous uint8 (rows, n_head, D // 32 * 18)")
+    rows, heads, rb = cache.shape
+    return Tensor.make(TYPE_Q4_0, [rb // Q4_0_BLOCK * QK4_0, heads, rows], [Q4_0_BLOCK, rb, heads * rb], cache.data_ptr())
+
+
+def move_rows_q4_0(dst, src, to, from_, delta=None, rope=None, stream=None):
+    """dst[to[i]] = src[from_[i]], with a rope the heads' first n_rot dims rotated on by delta and quantized again: cached
+    keys at other positions (a context that drops its oldest part, a cached passage behind another prompt).
+
+    dst, src: uint8 (rows, n_head, D//32*18) contiguous, dst may be src; to, from_: int64 (n,), entries outside a cache
+    are skipped; delta: int32 (4*n,), how far the positions t, h, w, e move; without delta and rope rows are copied (V).
+    In place a row that one entry reads must be no other entry's to (from_ == to is fine)."""
+    if stream is None and (rope is None or isinstance(rope, Rope)):
+        rc = (_host or _load_host()).move_rows(dst, src, to, from_, delta, rope)
+        if rc is not None:
+            if rc:
+                _check(rc)
+            return dst
+    with _on(dst.device, src=src, to=to, from_=from_, delta=delta):
+        td, ts = _heads_desc(dst, "dst"), _heads_desc(src, "src")
+        for t, name in ((to, "to"), (from_, "from_")):
+            _need(t.dim() == 1 and t.dtype == torch.int64, f"{name} must be int64 (n,)")
+        tt, tf = (Tensor.make(TYPE_I64, [t.shape[0]], [t.stride(0) * 8], t.data_ptr()) for t in (to, from_))
+        tl = None if delta is None else _vec(delta, torch.int32, "delta")
+        _check(lib().sqa_move_rows_q4_0(ctypes.byref(td), ctypes.byref(ts), ctypes.byref(tt), ctypes.byref(tf), _ref(tl),
+                                        _ref(rope), _stream(stream)))
+    return dst
 
 
 def _producer_descs(src, norm_w, pos):
@@ -653,6 +724,112 @@ def paged_attn(q, k_pool, v_pool, table, q_start, kv_len, max_q, scale=None, max
     return out
 
 
+class PagedShare(collections.namedtuple("PagedShare", "members m_start m_pos token_group")):
+    """What paged_share gives for one step: the operands of paged_attn_shared."""
+
+    __slots__ = ()
+
+
+def paged_share(q_start, kv_len, group, shared_len, members, m_start=None, m_pos=None, token_group=None, pos=None, stream=None):
+    """Which of a step's tokens go with which shared prefix, on the GPU, once per step: request b continues the first
+    shared_len[group[b]] keys of its group (group: int32 (B,), outside [0, G) for none; shared_len: int32 (G,)).
+
+    members: int32 (T,), made into the members' token rows by group, request and token; m_start: int32 (G + 1,) where a
+    group's begin; m_pos: int32 (T,) their positions behind the shared keys; token_group: int32 (T,) the group of every
+    token row, -1 for none. Those not given are made here; all are returned as a PagedShare. pos: int32 (4 * T,) as
+    paged_plan wrote it: the members' rotary positions are moved behind the shared keys (None: left alone). Requests with
+    kv_len <= 0 (refused ones) and groups of no keys have no members."""
+    if m_start is None or m_pos is None or token_group is None:
+        _need(stream is None or members.is_cuda, "tensors must be on the GPU")
+
+        def new(t, n):
+            if t is not None:
+                return t
+            return _make(stream, members.device, lambda: torch.empty(n, dtype=torch.int32, device=members.device))
+
+        T = members.shape[0]
+        m_start, m_pos, token_group = new(m_start, shared_len.shape[0] + 1), new(m_pos, T), new(token_group, T)
+    share = PagedShare(members, m_start, m_pos, token_group)
+    if stream is None:
+        rc = (_host or _load_host()).share(q_start, kv_len, group, shared_len, *share, pos)
+        if rc is not None:
+            if rc:
+                _check(rc)
+            return share
+    names = ("q_start", "kv_len", "group", "shared_len", "members", "m_start", "m_pos", "token_group", "pos")
+    ts = dict(zip(names, (q_start, kv_len, group, shared_len, *share, pos)))
+    with _on(members.device, **ts):
+        d = [None if t is None else _vec(t, torch.int32, name) for name, t in ts.items()]
+        _check(lib().sqa_paged_share(*[_ref(t) for t in d], _stream(stream)))
+    return share
+
+
+def paged_attn_shared_workspace_size(q, k_pool, table, shared_table, max_q):
+    """Workspace bytes of paged_attn_shared for these shapes (a smaller one takes fewer splits)."""
+    tq, tk, tt, ts = _tokens_desc(q, "q"), _pool_desc(k_pool, "k_pool"), _table_desc(table), _table_desc(shared_table)
+    return int(lib().sqa_paged_attn_shared_workspace_size(ctypes.byref(tq), ctypes.byref(tk), ctypes.byref(tt),
+                                                          ctypes.byref(ts), int(max_q)))
+
+
+def supports_paged_attn_shared(q, k_pool, table, shared_table, max_q, scale=None, max_bias=0.0, softcap=0.0):
+    n_tok, H, D = q.shape
+    scale = D ** -0.5 if scale is None else scale
+    tq, tk, tt, ts = _tokens_desc(q, "q"), _pool_desc(k_pool, "k_pool"), _table_desc(table), _table_desc(shared_table)
+    to = Tensor.make(TYPE_F32, [D, H, n_tok, 1], [4, D * 4, H * D * 4], 16)
+    return bool(lib().sqa_supports_paged_attn_shared(ctypes.byref(tq), ctypes.byref(tk), ctypes.byref(tk), ctypes.byref(tt),
+                                                     ctypes.byref(ts), int(max_q), scale, max_bias, softcap, ctypes.byref(to)))
+
+
+def paged_attn_shared(q, k_pool, v_pool, table, q_start, kv_len, shared_table, shared_len, share, max_q, scale=None,
+                      max_bias=0.0, softcap=0.0, prefix=None, gate=None, out=None, workspace=None, stream=None):
+    """paged_attn of requests that continue shared prefixes: the tokens of group g see the first shared_len[g] keys of
+    the pages in shared_table[g], read once for all of them, and their own keys as in paged_attn, under one softmax.
+
+    shared_table: int32 (G, W'), may be table itself with a place of the batch as the group; shared_len: int32 (G,);
+    share: paged_share's PagedShare of this step (T == n_tok); the rest as in paged_attn."""
+    if stream is None and out is not None and workspace is not None and isinstance(share, tuple) and len(share) == 4:
+        rc = (_host or _load_host()).attn_shared(q, k_pool, v_pool, table, q_start, kv_len, prefix, shared_table, shared_len,
+                                                 *share, max_q, scale, max_bias, softcap, gate, out, workspace)
+        if rc is not None:
+            if rc:
+                _check(rc)
+            return out
+    members, m_start, m_pos, token_group = share
+    with _on(q.device, k_pool=k_pool, v_pool=v_pool, table=table, q_start=q_start, kv_len=kv_len, prefix=prefix,
+             shared_table=shared_table, shared_len=shared_len, members=members, m_start=m_start, m_pos=m_pos,
+             token_group=token_group, gate=gate, out=out, workspace=workspace):
+        tq, tk, tv = _tokens_desc(q, "q"), _pool_desc(k_pool, "k_pool"), _pool_desc(v_pool, "v_pool")
+        n_tok, H, D = q.shape
+        scale = D ** -0.5 if scale is None else scale
+        if out is None:
+            out = _make(stream, q.device, lambda: torch.zeros((n_tok, H, D), dtype=torch.float32, device=q.device))
+        _need(out.dtype == torch.float32 and out.dim() == 3 and out.is_contiguous(), "out must be contiguous float32 (n_tok, H, D)")
+        tt, tst, to = _table_desc(table), _table_desc(shared_table), out_desc(out)
+        i32 = torch.int32
+        tp = None if prefix is None else _vec(prefix, i32, "prefix")
+        d = [_vec(t, i32, name) for t, name in ((q_start, "q_start"), (kv_len, "kv_len"))]
+        e = [_vec(t, i32, name) for t, name in ((shared_len, "shared_len"), (members, "members"), (m_start, "m_start"),
+                                                (m_pos, "m_pos"), (token_group, "token_group"))]
+        tg = None
+        if gate is not None:
+            _need(gate.dim() == 3 and gate.dtype == torch.float32 and gate.shape == q.shape and
+                  (gate.shape[2] <= 1 or gate.stride(2) == 1), "gate must be float32 like q")
+            tg = Tensor.make(TYPE_F32, [D, H, n_tok, 1], [4, gate.stride(1) * 4, gate.stride(0) * 4], gate.data_ptr())
+        _need(q.shape[2] <= 1 or q.stride(2) == 1, "q rows must have unit element stride")
+        if workspace is None:
+            need = int(lib().sqa_paged_attn_shared_workspace_size(ctypes.byref(tq), ctypes.byref(tk), ctypes.byref(tt),
+                                                                  ctypes.byref(tst), int(max_q)))
+            workspace = _make(stream, q.device, lambda: _workspace(need, q.device)[0])
+        _need(workspace is None or workspace.is_contiguous(), "workspace must be contiguous")
+        _check(lib().sqa_paged_attn_shared(ctypes.byref(tq), ctypes.byref(tk), ctypes.byref(tv), ctypes.byref(tt),
+                                           *[ctypes.byref(t) for t in d], _ref(tp), ctypes.byref(tst),
+                                           *[ctypes.byref(t) for t in e], int(max_q), scale, max_bias, softcap, _ref(tg),
+                                           ctypes.byref(to), workspace.data_ptr() if workspace is not None else None,
+                                           workspace.numel() * workspace.element_size() if workspace is not None else 0,
+                                           _stream(stream)))
+    return out
+
+
 def _lora_descs(base, x, a, b, gate, out):
     for t, name in ((base, "base"), (x, "x"), (gate, "gate"), (out, "out")):
         _need(t is None or (t.dim() == 2 and t.dtype == torch.float32 and (t.shape[1] <= 1 or t.stride(1) == 1)),
@@ -792,6 +969,16 @@ class KvCache:
         _check(lib().sqa_kv_cache_append(self._h, slot, ctypes.byref(tk), ctypes.byref(tv), ctypes.byref(ti),
                                          _stream(stream)))
 
+    def read(self, slot, idx, which="k", out=None, dtype=torch.float32, stream=None):
+        """Layer `slot`'s cached K or V of rows idx (int64) as values (n, Hkv*D), float32 or float16."""
+        return get_rows_q4_0((self.k if which == "k" else self.v)[slot], idx, out=out, dtype=dtype, stream=stream)
+
+    def move(self, slot, to, from_, delta, rope, stream=None):
+        """Rows from_ of layer `slot` to rows to, K rotated on by delta (int32 (4*n,)) and V as it is; a row of from_
+        must be no other entry's to (a long move down goes in pieces of at most its own distance, lowest first)."""
+        move_rows_q4_0(self.k[slot], self.k[slot], to, from_, delta, rope, stream=stream)
+        move_rows_q4_0(self.v[slot], self.v[slot], to, from_, stream=stream)
+
     def workspace_size(self, slot, q):
         """Workspace bytes of attend() for q over the current [0, n_kv_padded) views."""
         n_q, H, D = q.shape
@@ -880,10 +1067,38 @@ class PagedKvCache:
             set_rows_q4_0(self.rows(layer, "k"), k_cur, step.slots)
             set_rows_q4_0(self.rows(layer, "v"), v_cur, step.slots)
 
-    def workspace_size(self, q, max_q):
+    def read(self, layer, slots, which="k", out=None, dtype=torch.float32, stream=None):
+        """The layer's cached K or V at pool rows slots (int64, -1 reads as zeros) as values (n, Hkv*D)."""
+        return get_rows_q4_0(self.rows(layer, which), slots, out=out, dtype=dtype, stream=stream)
+
+    def move(self, layer, to, from_, delta, rope, stream=None):
+        """Pool rows from_ of the layer to rows to, K rotated on by delta (int32 (4*n,)) and V as it is; a row of from_
+        must be no other entry's to."""
+        move_rows_q4_0(self.rows(layer, "k"), self.rows(layer, "k"), to, from_, delta, rope, stream=stream)
+        move_rows_q4_0(self.rows(layer, "v"), self.rows(layer, "v"), to, from_, stream=stream)
+
+    def new_share(self, n_rows):
+        """Buffers of share() for steps of up to n_rows tokens (kept by the caller, reused step after step)."""
+        dev = self.table.device
+        return PagedShare(*(torch.zeros(n, dtype=torch.int32, device=dev)
+                            for n in (n_rows, self.table.shape[0] + 1, n_rows, n_rows)))
+
+    def share(self, parent, step, share, stream=None):
+        """After plan(): request b of this step continues all cached keys of place parent[b] (int32 (max_requests,),
+        -1 for none), which holds a prompt for several requests; its own pages and lengths count its own tokens only.
+        The members' positions in step.pos move behind the parent's keys. A parent has no parent that counts, and must
+        not end or grow while others continue it."""
+        return paged_share(step.q_start, step.kv_len, parent, step.n_past, *share, pos=step.pos, stream=stream)
+
+    def workspace_size(self, q, max_q, share=None):
+        if share is not None:
+            return paged_attn_shared_workspace_size(q, self.k[0], self.table, self.table, max_q)
         return paged_attn_workspace_size(q, self.k[0], self.table, max_q)
 
-    def attend(self, layer, q, step, max_q, **options):
-        """paged_attn of the step's tokens over the layer's pages (options: scale, max_bias, softcap, prefix, gate,
-        out, workspace, stream)."""
+    def attend(self, layer, q, step, max_q, share=None, **options):
+        """paged_attn of the step's tokens over the layer's pages, with share() paged_attn_shared (options: scale,
+        max_bias, softcap, prefix, gate, out, workspace, stream)."""
+        if share is not None:
+            return paged_attn_shared(q, self.k[layer], self.v[layer], self.table, step.q_start, step.kv_len, self.table,
+                                     step.n_past, share, max_q, **options)
         return paged_attn(q, self.k[layer], self.v[layer], self.table, step.q_start, step.kv_len, max_q, **options)

@@ -183,6 +183,68 @@ PyObject *set_rows(PyObject *, PyObject *const *a, Py_ssize_t n) {
     });
 }
 
+// every tensor of a call on the current device (the general path switches to theirs)
+void here(std::initializer_list<PyObject *> ts) {
+    const int dev = (int)c10::hip::current_device();
+    for (PyObject *o : ts) {
+        if (o == Py_None) continue;
+        const at::Tensor &t = tensor(o);
+        need(t.is_cuda() && t.get_device() == dev);
+    }
+}
+
+// (n,) row indices
+sqa_tensor places(const at::Tensor &t) {
+    need(t.dim() == 1 && t.scalar_type() == at::kLong);
+    return index(t, SQA_TYPE_I64, t.stride(0) * 8);
+}
+
+// cache, idx, out
+PyObject *get_rows(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    return answer([&]() -> int {
+        need(n == 3);
+        here({a[0], a[1], a[2]});
+        const at::Tensor &c = tensor(a[0]), &o = tensor(a[2]);
+        need(c.dim() >= 2 && c.scalar_type() == at::kByte && c.is_contiguous() && o.dim() == 2 &&
+             (o.scalar_type() == at::kFloat || o.scalar_type() == at::kHalf) && (o.size(1) <= 1 || o.stride(1) == 1));
+        const int64_t ne0 = o.size(1), e = (int64_t)o.element_size(), s = o.stride(0) * e;
+        const sqa_tensor ts = cache_rows(c, ne0), ti = places(tensor(a[1])),
+                         to = make(e == 4 ? SQA_TYPE_F32 : SQA_TYPE_F16, o, ne0, o.size(0), 1, e, s, s * o.size(0), s * o.size(0));
+        void *st = stream();
+        return without_gil([&] { return sqa_get_rows_q4_0(&to, &ts, &ti, st); });
+    });
+}
+
+// dst, src, to, from, delta, rope (both or neither None)
+PyObject *move_rows(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    Py_buffer view{};
+    PyObject *r = answer([&]() -> int {
+        need(n == 6);
+        here({a[0], a[1], a[2], a[3], a[4]});
+        auto heads = [](const at::Tensor &t) {
+            need(t.dim() == 3 && t.scalar_type() == at::kByte && t.is_contiguous() && t.size(2) % SQA_Q4_0_BLOCK_BYTES == 0);
+            const int64_t rb = t.size(2), row = rb * t.size(1);
+            return make(SQA_TYPE_Q4_0, t, rb / SQA_Q4_0_BLOCK_BYTES * SQA_QK4_0, t.size(1), t.size(0), SQA_Q4_0_BLOCK_BYTES, rb,
+                        row, row * t.size(0));
+        };
+        const sqa_tensor td = heads(tensor(a[0])), ts = heads(tensor(a[1])), tt = places(tensor(a[2])), tf = places(tensor(a[3]));
+        sqa_tensor tl;
+        const bool turn = a[4] != Py_None;
+        need(turn == (a[5] != Py_None));
+        if (turn) {
+            const at::Tensor &d = tensor(a[4]);
+            need(d.dim() == 1 && d.scalar_type() == at::kInt && d.is_contiguous());
+            tl = index(d, SQA_TYPE_I32, 4);
+            need(PyObject_GetBuffer(a[5], &view, PyBUF_SIMPLE) == 0 && view.len == (Py_ssize_t)sizeof(sqa_rope));
+        }
+        const sqa_rope *rope = turn ? (const sqa_rope *)view.buf : nullptr;
+        void *st = stream();
+        return without_gil([&] { return sqa_move_rows_q4_0(&td, &ts, &tt, &tf, turn ? &tl : nullptr, rope, st); });
+    });
+    if (view.obj) PyBuffer_Release(&view);
+    return r;
+}
+
 // cache or out, src, norm_w, eps, pos, rope, idx (None: F32 output)
 PyObject *rope_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
     Py_buffer view{};
@@ -279,16 +341,6 @@ sqa_tensor pool_view(const at::Tensor &t) {  // (n_pages, page, Hkv, bytes) -> [
     return d;
 }
 
-// every tensor of a call on the current device (the general path switches to theirs)
-void here(std::initializer_list<PyObject *> ts) {
-    const int dev = (int)c10::hip::current_device();
-    for (PyObject *o : ts) {
-        if (o == Py_None) continue;
-        const at::Tensor &t = tensor(o);
-        need(t.is_cuda() && t.get_device() == dev);
-    }
-}
-
 // state, ring, table, n_past, n_new, page, then the step: state, n_past, q_start, kv_len, slots, pos
 PyObject *plan(PyObject *, PyObject *const *a, Py_ssize_t n) {
     return answer([&]() -> int {
@@ -307,6 +359,55 @@ PyObject *plan(PyObject *, PyObject *const *a, Py_ssize_t n) {
     });
 }
 
+// q_start, kv_len, group, shared_len, members, m_start, m_pos, token_group, pos
+PyObject *share(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    return answer([&]() -> int {
+        need(n == 9);
+        here({a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7], a[8]});
+        sqa_tensor t[9];
+        for (int i = 0; i < 8; ++i) t[i] = ints(tensor(a[i]));
+        const bool pos = a[8] != Py_None;
+        if (pos) t[8] = ints(tensor(a[8]));
+        void *s = stream();
+        return without_gil([&] {
+            return sqa_paged_share(&t[0], &t[1], &t[2], &t[3], &t[4], &t[5], &t[6], &t[7], pos ? &t[8] : nullptr, s);
+        });
+    });
+}
+
+sqa_tensor gate_view(const at::Tensor &t, const at::Tensor &q) {
+    need(t.dim() == 3 && t.scalar_type() == at::kFloat && t.sizes() == q.sizes() && (t.size(2) <= 1 || t.stride(2) == 1));
+    return make(SQA_TYPE_F32, t, q.size(2), q.size(1), q.size(0), 4, t.stride(1) * 4, t.stride(0) * 4, t.stride(0) * 4 * q.size(0));
+}
+
+// q, k_pool, v_pool, table, q_start, kv_len, prefix, shared_table, shared_len, members, m_start, m_pos, token_group,
+// max_q, scale, max_bias, softcap, gate, out, workspace
+PyObject *attn_shared(PyObject *, PyObject *const *a, Py_ssize_t n) {
+    return answer([&]() -> int {
+        need(n == 20);
+        here({a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7], a[8], a[9], a[10], a[11], a[12], a[17], a[18], a[19]});
+        const at::Tensor &q = tensor(a[0]), &o = tensor(a[18]), &ws = tensor(a[19]);
+        need(q.dim() == 3 && q.scalar_type() == at::kFloat && o.scalar_type() == at::kFloat && ws.is_contiguous() &&
+             (q.size(2) <= 1 || q.stride(2) == 1));
+        const sqa_tensor tq = q_view(q), tk = pool_view(tensor(a[1])), tv = pool_view(tensor(a[2])),
+                         tt = table_view(tensor(a[3])), ts = ints(tensor(a[4])), tl = ints(tensor(a[5])),
+                         st = table_view(tensor(a[7])), sl = ints(tensor(a[8])), me = ints(tensor(a[9])),
+                         ms = ints(tensor(a[10])), mp = ints(tensor(a[11])), tr = ints(tensor(a[12])), to = out_view(o);
+        sqa_tensor tp, tg;
+        const bool prefix = a[6] != Py_None, gate = a[17] != Py_None;
+        if (prefix) tp = ints(tensor(a[6]));
+        if (gate) tg = gate_view(tensor(a[17]), q);
+        const int64_t max_q = integer(a[13]);
+        const float scale = scale_of(a[14], q), bias = (float)real(a[15]), cap = (float)real(a[16]);
+        void *wp = ws.data_ptr(), *s = stream();
+        const size_t wb = (size_t)ws.nbytes();
+        return without_gil([&] {
+            return sqa_paged_attn_shared(&tq, &tk, &tv, &tt, &ts, &tl, prefix ? &tp : nullptr, &st, &sl, &me, &ms, &mp, &tr,
+                                         max_q, scale, bias, cap, gate ? &tg : nullptr, &to, wp, wb, s);
+        });
+    });
+}
+
 // q, k_pool, v_pool, table, q_start, kv_len, prefix, max_q, scale, max_bias, softcap, gate, out, workspace
 PyObject *paged_attn(PyObject *, PyObject *const *a, Py_ssize_t n) {
     return answer([&]() -> int {
@@ -320,12 +421,7 @@ PyObject *paged_attn(PyObject *, PyObject *const *a, Py_ssize_t n) {
         sqa_tensor tp, tg;
         const bool prefix = a[6] != Py_None, gate = a[11] != Py_None;
         if (prefix) tp = ints(tensor(a[6]));
-        if (gate) {
-            const at::Tensor &t = tensor(a[11]);
-            need(t.dim() == 3 && t.scalar_type() == at::kFloat && t.sizes() == q.sizes() && (t.size(2) <= 1 || t.stride(2) == 1));
-            tg = make(SQA_TYPE_F32, t, q.size(2), q.size(1), q.size(0), 4, t.stride(1) * 4, t.stride(0) * 4,
-                      t.stride(0) * 4 * q.size(0));
-        }
+        if (gate) tg = gate_view(tensor(a[11]), q);
         const int64_t max_q = integer(a[7]);
         const float scale = scale_of(a[8], q), bias = (float)real(a[9]), cap = (float)real(a[10]);
         void *wp = ws.data_ptr(), *st = stream();
@@ -368,7 +464,8 @@ PyMethodDef methods[] = {
 #define SQA_FN(f) {#f, (PyCFunction)(void (*)(void))f, METH_FASTCALL, nullptr}
     SQA_FN(fa),        SQA_FN(fa_causal), SQA_FN(fill_mask), SQA_FN(set_rows),
     SQA_FN(rope_norm), SQA_FN(out_proj),  SQA_FN(append),    SQA_FN(plan),
-    SQA_FN(paged_attn), SQA_FN(lora),     {nullptr, nullptr, 0, nullptr},
+    SQA_FN(paged_attn), SQA_FN(lora),     SQA_FN(get_rows),  SQA_FN(move_rows),
+    SQA_FN(share),     SQA_FN(attn_shared), {nullptr, nullptr, 0, nullptr},
 #undef SQA_FN
 };
 

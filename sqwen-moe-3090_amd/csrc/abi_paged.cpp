@@ -2,40 +2,13 @@
 // argument checks, support queries and dispatch.
 #include <math.h>
 
+#include <initializer_list>
+
+#include "checks.hpp"
 #include "paged.hpp"
 
 namespace sqa {
 namespace {
-
-bool dense1(const sqa_tensor *t, int type, int64_t n, int64_t esize) {
-    return t->type == type && t->ne[0] == n && t->ne[1] == 1 && t->ne[2] == 1 && t->ne[3] == 1 &&
-           (n <= 1 || t->nb[0] == (uint64_t)esize) && (n == 0 || (t->data && (uintptr_t)t->data % esize == 0));
-}
-
-// n rows of `len` bytes, `step` bytes apart
-struct Rows {
-    uintptr_t at;
-    uint64_t len, step;
-    int64_t n;
-    uintptr_t end() const { return at + (uint64_t)(n - 1) * step + len; }
-};
-
-Rows rows_of(const sqa_tensor *t) {  // ne[1] rows of ne[0] 4-byte values
-    return Rows{(uintptr_t)t->data, 4 * (uint64_t)t->ne[0], t->nb[1], t->ne[1]};
-}
-Rows run_of(const sqa_tensor *t, uint64_t bytes) { return Rows{(uintptr_t)t->data, bytes, 0, bytes ? 1 : 0}; }
-
-// Whether two sets of rows share a byte. Rows of one step, such as parts of a wider buffer's
-// columns, may lie between each other; of different steps, all that lies between is taken as theirs.
-bool meet(const Rows &a, const Rows &b) {
-    if (a.n < 1 || b.n < 1 || a.end() <= b.at || b.end() <= a.at) return false;
-    const uint64_t step = a.n == 1 ? b.step : a.step;
-    if ((a.n > 1 && b.n > 1 && a.step != b.step) || (a.n == 1 && b.n == 1) || a.len > step || b.len > step) return true;
-    const uint64_t r = b.at >= a.at ? (b.at - a.at) % step : (step - (a.at - b.at) % step) % step;  // b's start in a's row
-    return r < a.len || step - r < b.len;
-}
-
-bool power_of_two(int64_t x) { return x > 0 && (x & (x - 1)) == 0; }
 
 int check_table(const sqa_tensor *t, const char *what) {
     if (t->type != SQA_TYPE_I32 || t->ne[2] != 1 || t->ne[3] != 1 || t->ne[0] < 1 || t->ne[1] < 1)
@@ -51,8 +24,7 @@ int check_table(const sqa_tensor *t, const char *what) {
 }
 
 int check_paged(const sqa_tensor *q, const sqa_tensor *k, const sqa_tensor *v, const sqa_tensor *table, int64_t max_q,
-                float scale, float max_bias, float softcap, const sqa_tensor *dst) {
-    const char *what = "paged_attn";
+                float scale, float max_bias, float softcap, const sqa_tensor *dst, const char *what = "paged_attn") {
     if (!q || !k || !v || !table || !dst) return set_error(SQA_ERR_INVALID, "%s: null tensor", what);
     if (q->type != SQA_TYPE_F32 || dst->type != SQA_TYPE_F32)
         return set_error(SQA_ERR_UNSUPPORTED, "%s: q and dst must be F32", what);
@@ -100,6 +72,66 @@ int check_paged(const sqa_tensor *q, const sqa_tensor *k, const sqa_tensor *v, c
     if (!isfinite(max_bias) || max_bias < 0.0f || !isfinite(softcap) || softcap < 0.0f)
         return set_error(SQA_ERR_INVALID, "%s: max_bias and logit_softcap must be finite and not negative", what);
     return SQA_OK;
+}
+
+int check_shared(const sqa_tensor *q, const sqa_tensor *k, const sqa_tensor *v, const sqa_tensor *table,
+                 const sqa_tensor *shared_table, int64_t max_q, float scale, float max_bias, float softcap, const sqa_tensor *dst) {
+    const char *what = "paged_attn_shared";
+    int rc = check_paged(q, k, v, table, max_q, scale, max_bias, softcap, dst, what);
+    if (rc) return rc;
+    if (!shared_table) return set_error(SQA_ERR_INVALID, "%s: null tensor", what);
+    rc = check_table(shared_table, what);
+    if (rc) return rc;
+    if (shared_table->ne[0] * k->ne[2] > INT32_MAX)
+        return set_error(SQA_ERR_UNSUPPORTED, "%s: table rows of more than 2^31 tokens", what);
+    return SQA_OK;
+}
+
+// The arrays of a call beside q, the pools and the table.
+int check_arrays(const sqa_tensor *q, const sqa_tensor *table, const sqa_tensor *q_start, const sqa_tensor *kv_len,
+                 const sqa_tensor *prefix, const sqa_tensor *gate, const sqa_tensor *dst, const char *what) {
+    const int64_t B = table->ne[1];
+    if (!q_start || !kv_len) return set_error(SQA_ERR_INVALID, "%s: null tensor", what);
+    if (!dense1(q_start, SQA_TYPE_I32, B + 1, 4) || !dense1(kv_len, SQA_TYPE_I32, B, 4) ||
+        (prefix && !dense1(prefix, SQA_TYPE_I32, B, 4)))
+        return set_error(SQA_ERR_INVALID, "%s: q_start, kv_len and prefix must be contiguous I32 of B + 1, B and B entries", what);
+    if (gate && (gate->type != SQA_TYPE_F32 || gate->ne[0] != dst->ne[0] || gate->ne[1] != dst->ne[1] ||
+                 gate->ne[2] != dst->ne[2] || gate->ne[3] != 1 || gate->nb[0] != 4 || gate->nb[1] % 4 || gate->nb[2] % 4 ||
+                 (uintptr_t)gate->data % 4 || (q->ne[1] > 0 && !gate->data)))
+        return set_error(SQA_ERR_INVALID, "%s: gate must be F32 [D, H, n_tok]", what);
+    return SQA_OK;
+}
+
+Rows table_rows(const sqa_tensor *t) { return Rows{(uintptr_t)t->data, 4 * (uint64_t)t->ne[0], t->nb[1], t->ne[1]}; }
+
+// Whether dst or the workspace meets another array (`more`: further ones). Some rows of dst, and the
+// workspace, are written while others are computed. A row of q or gate is read for no row of dst but
+// its own, so that q or gate may be dst itself.
+bool clash(const sqa_tensor *q, const sqa_tensor *k, const sqa_tensor *v, const sqa_tensor *table, const sqa_tensor *q_start,
+           const sqa_tensor *kv_len, const sqa_tensor *prefix, const sqa_tensor *gate, const sqa_tensor *dst, void *workspace,
+           size_t workspace_bytes, std::initializer_list<Rows> more) {
+    const int64_t n_tok = q->ne[1], H = q->ne[2], B = table->ne[1];
+    auto heads = [&](const sqa_tensor *t, uint64_t token, uint64_t head) {  // its rows, by token or by head
+        const uint64_t row = 4 * (uint64_t)kHeadDim, by_token = row + (uint64_t)(H - 1) * head;
+        return token >= by_token || n_tok == 1 ? Rows{(uintptr_t)t->data, by_token, token, n_tok}
+                                               : Rows{(uintptr_t)t->data, row + (uint64_t)(n_tok - 1) * token, head, H};
+    };
+    auto same = [&](const sqa_tensor *t, uint64_t token, uint64_t head) {  // dst itself
+        return t->data == dst->data && (n_tok == 1 || token == dst->nb[2]) && (H == 1 || head == dst->nb[1]);
+    };
+    auto pages = [&](const sqa_tensor *t) { return Rows{(uintptr_t)t->data, t->nb[2] * (uint64_t)t->ne[2], t->nb[3], t->ne[3]}; };
+    const Rows out = run_of(dst, 4ull * kHeadDim * (uint64_t)(H * n_tok)), rows_q = heads(q, q->nb[1], q->nb[2]);
+    const Rows ws{(uintptr_t)workspace, workspace_bytes, 0, workspace ? 1 : 0};
+    bool bad = meet(out, ws) || meet(ws, rows_q) || (!same(q, q->nb[1], q->nb[2]) && meet(out, rows_q));
+    if (gate) {
+        const Rows rows_g = heads(gate, gate->nb[2], gate->nb[1]);
+        bad |= meet(ws, rows_g) || (!same(gate, gate->nb[2], gate->nb[1]) && meet(out, rows_g));
+    }
+    for (const Rows &r : {pages(k), pages(v), table_rows(table), run_of(q_start, 4 * (uint64_t)(B + 1)),
+                          run_of(kv_len, 4 * (uint64_t)B), prefix ? run_of(prefix, 4 * (uint64_t)B) : Rows{}})
+        bad |= meet(out, r) || meet(ws, r);
+    for (const Rows &r : more) bad |= meet(out, r) || meet(ws, r);
+    return bad;
 }
 
 int check_lora(const sqa_tensor *base, const sqa_tensor *x, const sqa_tensor *gate, const sqa_tensor *a,
@@ -212,46 +244,88 @@ int sqa_paged_attn(const sqa_tensor *q, const sqa_tensor *k, const sqa_tensor *v
     const char *what = "paged_attn";
     const int rc = check_paged(q, k, v, table, max_q, scale, max_bias, logit_softcap, dst);
     if (rc) return rc;
-    const int64_t B = table->ne[1];
-    if (!q_start || !kv_len) return set_error(SQA_ERR_INVALID, "%s: null tensor", what);
-    if (!dense1(q_start, SQA_TYPE_I32, B + 1, 4) || !dense1(kv_len, SQA_TYPE_I32, B, 4) ||
-        (prefix && !dense1(prefix, SQA_TYPE_I32, B, 4)))
-        return set_error(SQA_ERR_INVALID, "%s: q_start, kv_len and prefix must be contiguous I32 of B + 1, B and B entries", what);
-    if (gate && (gate->type != SQA_TYPE_F32 || gate->ne[0] != dst->ne[0] || gate->ne[1] != dst->ne[1] ||
-                 gate->ne[2] != dst->ne[2] || gate->ne[3] != 1 || gate->nb[0] != 4 || gate->nb[1] % 4 || gate->nb[2] % 4 ||
-                 (uintptr_t)gate->data % 4 || (q->ne[1] > 0 && !gate->data)))
-        return set_error(SQA_ERR_INVALID, "%s: gate must be F32 [D, H, n_tok]", what);
+    if (const int bad = check_arrays(q, table, q_start, kv_len, prefix, gate, dst, what)) return bad;
     if (q->ne[1] == 0) return SQA_OK;
-    // Some rows of dst, and the workspace, are written while others are computed. A row of q or
-    // gate is read for no row of dst but its own.
-    const int64_t n_tok = q->ne[1], H = q->ne[2];
-    auto heads = [&](const sqa_tensor *t, uint64_t token, uint64_t head) {  // its rows, by token or by head
-        const uint64_t row = 4 * (uint64_t)kHeadDim, by_token = row + (uint64_t)(H - 1) * head;
-        return token >= by_token || n_tok == 1 ? Rows{(uintptr_t)t->data, by_token, token, n_tok}
-                                               : Rows{(uintptr_t)t->data, row + (uint64_t)(n_tok - 1) * token, head, H};
-    };
-    auto same = [&](const sqa_tensor *t, uint64_t token, uint64_t head) {  // dst itself
-        return t->data == dst->data && (n_tok == 1 || token == dst->nb[2]) && (H == 1 || head == dst->nb[1]);
-    };
-    auto pages = [&](const sqa_tensor *t) { return Rows{(uintptr_t)t->data, t->nb[2] * (uint64_t)t->ne[2], t->nb[3], t->ne[3]}; };
-    const Rows out = run_of(dst, 4ull * kHeadDim * (uint64_t)(H * n_tok)), tab{(uintptr_t)table->data, 4 * (uint64_t)table->ne[0], table->nb[1], B};
-    const Rows rows_q = heads(q, q->nb[1], q->nb[2]);
-    const size_t most = paged_attn_workspace(n_tok, H, k->ne[1], B, max_q);
-    const Rows ws{(uintptr_t)workspace, workspace_bytes < most ? workspace_bytes : most, 0, workspace ? 1 : 0};
-    bool clash = meet(out, ws) || meet(ws, rows_q) || (!same(q, q->nb[1], q->nb[2]) && meet(out, rows_q));
-    if (gate) {
-        const Rows rows_g = heads(gate, gate->nb[2], gate->nb[1]);
-        clash |= meet(ws, rows_g) || (!same(gate, gate->nb[2], gate->nb[1]) && meet(out, rows_g));
-    }
-    for (const Rows &r : {pages(k), pages(v), tab, run_of(q_start, 4 * (uint64_t)(B + 1)), run_of(kv_len, 4 * (uint64_t)B),
-                          prefix ? run_of(prefix, 4 * (uint64_t)B) : Rows{}})
-        clash |= meet(out, r) || meet(ws, r);
-    if (clash)
+    const size_t most = paged_attn_workspace(q->ne[1], q->ne[2], k->ne[1], table->ne[1], max_q);
+    if (clash(q, k, v, table, q_start, kv_len, prefix, gate, dst, workspace, workspace_bytes < most ? workspace_bytes : most, {}))
         return set_error(SQA_ERR_INVALID, "%s: dst and the workspace must not overlap another array, but for a q or gate that is dst itself",
                          what);
     const PagedArgs a{q, k, v, table, q_start, kv_len, prefix, gate, dst, max_q, scale, max_bias, logit_softcap,
                       workspace, workspace_bytes};
     return launch_paged_attn(a, (hipStream_t)stream);
+}
+
+int sqa_paged_share(const sqa_tensor *q_start, const sqa_tensor *kv_len, const sqa_tensor *group, const sqa_tensor *shared_len,
+                    const sqa_tensor *members, const sqa_tensor *m_start, const sqa_tensor *m_pos,
+                    const sqa_tensor *token_group, const sqa_tensor *pos, void *stream) {
+    const char *what = "paged_share";
+    for (const sqa_tensor *t : {q_start, kv_len, group, shared_len, members, m_start, m_pos, token_group})
+        if (!t) return set_error(SQA_ERR_INVALID, "%s: null tensor", what);
+    const int64_t B = kv_len->ne[0], G = shared_len->ne[0], T = members->ne[0];
+    if (B < 1 || G < 1 || T < 0) return set_error(SQA_ERR_INVALID, "%s: no requests or groups", what);
+    if (B > kMaxRequests || G > kMaxRequests)
+        return set_error(SQA_ERR_UNSUPPORTED, "%s: %lld requests, %lld groups (at most %d)", what, (long long)B, (long long)G, kMaxRequests);
+    if (T > (1 << 24)) return set_error(SQA_ERR_UNSUPPORTED, "%s: more than 2^24 token rows", what);
+    if (!dense1(kv_len, SQA_TYPE_I32, B, 4) || !dense1(group, SQA_TYPE_I32, B, 4) || !dense1(q_start, SQA_TYPE_I32, B + 1, 4) ||
+        !dense1(shared_len, SQA_TYPE_I32, G, 4) || !dense1(m_start, SQA_TYPE_I32, G + 1, 4) || !dense1(members, SQA_TYPE_I32, T, 4) ||
+        !dense1(m_pos, SQA_TYPE_I32, T, 4) || !dense1(token_group, SQA_TYPE_I32, T, 4) || (pos && !dense1(pos, SQA_TYPE_I32, 4 * T, 4)))
+        return set_error(SQA_ERR_INVALID, "%s: arrays must be contiguous I32, of B, B + 1, G, G + 1, T and 4 T entries", what);
+    // Every workgroup reads the inputs while others write (what is written stands first).
+    const sqa_tensor *all[] = {members, m_start, m_pos, token_group, pos, q_start, kv_len, group, shared_len};
+    for (int i = 0; i < 5; ++i)
+        for (int j = i + 1; j < 9; ++j)
+            if (all[i] && all[j] && meet(run_of(all[i], 4 * (uint64_t)all[i]->ne[0]), run_of(all[j], 4 * (uint64_t)all[j]->ne[0])))
+                return set_error(SQA_ERR_INVALID, "%s: what the call writes must not overlap its other arrays", what);
+    const ShareArgs a{(const int32_t *)q_start->data, (const int32_t *)kv_len->data, (const int32_t *)group->data,
+                      (const int32_t *)shared_len->data, (int32_t *)members->data, (int32_t *)m_start->data,
+                      (int32_t *)m_pos->data, (int32_t *)token_group->data, pos ? (int32_t *)pos->data : nullptr,
+                      (int)B, (int)G, (int)T};
+    return launch_paged_share(a, (hipStream_t)stream);
+}
+
+int sqa_supports_paged_attn_shared(const sqa_tensor *q, const sqa_tensor *k, const sqa_tensor *v, const sqa_tensor *table,
+                                   const sqa_tensor *shared_table, int64_t max_q, float scale, float max_bias,
+                                   float logit_softcap, const sqa_tensor *dst) {
+    return check_shared(q, k, v, table, shared_table, max_q, scale, max_bias, logit_softcap, dst) == SQA_OK ? 1 : 0;
+}
+
+size_t sqa_paged_attn_shared_workspace_size(const sqa_tensor *q, const sqa_tensor *k, const sqa_tensor *table,
+                                            const sqa_tensor *shared_table, int64_t max_q) {
+    if (sqa_paged_attn_workspace_size(q, k, table, max_q) == 0 || !shared_table || shared_table->ne[1] < 1 ||
+        shared_table->ne[1] > kMaxRequests)
+        return 0;
+    return paged_shared_workspace(q->ne[1], q->ne[2], k->ne[1], table->ne[1], shared_table->ne[1], max_q);
+}
+
+int sqa_paged_attn_shared(const sqa_tensor *q, const sqa_tensor *k, const sqa_tensor *v, const sqa_tensor *table,
+                          const sqa_tensor *q_start, const sqa_tensor *kv_len, const sqa_tensor *prefix,
+                          const sqa_tensor *shared_table, const sqa_tensor *shared_len, const sqa_tensor *members,
+                          const sqa_tensor *m_start, const sqa_tensor *m_pos, const sqa_tensor *token_group, int64_t max_q,
+                          float scale, float max_bias, float logit_softcap, const sqa_tensor *gate, const sqa_tensor *dst,
+                          void *workspace, size_t workspace_bytes, void *stream) {
+    const char *what = "paged_attn_shared";
+    int rc = check_shared(q, k, v, table, shared_table, max_q, scale, max_bias, logit_softcap, dst);
+    if (!rc) rc = check_arrays(q, table, q_start, kv_len, prefix, gate, dst, what);
+    if (rc) return rc;
+    const int64_t n_tok = q->ne[1], B = table->ne[1], G = shared_table->ne[1];
+    if (!shared_len || !members || !m_start || !m_pos || !token_group) return set_error(SQA_ERR_INVALID, "%s: null tensor", what);
+    if (!dense1(shared_len, SQA_TYPE_I32, G, 4) || !dense1(m_start, SQA_TYPE_I32, G + 1, 4) ||
+        !dense1(members, SQA_TYPE_I32, n_tok, 4) || !dense1(m_pos, SQA_TYPE_I32, n_tok, 4) ||
+        !dense1(token_group, SQA_TYPE_I32, n_tok, 4))
+        return set_error(SQA_ERR_INVALID, "%s: shared_len, m_start, members, m_pos and token_group must be contiguous I32 of G, "
+                         "G + 1 and n_tok entries", what);
+    if (n_tok == 0) return SQA_OK;
+    const size_t most = paged_shared_workspace(n_tok, q->ne[2], k->ne[1], B, G, max_q);
+    const uint64_t g4 = 4 * (uint64_t)G, t4 = 4 * (uint64_t)n_tok;
+    if (clash(q, k, v, table, q_start, kv_len, prefix, gate, dst, workspace, workspace_bytes < most ? workspace_bytes : most,
+              {table_rows(shared_table), run_of(shared_len, g4), run_of(m_start, g4 + 4), run_of(members, t4), run_of(m_pos, t4),
+               run_of(token_group, t4)}))
+        return set_error(SQA_ERR_INVALID, "%s: dst and the workspace must not overlap another array, but for a q or gate that is dst itself",
+                         what);
+    const SharedArgs a{{q, k, v, table, q_start, kv_len, prefix, gate, dst, max_q, scale, max_bias, logit_softcap, workspace,
+                        workspace_bytes},
+                       shared_table, shared_len, members, m_start, m_pos, token_group};
+    return launch_paged_shared(a, (hipStream_t)stream);
 }
 
 int sqa_supports_lora_add(const sqa_tensor *base, const sqa_tensor *x, const sqa_tensor *gate, const sqa_tensor *a,

@@ -16,6 +16,22 @@ struct PagedArgs {
 size_t paged_attn_workspace(int64_t n_tok, int64_t H, int64_t Hkv, int64_t B, int64_t max_q);
 int launch_paged_attn(const PagedArgs &a, hipStream_t s);
 
+// A call whose groups of requests share prefixes: their pages and lengths, and the step's plan of members.
+struct SharedArgs {
+    PagedArgs own;
+    const sqa_tensor *table, *len, *members, *m_start, *m_pos, *token_group;
+};
+size_t paged_shared_workspace(int64_t n_tok, int64_t H, int64_t Hkv, int64_t B, int64_t groups, int64_t max_q);
+int launch_paged_shared(const SharedArgs &a, hipStream_t s);
+
+struct ShareArgs {
+    const int32_t *q_start, *kv_len, *group, *shared_len;
+    int32_t *members, *m_start, *m_pos, *token_group;
+    int32_t *pos;  // or null
+    int B, n_groups, T;
+};
+int launch_paged_share(const ShareArgs &a, hipStream_t s);
+
 struct PlanArgs {
     const int32_t *n_past, *n_new;
     int32_t *table;

@@ -222,17 +222,7 @@ int launch_combine(const Call &c, hipStream_t s) {
     return hip_status(hipGetLastError(), "paged_attn merge launch");
 }
 
-}  // namespace paged
-
-using namespace paged;
-
-size_t paged_attn_workspace(int64_t n_tok, int64_t H, int64_t Hkv, int64_t B, int64_t max_q) {
-    if (n_tok < 1) return 0;
-    const Plan p = plan(n_tok, H, Hkv, B, max_q);
-    return p.where + p.work + (size_t)p.slots_d * p.slot_d + (size_t)p.slots_c * p.slot_c + 512;
-}
-
-int launch_paged_attn(const PagedArgs &a, hipStream_t s) {
+Call call_of(const PagedArgs &a) {
     const sqa_tensor &q = *a.q, &k = *a.k;
     Call c{};
     c.q = (const char *)q.data, c.q_nb1 = (int64_t)q.nb[1], c.q_nb2 = (int64_t)q.nb[2];
@@ -260,7 +250,21 @@ int launch_paged_attn(const PagedArgs &a, hipStream_t s) {
     c.gate_nb1 = a.gate ? (int64_t)a.gate->nb[1] : 0, c.gate_nb2 = a.gate ? (int64_t)a.gate->nb[2] : 0;
     c.dst = (float *)a.dst->data;
     c.cus = device_cu_count();
+    return c;
+}
 
+}  // namespace paged
+
+using namespace paged;
+
+size_t paged_attn_workspace(int64_t n_tok, int64_t H, int64_t Hkv, int64_t B, int64_t max_q) {
+    if (n_tok < 1) return 0;
+    const Plan p = plan(n_tok, H, Hkv, B, max_q);
+    return p.where + p.work + (size_t)p.slots_d * p.slot_d + (size_t)p.slots_c * p.slot_c + 512;
+}
+
+int launch_paged_attn(const PagedArgs &a, hipStream_t s) {
+    Call c = call_of(a);
     const Plan p = plan(c.n_tok, c.H, c.Hkv, c.B, a.max_q);
     const size_t need = p.where + p.work + (size_t)p.least_d * p.slot_d + 512;
     if (!a.ws || a.ws_bytes < need)

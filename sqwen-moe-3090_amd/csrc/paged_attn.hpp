@@ -184,6 +184,9 @@ __device__ __forceinline__ float gate_by(float x, float g) {
     return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * g));
 }
 
+// What a call's arguments say of it (no workspace yet).
+Call call_of(const PagedArgs &a);
+
 int launch_few(const Call &c, hipStream_t s);      // paged_decode.hip
 int launch_many(const Call &c, hipStream_t s);     // paged_chunk.hip
 int launch_combine(const Call &c, hipStream_t s);  // paged_attn.hip
