@@ -5,6 +5,7 @@
 // in the call) go to paged_decode.hip, the others to paged_chunk.hip.
 #include <float.h>
 
+#include "paged_merge.hpp"
 #include "paged_work.hpp"
 
 namespace sqa {
@@ -17,33 +18,10 @@ typedef float floatx4 __attribute__((ext_vector_type(4)));
 // Merge of a row's partials: out = sum_s acc_s 2^(m_s - M) / sum_s l_s 2^(m_s - M), M = max m_s,
 // then the gate. m is in base 2 as the kernels hold it: through base e and back, 50 nats lost 2e-6
 // of a split's weight. A partial whose m is -inf (no key seen) may hold anything.
-struct Row {
-    const float *acc, *ml;  // of the row in its first slot
-    int64_t step;           // floats of acc between its splits (ml: step / 128)
-    int n;                  // 0: nothing to do
-};
-
 __device__ __forceinline__ Row row_of(const Call &c, int t, int h) {
-    Row r{nullptr, nullptr, 0, 0};
     const int4 w = c.where[t];
-    if (t < c.q_start[0] || t >= c.q_start[c.B]) return r;  // of no request: w was not written
-    const int form = w.w & 3, step = w.w >> 2, kvh = group_of(c, h), row = w.z + h - kvh * c.G;
-    const int rows = form == kFew ? c.rows_d : c.rows_c;
-    const int64_t heads = form == kFew ? 1 : (int64_t)w.y * step, first = w.x + kvh * heads;
-    // (arrays that are no plan's may leave here what the workspace held: any four numbers)
-    if (form == kDone || w.x < 0 || step < 1 || w.y < 1 || w.y > 256 || row < 0 || row >= rows ||
-        first + (int64_t)(w.y - 1) * step >= (form == kFew ? c.slots_d : c.slots_c))
-        return r;
-    const int64_t at = first * rows + row;
-    r.acc = (form == kFew ? c.acc_d : c.acc_c) + at * 256;
-    r.ml = (form == kFew ? c.ml_d : c.ml_c) + at * 2;
-    r.step = (int64_t)step * rows * 256;
-    r.n = w.y;
-    return r;
-}
-
-__device__ __forceinline__ const float *gate_row(const Call &c, int t, int h) {
-    return reinterpret_cast<const float *>(c.gate + t * c.gate_nb2 + h * c.gate_nb1);
+    if (t < c.q_start[0] || t >= c.q_start[c.B]) return Row{nullptr, nullptr, 0, 0};  // of no request: w was not written
+    return partials(c, w, h);
 }
 
 // Few rows of many splits: 16 workgroups per row, 16 dims each; a thread holds one dim
@@ -167,17 +145,29 @@ __global__ __launch_bounds__(kThreads) void merge_rows_kernel(Call c) {
     }
 }
 
-size_t al256(size_t x) { return (x + 255) & ~(size_t)255; }
+}  // namespace
 
-// What a call launches, and its workspace: the tokens' entries, the many-row plan, the slots of the
-// few-row kernel, then those of the many-row kernel.
-struct Plan {
-    int most_d, rows_d, rows_c;  // of Call
-    int64_t slots_d, least_d, slots_c, grid_c;
-    size_t where, work, slot_d, slot_c;
-};
+int launch_combine(const Call &c, hipStream_t s) {
+    const int prof = profile_start("paged_merge", s);
+    const int64_t rows = (int64_t)c.n_tok * c.H;
+    // 16 workgroups a row below 128 rows: requests of 8000 keys with 16 rows each, the whole call
+    // with these and with a wavefront a row: 16 rows 11.5 and 23.9 us, 64 15.3 and 17.4, 112 20.9
+    // and 20.7, 128 22.8 and 21.8, 192 26.9 and 24.8.
+    if (rows < 128) {
+        merge_dims_kernel<<<dim3((unsigned)rows, 16), dim3(kThreads), 0, s>>>(c);
+    } else {
+        // four heads a wavefront where that leaves wavefronts enough for the chip
+        const bool four = rows > 8192 && c.H >= 16;
+        const dim3 grid((unsigned)((c.H + (four ? 16 : 4) - 1) / (four ? 16 : 4)),
+                        (unsigned)(c.n_tok < (1 << 15) ? c.n_tok : 1 << 15), (unsigned)((c.n_tok + (1 << 15) - 1) >> 15));
+        if (four) merge_rows_kernel<4><<<grid, dim3(kThreads), 0, s>>>(c);
+        else merge_rows_kernel<1><<<grid, dim3(kThreads), 0, s>>>(c);
+    }
+    profile_stop(prof, s);
+    return hip_status(hipGetLastError(), "paged_attn merge launch");
+}
 
-Plan plan(int64_t n_tok, int64_t H, int64_t Hkv, int64_t B, int64_t max_q) {
+Plan plan_of(int64_t n_tok, int64_t H, int64_t Hkv, int64_t B, int64_t max_q) {
     Plan p{};
     const int64_t G = H / Hkv, rows = (max_q < n_tok ? max_q : n_tok) * G, cus = device_cu_count();
     const int64_t active = B < n_tok ? B : n_tok;
@@ -200,26 +190,35 @@ Plan plan(int64_t n_tok, int64_t H, int64_t Hkv, int64_t B, int64_t max_q) {
     return p;
 }
 
-}  // namespace
+size_t least_bytes(const Plan &p) { return p.where + p.work + (size_t)p.least_d * p.slot_d + 512; }
+size_t full_bytes(const Plan &p) {
+    return p.where + p.work + (size_t)p.slots_d * p.slot_d + (size_t)p.slots_c * p.slot_c + 512;
+}
 
-int launch_combine(const Call &c, hipStream_t s) {
-    const int prof = profile_start("paged_merge", s);
-    const int64_t rows = (int64_t)c.n_tok * c.H;
-    // 16 workgroups a row below 128 rows: requests of 8000 keys with 16 rows each, the whole call
-    // with these and with a wavefront a row: 16 rows 11.5 and 23.9 us, 64 15.3 and 17.4, 112 20.9
-    // and 20.7, 128 22.8 and 21.8, 192 26.9 and 24.8.
-    if (rows < 128) {
-        merge_dims_kernel<<<dim3((unsigned)rows, 16), dim3(kThreads), 0, s>>>(c);
-    } else {
-        // four heads a wavefront where that leaves wavefronts enough for the chip
-        const bool four = rows > 8192 && c.H >= 16;
-        const dim3 grid((unsigned)((c.H + (four ? 16 : 4) - 1) / (four ? 16 : 4)),
-                        (unsigned)(c.n_tok < (1 << 15) ? c.n_tok : 1 << 15), (unsigned)((c.n_tok + (1 << 15) - 1) >> 15));
-        if (four) merge_rows_kernel<4><<<grid, dim3(kThreads), 0, s>>>(c);
-        else merge_rows_kernel<1><<<grid, dim3(kThreads), 0, s>>>(c);
-    }
-    profile_stop(prof, s);
-    return hip_status(hipGetLastError(), "paged_attn merge launch");
+int lay_out(Call &c, const Plan &p, void *ws, size_t ws_bytes, const char *what) {
+    const size_t need = least_bytes(p);
+    if (!ws || ws_bytes < need)
+        return set_error(SQA_ERR_WORKSPACE, "%s: workspace %zu bytes < %zu needed", what, ws ? ws_bytes : (size_t)0, need);
+    if (p.grid_c > INT32_MAX) return set_error(SQA_ERR_UNSUPPORTED, "%s: too many query tiles", what);
+    size_t left = ws_bytes - 512 - p.where - p.work;
+    c.most_d = p.most_d, c.rows_d = p.rows_d, c.rows_c = p.rows_c, c.grid_c = (int)p.grid_c;
+    auto take = [&left](int64_t slots, size_t bytes) {
+        if (!slots || (size_t)slots > left / bytes) slots = slots ? (int64_t)(left / bytes) : 0;
+        left -= (size_t)slots * bytes;
+        return (int)slots;
+    };
+    c.slots_d = take(p.slots_d, p.slot_d);
+    c.slots_c = take(p.slots_c, p.slot_c);
+    c.room = c.slots_d / c.Hkv;
+    c.few_pieces = c.cus / c.Hkv, c.all_pieces = 2 * c.cus / c.Hkv;
+    uint8_t *base = reinterpret_cast<uint8_t *>(((uintptr_t)ws + 255) & ~(uintptr_t)255);
+    c.where = reinterpret_cast<int4 *>(base);
+    c.work = reinterpret_cast<int *>(base + p.where);
+    c.acc_d = reinterpret_cast<float *>(base + p.where + p.work);
+    c.acc_c = c.acc_d + (size_t)c.slots_d * c.rows_d * kHeadDim;
+    c.ml_d = c.acc_c + (size_t)c.slots_c * c.rows_c * kHeadDim;
+    c.ml_c = c.ml_d + (size_t)c.slots_d * c.rows_d * 2;
+    return SQA_OK;
 }
 
 Call call_of(const PagedArgs &a) {
@@ -259,37 +258,16 @@ using namespace paged;
 
 size_t paged_attn_workspace(int64_t n_tok, int64_t H, int64_t Hkv, int64_t B, int64_t max_q) {
     if (n_tok < 1) return 0;
-    const Plan p = plan(n_tok, H, Hkv, B, max_q);
-    return p.where + p.work + (size_t)p.slots_d * p.slot_d + (size_t)p.slots_c * p.slot_c + 512;
+    const Plan p = plan_of(n_tok, H, Hkv, B, max_q);
+    return full_bytes(p);
 }
 
 int launch_paged_attn(const PagedArgs &a, hipStream_t s) {
     Call c = call_of(a);
-    const Plan p = plan(c.n_tok, c.H, c.Hkv, c.B, a.max_q);
-    const size_t need = p.where + p.work + (size_t)p.least_d * p.slot_d + 512;
-    if (!a.ws || a.ws_bytes < need)
-        return set_error(SQA_ERR_WORKSPACE, "paged_attn: workspace %zu bytes < %zu needed", a.ws ? a.ws_bytes : (size_t)0, need);
-    if (p.grid_c > INT32_MAX) return set_error(SQA_ERR_UNSUPPORTED, "paged_attn: too many query tiles");
-    size_t left = a.ws_bytes - 512 - p.where - p.work;
-    c.most_d = p.most_d, c.rows_d = p.rows_d, c.rows_c = p.rows_c, c.grid_c = (int)p.grid_c;
-    auto take = [&left](int64_t slots, size_t bytes) {
-        if (!slots || (size_t)slots > left / bytes) slots = slots ? (int64_t)(left / bytes) : 0;
-        left -= (size_t)slots * bytes;
-        return (int)slots;
-    };
-    c.slots_d = take(p.slots_d, p.slot_d);
-    c.slots_c = take(p.slots_c, p.slot_c);
-    c.room = c.slots_d / c.Hkv;
-    c.few_pieces = c.cus / c.Hkv, c.all_pieces = 2 * c.cus / c.Hkv;
-    uint8_t *base = reinterpret_cast<uint8_t *>(((uintptr_t)a.ws + 255) & ~(uintptr_t)255);
-    c.where = reinterpret_cast<int4 *>(base);
-    c.work = reinterpret_cast<int *>(base + p.where);
-    c.acc_d = reinterpret_cast<float *>(base + p.where + p.work);
-    c.acc_c = c.acc_d + (size_t)c.slots_d * c.rows_d * kHeadDim;
-    c.ml_d = c.acc_c + (size_t)c.slots_c * c.rows_c * kHeadDim;
-    c.ml_c = c.ml_d + (size_t)c.slots_d * c.rows_d * 2;
-
-    int rc = launch_few(c, s);
+    const Plan p = plan_of(c.n_tok, c.H, c.Hkv, c.B, a.max_q);
+    int rc = lay_out(c, p, a.ws, a.ws_bytes, "paged_attn");
+    if (rc) return rc;
+    rc = launch_few(c, s);
     if (rc) return rc;
     if (p.rows_c) {
         rc = launch_many(c, s);

@@ -1,6 +1,8 @@
 // paged_attn.hpp - device code that the attention kernels over a paged pool share:
 // the requests of a call, how its keys are split over workgroups, the score options.
 #pragma once
+#include <type_traits>
+
 #include "paged.hpp"
 
 namespace sqa {
@@ -16,6 +18,10 @@ typedef float float4a __attribute__((ext_vector_type(4), aligned(4)));
 // heads 1 (kFew) or slots * step (kMany).
 constexpr int kDone = 0;  // nothing to merge: the row is written, or left as it was
 constexpr int kFew = 1, kMany = 2;
+constexpr int kWhole = 3;  // one part, normalised, in OwnCall::dst and ::stats
+
+// P of every partial carries this power of two, l with it (which cancels in a merge).
+constexpr int kPBits = 6;
 
 // What a call's kernels know of it.
 struct Call {
@@ -52,6 +58,20 @@ struct Call {
     int cus;
 };
 
+// The own part of a call whose groups share prefixes: every row goes through the merge, those of
+// one split normalised (dst is then a buffer of the workspace) with their (m, l) in stats.
+struct OwnCall : Call {
+    float *stats;  // [n_tok][H][2]
+};
+// The shared part: `requests` are groups, q_start their members' first places, kv_len the
+// prefixes' lengths. Every token sees every key, and no part is whole.
+struct SharedCall : Call {
+    const int32_t *members;  // [n_tok] token rows by group
+    const int32_t *m_pos;    // their positions
+};
+template <class C> inline constexpr bool kIsShared = std::is_same<C, SharedCall>::value;
+template <class C> inline constexpr bool kIsOwn = std::is_same<C, OwnCall>::value;
+
 // A request's tokens and keys. Anything the arrays may hold leaves rows inside
 // [0, n_tok) and keys inside [0, most_kv).
 struct Request {
@@ -69,6 +89,17 @@ __device__ __forceinline__ Request request(const Call &c, int b) {
     r.n = min(max(s1, r.q0), c.n_tok) - r.q0;
     r.kv = (int)min((int64_t)max(len, 0), c.most_kv);
     r.pos0 = max(len, 0) - r.n;
+    return r;
+}
+
+__device__ __forceinline__ Request request(const SharedCall &c, int b) {
+    Request r;
+    const int s0 = c.q_start[b], s1 = c.q_start[b + 1], len = c.kv_len[b];
+    r.prefix = INT32_MAX;
+    r.q0 = min(max(s0, 0), c.n_tok);
+    r.kv = (int)min((int64_t)max(len, 0), c.most_kv);
+    r.n = r.kv ? min(max(s1, r.q0), c.n_tok) - r.q0 : 0;
+    r.pos0 = 0;
     return r;
 }
 
@@ -116,7 +147,8 @@ __device__ __forceinline__ int wave_max(int x) {  // of values >= 0
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
 // The request of a workgroup (b wave-uniform).
-__device__ __forceinline__ Request uniform_request(const Call &c, int b) {
+template <class C>
+__device__ __forceinline__ Request uniform_request(const C &c, int b) {
     const Request r = request(c, b);
     return Request{uniform(r.q0), uniform(r.n), uniform(r.kv), uniform(r.pos0), uniform(r.prefix)};
 }
@@ -184,11 +216,31 @@ __device__ __forceinline__ float gate_by(float x, float g) {
     return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * g));
 }
 
-// What a call's arguments say of it (no workspace yet).
+// What a call launches, and its workspace: the tokens' entries, the many-row plan, the slots of the
+// few-row kernel, then those of the many-row kernel.
+struct Plan {
+    int most_d, rows_d, rows_c;  // of Call
+    int64_t slots_d, least_d, slots_c, grid_c;
+    size_t where, work, slot_d, slot_c;
+};
+Plan plan_of(int64_t n_tok, int64_t H, int64_t Hkv, int64_t B, int64_t max_q);
+size_t least_bytes(const Plan &p);
+size_t full_bytes(const Plan &p);
+// What a call's arguments say of it, and its workspace's parts.
 Call call_of(const PagedArgs &a);
+int lay_out(Call &c, const Plan &p, void *ws, size_t ws_bytes, const char *what);
 
+inline size_t al256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+struct SharedCalls {
+    OwnCall own;
+    SharedCall shared;
+};
 int launch_few(const Call &c, hipStream_t s);      // paged_decode.hip
+int launch_few(const SharedCalls &c, hipStream_t s);  // the own part, and the plan of both
 int launch_many(const Call &c, hipStream_t s);     // paged_chunk.hip
+int launch_many(const OwnCall &c, hipStream_t s);
+int launch_many(const SharedCall &c, hipStream_t s);
 int launch_combine(const Call &c, hipStream_t s);  // paged_attn.hip
 
 }  // namespace paged

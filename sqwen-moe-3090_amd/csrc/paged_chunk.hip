@@ -68,7 +68,7 @@ constexpr int kLdsBytes = kLdsRaw + 4 * kRawTile + 16;
 static_assert(kLdsBytes <= 160 * 1024, "LDS budget");
 static_assert(kLdsRaw % 16 == 0 && kKStage % 16 == 0 && kVStage % 16 == 0, "alignment of the stages");
 constexpr int kSlack = 8;  // log2 of the largest P the lazy rescale admits
-constexpr int kEp = 6;     // P travels as P 2^kEp (at most 2^14)
+constexpr int kEp = kPBits;  // P travels as P 2^kEp (at most 2^14)
 constexpr int kMaxE = 24;  // of the V scales: makes the smallest fp16 one
 
 // max(x, x of lane ^ 16) and max(x, x of lane ^ 32) with gfx950's row swaps (no
@@ -273,7 +273,8 @@ struct QRow {
 
 // ---------------------------------------------------------------- work split
 
-__device__ __forceinline__ Item many_item(const Call &c, int lin, int qb) {
+template <class C>
+__device__ __forceinline__ Item many_item(const C &c, int lin, int qb) {
     Item it{};
     const Work w = *reinterpret_cast<const Work *>(c.work);
     it = reinterpret_cast<const Item *>(c.work + kListAt)[min(lin, kListed - 1)];  // beside it, used if there is a list
@@ -307,9 +308,12 @@ __device__ __forceinline__ Item many_item(const Call &c, int lin, int qb) {
     return it;
 }
 
-// kRG = 2: 128 query rows a workgroup; 1: 64 rows. OPT: the logits are capped or biased.
-template <int kRG, bool OPT>
-__global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
+// kRG = 2: 128 query rows a workgroup; 1: 64 rows. OPT: the logits are capped or biased. C: Call,
+// or one of the two parts of a call whose groups share prefixes: in the shared one a tile's
+// tokens are members of a group, wherever their rows are.
+template <int kRG, bool OPT, class C>
+__global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(C p) {
+    constexpr bool kShared = kIsShared<C>, kOwn = kIsOwn<C>;
     extern __shared__ __align__(16) uint8_t smem[];
     const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -323,11 +327,20 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
     const Request rq{uniform(it.rq.q0), uniform(it.rq.n), uniform(it.rq.kv), uniform(it.rq.pos0), uniform(it.rq.prefix)};
     const int q_base = it.tile * qb;        // its first token in the request
     const int q_top = min(q_base + qb, rq.n);
-    const bool whole = it.splits == 1;      // of the keys: the result goes out from here
+    const bool whole = !kShared && it.splits == 1;  // of the keys: the result goes out from here
     const int slot = it.slot + (it.kvh * it.splits + it.split) * it.tiles + it.tile;
-    if (it.split == 0 && it.kvh == 0 && tid < q_top - q_base)
-        p.where[rq.q0 + q_base + tid] =
-            whole ? make_int4(0, 0, 0, kDone) : make_int4(it.slot + it.tile, it.splits, tid * p.G, 4 * it.tiles + kMany);
+    // row of the tile's token i; a member that no plan wrote may be any number (< 0: none then)
+    auto row_at = [&](int i) {
+        if constexpr (kShared) {
+            const int t = p.members[rq.q0 + i];
+            return (uint32_t)t < (uint32_t)p.n_tok ? t : -1;
+        }
+        return rq.q0 + i;
+    };
+    int own_row = 0;
+    if (it.split == 0 && it.kvh == 0 && tid < q_top - q_base && (own_row = row_at(q_base + tid)) >= 0)
+        p.where[own_row] =
+            whole ? make_int4(0, 0, 0, kOwn ? kWhole : kDone) : make_int4(it.slot + it.tile, it.splits, tid * p.G, 4 * it.tiles + kMany);
 
     // Key range: the split, cut at the last key any token of the tile sees.
     const int k_begin = it.t0 * kPK;
@@ -386,9 +399,12 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
             const int i = group_of(p, r), h = kvh * p.G + r - i * p.G;
             const bool ok = q_base + i < q_top;
             my_see[rg] = ok ? sees(rq, q_base + i) : 0;
+            const int row = kShared && ok ? row_at(q_base + i) : rq.q0 + q_base + i;
             my_pos[rg] = rq.pos0 + q_base + i;
+            if constexpr (kShared) my_pos[rg] = OPT && ok ? p.m_pos[rq.q0 + q_base + i] : 0;
             my_slope[rg] = OPT && p.bias != 0.0f ? slope2(p, h) : 0.0f;
-            qrow[rg].load(p, ok ? rq.q0 + q_base + i : rq.q0, h, g);
+            if constexpr (kShared) qrow[rg].load(p, ok && row >= 0 ? row : 0, h, g);
+            else qrow[rg].load(p, ok ? row : rq.q0, h, g);
             row_ok[rg] = ok;
             m_run[rg] = -INFINITY;
             l_part[rg] = 0.0f;
@@ -770,11 +786,11 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
             for (int T = 0; T < 16; ++T) x[T] = from[16 * T];
         }
     };
-    if (whole && p.gate) load_gate(0, gv[0]);
+    if (!kOwn && whole && p.gate) load_gate(0, gv[0]);
 #pragma unroll
     for (int k = 0; k < 4 * kRG; ++k) {
         const int rg = k >> 2, i = k & 3, r = 16 * kRG * w + 16 * rg + 4 * g + i;
-        if (whole && p.gate && k + 1 < 4 * kRG) load_gate(k + 1, gv[(k + 1) & 1]);
+        if (!kOwn && whole && p.gate && k + 1 < 4 * kRG) load_gate(k + 1, gv[(k + 1) & 1]);
         int h;
         const int tok = token_of(k, &h);
         if (tok >= q_top) continue;
@@ -786,10 +802,16 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
             float o[16];
 #pragma unroll
             for (int T = 0; T < 16; ++T) o[T] = __builtin_amdgcn_ldexpf(acc[rg][T][i], e_out[T >> 2]) * inv;
-            if (p.gate) {
+            if (!kOwn && p.gate) {
 #pragma unroll
                 for (int T = 0; T < 16; ++T) o[T] = gate_by(o[T], gv[k & 1][T]);
             }
+            if constexpr (kOwn)
+                if (n == 0) {
+                    float *ml_to = p.stats + ((int64_t)(rq.q0 + tok) * p.H + h) * 2;
+                    store_through(ml_to, lrow != lrow ? lrow : mrow);
+                    store_through(ml_to + 1, lrow);
+                }
 #pragma unroll
             for (int T = 0; T < 16; ++T) store_through(to + 16 * T, o[T]);
         } else {
@@ -807,27 +829,32 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(Call p) {
     }
 }
 
-}  // namespace
-
-int launch_many(const Call &c, hipStream_t s) {
+template <class C>
+int launch(const C &c, const char *name, hipStream_t s) {
     const bool opt = c.cap2 != 0.0f || c.bias != 0.0f;
     static std::once_flag once;  // the LDS limit is raised once per process
     static hipError_t err = hipSuccess;
     std::call_once(once, [] {
-        for (const void *f : {(const void *)paged_many_kernel<1, false>, (const void *)paged_many_kernel<1, true>,
-                              (const void *)paged_many_kernel<2, false>, (const void *)paged_many_kernel<2, true>})
+        for (const void *f : {(const void *)paged_many_kernel<1, false, C>, (const void *)paged_many_kernel<1, true, C>,
+                              (const void *)paged_many_kernel<2, false, C>, (const void *)paged_many_kernel<2, true, C>})
             if (err == hipSuccess) err = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsBytes);
     });
     if (err != hipSuccess) return hip_status(err, "paged_attn LDS attribute");
     const dim3 grid((unsigned)c.grid_c);
-    const int prof = profile_start("paged_chunk", s);
-    if (c.rows_c == 64 && opt) paged_many_kernel<1, true><<<grid, dim3(kThreads), kLdsBytes, s>>>(c);
-    else if (c.rows_c == 64) paged_many_kernel<1, false><<<grid, dim3(kThreads), kLdsBytes, s>>>(c);
-    else if (opt) paged_many_kernel<2, true><<<grid, dim3(kThreads), kLdsBytes, s>>>(c);
-    else paged_many_kernel<2, false><<<grid, dim3(kThreads), kLdsBytes, s>>>(c);
+    const int prof = profile_start(name, s);
+    if (c.rows_c == 64 && opt) paged_many_kernel<1, true, C><<<grid, dim3(kThreads), kLdsBytes, s>>>(c);
+    else if (c.rows_c == 64) paged_many_kernel<1, false, C><<<grid, dim3(kThreads), kLdsBytes, s>>>(c);
+    else if (opt) paged_many_kernel<2, true, C><<<grid, dim3(kThreads), kLdsBytes, s>>>(c);
+    else paged_many_kernel<2, false, C><<<grid, dim3(kThreads), kLdsBytes, s>>>(c);
     profile_stop(prof, s);
     return hip_status(hipGetLastError(), "paged_attn launch");
 }
+
+}  // namespace
+
+int launch_many(const Call &c, hipStream_t s) { return launch(c, "paged_chunk", s); }
+int launch_many(const OwnCall &c, hipStream_t s) { return launch(c, "paged_chunk", s); }
+int launch_many(const SharedCall &c, hipStream_t s) { return launch(c, "paged_shared", s); }
 
 }  // namespace paged
 }  // namespace sqa

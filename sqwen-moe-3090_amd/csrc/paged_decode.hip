@@ -32,6 +32,7 @@
 // 1.2 tiles of 18 KB a us, 5.7 TB/s on the chip) and about 8 us at a launch's start
 // and end: 16 requests of 100000 to 131071 keys 231 us, 4.6 TB/s (a copy: 4.98).
 #include <mutex>
+#include <type_traits>
 
 #define SQA_PLAN_CHUNKS
 #include "paged_work.hpp"
@@ -71,7 +72,7 @@ constexpr float kSlack = 8.0f;  // log2 of the largest P the lazy rescale admits
 // same values; with |d_v 2^E| < 2, A = P d_v 2^E stays below 2^15. (The range goes to P:
 // at P 2^-4 its lo part lay so deep in fp16's subnormals that the output was 1.4e-6 off
 // for 4096 keys, now 2e-7.)
-constexpr float kPShift = -6.0f;
+constexpr float kPShift = -(float)kPBits;
 // Largest d_v exponent E of the value wavefronts (d_v enters A as d_v 2^E): V
 // scales below 2^-20 lose low bits of A; 2^E stays two fp16 powers of two.
 constexpr int kMaxDvExp = 18;
@@ -286,8 +287,14 @@ __device__ __forceinline__ int lds_byte(int row, int c) {
 // TWO = true : up to 16 rows (rows 0-7 and 8-15 as two B sets, one A operand).
 // OPT: the logits are capped or biased. PLAN: a last workgroup plans the many-row kernel.
 // (128 registers a lane; TWO with OPT and PLAN keeps one more in scratch, the others none.)
-template <bool TWO, bool OPT, bool PLAN>
-__global__ __launch_bounds__(kThreads, 4) void paged_few_kernel(Call p) {
+// A: Call, or SharedCalls, whose shared part is planned beside the own one.
+__device__ __forceinline__ const Call &own_of(const Call &a) { return a; }
+__device__ __forceinline__ const Call &own_of(const SharedCalls &a) { return a.own; }
+
+template <bool TWO, bool OPT, bool PLAN, class A>
+__global__ __launch_bounds__(kThreads, 4) void paged_few_kernel(A a) {
+    constexpr bool kShared = !std::is_same<A, Call>::value;
+    const Call &p = own_of(a);
     extern __shared__ __align__(16) uint8_t smem[];
     const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // wave-uniform, in an SGPR
@@ -303,7 +310,12 @@ __global__ __launch_bounds__(kThreads, 4) void paged_few_kernel(Call p) {
     constexpr int kRowMask = TWO ? 15 : 7;  // rows 8-15 mirror rows 0-7 when only 8 exist
 
     if (PLAN && blockIdx.z == gridDim.z - 1) {
-        if (blockIdx.x == 0 && blockIdx.y == 0) plan_chunks(p, reinterpret_cast<int *>(smem));
+        if constexpr (kShared) {
+            if (blockIdx.x == 0 && blockIdx.y == 0) plan_chunks(a.shared, reinterpret_cast<int *>(smem));
+            if (blockIdx.x == 1 && blockIdx.y == 0 && p.rows_c) plan_chunks(p, reinterpret_cast<int *>(smem));
+        } else {
+            if (blockIdx.x == 0 && blockIdx.y == 0) plan_chunks(p, reinterpret_cast<int *>(smem));
+        }
         return;
     }
     // ---------------- piece and KV head of this workgroup ---------------------
@@ -312,7 +324,7 @@ __global__ __launch_bounds__(kThreads, 4) void paged_few_kernel(Call p) {
     const int kvh = (int)blockIdx.y;
     const int piece = (int)(8 * blockIdx.z + blockIdx.x);
     const Piece pc = few_piece(p, reinterpret_cast<int *>(smem), piece, p.most_d);
-    if (!PLAN && blockIdx.x + blockIdx.y + blockIdx.z == 0) skip_large(p);
+    if ((kShared ? p.rows_c == 0 : !PLAN) && blockIdx.x + blockIdx.y + blockIdx.z == 0) skip_large(p);
     // The workspace has slots for `room` pieces. Requests whose ranges of q_start overlap may be
     // more than there are tokens, which room counts on, and the grid is a multiple of 8 of them.
     if (pc.b < 0 || piece >= p.room) return;
@@ -1030,27 +1042,50 @@ __global__ __launch_bounds__(kThreads, 4) void paged_few_kernel(Call p) {
 }
 
 
+void raise_lds(hipError_t *err, const void *kernel) {
+    if (*err == hipSuccess) *err = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsBytes);
+}
+
+dim3 few_grid(const Call &c, bool plan) { return dim3(8, (unsigned)c.Hkv, (unsigned)((c.room + 7) / 8 + (plan ? 1 : 0))); }
+
 }  // namespace
 
 int launch_few(const Call &c, hipStream_t s) {
     const bool two = c.rows_d > 8, opt = c.cap2 != 0.0f || c.bias != 0.0f;
-    const dim3 grid(8, (unsigned)c.Hkv, (unsigned)((c.room + 7) / 8 + (c.rows_c ? 1 : 0)));
     typedef void (*Kernel)(Call);
     static const Kernel kernels[8] = {
-        paged_few_kernel<false, false, false>, paged_few_kernel<true, false, false>, paged_few_kernel<false, true, false>,
-        paged_few_kernel<true, true, false>,   paged_few_kernel<false, false, true>, paged_few_kernel<true, false, true>,
-        paged_few_kernel<false, true, true>,   paged_few_kernel<true, true, true>};
+        paged_few_kernel<false, false, false, Call>, paged_few_kernel<true, false, false, Call>,
+        paged_few_kernel<false, true, false, Call>,  paged_few_kernel<true, true, false, Call>,
+        paged_few_kernel<false, false, true, Call>,  paged_few_kernel<true, false, true, Call>,
+        paged_few_kernel<false, true, true, Call>,   paged_few_kernel<true, true, true, Call>};
     static std::once_flag once;  // the LDS limit is raised once per process
     static hipError_t err = hipSuccess;
     std::call_once(once, [] {
-        for (Kernel k : kernels)
-            if (err == hipSuccess) err = hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize, kLdsBytes);
+        for (Kernel k : kernels) raise_lds(&err, (const void *)k);
     });
     if (err != hipSuccess) return hip_status(err, "paged_attn LDS attribute");
     const int prof = profile_start("paged_decode", s);
-    kernels[two + 2 * opt + 4 * (c.rows_c != 0)]<<<grid, dim3(kThreads), kLdsBytes, s>>>(c);
+    kernels[two + 2 * opt + 4 * (c.rows_c != 0)]<<<few_grid(c, c.rows_c != 0), dim3(kThreads), kLdsBytes, s>>>(c);
     profile_stop(prof, s);
     return hip_status(hipGetLastError(), "paged_attn launch");
+}
+
+int launch_few(const SharedCalls &c, hipStream_t s) {
+    const bool two = c.own.rows_d > 8, opt = c.own.cap2 != 0.0f || c.own.bias != 0.0f;
+    typedef void (*Kernel)(SharedCalls);
+    static const Kernel kernels[4] = {
+        paged_few_kernel<false, false, true, SharedCalls>, paged_few_kernel<true, false, true, SharedCalls>,
+        paged_few_kernel<false, true, true, SharedCalls>, paged_few_kernel<true, true, true, SharedCalls>};
+    static std::once_flag once;
+    static hipError_t err = hipSuccess;
+    std::call_once(once, [] {
+        for (Kernel k : kernels) raise_lds(&err, (const void *)k);
+    });
+    if (err != hipSuccess) return hip_status(err, "paged_attn_shared LDS attribute");
+    const int prof = profile_start("paged_decode", s);
+    kernels[two + 2 * opt]<<<few_grid(c.own, true), dim3(kThreads), kLdsBytes, s>>>(c);
+    profile_stop(prof, s);
+    return hip_status(hipGetLastError(), "paged_attn_shared launch");
 }
 
 }  // namespace paged

@@ -1,92 +1,150 @@
-// paged_shared.hip - attention of a batch whose groups of requests share long prefixes: a
-// request's own pages and its group's pages under one softmax.
+// paged_shared.hip - attention of a batch whose groups of requests share long prefixes: what a
+// call launches, its workspace, and the merge of the two parts.
 //
-// The simple form: a wavefront takes one query row, 4 dims a lane, and goes through the
-// keys of the shared prefix and then its own with a running maximum and sum.
-#include "paged_attn.hpp"
+// A row's own keys go the way of paged_attn (paged_decode.hip, paged_chunk.hip). The keys of a
+// group's prefix meet the rows of all its tokens at once: the many-row kernel of paged_chunk.hip
+// takes tiles of 128 (or 64) rows out of the group's list of members, so that a key is read and
+// expanded once for that many rows instead of once for every request's 8. An extra workgroup of
+// the few-row launch plans the tiles and splits. Every row's parts (splits of its own keys and of
+// the prefix) then meet in the merge, M the largest of all their maxima:
+//   out = sum_s acc_s 2^(m_s - M) / sum_s l_s 2^(m_s - M), then the gate.
+#include "paged_merge.hpp"
+#include "paged_work.hpp"
 
 namespace sqa {
 namespace paged {
 namespace {
 
-struct Shared {
-    Call c;                   // own part
-    const int32_t *table;     // pages of the groups' prefixes
-    int64_t table_stride, most_kv;
-    const int32_t *len, *token_group;
-    int groups;
+constexpr int kThreads = 256;
+
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+
+struct Merge {
+    OwnCall own;
+    SharedCall shared;
+    const int32_t *token_group;
+    float *dst;
 };
 
-struct Online {
-    float m = -INFINITY, l = 0.0f, o[4] = {};
+// A wavefront takes R heads of a token together, 4 dims a lane; 64 / R parts at a time: lane
+// r * 64 / R + i holds part i's weight for head r. The own parts come first, then the prefix's.
+template <int R>
+__global__ __launch_bounds__(kThreads) void merge_shared_kernel(Merge p) {
+    constexpr int kS = 64 / R, kBatch = R >= 4 ? 2 : 8;
+    const OwnCall &c = p.own;
+    const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int t = (int)blockIdx.y + (int)(blockIdx.z << 15), h0 = ((int)blockIdx.x * 4 + wave) * R;
+    if (t >= c.n_tok || h0 >= c.H) return;
+    // (of no request: the entry was not written)
+    if (t < c.q_start[0] || t >= c.q_start[c.B]) return;
+    const int4 w1 = c.where[t];
+    const int g = p.token_group[t];
+    const bool member = g >= 0 && g < p.shared.B && p.shared.kv_len[g] > 0;
+    const int4 w2 = member ? p.shared.where[t] : make_int4(0, 0, 0, kDone);
+    const bool whole = (w1.w & 3) == kWhole;
+    Row a[R], b[R];
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+        const int h = min(h0 + k, c.H - 1);
+        a[k] = partials(c, w1, h);
+        if (whole) {
+            const int64_t at = (int64_t)t * c.H + h;
+            a[k] = Row{c.dst + at * 256, c.stats + at * 2, 0, 1};
+        }
+        b[k] = partials(p.shared, w2, h);
+    }
+    if (a[0].n == 0) return;  // of the token: all heads alike
+    const int n1 = a[0].n, n = n1 + b[0].n, k_own = lane / kS, i_own = lane % kS;
+    const float *ml1 = a[0].ml, *ml2 = b[0].ml;
+#pragma unroll
+    for (int k = 1; k < R; ++k) ml1 = k_own == k ? a[k].ml : ml1, ml2 = k_own == k ? b[k].ml : ml2;
+    floatx4 o[R], g4[R];
+    float M = -INFINITY, L = 0.0f;  // of head k_own
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+        o[k] = floatx4{0.f, 0.f, 0.f, 0.f};
+        if (c.gate) g4[k] = *reinterpret_cast<const float4a *>(gate_row(c, t, min(h0 + k, c.H - 1)) + 4 * lane);
+    }
+    for (int s0 = 0; s0 < n; s0 += kS) {
+        const int s = s0 + i_own;
+        const float *at = s < n1 ? ml1 + s * (a[0].step / 128) : ml2 + (s - n1) * (b[0].step / 128);
+        const float2 ml = s < n ? *reinterpret_cast<const float2 *>(at) : make_float2(-INFINITY, 0.0f);
+        float m = ml.x;
+#pragma unroll
+        for (int x = 1; x < kS; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
+        const float Mn = fmaxf(M, m), al = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - Mn);
+        const float e = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - Mn);
+        float l = ml.x == -INFINITY ? 0.0f : ml.y * e;
+        const float w = whole && s == 0 ? l : e;  // a whole part comes normalised
+#pragma unroll
+        for (int x = 1; x < kS; x <<= 1) l += __shfl_xor(l, x);
+        L = L * al + l;
+        M = Mn;
+#pragma unroll
+        for (int k = 0; k < R; ++k) o[k] *= __int_as_float(__builtin_amdgcn_readlane(__float_as_int(al), k * kS));
+        const int end = min(n - s0, kS);
+        for (int s1 = 0; s1 < end; s1 += kBatch) {
+            floatx4 x[kBatch][R];
+            float wt[kBatch][R];
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j)
+#pragma unroll
+                for (int k = 0; k < R; ++k) {
+                    const int i = s0 + s1 + j;
+                    wt[j][k] = s1 + j < end ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), k * kS + min(s1 + j, kS - 1))) : 0.0f;
+                    const float *from = i < n1 ? a[k].acc + i * a[k].step : b[k].acc + (i - n1) * b[k].step;
+                    if (wt[j][k] != 0.0f) x[j][k] = *reinterpret_cast<const floatx4 *>(from + 4 * lane);
+                }
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j)
+#pragma unroll
+                for (int k = 0; k < R; ++k)
+                    if (wt[j][k] != 0.0f) o[k] += x[j][k] * wt[j][k];
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+        if (h0 + k >= c.H) break;
+        const float Lk = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(L), k * kS));
+        const float inv = Lk == 0.0f ? 0.0f : 1.0f / Lk;
+        floatx4 x = o[k] * inv;
+        if (c.gate) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = gate_by(x[i], g4[k][i]);
+        }
+        *reinterpret_cast<floatx4 *>(p.dst + ((int64_t)t * c.H + h0 + k) * kHeadDim + 4 * lane) = x;
+    }
+}
+
+// The workspace of a call: stats and results of rows of one part (where there is a chunk kernel),
+// the shared part's entries, plan and slots, then the own part's.
+struct Space {
+    Plan own, shared;
+    size_t stats, whole;
+    size_t fixed() const { return stats + whole; }
+    size_t least_shared() const { return shared.where + shared.work + (size_t)least_slots * shared.slot_c + 512; }
+    size_t full_shared() const { return shared.where + shared.work + (size_t)shared.slots_c * shared.slot_c + 512; }
+    int64_t least_slots;
 };
 
-// Sum over the wavefront.
-__device__ __forceinline__ float wsum(float x) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o);
-    return x;
-}
-
-// A lane's 4 dims of a head row: byte pair within its block.
-__device__ __forceinline__ void row4(const uint8_t *row, int lane, float (&x)[4]) {
-    const uint8_t *b = row + (lane >> 3) * SQA_Q4_0_BLOCK_BYTES;
-    const int t = lane & 7;
-    const float d = (float)*reinterpret_cast<const _Float16 *>(b);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = (float)((b[2 + 4 * (t & 3) + j] >> (t < 4 ? 0 : 4) & 15) - 8) * d;
-}
-
-__device__ void keys(const Call &c, const int32_t *row, int n, int kvh, int lane, const float (&q)[4], float slope, int far,
-                     Online &a) {
-    for (int j = 0; j < n; ++j) {
-        const int id = row[j >> c.lp];
-        if ((uint32_t)id >= (uint32_t)c.n_pages) continue;
-        const int64_t at = (int64_t)(j & (c.page - 1)) * c.row_bytes + kvh * kHeadRowBytes;
-        float k[4];
-        row4(c.k + id * c.k_page + at, lane, k);
-        float s[1] = {wsum(fmaf(q[0], k[0], fmaf(q[1], k[1], fmaf(q[2], k[2], q[3] * k[3]))))};
-        if (c.cap2 != 0.0f) cap_logits(s, c.cap2, c.cap_inv, 0.0f);
-        if (c.bias != 0.0f) s[0] = fmaf(-slope, fabsf((float)(far - j)), s[0]);
-        const float m = fmaxf(a.m, s[0]), al = a.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(a.m - m);
-        const float p = s[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s[0] - m);
-        row4(c.v + id * c.v_page + at, lane, k);
-        a.m = m, a.l = fmaf(a.l, al, p);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) a.o[i] = fmaf(a.o[i], al, p * k[i]);
+Space space(int64_t n_tok, int64_t H, int64_t Hkv, int64_t B, int64_t groups, int64_t max_q) {
+    Space s{};
+    s.own = plan_of(n_tok, H, Hkv, B, max_q);
+    if (s.own.rows_c) {
+        s.stats = al256((size_t)(n_tok * H) * 8);
+        s.whole = al256((size_t)(n_tok * H) * kHeadDim * 4);
     }
-}
-
-__global__ __launch_bounds__(256) void shared_simple_kernel(Shared p) {
-    const Call &c = p.c;
-    const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int t = (int)(row / c.H), h = (int)(row - (int64_t)t * c.H);
-    if (t >= c.n_tok || t < c.q_start[0] || t >= c.q_start[c.B]) return;
-    int lo = 0, hi = c.B;  // the request: the last one that starts at or before t
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (c.q_start[mid] <= t) lo = mid;
-        else hi = mid;
-    }
-    const Request rq = request(c, lo);
-    const float4a x = *reinterpret_cast<const float4a *>(c.q + t * c.q_nb1 + h * c.q_nb2 + 16 * lane);
-    float q[4], amax = 0.0f;
-    for (int i = 0; i < 4; ++i) amax = fmaxf(amax, fabsf(x[i]));
-    for (int o = 1; o < 8; o <<= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
-    const float d = (float)(_Float16)(amax / 127.f) * c.qscale, id = amax != 0.0f ? 127.f / amax : 0.0f;
-    for (int i = 0; i < 4; ++i) q[i] = rintf(x[i] * id) * d;
-    const float slope = c.bias != 0.0f ? slope2(c, h) : 0.0f;
-    const int kvh = group_of(c, h), g = p.token_group[t], i = t - rq.q0;
-    const int len = g >= 0 && g < p.groups ? (int)min((int64_t)max(p.len[g], 0), p.most_kv) : 0;
-    Online a;
-    keys(c, p.table + (len ? g * p.table_stride : 0), len, kvh, lane, q, slope, len + rq.pos0 + i, a);
-    keys(c, c.table + lo * c.table_stride, sees(rq, i), kvh, lane, q, slope, rq.pos0 + i, a);
-    const float *gate = c.gate ? reinterpret_cast<const float *>(c.gate + t * c.gate_nb2 + h * c.gate_nb1) + 4 * lane : nullptr;
-    for (int k = 0; k < 4; ++k) {
-        const float o = a.l == 0.0f ? 0.0f : a.o[k] / a.l;
-        c.dst[((int64_t)t * c.H + h) * kHeadDim + 4 * lane + k] = gate ? gate_by(o, gate[k]) : o;
-    }
+    const int64_t G = H / Hkv, cus = device_cu_count(), active = groups < n_tok ? groups : n_tok;
+    Plan &p = s.shared;
+    p.rows_c = n_tok * G <= 64 ? 64 : 128;
+    p.where = al256((size_t)n_tok * 16);
+    p.work = al256(work_bytes(groups));
+    p.slot_c = (size_t)p.rows_c * (kHeadDim + 2) * 4;
+    // every tile of members is a slot, at least: whole tiles and a last one of every group
+    s.least_slots = (n_tok / (p.rows_c / G) + active) * Hkv;
+    p.slots_c = s.least_slots + cus > 3 * cus ? s.least_slots + cus : 3 * cus;
+    p.grid_c = (p.slots_c + 7) & ~(int64_t)7;
+    return s;
 }
 
 }  // namespace
@@ -95,23 +153,65 @@ __global__ __launch_bounds__(256) void shared_simple_kernel(Shared p) {
 using namespace paged;
 
 size_t paged_shared_workspace(int64_t n_tok, int64_t H, int64_t Hkv, int64_t B, int64_t groups, int64_t max_q) {
-    (void)H, (void)Hkv, (void)B, (void)groups, (void)max_q;
-    return n_tok ? 512 : 0;
+    if (n_tok < 1) return 0;
+    const Space s = space(n_tok, H, Hkv, B, groups, max_q);
+    return s.fixed() + full_bytes(s.own) + s.full_shared() + 512;
 }
 
 int launch_paged_shared(const SharedArgs &a, hipStream_t s) {
-    if (!a.own.ws || a.own.ws_bytes < 512)
-        return set_error(SQA_ERR_WORKSPACE, "paged_attn_shared: workspace %zu bytes < 512 needed", a.own.ws ? a.own.ws_bytes : (size_t)0);
-    Shared p{};
-    p.c = call_of(a.own);
-    p.table = (const int32_t *)a.table->data, p.table_stride = (int64_t)a.table->nb[1] / 4;
-    p.most_kv = a.table->ne[0] << p.c.lp;
-    p.len = (const int32_t *)a.len->data, p.token_group = (const int32_t *)a.token_group->data;
-    p.groups = (int)a.table->ne[1];
-    const int prof = profile_start("paged_shared", s);
-    shared_simple_kernel<<<dim3((unsigned)(((int64_t)p.c.n_tok * p.c.H + 3) / 4)), dim3(256), 0, s>>>(p);
+    const char *what = "paged_attn_shared";
+    Merge m{};
+    static_cast<Call &>(m.own) = call_of(a.own);
+    m.dst = m.own.dst;
+    SharedCall &c = m.shared;
+    static_cast<Call &>(c) = m.own;
+    c.table = (const int32_t *)a.table->data, c.table_stride = (int64_t)a.table->nb[1] / 4;
+    c.most_kv = a.table->ne[0] << c.lp;
+    c.B = (int)a.table->ne[1];
+    c.q_start = (const int32_t *)a.m_start->data, c.kv_len = (const int32_t *)a.len->data;
+    c.prefix = nullptr;
+    c.members = (const int32_t *)a.members->data, c.m_pos = (const int32_t *)a.m_pos->data;
+    m.token_group = (const int32_t *)a.token_group->data;
+
+    const Space sp = space(c.n_tok, c.H, c.Hkv, m.own.B, c.B, a.own.max_q);
+    const size_t least_own = least_bytes(sp.own), least = sp.fixed() + least_own + sp.least_shared() + 512;
+    if (!a.own.ws || a.own.ws_bytes < least)
+        return set_error(SQA_ERR_WORKSPACE, "%s: workspace %zu bytes < %zu needed", what, a.own.ws ? a.own.ws_bytes : (size_t)0, least);
+    if (sp.shared.grid_c > INT32_MAX) return set_error(SQA_ERR_UNSUPPORTED, "%s: too many query tiles", what);
+    uint8_t *base = reinterpret_cast<uint8_t *>(((uintptr_t)a.own.ws + 255) & ~(uintptr_t)255);
+    m.own.stats = reinterpret_cast<float *>(base);
+    m.own.dst = reinterpret_cast<float *>(base + sp.stats);
+    base += sp.fixed();
+    // what is left beyond the least: to the shared part as much as it takes, the rest to the own one
+    // (half of it at least)
+    const size_t more = a.own.ws_bytes - least, take = sp.full_shared() - sp.least_shared();
+    const size_t own_take = full_bytes(sp.own) - least_own, half = more / 2 < own_take ? more / 2 : own_take;
+    const size_t shared_bytes = sp.least_shared() + (take < more - half ? take : more - half);
+    c.rows_c = sp.shared.rows_c, c.grid_c = (int)sp.shared.grid_c;
+    c.where = reinterpret_cast<int4 *>(base);
+    c.work = reinterpret_cast<int *>(base + sp.shared.where);
+    c.slots_c = (int)((shared_bytes - 512 - sp.shared.where - sp.shared.work) / sp.shared.slot_c);
+    if (c.slots_c > sp.shared.slots_c) c.slots_c = (int)sp.shared.slots_c;
+    c.acc_c = reinterpret_cast<float *>(base + sp.shared.where + sp.shared.work);
+    c.ml_c = c.acc_c + (size_t)c.slots_c * c.rows_c * kHeadDim;
+    c.most_d = c.slots_d = c.rows_d = 0;
+    uint8_t *rest = reinterpret_cast<uint8_t *>(((uintptr_t)(c.ml_c + (size_t)c.slots_c * c.rows_c * 2) + 255) & ~(uintptr_t)255);
+    int rc = lay_out(m.own, sp.own, rest, (size_t)((uint8_t *)a.own.ws + a.own.ws_bytes - rest), what);
+    if (rc) return rc;
+
+    rc = launch_few(SharedCalls{m.own, c}, s);
+    if (!rc && m.own.rows_c) rc = launch_many(m.own, s);
+    if (!rc) rc = launch_many(c, s);
+    if (rc) return rc;
+
+    const int prof = profile_start("paged_shared_merge", s);
+    const bool four = (int64_t)c.n_tok * c.H > 8192 && c.H >= 16;
+    const dim3 grid((unsigned)((c.H + (four ? 16 : 4) - 1) / (four ? 16 : 4)), (unsigned)(c.n_tok < (1 << 15) ? c.n_tok : 1 << 15),
+                    (unsigned)((c.n_tok + (1 << 15) - 1) >> 15));
+    if (four) merge_shared_kernel<4><<<grid, dim3(kThreads), 0, s>>>(m);
+    else merge_shared_kernel<1><<<grid, dim3(kThreads), 0, s>>>(m);
     profile_stop(prof, s);
-    return hip_status(hipGetLastError(), "paged_attn_shared launch");
+    return hip_status(hipGetLastError(), "paged_attn_shared merge launch");
 }
 
 }  // namespace sqa

@@ -76,9 +76,14 @@ __device__ constexpr int kTried[kChoices] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20
 constexpr float kWg = 4.5f, kMerge = 0.7f, kMergeSlot = 0.014f;
 constexpr int kCounted = 64, kLevels = 8, kRounds = 4;
 
+// Groups of a shared prefix are requests whose tokens all see all keys and whose parts all go
+// through the merge.
+//
 // Run by all 512 threads of one workgroup; lds: 512 + 6 * 2600 + 1 words, or 512 + B + 1.
 // Lanes are requests (a run of them above 512), then lengths that are tried, then items.
-__device__ __forceinline__ void plan_chunks(const Call &c, int *lds) {
+template <class C>
+__device__ __forceinline__ void plan_chunks(const C &c, int *lds) {
+    constexpr bool kAll = kIsShared<C>;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, qb = c.rows_c / c.G;
     Work *out = reinterpret_cast<Work *>(c.work);
     int *first = c.work + kFirstAt, *slot = first + c.B + 1;
@@ -101,7 +106,7 @@ __device__ __forceinline__ void plan_chunks(const Call &c, int *lds) {
         const int T = chunk_tiles(c, r, qb, &kt);
         // query tile i of T ends (T - 1 - i) * qb keys before the last one
         const float all = (float)T * (float)kt;
-        work += fmaxf(all - 0.5f * (float)T * (float)(T - 1) * (float)qb / kChunkKeys, 0.5f * all);
+        work += kAll ? all : fmaxf(all - 0.5f * (float)T * (float)(T - 1) * (float)qb / kChunkKeys, 0.5f * all);
         wgs += T;
         longest = max(longest, kt);
     }
@@ -131,7 +136,7 @@ __device__ __forceinline__ void plan_chunks(const Call &c, int *lds) {
         int kt;
         const int T = chunk_tiles(c, load(b), qb, &kt), n = T * div_ceil(kt, l_j);
         n_j += n;
-        split_j += kt > l_j ? n : 0;
+        split_j += kAll || kt > l_j ? n : 0;
     }
     n_j += __shfl_xor(n_j, 16), split_j += __shfl_xor(split_j, 16);
     n_j += __shfl_xor(n_j, 32), split_j += __shfl_xor(split_j, 32);
@@ -204,7 +209,7 @@ __device__ __forceinline__ void plan_chunks(const Call &c, int *lds) {
         const int T = chunk_tiles(c, load(b), qb, &kt), S = div_ceil(kt, len), k = T * S * c.Hkv;
         start[b] = items;
         items += k;
-        slots += S > 1 ? k : 0;
+        slots += kAll || S > 1 ? k : 0;
     }
     const int upto = wave_scan(items), slots_upto = wave_scan(slots);
     if (lane == 63) sums[wave] = upto, sums[8 + wave] = slots_upto;
@@ -217,7 +222,7 @@ __device__ __forceinline__ void plan_chunks(const Call &c, int *lds) {
         (void)chunk_tiles(c, load(b), qb, &kt);
         first[b] = start[b] + before;
         slot[b] = slots_before;
-        slots_before += kt > len ? k : 0;
+        slots_before += kAll || kt > len ? k : 0;
     }
     __syncthreads();
     for (int b = b0; b < b1; ++b) start[b] += before;
