@@ -99,7 +99,7 @@ int sqa_supports_set_rows(const sqa_tensor *dst, const sqa_tensor *src, const sq
  *   src: Q4_0 [ne0, src_rows] (row stride src->nb[1], even)
  *   idx: I64 [n_rows] (element stride idx->nb[0]); rows may come more than once
  *   dst: F32 or F16 [ne0, n_rows] (row stride dst->nb[1], elements contiguous)
- * ne0 % 32 == 0. An index outside [0, src->ne[1]) reads as a row of zeros (the slots of -1 that a
+ * ne0 % 32 == 0, ne0 <= 2^17. An index outside [0, src->ne[1]) reads as a row of zeros (the slots of -1 that a
  * page plan gives). dst must not overlap src or idx.
  */
 int sqa_get_rows_q4_0(const sqa_tensor *dst, const sqa_tensor *src, const sqa_tensor *idx, void *stream);
@@ -170,7 +170,7 @@ int sqa_supports_rope_norm(const sqa_tensor *dst, const sqa_tensor *src, const s
  * (quantize_row_q4_0), the others' bytes stay. D of 64, 128 or 256 with a rope.
  * In place (dst is src) a row that one entry reads must be no other entry's to[]: from == to is
  * fine, as are ranges that do not meet; otherwise, and where to[] names a row twice, that row is
- * unspecified. dst overlaps nothing else.
+ * unspecified. dst overlaps nothing else. D * n_head <= 2^17.
  */
 int sqa_move_rows_q4_0(const sqa_tensor *dst, const sqa_tensor *src, const sqa_tensor *to, const sqa_tensor *from,
                        const sqa_tensor *delta, const sqa_rope *rope, void *stream);

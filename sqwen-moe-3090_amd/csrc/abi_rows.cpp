@@ -33,7 +33,7 @@ int check_get(const sqa_tensor *dst, const sqa_tensor *src, const sqa_tensor *id
         return set_error(SQA_ERR_INVALID, "%s: src and dst must be [ne0, rows]", what);
     if (ne0 < 1 || ne0 % SQA_QK4_0 || dst->ne[0] != ne0)
         return set_error(SQA_ERR_INVALID, "%s: rows must be equally long, a multiple of 32 values", what);
-    if (ne0 > (1 << 24) || n > (1 << 28) || n * (ne0 / 32) > ((int64_t)1 << 35))
+    if (ne0 > kMostRowValues || n > kMostRowCount)
         return set_error(SQA_ERR_UNSUPPORTED, "%s: sizes out of range", what);
     const int rc = check_index(idx, n, what, "idx");
     if (rc) return rc;
@@ -64,7 +64,7 @@ int check_move(const sqa_tensor *dst, const sqa_tensor *src, const sqa_tensor *t
             return set_error(SQA_ERR_UNSUPPORTED, "%s: rows must be contiguous blocks at even addresses", what);
         if (t->ne[2] > 1 && t->nb[2] < row * (uint64_t)heads) return set_error(SQA_ERR_INVALID, "%s: rows overlap", what);
     }
-    if (n < 0 || n > (1 << 28) || D > (1 << 20) || heads > (1 << 12) || n * heads * (D / 32) > ((int64_t)1 << 35))
+    if (n < 0 || n > kMostRowCount || D > kMostRowValues || heads > kMostRowValues || heads * D > kMostRowValues)
         return set_error(SQA_ERR_UNSUPPORTED, "%s: sizes out of range", what);
     int rc = check_index(to, n, what, "to");
     if (!rc) rc = check_index(from, n, what, "from");
@@ -86,6 +86,10 @@ int check_move(const sqa_tensor *dst, const sqa_tensor *src, const sqa_tensor *t
         return set_error(SQA_ERR_UNSUPPORTED, "%s: ext_factor != 0 (YaRN ramp) is not supported", what);
     if (!std::isfinite(rope->freq_base) || rope->freq_base <= 0.0f || !std::isfinite(rope->freq_scale))
         return set_error(SQA_ERR_INVALID, "%s: freq_base must be positive, freq_scale finite", what);
+    // the fastest of the pairs; the kernel's reduction is for angles below 3e9
+    const double fast = fmax(1.0, pow((double)rope->freq_base, -2.0 * (rope->n_rot / 2 - 1) / rope->n_rot)) * fabs((double)rope->freq_scale);
+    if (!(fast <= kMostFreq))
+        return set_error(SQA_ERR_UNSUPPORTED, "%s: rotation pairs of more than %g radians a position", what, kMostFreq);
     return SQA_OK;
 }
 
@@ -139,9 +143,12 @@ int sqa_move_rows_q4_0(const sqa_tensor *dst, const sqa_tensor *src, const sqa_t
     if (rope) {
         p.delta = (const int32_t *)delta->data;
         p.n_rot = rope->n_rot;
-        for (int k = 0; k < 4; ++k) p.sections[k] = rope->sections[k], p.sect += rope->sections[k];
-        for (int k = 0; k < p.n_rot / 2; ++k)
+        const int32_t *n = rope->sections, sect = n[0] + n[1] + n[2] + n[3];
+        for (int k = 0; k < p.n_rot / 2; ++k) {
             p.freq[k] = (double)rope->freq_scale * pow((double)rope->freq_base, -2.0 * k / p.n_rot);
+            const int s = k % sect, c = s % 3;  // the sections' interleaved order, t h w
+            p.component[k] = s >= 3 * n[c] ? 3 : (uint8_t)c;
+        }
     }
     return launch_move_rows_q4_0(p, (hipStream_t)stream);
 }

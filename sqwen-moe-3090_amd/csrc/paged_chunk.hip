@@ -314,6 +314,11 @@ __device__ __forceinline__ Item many_item(const C &c, int lin, int qb) {
 template <int kRG, bool OPT, class C>
 __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(C p) {
     constexpr bool kShared = kIsShared<C>, kOwn = kIsOwn<C>;
+    // Who expands K: the score waves, between their MFMAs, or with the options, whose score waves have
+    // no registers left for it (spills: 45 us became 74), the value waves as they do V. Both tensors in
+    // the score waves: 1278 us where this is 1184 and all in the value waves 1231 (2040 tokens behind
+    // 16000 shared keys).
+    constexpr bool kScoreK = !OPT;
     extern __shared__ __align__(16) uint8_t smem[];
     const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -425,6 +430,8 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(C p) {
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf) k_off[bp][hf] = n * 512 + 16 * ((4 * bp + g) ^ (n & 7)) + 8 * (hf ^ nh);
         const int p_off = w * (kRG * 2048) + 16 * lane;  // P slots [w][rg][half][lane]
+        Expand ex;
+        ex.init(w, lane);
 
         int ida = id_of(0, 0), idb = id_of(0, 1);  // pages of the tile's two groups
         for (int t = 0; t <= n_tiles && n_tiles > 0; ++t) {
@@ -454,6 +461,8 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(C p) {
             // d_k of the lane's four C rows 16kg + 4g + i, block b: 8 bytes at
             // Dk[b][16kg + 4g]
             const uint8_t *dkb = smem + (t & 1) * kKStage + kOffDk + 8 * g;
+            // the expansion of the next K tile goes between the MFMAs (the value waves did the first two)
+            if (kScoreK && t > 0) ex.read_k(smem, t + 1);
             // Software-pipelined by one step: step j = (block j >> 1, key group j & 1)
             // issues its MFMAs, then the d_k scaling of step j - 1 runs while they
             // execute. The scheduling barrier keeps the compiler from pulling the
@@ -493,6 +502,7 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(C p) {
 #pragma unroll
                     for (int rg = 0; rg < kRG; ++rg) cp[rg] = cn[rg];
                 }
+                if (kScoreK && t > 0 && j >= 8 && j < 16 && j % 2 == 0) ex.store_k(smem, t + 1, (j - 8) / 2);
             }
             float s[kRG][8];  // keys 8g + jj, base-2 logits
 #pragma unroll
@@ -724,7 +734,7 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(C p) {
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) bvn[hf] = lds_half8(smem, vb0 + 1024 * hf, vb1 + 1024 * hf);
         ex.read_v(smem, t);
-        ex.read_k(smem, t + 1);
+        if (!kScoreK) ex.read_k(smem, t + 1);
 #pragma unroll
         for (int b = 0; b < 8; ++b) {
             const half8 bv[2] = {bvn[0], bvn[1]};
@@ -763,7 +773,7 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(C p) {
             if (b == 1) scales(t, x0, y0);
             if (b == 2) ex.store_v(smem, t, 0);
             if (b == 3) ex.store_v(smem, t, 1);
-            if (b >= 4) ex.store_k(smem, t + 1, b - 4);
+            if (!kScoreK && b >= 4) ex.store_k(smem, t + 1, b - 4);
         }
     }
     __syncthreads();  // m and l of the rows ...

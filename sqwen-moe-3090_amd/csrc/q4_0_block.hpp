@@ -11,6 +11,16 @@
 
 namespace sqa {
 
+// x of another lane of the 8: quad permutes, row_half_mirror, row_shl:4.
+template <int kCtrl, typename T>
+__device__ __forceinline__ T dpp8(T x) {
+    int i;
+    __builtin_memcpy(&i, &x, 4);
+    i = __builtin_amdgcn_update_dpp(i, i, kCtrl, 0xf, 0xf, false);
+    __builtin_memcpy(&x, &i, 4);
+    return x;
+}
+
 // v: this lane's 4 values (block elements 4t..4t+3, t = lane & 7); blk: the
 // 18-byte block. All 8 lanes of the group must call it together.
 __device__ __forceinline__ void quantize_q4_0_block8(const float v[4], int t, uint8_t *blk) {
@@ -19,21 +29,21 @@ __device__ __forceinline__ void quantize_q4_0_block8(const float v[4], int t, ui
     // fma (v_fmaak_f32), and a value whose x*id lies within half an ulp below a
     // half-integer then truncated to the code below ggml's
 #pragma clang fp contract(off)
-    // Lane-local first-occurrence maximum of |x|; index 32 marks "none".
-    float amax = 0.0f, mx = 0.0f;
-    int im = 32;
+    // The largest |x| of the 8 lanes (a NaN counts as none), then the first element that has it and its
+    // sign as one number, by DPP within 8 lanes: neighbours, neighbouring pairs, the mirrored half.
+    float top = fmaxf(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fabsf(v[2])), fabsf(v[3]));
+    top = fmaxf(top, 0.0f);
+    top = fmaxf(top, dpp8<0xB1>(top));
+    top = fmaxf(top, dpp8<0x4E>(top));
+    top = fmaxf(top, dpp8<0x141>(top));
+    uint32_t first = 64;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const float a = fabsf(v[j]);
-        if (amax < a) { amax = a; mx = v[j]; im = 4 * t + j; }
-    }
-#pragma unroll
-    for (int off = 4; off >= 1; off >>= 1) {
-        const float a2 = __shfl_xor(amax, off, 8);
-        const float m2 = __shfl_xor(mx, off, 8);
-        const int i2 = __shfl_xor(im, off, 8);
-        if (a2 > amax || (a2 == amax && i2 < im)) { amax = a2; mx = m2; im = i2; }
-    }
+    for (int j = 3; j >= 0; --j)
+        first = fabsf(v[j]) == top ? (uint32_t)(8 * t + 2 * j) | __float_as_uint(v[j]) >> 31 : first;
+    first = min(first, dpp8<0xB1>(first));
+    first = min(first, dpp8<0x4E>(first));
+    first = min(first, dpp8<0x141>(first));
+    const float mx = top == 0.0f ? 0.0f : first & 1 ? -top : top;
 
     const float d = mx / -8.0f;
     const float id = d != 0.0f ? __fdiv_rn(1.0f, d) : 0.0f;
@@ -46,7 +56,7 @@ __device__ __forceinline__ void quantize_q4_0_block8(const float v[4], int t, ui
         word |= (uint32_t)(c & 0xff) << (8 * j);
     }
     // qs[j] = code[j] | code[j+16] << 4: lanes 0..3 take the high nibbles from lanes 4..7.
-    const uint32_t hi = __shfl_down(word, 4, 8);
+    const uint32_t hi = dpp8<0x104>(word);
     if (t < 4) {
         const uint32_t qs = word | (hi << 4);
         uint16_t *p = reinterpret_cast<uint16_t *>(blk + 2 + 4 * t);

@@ -14,10 +14,17 @@ struct GetRows {
     int64_t dst_nb1;
     int64_t n;    // rows
     int blocks;   // q4_0 blocks of a row
+    // set by the launch: its first row, rows of a workgroup, reciprocal of a row's units
+    int64_t first;
+    int rows;
+    float recip;
 };
-int launch_get_rows_q4_0(const GetRows &p, bool half, hipStream_t s);
+int launch_get_rows_q4_0(GetRows p, bool half, hipStream_t s);
 
 constexpr int kMostRot = 256;  // rotated dims of a head
+constexpr double kMostFreq = 1.25;  // radians a position: times 2^31 positions, below 3e9
+constexpr int64_t kMostRowValues = 1 << 17;  // of a row: what the kernels' divisions by a reciprocal are exact for
+constexpr int64_t kMostRowCount = (int64_t)1 << 40;
 
 // Rows moved: dst[to[i]] = src[from[i]], the first n_rot dims of every head rotated.
 struct MoveRows {
@@ -30,9 +37,14 @@ struct MoveRows {
     int64_t n;
     int heads, head_dim;
     int n_rot;             // 0: rows are copied
-    int sections[4], sect; // sect: the sections' sum
-    double freq[kMostRot / 2];  // radians a position, of every rotation pair
+    // of every rotation pair: radians a position, which position (t, h, w, e) turns it
+    double freq[kMostRot / 2];
+    uint8_t component[kMostRot / 2];
+    // set by the launch: its first row, rows of a workgroup, reciprocals of what its threads divide by
+    int64_t first;
+    int rows;
+    float recip_half, recip_turned, recip_lanes, recip_copy, recip_rest;
 };
-int launch_move_rows_q4_0(const MoveRows &p, hipStream_t s);
+int launch_move_rows_q4_0(MoveRows p, hipStream_t s);
 
 }  // namespace sqa

@@ -72,10 +72,11 @@ def test_get_rows_gives_what_set_rows_wrote(sqa, dev):
     kv.begin_step(300)
     kv.append(1, x, 2 * x, idx)
     k, v = kv.read(1, idx), kv.read(1, idx, "v", dtype=torch.float16)
-    # a code is off by at most half a step, its largest value's by none (8 d is the value but for d's float16), and
-    # where that value is positive the opposite end, 7 of 8 steps, by a whole one
+    # A code is off by at most half a step d = top / 8, and at the end opposite the largest value, which 7 steps reach,
+    # by a whole one. The scale is then rounded to float16, by 2^-11 of it at most, and a code of up to 8 carries 8 times
+    # that: 8 * 2^-11 d = 2^-8 d beside the whole step.
     top = x.view(300, 16, 32).abs().amax(-1, keepdim=True)
-    assert ((k.view(300, 16, 32) - x.view(300, 16, 32)).abs() <= top / 8 * 1.001).all()
+    assert ((k.view(300, 16, 32) - x.view(300, 16, 32)).abs() <= top / 8 * (1 + 2.0 ** -8)).all()
     again = torch.zeros_like(kv.k[1])
     sqa.set_rows_q4_0(again, k, idx)
     assert torch.equal(again[idx], kv.k[1][idx])  # values on the grid quantize to themselves
