@@ -2,7 +2,7 @@
 // counterparts of set_rows_q4_0.hip.
 //
 // Both are one pass over the rows. get_rows is bound by the bytes it reads and writes: 131072
-// rows of 512 values as F16 45 us, 3.9 TB/s (F32 86 us, 3.6; a copy 4.8). move_rows of 100001 such
+// rows of 512 values as F16 28 us, 6.2 TB/s, F32 45 us, 6.8 (a copy 4.8). move_rows of 100001 such
 // rows 25 us: vector instructions (15 us without the rotated blocks, 14 of them with a table that
 // costs nothing) and, below 20000 rows, four memory latencies in a row. A workgroup
 // takes a run of rows; its threads go through the rows' units of a fixed size, whose row
@@ -21,44 +21,56 @@ constexpr int kThreads = 256;
 typedef uint32_t uint32a __attribute__((aligned(2)));
 typedef uint32_t uint32x2a __attribute__((ext_vector_type(2), aligned(2)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef uint32_t uint32x4 __attribute__((ext_vector_type(4)));
 
 // u / n for 0 <= u <= 2^20 by the reciprocal of n: u + 1/2 is half of 1 / n or more from a whole
 // quotient, and the float product off by 2^-22 of it (32-bit multiplications take four times as long).
 __device__ __forceinline__ int div_by(int u, float recip) { return (int)(((float)u + 0.5f) * recip); }
 __device__ __forceinline__ int mul(int a, int b) { return __mul24(a, b); }  // below 2^23 each
 
-// get_rows: a unit is 8 values, 8 bytes of codes (low or high nibbles) and their block's
-// scale; 16 bytes of F16 or two times 16 of F32 go out. Rows whose ends are not 16 bytes
+// get_rows: a unit is the 16 bytes that a lane stores, 8 values of F16 or 4 of F32: their codes
+// (low or high nibbles of 8 or 4 bytes) and their block's scale. Rows whose starts are not 16 bytes
 // apart, or at such addresses, go out value by value.
-template <bool kHalf, bool kVec>
+template <bool kHalf, bool kVec, bool kStream>
 __global__ __launch_bounds__(kThreads) void get_rows_q4_0_kernel(GetRows p) {
-    const int units = p.blocks * 4;
+    constexpr int kVals = kHalf ? 8 : 4, kPer = 32 / kVals;  // units of a block
+    const int units = p.blocks * kPer;
     const int64_t i0 = p.first + (int64_t)blockIdx.x * p.rows;
     for (int u = threadIdx.x; u < (int)min((int64_t)p.rows, p.n - i0) * units; u += kThreads) {
-        const int k = div_by(u, p.recip), c = u - mul(k, units), b = c >> 2, t = c & 3;
+        const int k = div_by(u, p.recip), c = u - mul(k, units), b = c / kPer, t = c % kPer;
         const int64_t i = i0 + k, r = *reinterpret_cast<const int64_t *>(p.idx + i * p.idx_nb0);
-        float v[8] = {};
+        float v[kVals] = {};
         if (r >= 0 && r < p.src_rows) {
             const uint8_t *from = p.src + r * p.src_nb1 + b * SQA_Q4_0_BLOCK_BYTES;
             const float d = (float)*reinterpret_cast<const _Float16 *>(from);
-            const uint32x2a q = *reinterpret_cast<const uint32x2a *>(from + 2 + 8 * (t & 1));
-            const int sh = t & 2 ? 4 : 0;
+            from += 2 + kVals * (t % (kPer / 2));
+            uint32_t q[kVals / 4];
+            if constexpr (kHalf) {
+                const uint32x2a x = *reinterpret_cast<const uint32x2a *>(from);
+                q[0] = x[0], q[1] = x[1];
+            } else {
+                q[0] = *reinterpret_cast<const uint32a *>(from);
+            }
+            const int sh = t < kPer / 2 ? 0 : 4;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = (float)((int)(q[j >> 2] >> (8 * (j & 3) + sh) & 15) - 8) * d;
+            for (int j = 0; j < kVals; ++j) v[j] = (float)((int)(q[j >> 2] >> (8 * (j & 3) + sh) & 15) - 8) * d;
         }
-        char *row = p.dst + i * p.dst_nb1 + (int64_t)c * (kHalf ? 16 : 32);
-        if constexpr (kHalf && kVec) {
-            half8 h;
+        char *row = p.dst + i * p.dst_nb1 + (int64_t)c * 16;
+        if constexpr (kVec) {
+            uint32x4 x;
+            if constexpr (kHalf) {
+                half8 h;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) h[j] = (_Float16)v[j];
-            *reinterpret_cast<half8 *>(row) = h;
-        } else if constexpr (kVec) {
-            *reinterpret_cast<floatx4 *>(row) = floatx4{v[0], v[1], v[2], v[3]};
-            *reinterpret_cast<floatx4 *>(row + 16) = floatx4{v[4], v[5], v[6], v[7]};
+                for (int j = 0; j < kVals; ++j) h[j] = (_Float16)v[j];
+                __builtin_memcpy(&x, &h, 16);
+            } else {
+                __builtin_memcpy(&x, v, 16);
+            }
+            if constexpr (kStream) __builtin_nontemporal_store(x, reinterpret_cast<uint32x4 *>(row));
+            else *reinterpret_cast<uint32x4 *>(row) = x;
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < kVals; ++j) {
                 if constexpr (kHalf) reinterpret_cast<_Float16 *>(row)[j] = (_Float16)v[j];
                 else reinterpret_cast<float *>(row)[j] = v[j];
             }
@@ -96,7 +108,6 @@ __device__ __forceinline__ float2 cos_sin(double x) {
 // of kTurns rotated units, or kCopies copied ones, in flight together. In place all loads of a row's
 // rotated blocks stand before its stores (a row's lanes may be in two wavefronts).
 typedef uint32_t Bytes12 __attribute__((ext_vector_type(3), aligned(4)));
-typedef uint32_t Bytes16 __attribute__((ext_vector_type(4)));
 constexpr int kTurns = 2, kCopies = 4;
 
 template <typename Copy, int kStep>
@@ -211,14 +222,24 @@ void launch_all(P &p, const char *name, hipStream_t s, F launch) {
 
 }  // namespace
 
+// Results of more than this go past the caches: 268 MB of F32 87 us with ordinary stores and 45 so,
+// 134 MB of F16 50 and 28; with a kernel that reads them right after (in us, both together) 182
+// and 172, 91 and 88; but 66 MB 45.5 and 47.3, 33 MB 23.3 and 25.5: those stay in the last cache.
+constexpr int64_t kStreamBytes = 96 << 20;
+
 int launch_get_rows_q4_0(GetRows p, bool half, hipStream_t s) {
     if (p.n == 0) return SQA_OK;
-    const int64_t units = 4 * (int64_t)p.blocks;
+    const int64_t units = (half ? 4 : 8) * (int64_t)p.blocks, bytes = p.n * 16 * units;
     p.rows = rows_of_workgroup(p.n, units, 4, 16);
     p.recip = recip(units);
     const bool vec = (uintptr_t)p.dst % 16 == 0 && (p.dst_nb1 % 16 == 0 || p.n == 1);
-    const auto kernel = half ? (vec ? get_rows_q4_0_kernel<true, true> : get_rows_q4_0_kernel<true, false>)
-                             : (vec ? get_rows_q4_0_kernel<false, true> : get_rows_q4_0_kernel<false, false>);
+    const bool stream = bytes > kStreamBytes;
+    const auto kernel = half ? (!vec     ? get_rows_q4_0_kernel<true, false, false>
+                                : stream ? get_rows_q4_0_kernel<true, true, true>
+                                         : get_rows_q4_0_kernel<true, true, false>)
+                             : (!vec     ? get_rows_q4_0_kernel<false, false, false>
+                                : stream ? get_rows_q4_0_kernel<false, true, true>
+                                         : get_rows_q4_0_kernel<false, true, false>);
     launch_all(p, "get_rows_q4_0", s, [&](dim3 grid) { kernel<<<grid, dim3(kThreads), 0, s>>>(p); });
     return hip_status(hipGetLastError(), "get_rows_q4_0 launch");
 }
@@ -238,7 +259,7 @@ int launch_move_rows_q4_0(MoveRows p, hipStream_t s) {
     p.recip_turned = recip(lanes * p.heads), p.recip_lanes = recip(lanes);
     p.recip_copy = recip(rest * p.heads), p.recip_rest = recip(rest);
     const size_t lds = (size_t)p.rows * (16 + (p.n_rot / 2) * sizeof(float2));
-    const auto kernel = step == 16   ? move_rows_q4_0_kernel<Bytes16, 16>
+    const auto kernel = step == 16   ? move_rows_q4_0_kernel<uint32x4, 16>
                         : step == 12 ? move_rows_q4_0_kernel<Bytes12, 12>
                                      : move_rows_q4_0_kernel<uint16_t, 2>;
     launch_all(p, "move_rows_q4_0", s, [&](dim3 grid) { kernel<<<grid, dim3(kThreads), lds, s>>>(p); });
