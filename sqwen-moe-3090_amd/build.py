@@ -43,6 +43,7 @@ def sources():
 EXTRA_FLAGS = {
     "fa_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
     "paged_chunk.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
+    "paged_chunk_shared.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
 }
 
 

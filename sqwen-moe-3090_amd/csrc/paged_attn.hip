@@ -167,30 +167,36 @@ int launch_combine(const Call &c, hipStream_t s) {
     return hip_status(hipGetLastError(), "paged_attn merge launch");
 }
 
-Plan plan_of(int64_t n_tok, int64_t H, int64_t Hkv, int64_t B, int64_t max_q) {
+Plan plan_of(int64_t n_tok, int64_t H, int64_t Hkv, int64_t B, int64_t max_q, int64_t groups) {
     Plan p{};
     const int64_t G = H / Hkv, rows = (max_q < n_tok ? max_q : n_tok) * G, cus = device_cu_count();
     const int64_t active = B < n_tok ? B : n_tok;
     p.most_d = rows <= 8 || (rows > 16 && G <= 8) ? 8 : 16;
+    if (groups && rows <= 8 && n_tok * G > 8 && n_tok * G <= 16) p.most_d = 16;  // a group may be all the tokens
     p.rows_d = p.most_d;
     const int64_t P = 2 * cus / Hkv;  // pieces that are wanted at most
-    p.slots_d = ((P < 1 ? 1 : P) + active) * Hkv;
-    p.least_d = (1 + active) * Hkv;
+    const int64_t parts = active + (groups < n_tok ? groups : n_tok);
+    p.slots_d = ((P < 1 ? 1 : P) + parts) * Hkv;
+    p.least_d = (1 + parts) * Hkv;
     p.where = al256((size_t)n_tok * 16);
     p.slot_d = (size_t)p.rows_d * (kHeadDim + 2) * 4;
-    if (rows > p.most_d) {
-        p.rows_c = rows <= 64 ? 64 : 128;
+    if (rows > p.most_d || (groups && n_tok * G > p.most_d)) {
+        p.rows_c = (groups ? n_tok * G : rows) <= 64 ? 64 : 128;
         // whole query tiles and a last one of every request; three rounds where that is less
-        const int64_t wgs = (n_tok / (p.rows_c / G) + active) * Hkv;
-        p.grid_c = (wgs + cus > 3 * cus ? wgs + cus : 3 * cus) + 7 & ~(int64_t)7;
-        p.slots_c = 3 * cus;
-        p.work = al256(work_bytes(B));
+        const int64_t tile = p.rows_c / G, wgs = (n_tok / tile + active) * Hkv;
+        // those of the groups, each of them a slot at least
+        p.least_c = groups ? (n_tok / tile + (groups < n_tok ? groups : n_tok)) * Hkv : 0;
+        p.grid_c = (wgs + p.least_c + cus > 3 * cus ? wgs + p.least_c + cus : 3 * cus) + 7 & ~(int64_t)7;
+        p.slots_c = p.least_c + cus > 3 * cus ? p.least_c + cus : 3 * cus;
+        p.work = al256(work_bytes(B + groups));
         p.slot_c = (size_t)p.rows_c * (kHeadDim + 2) * 4;
     }
     return p;
 }
 
-size_t least_bytes(const Plan &p) { return p.where + p.work + (size_t)p.least_d * p.slot_d + 512; }
+size_t least_bytes(const Plan &p) {
+    return p.where + p.work + (size_t)p.least_d * p.slot_d + (size_t)p.least_c * p.slot_c + 512;
+}
 size_t full_bytes(const Plan &p) {
     return p.where + p.work + (size_t)p.slots_d * p.slot_d + (size_t)p.slots_c * p.slot_c + 512;
 }
@@ -207,7 +213,9 @@ int lay_out(Call &c, const Plan &p, void *ws, size_t ws_bytes, const char *what)
         left -= (size_t)slots * bytes;
         return (int)slots;
     };
+    left -= (size_t)p.least_c * p.slot_c;  // what the chunk kernel cannot do without
     c.slots_d = take(p.slots_d, p.slot_d);
+    left += (size_t)p.least_c * p.slot_c;
     c.slots_c = take(p.slots_c, p.slot_c);
     c.room = c.slots_d / c.Hkv;
     c.few_pieces = c.cus / c.Hkv, c.all_pieces = 2 * c.cus / c.Hkv;

@@ -58,19 +58,26 @@ struct Call {
     int cus;
 };
 
-// The own part of a call whose groups share prefixes: every row goes through the merge, those of
-// one split normalised (dst is then a buffer of the workspace) with their (m, l) in stats.
-struct OwnCall : Call {
-    float *stats;  // [n_tok][H][2]
+// A call whose groups share prefixes: what the kernels deal out are its entries, the requests
+// over their own keys and behind them the groups over their prefixes. A group's tokens are
+// members, wherever their rows are; every one sees every key of the prefix. All rows go through
+// the merge: those of a request in one part normalised, in `whole` with their (m, l) in stats.
+struct Parts : Call {
+    int groups;
+    const int32_t *g_table;       // pages of the prefixes
+    int64_t g_stride, g_most_kv;  // as table_stride and most_kv
+    const int32_t *g_len;         // [groups] keys
+    const int32_t *m_start;       // [groups + 1]
+    const int32_t *members;       // [n_tok] token rows by group
+    const int32_t *m_pos;         // their positions
+    int4 *g_where;                // [n_tok] as where, of the groups' parts
+    float *whole, *stats;         // [n_tok][H][256], [n_tok][H][2]
 };
-// The shared part: `requests` are groups, q_start their members' first places, kv_len the
-// prefixes' lengths. Every token sees every key, and no part is whole.
-struct SharedCall : Call {
-    const int32_t *members;  // [n_tok] token rows by group
-    const int32_t *m_pos;    // their positions
-};
-template <class C> inline constexpr bool kIsShared = std::is_same<C, SharedCall>::value;
-template <class C> inline constexpr bool kIsOwn = std::is_same<C, OwnCall>::value;
+template <class C> inline constexpr bool kIsParts = std::is_same<C, Parts>::value;
+__device__ __forceinline__ int entries(const Call &c) { return c.B; }
+__device__ __forceinline__ int entries(const Parts &c) { return c.B + c.groups; }
+__device__ __forceinline__ bool is_group(const Call &, int) { return false; }
+__device__ __forceinline__ bool is_group(const Parts &c, int b) { return b >= c.B; }
 
 // A request's tokens and keys. Anything the arrays may hold leaves rows inside
 // [0, n_tok) and keys inside [0, most_kv).
@@ -92,15 +99,24 @@ __device__ __forceinline__ Request request(const Call &c, int b) {
     return r;
 }
 
-__device__ __forceinline__ Request request(const SharedCall &c, int b) {
+// Of entry b; a group's tokens are counted by their places among the members.
+__device__ __forceinline__ Request request(const Parts &c, int b) {
+    if (!is_group(c, b)) return request(static_cast<const Call &>(c), b);
     Request r;
-    const int s0 = c.q_start[b], s1 = c.q_start[b + 1], len = c.kv_len[b];
-    r.prefix = INT32_MAX;
+    const int g = b - c.B, s0 = c.m_start[g], s1 = c.m_start[g + 1], len = c.g_len[g];
+    r.prefix = INT32_MAX, r.pos0 = 0;
+    r.kv = (int)min((int64_t)max(len, 0), c.g_most_kv);
     r.q0 = min(max(s0, 0), c.n_tok);
-    r.kv = (int)min((int64_t)max(len, 0), c.most_kv);
     r.n = r.kv ? min(max(s1, r.q0), c.n_tok) - r.q0 : 0;
-    r.pos0 = 0;
     return r;
+}
+
+// Row of token i of an entry; a member that no plan wrote may be any number (< 0: none then).
+__device__ __forceinline__ int row_of_token(const Call &, const Request &r, bool, int i) { return r.q0 + i; }
+__device__ __forceinline__ int row_of_token(const Parts &c, const Request &r, bool group, int i) {
+    if (!group) return r.q0 + i;
+    const int t = c.members[r.q0 + i];
+    return (uint32_t)t < (uint32_t)c.n_tok ? t : -1;
 }
 
 // Keys [0, sees) that token i sees.
@@ -159,6 +175,11 @@ typedef const __attribute__((address_space(4))) int32_t *TableRow;
 __device__ __forceinline__ TableRow table_row(const Call &c, int b) {
     const uint64_t at = (uint64_t)(uintptr_t)(c.table + (int64_t)b * c.table_stride);
     return reinterpret_cast<TableRow>(((uint64_t)(uint32_t)uniform((int)(at >> 32)) << 32) | (uint32_t)uniform((int)(uint32_t)at));
+}
+__device__ __forceinline__ TableRow table_row(const Parts &c, int b) {
+    Call of = c;
+    if (is_group(c, b)) of.table = c.g_table, of.table_stride = c.g_stride, b -= c.B;
+    return table_row(of, b);
 }
 __device__ __forceinline__ int page_id(TableRow row, int i) { return row[i]; }
 
@@ -220,10 +241,11 @@ __device__ __forceinline__ float gate_by(float x, float g) {
 // few-row kernel, then those of the many-row kernel.
 struct Plan {
     int most_d, rows_d, rows_c;  // of Call
-    int64_t slots_d, least_d, slots_c, grid_c;
+    int64_t slots_d, least_d, slots_c, least_c, grid_c;
     size_t where, work, slot_d, slot_c;
 };
-Plan plan_of(int64_t n_tok, int64_t H, int64_t Hkv, int64_t B, int64_t max_q);
+// (groups: of a call that shares prefixes, whose groups of few rows are the few-row kernel's too)
+Plan plan_of(int64_t n_tok, int64_t H, int64_t Hkv, int64_t B, int64_t max_q, int64_t groups = 0);
 size_t least_bytes(const Plan &p);
 size_t full_bytes(const Plan &p);
 // What a call's arguments say of it, and its workspace's parts.
@@ -232,16 +254,11 @@ int lay_out(Call &c, const Plan &p, void *ws, size_t ws_bytes, const char *what)
 
 inline size_t al256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-struct SharedCalls {
-    OwnCall own;
-    SharedCall shared;
-};
-int launch_few(const Call &c, hipStream_t s);      // paged_decode.hip
-int launch_few(const SharedCalls &c, hipStream_t s);  // the own part, and the plan of both
-int launch_many(const Call &c, hipStream_t s);     // paged_chunk.hip
-int launch_many(const OwnCall &c, hipStream_t s);
-int launch_many(const SharedCall &c, hipStream_t s);
-int launch_combine(const Call &c, hipStream_t s);  // paged_attn.hip
+int launch_few(const Call &c, hipStream_t s);          // paged_decode.hip
+int launch_few(const Parts &c, hipStream_t s);  // the own part, and the plan of both
+int launch_many(const Call &c, hipStream_t s);         // paged_chunk.hip
+int launch_many(const Parts &c, hipStream_t s);  // paged_chunk_shared.hip
+int launch_combine(const Call &c, hipStream_t s);      // paged_attn.hip
 
 }  // namespace paged
 }  // namespace sqa

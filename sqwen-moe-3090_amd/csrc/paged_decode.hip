@@ -76,7 +76,7 @@ constexpr float kPShift = -(float)kPBits;
 // Largest d_v exponent E of the value wavefronts (d_v enters A as d_v 2^E): V
 // scales below 2^-20 lose low bits of A; 2^E stays two fp16 powers of two.
 constexpr int kMaxDvExp = 18;
-static_assert(kMaxRequests * 4 <= kLdsBytes, "tiles of every request");
+static_assert(2 * kMaxRequests * 4 <= kLdsBytes, "tiles of every request and group");
 static_assert(2 * kLdsBytes <= 160 * 1024, "two workgroups per CU");
 static_assert((512 + 6 * 2600 + 8) * 4 <= kLdsBytes && (512 + kMaxRequests + 8) * 4 <= kLdsBytes, "the plan's LDS");
 static_assert(4 * 2 * 64 * 32 <= (kVStages - 1) * kTensorBytes, "Q operands must fit in V stages 1..2");
@@ -153,9 +153,9 @@ struct Piece {
 
 constexpr int kLengths = 8;
 
-// Tiles of request b, r; 0: none of this kernel's.
-__device__ __forceinline__ int tiles_of(const Call &c, int b, const Request &r, int most) {
-    return b >= c.B || r.n == 0 || r.n * c.G > most ? 0 : max((r.kv + kTileKeys - 1) / kTileKeys, 1);
+// Tiles of entry b of B, r; 0: none of this kernel's.
+__device__ __forceinline__ int tiles_of(const Call &c, int b, int B, const Request &r, int most) {
+    return b >= B || r.n == 0 || r.n * c.G > most ? 0 : max((r.kv + kTileKeys - 1) / kTileKeys, 1);
 }
 
 // Piece length: from total / P up to nearly twice that, the shortest whose pieces number
@@ -167,20 +167,21 @@ __device__ __forceinline__ int tiles_of(const Call &c, int b, const Request &r, 
 // a wavefront's lanes, more in LDS (read again from memory for each of the sums, 1000
 // requests of up to 500 keys took 181 us instead of 140; 16 a lane, the code for it cost
 // every call 1.3 us).
-__device__ __forceinline__ Piece few_piece(const Call &c, int *lds, int piece, int most) {
-    const int lane = threadIdx.x & 63;
-    const bool small = c.B <= 64;
-    const Request mine = request(c, min(lane, c.B - 1));
-    const int own = tiles_of(c, lane, mine, most);
+template <class C>
+__device__ __forceinline__ Piece few_piece(const C &c, int *lds, int piece, int most) {
+    const int lane = threadIdx.x & 63, B = entries(c);
+    const bool small = B <= 64;
+    const Request mine = request(c, min(lane, B - 1));
+    const int own = tiles_of(c, lane, B, mine, most);
     if (!small) {
-        for (int b = threadIdx.x; b < c.B; b += kThreads) lds[b] = tiles_of(c, b, request(c, b), most);
+        for (int b = threadIdx.x; b < B; b += kThreads) lds[b] = tiles_of(c, b, B, request(c, b), most);
         __syncthreads();
     }
-    auto tiles = [&](int b0) { return small ? own : b0 + lane < c.B ? lds[b0 + lane] : 0; };
+    auto tiles = [&](int b0) { return small ? own : b0 + lane < B ? lds[b0 + lane] : 0; };
     int total = 0, longest = 0, active = 0;
-    for (int b0 = 0; b0 < c.B; b0 += 64) {
+    for (int b0 = 0; b0 < B; b0 += 64) {
         const int t = tiles(b0);
-        total += min(t, 1 << 18);  // 2^12 requests: below 2^31
+        total += min(t, 1 << 17);  // 2^13 entries: below 2^31
         longest = max(longest, t);
         active += t > 0;
     }
@@ -194,19 +195,19 @@ __device__ __forceinline__ Piece few_piece(const Call &c, int *lds, int piece, i
     // (no request has more than 2^25 tiles; lengths of up to 15 times this have to fit an int)
     const int base = min(max(max(share, (longest + kMostSplits - 1) / kMostSplits), 1), 1 << 25);
     int len = 0;
-    if (c.B <= 256) {
+    if (B <= 256) {
         int lo = base, hi = 2 * base;  // the first length that will do, if it is below hi
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
             int k = 0;
-            for (int b0 = 0; b0 < c.B; b0 += 64) k += div_ceil(tiles(b0), mid);
+            for (int b0 = 0; b0 < B; b0 += 64) k += div_ceil(tiles(b0), mid);
             if (wave_sum(k) <= P) hi = mid;
             else lo = mid + 1;
         }
         len = lo < 2 * base ? lo : 0;
     }
     int n[kLengths] = {};
-    for (int b0 = 0; b0 < c.B && len == 0; b0 += 64) {
+    for (int b0 = 0; b0 < B && len == 0; b0 += 64) {
         const int t = tiles(b0);
 #pragma unroll
         for (int j = 0; j < kLengths; ++j) {
@@ -220,7 +221,7 @@ __device__ __forceinline__ Piece few_piece(const Call &c, int *lds, int piece, i
     if (len == 0) len = wave_sum(n[0]) <= c.room ? base : 1 << 25;  // 2^25 tiles: every request whole
     Piece pc{-1, 0, 1, 0, 0, 0, {}};
     int first = 0;
-    for (int b0 = 0; b0 < c.B && first <= piece; b0 += 64) {
+    for (int b0 = 0; b0 < B && first <= piece; b0 += 64) {
         const int t = tiles(b0);
         const int k = div_ceil(t, len);
         const int upto = first + wave_scan(k);
@@ -287,14 +288,10 @@ __device__ __forceinline__ int lds_byte(int row, int c) {
 // TWO = true : up to 16 rows (rows 0-7 and 8-15 as two B sets, one A operand).
 // OPT: the logits are capped or biased. PLAN: a last workgroup plans the many-row kernel.
 // (128 registers a lane; TWO with OPT and PLAN keeps one more in scratch, the others none.)
-// A: Call, or SharedCalls, whose shared part is planned beside the own one.
-__device__ __forceinline__ const Call &own_of(const Call &a) { return a; }
-__device__ __forceinline__ const Call &own_of(const SharedCalls &a) { return a.own; }
+// C: Call, or Parts, whose groups of few rows are pieces too.
 
-template <bool TWO, bool OPT, bool PLAN, class A>
-__global__ __launch_bounds__(kThreads, 4) void paged_few_kernel(A a) {
-    constexpr bool kShared = !std::is_same<A, Call>::value;
-    const Call &p = own_of(a);
+template <bool TWO, bool OPT, bool PLAN, class C>
+__global__ __launch_bounds__(kThreads, 4) void paged_few_kernel(C p) {
     extern __shared__ __align__(16) uint8_t smem[];
     const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // wave-uniform, in an SGPR
@@ -310,12 +307,7 @@ __global__ __launch_bounds__(kThreads, 4) void paged_few_kernel(A a) {
     constexpr int kRowMask = TWO ? 15 : 7;  // rows 8-15 mirror rows 0-7 when only 8 exist
 
     if (PLAN && blockIdx.z == gridDim.z - 1) {
-        if constexpr (kShared) {
-            if (blockIdx.x == 0 && blockIdx.y == 0) plan_chunks(a.shared, reinterpret_cast<int *>(smem));
-            if (blockIdx.x == 1 && blockIdx.y == 0 && p.rows_c) plan_chunks(p, reinterpret_cast<int *>(smem));
-        } else {
-            if (blockIdx.x == 0 && blockIdx.y == 0) plan_chunks(p, reinterpret_cast<int *>(smem));
-        }
+        if (blockIdx.x == 0 && blockIdx.y == 0) plan_chunks(p, reinterpret_cast<int *>(smem));
         return;
     }
     // ---------------- piece and KV head of this workgroup ---------------------
@@ -324,15 +316,19 @@ __global__ __launch_bounds__(kThreads, 4) void paged_few_kernel(A a) {
     const int kvh = (int)blockIdx.y;
     const int piece = (int)(8 * blockIdx.z + blockIdx.x);
     const Piece pc = few_piece(p, reinterpret_cast<int *>(smem), piece, p.most_d);
-    if ((kShared ? p.rows_c == 0 : !PLAN) && blockIdx.x + blockIdx.y + blockIdx.z == 0) skip_large(p);
+    if (!PLAN && blockIdx.x + blockIdx.y + blockIdx.z == 0) skip_large(p);
     // The workspace has slots for `room` pieces. Requests whose ranges of q_start overlap may be
     // more than there are tokens, which room counts on, and the grid is a multiple of 8 of them.
     if (pc.b < 0 || piece >= p.room) return;
     const Request rq = pc.rq;
     const int rows = rq.n * p.G;
     const int slot = (pc.first + pc.split) * p.Hkv + kvh;
-    if (pc.split == 0 && kvh == 0 && tid < rq.n)
-        p.where[rq.q0 + tid] = make_int4(pc.first * p.Hkv, pc.n, tid * p.G, p.Hkv * 4 + kFew);
+    const bool shared = is_group(p, pc.b);
+    int4 *where = p.where;
+    if constexpr (kIsParts<C>) where = shared ? p.g_where : where;
+    int own_row = 0;
+    if (pc.split == 0 && kvh == 0 && tid < rq.n && (own_row = row_of_token(p, rq, shared, tid)) >= 0)
+        where[own_row] = make_int4(pc.first * p.Hkv, pc.n, tid * p.G, p.Hkv * 4 + kFew);
     const int k0 = pc.t0 * kTileKeys;
     const int k1 = min(pc.t1 * kTileKeys, rq.kv);
     const int n_tiles = uniform(k1 > k0 ? (k1 - k0 + kTileKeys - 1) / kTileKeys : 0);
@@ -387,11 +383,13 @@ __global__ __launch_bounds__(kThreads, 4) void paged_few_kernel(A a) {
 #pragma unroll
             for (int set = 0; set < kSets; ++set) {
                 const int r = 8 * set + (n & 7);
-                const bool row_ok = r < rows;
+                bool row_ok = r < rows;
                 const int t = group_of(p, r);
                 const int hq = kvh * p.G + (r - t * p.G);
+                const int at = row_ok ? row_of_token(p, rq, shared, t) : 0;
+                if constexpr (kIsParts<C>) row_ok = row_ok && at >= 0;
                 const float *qrow = reinterpret_cast<const float *>(
-                    p.q + (row_ok ? (int64_t)(rq.q0 + t) * p.q_nb1 + (int64_t)hq * p.q_nb2 : 0));
+                    p.q + (row_ok ? (int64_t)at * p.q_nb1 + (int64_t)hq * p.q_nb2 : 0));
                 const int blk = 2 * pr + (n >> 3);
                 float x[16];
 #pragma unroll
@@ -460,7 +458,9 @@ __global__ __launch_bounds__(kThreads, 4) void paged_few_kernel(A a) {
         const bool my_ok = my_r < rows;
         const int my_t = my_ok ? group_of(p, my_r) : 0;
         const int my_see = sees(rq, my_t);  // keys that the row sees
-        const int my_pos = rq.pos0 + my_t;
+        int my_pos = rq.pos0 + my_t;
+        if constexpr (kIsParts<C> && OPT)
+            if (shared) my_pos = my_ok ? p.m_pos[rq.q0 + my_t] : 0;
         float my_slope = 0.0f;
         if (OPT && p.bias != 0.0f) my_slope = slope2(p, kvh * p.G + my_r - my_t * p.G);
         const bool row_writer = TWO || n < 8;  // lanes n >= 8 mirror rows 0-7 when only 8 exist
@@ -1070,12 +1070,14 @@ int launch_few(const Call &c, hipStream_t s) {
     return hip_status(hipGetLastError(), "paged_attn launch");
 }
 
-int launch_few(const SharedCalls &c, hipStream_t s) {
-    const bool two = c.own.rows_d > 8, opt = c.own.cap2 != 0.0f || c.own.bias != 0.0f;
-    typedef void (*Kernel)(SharedCalls);
-    static const Kernel kernels[4] = {
-        paged_few_kernel<false, false, true, SharedCalls>, paged_few_kernel<true, false, true, SharedCalls>,
-        paged_few_kernel<false, true, true, SharedCalls>, paged_few_kernel<true, true, true, SharedCalls>};
+int launch_few(const Parts &c, hipStream_t s) {
+    const bool two = c.rows_d > 8, opt = c.cap2 != 0.0f || c.bias != 0.0f;
+    typedef void (*Kernel)(Parts);
+    static const Kernel kernels[8] = {
+        paged_few_kernel<false, false, false, Parts>, paged_few_kernel<true, false, false, Parts>,
+        paged_few_kernel<false, true, false, Parts>,  paged_few_kernel<true, true, false, Parts>,
+        paged_few_kernel<false, false, true, Parts>,  paged_few_kernel<true, false, true, Parts>,
+        paged_few_kernel<false, true, true, Parts>,   paged_few_kernel<true, true, true, Parts>};
     static std::once_flag once;
     static hipError_t err = hipSuccess;
     std::call_once(once, [] {
@@ -1083,7 +1085,8 @@ int launch_few(const SharedCalls &c, hipStream_t s) {
     });
     if (err != hipSuccess) return hip_status(err, "paged_attn_shared LDS attribute");
     const int prof = profile_start("paged_decode", s);
-    kernels[two + 2 * opt]<<<few_grid(c.own, true), dim3(kThreads), kLdsBytes, s>>>(c);
+    const bool plan = c.rows_c != 0;
+    kernels[two + 2 * opt + 4 * plan]<<<few_grid(c, plan), dim3(kThreads), kLdsBytes, s>>>(c);
     profile_stop(prof, s);
     return hip_status(hipGetLastError(), "paged_attn_shared launch");
 }

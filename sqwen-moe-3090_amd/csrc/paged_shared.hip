@@ -5,7 +5,8 @@
 // group's prefix meet the rows of all its tokens at once: the many-row kernel of paged_chunk.hip
 // takes tiles of 128 (or 64) rows out of the group's list of members, so that a key is read and
 // expanded once for that many rows instead of once for every request's 8. An extra workgroup of
-// the few-row launch plans the tiles and splits. Every row's parts (splits of its own keys and of
+// the few-row launch plans the tiles and splits. Groups of few rows (a token or two) are pieces of
+// the few-row kernel, beside the requests. Every row's parts (splits of its own keys and of
 // the prefix) then meet in the merge, M the largest of all their maxima:
 //   out = sum_s acc_s 2^(m_s - M) / sum_s l_s 2^(m_s - M), then the gate.
 #include "paged_merge.hpp"
@@ -20,10 +21,8 @@ constexpr int kThreads = 256;
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 
 struct Merge {
-    OwnCall own;
-    SharedCall shared;
+    Parts parts;
     const int32_t *token_group;
-    float *dst;
 };
 
 // A wavefront takes R heads of a token together, 4 dims a lane; 64 / R parts at a time: lane
@@ -31,7 +30,7 @@ struct Merge {
 template <int R>
 __global__ __launch_bounds__(kThreads) void merge_shared_kernel(Merge p) {
     constexpr int kS = 64 / R, kBatch = R >= 4 ? 2 : 8;
-    const OwnCall &c = p.own;
+    const Parts &c = p.parts;
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int t = (int)blockIdx.y + (int)(blockIdx.z << 15), h0 = ((int)blockIdx.x * 4 + wave) * R;
     if (t >= c.n_tok || h0 >= c.H) return;
@@ -39,8 +38,8 @@ __global__ __launch_bounds__(kThreads) void merge_shared_kernel(Merge p) {
     if (t < c.q_start[0] || t >= c.q_start[c.B]) return;
     const int4 w1 = c.where[t];
     const int g = p.token_group[t];
-    const bool member = g >= 0 && g < p.shared.B && p.shared.kv_len[g] > 0;
-    const int4 w2 = member ? p.shared.where[t] : make_int4(0, 0, 0, kDone);
+    const bool member = g >= 0 && g < c.groups && c.g_len[g] > 0;
+    const int4 w2 = member ? c.g_where[t] : make_int4(0, 0, 0, kDone);
     const bool whole = (w1.w & 3) == kWhole;
     Row a[R], b[R];
 #pragma unroll
@@ -49,9 +48,9 @@ __global__ __launch_bounds__(kThreads) void merge_shared_kernel(Merge p) {
         a[k] = partials(c, w1, h);
         if (whole) {
             const int64_t at = (int64_t)t * c.H + h;
-            a[k] = Row{c.dst + at * 256, c.stats + at * 2, 0, 1};
+            a[k] = Row{c.whole + at * 256, c.stats + at * 2, 0, 1};
         }
-        b[k] = partials(p.shared, w2, h);
+        b[k] = partials(c, w2, h);
     }
     if (a[0].n == 0) return;  // of the token: all heads alike
     const int n1 = a[0].n, n = n1 + b[0].n, k_own = lane / kS, i_own = lane % kS;
@@ -112,38 +111,26 @@ __global__ __launch_bounds__(kThreads) void merge_shared_kernel(Merge p) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] = gate_by(x[i], g4[k][i]);
         }
-        *reinterpret_cast<floatx4 *>(p.dst + ((int64_t)t * c.H + h0 + k) * kHeadDim + 4 * lane) = x;
+        *reinterpret_cast<floatx4 *>(c.dst + ((int64_t)t * c.H + h0 + k) * kHeadDim + 4 * lane) = x;
     }
 }
 
-// The workspace of a call: stats and results of rows of one part (where there is a chunk kernel),
-// the shared part's entries, plan and slots, then the own part's.
+// Workspace of a call: the groups' entries, stats and results of requests in one part (where there
+// is a chunk kernel), then what a call without groups has.
 struct Space {
-    Plan own, shared;
-    size_t stats, whole;
-    size_t fixed() const { return stats + whole; }
-    size_t least_shared() const { return shared.where + shared.work + (size_t)least_slots * shared.slot_c + 512; }
-    size_t full_shared() const { return shared.where + shared.work + (size_t)shared.slots_c * shared.slot_c + 512; }
-    int64_t least_slots;
+    Plan plan;
+    size_t where, stats, whole;
+    size_t more() const { return where + stats + whole + 256; }
 };
 
 Space space(int64_t n_tok, int64_t H, int64_t Hkv, int64_t B, int64_t groups, int64_t max_q) {
     Space s{};
-    s.own = plan_of(n_tok, H, Hkv, B, max_q);
-    if (s.own.rows_c) {
+    s.plan = plan_of(n_tok, H, Hkv, B, max_q, groups);
+    s.where = al256((size_t)n_tok * 16);
+    if (s.plan.rows_c) {  // (also where max_q says that no request is the chunk kernel's)
         s.stats = al256((size_t)(n_tok * H) * 8);
         s.whole = al256((size_t)(n_tok * H) * kHeadDim * 4);
     }
-    const int64_t G = H / Hkv, cus = device_cu_count(), active = groups < n_tok ? groups : n_tok;
-    Plan &p = s.shared;
-    p.rows_c = n_tok * G <= 64 ? 64 : 128;
-    p.where = al256((size_t)n_tok * 16);
-    p.work = al256(work_bytes(groups));
-    p.slot_c = (size_t)p.rows_c * (kHeadDim + 2) * 4;
-    // every tile of members is a slot, at least: whole tiles and a last one of every group
-    s.least_slots = (n_tok / (p.rows_c / G) + active) * Hkv;
-    p.slots_c = s.least_slots + cus > 3 * cus ? s.least_slots + cus : 3 * cus;
-    p.grid_c = (p.slots_c + 7) & ~(int64_t)7;
     return s;
 }
 
@@ -155,53 +142,34 @@ using namespace paged;
 size_t paged_shared_workspace(int64_t n_tok, int64_t H, int64_t Hkv, int64_t B, int64_t groups, int64_t max_q) {
     if (n_tok < 1) return 0;
     const Space s = space(n_tok, H, Hkv, B, groups, max_q);
-    return s.fixed() + full_bytes(s.own) + s.full_shared() + 512;
+    return s.more() + full_bytes(s.plan);
 }
 
 int launch_paged_shared(const SharedArgs &a, hipStream_t s) {
     const char *what = "paged_attn_shared";
     Merge m{};
-    static_cast<Call &>(m.own) = call_of(a.own);
-    m.dst = m.own.dst;
-    SharedCall &c = m.shared;
-    static_cast<Call &>(c) = m.own;
-    c.table = (const int32_t *)a.table->data, c.table_stride = (int64_t)a.table->nb[1] / 4;
-    c.most_kv = a.table->ne[0] << c.lp;
-    c.B = (int)a.table->ne[1];
-    c.q_start = (const int32_t *)a.m_start->data, c.kv_len = (const int32_t *)a.len->data;
-    c.prefix = nullptr;
+    Parts &c = m.parts;
+    static_cast<Call &>(c) = call_of(a.own);
+    c.groups = (int)a.table->ne[1];
+    c.g_table = (const int32_t *)a.table->data, c.g_stride = (int64_t)a.table->nb[1] / 4;
+    c.g_most_kv = a.table->ne[0] << c.lp;
+    c.g_len = (const int32_t *)a.len->data, c.m_start = (const int32_t *)a.m_start->data;
     c.members = (const int32_t *)a.members->data, c.m_pos = (const int32_t *)a.m_pos->data;
     m.token_group = (const int32_t *)a.token_group->data;
 
-    const Space sp = space(c.n_tok, c.H, c.Hkv, m.own.B, c.B, a.own.max_q);
-    const size_t least_own = least_bytes(sp.own), least = sp.fixed() + least_own + sp.least_shared() + 512;
+    const Space sp = space(c.n_tok, c.H, c.Hkv, c.B, c.groups, a.own.max_q);
+    const size_t least = sp.more() + least_bytes(sp.plan);
     if (!a.own.ws || a.own.ws_bytes < least)
         return set_error(SQA_ERR_WORKSPACE, "%s: workspace %zu bytes < %zu needed", what, a.own.ws ? a.own.ws_bytes : (size_t)0, least);
-    if (sp.shared.grid_c > INT32_MAX) return set_error(SQA_ERR_UNSUPPORTED, "%s: too many query tiles", what);
     uint8_t *base = reinterpret_cast<uint8_t *>(((uintptr_t)a.own.ws + 255) & ~(uintptr_t)255);
-    m.own.stats = reinterpret_cast<float *>(base);
-    m.own.dst = reinterpret_cast<float *>(base + sp.stats);
-    base += sp.fixed();
-    // what is left beyond the least: to the shared part as much as it takes, the rest to the own one
-    // (half of it at least)
-    const size_t more = a.own.ws_bytes - least, take = sp.full_shared() - sp.least_shared();
-    const size_t own_take = full_bytes(sp.own) - least_own, half = more / 2 < own_take ? more / 2 : own_take;
-    const size_t shared_bytes = sp.least_shared() + (take < more - half ? take : more - half);
-    c.rows_c = sp.shared.rows_c, c.grid_c = (int)sp.shared.grid_c;
-    c.where = reinterpret_cast<int4 *>(base);
-    c.work = reinterpret_cast<int *>(base + sp.shared.where);
-    c.slots_c = (int)((shared_bytes - 512 - sp.shared.where - sp.shared.work) / sp.shared.slot_c);
-    if (c.slots_c > sp.shared.slots_c) c.slots_c = (int)sp.shared.slots_c;
-    c.acc_c = reinterpret_cast<float *>(base + sp.shared.where + sp.shared.work);
-    c.ml_c = c.acc_c + (size_t)c.slots_c * c.rows_c * kHeadDim;
-    c.most_d = c.slots_d = c.rows_d = 0;
-    uint8_t *rest = reinterpret_cast<uint8_t *>(((uintptr_t)(c.ml_c + (size_t)c.slots_c * c.rows_c * 2) + 255) & ~(uintptr_t)255);
-    int rc = lay_out(m.own, sp.own, rest, (size_t)((uint8_t *)a.own.ws + a.own.ws_bytes - rest), what);
+    c.g_where = reinterpret_cast<int4 *>(base);
+    c.stats = reinterpret_cast<float *>(base + sp.where);
+    c.whole = reinterpret_cast<float *>(base + sp.where + sp.stats);
+    int rc = lay_out(c, sp.plan, base + sp.more() - 256, a.own.ws_bytes - sp.more(), what);
     if (rc) return rc;
 
-    rc = launch_few(SharedCalls{m.own, c}, s);
-    if (!rc && m.own.rows_c) rc = launch_many(m.own, s);
-    if (!rc) rc = launch_many(c, s);
+    rc = launch_few(c, s);
+    if (!rc && c.rows_c) rc = launch_many(c, s);
     if (rc) return rc;
 
     const int prof = profile_start("paged_shared_merge", s);

@@ -31,7 +31,7 @@ struct Item {
 };
 static_assert(sizeof(Item) == 64, "one scalar load");
 
-// Words: Work | list [kListed] of Item | first item of every request [B + 1] | first slot [B]
+// Words: Work | list [kListed] of Item | first item of every entry [E + 1] | first slot [E]
 constexpr int kListAt = 16, kFirstAt = kListAt + 16 * kListed;
 __host__ __device__ inline size_t work_bytes(int64_t B) { return (size_t)(kFirstAt + 2 * B + 4) * 4; }
 
@@ -83,30 +83,31 @@ constexpr int kCounted = 64, kLevels = 8, kRounds = 4;
 // Lanes are requests (a run of them above 512), then lengths that are tried, then items.
 template <class C>
 __device__ __forceinline__ void plan_chunks(const C &c, int *lds) {
-    constexpr bool kAll = kIsShared<C>;
+    const int E = entries(c);
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, qb = c.rows_c / c.G;
     Work *out = reinterpret_cast<Work *>(c.work);
-    int *first = c.work + kFirstAt, *slot = first + c.B + 1;
+    int *first = c.work + kFirstAt, *slot = first + E + 1;
     Item *list = reinterpret_cast<Item *>(c.work + kListAt);
     int *sums = lds, *start = lds + 512;                      // start: first item of every request
-    Request *known = reinterpret_cast<Request *>(start + c.B + 1);
-    const int per = (c.B + 511) / 512, b0 = min(tid * per, c.B), b1 = min(b0 + per, c.B);
-    const bool kept = c.B <= 2600;  // in LDS; larger batches read them again
+    Request *known = reinterpret_cast<Request *>(start + E + 1);
+    const int per = (E + 511) / 512, b0 = min(tid * per, E), b1 = min(b0 + per, E);
+    const bool kept = E <= 2600;  // in LDS; larger batches read them again
     auto load = [&](int b) {
         return kept ? known[b] : request(c, b);
     };
 
-    int wgs = 0, longest = 0, tokens = 0;
+    int wgs = 0, longest = 0, tokens = 0, members = 0;
     float work = 0.0f;  // key tiles that all query tiles see together
     for (int b = b0; b < b1; ++b) {
         const Request r = request(c, b);
         if (kept) known[b] = r;
-        tokens = min(tokens + r.n, c.n_tok + 1);
+        int &count = is_group(c, b) ? members : tokens;
+        count = min(count + r.n, c.n_tok + 1);
         int kt;
         const int T = chunk_tiles(c, r, qb, &kt);
         // query tile i of T ends (T - 1 - i) * qb keys before the last one
         const float all = (float)T * (float)kt;
-        work += kAll ? all : fmaxf(all - 0.5f * (float)T * (float)(T - 1) * (float)qb / kChunkKeys, 0.5f * all);
+        work += is_group(c, b) ? all : fmaxf(all - 0.5f * (float)T * (float)(T - 1) * (float)qb / kChunkKeys, 0.5f * all);
         wgs += T;
         longest = max(longest, kt);
     }
@@ -115,14 +116,20 @@ __device__ __forceinline__ void plan_chunks(const C &c, int *lds) {
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) work += __shfl_xor(work, o);
     tokens = min(wave_sum(tokens), c.n_tok + 1);  // (64 (2^24 + 1) at most)
-    if (lane == 0) sums[wave] = wgs, sums[8 + wave] = longest, sums[16 + wave] = __float_as_int(work), sums[24 + wave] = tokens;
+    members = kIsParts<C> ? min(wave_sum(members), c.n_tok + 1) : 0;
+    if (lane == 0) {
+        sums[wave] = wgs, sums[8 + wave] = longest, sums[16 + wave] = __float_as_int(work), sums[24 + wave] = tokens;
+        sums[32 + wave] = members;
+    }
     __syncthreads();
-    wgs = longest = tokens = 0, work = 0.0f;
-    for (int w = 0; w < 8; ++w)
+    wgs = longest = tokens = members = 0, work = 0.0f;
+    for (int w = 0; w < 8; ++w) {
         wgs += sums[w], longest = max(longest, sums[8 + w]), work += __int_as_float(sums[16 + w]), tokens += sums[24 + w];
+        members += sums[32 + w];
+    }
     // More tokens than there are: ranges of q_start overlap. The sums of tiles below, and the
     // workgroups and slots that the host provided, are for disjoint ones.
-    if (wgs == 0 || tokens > c.n_tok) {
+    if (wgs == 0 || tokens > c.n_tok || members > c.n_tok) {
         if (tid == 0) *out = Work{1, 0, 0, 0};
         return;
     }
@@ -132,11 +139,11 @@ __device__ __forceinline__ void plan_chunks(const C &c, int *lds) {
     // split ones; 32 requests at a time
     const int j = lane & (kChoices - 1), l_j = max(div_ceil(longest, kTried[j]), 2);
     int n_j = 0, split_j = 0;
-    for (int b = 4 * wave + (lane >> 4); b < c.B; b += 32) {
+    for (int b = 4 * wave + (lane >> 4); b < E; b += 32) {
         int kt;
         const int T = chunk_tiles(c, load(b), qb, &kt), n = T * div_ceil(kt, l_j);
         n_j += n;
-        split_j += kAll || kt > l_j ? n : 0;
+        split_j += is_group(c, b) || kt > l_j ? n : 0;
     }
     n_j += __shfl_xor(n_j, 16), split_j += __shfl_xor(split_j, 16);
     n_j += __shfl_xor(n_j, 32), split_j += __shfl_xor(split_j, 32);
@@ -147,11 +154,11 @@ __device__ __forceinline__ void plan_chunks(const C &c, int *lds) {
     const int64_t N = (int64_t)n_j * c.Hkv, slots_j = (int64_t)split_j * c.Hkv;
     const int part_j = min(l_j, longest);
     const float part = (float)part_j, cus = (float)c.cus;
-    const bool counted = c.B <= kCounted;
+    const bool counted = E <= kCounted;
     if (counted) {  // wavefront w: query tiles times splits of at least (w + 1) / 8 of a part
         const int x = div_ceil(part_j * (wave + 1), kLevels);
         int n_x = 0;
-        for (int b = lane >> 4; b < c.B && N > c.cus && N <= kRounds * c.cus; b += 4) {
+        for (int b = lane >> 4; b < E && N > c.cus && N <= kRounds * c.cus; b += 4) {
             const Request r = load(b);
             if (r.n * c.G <= c.most_d) continue;
             int kt;
@@ -209,7 +216,7 @@ __device__ __forceinline__ void plan_chunks(const C &c, int *lds) {
         const int T = chunk_tiles(c, load(b), qb, &kt), S = div_ceil(kt, len), k = T * S * c.Hkv;
         start[b] = items;
         items += k;
-        slots += kAll || S > 1 ? k : 0;
+        slots += is_group(c, b) || S > 1 ? k : 0;
     }
     const int upto = wave_scan(items), slots_upto = wave_scan(slots);
     if (lane == 63) sums[wave] = upto, sums[8 + wave] = slots_upto;
@@ -222,15 +229,15 @@ __device__ __forceinline__ void plan_chunks(const C &c, int *lds) {
         (void)chunk_tiles(c, load(b), qb, &kt);
         first[b] = start[b] + before;
         slot[b] = slots_before;
-        slots_before += kAll || kt > len ? k : 0;
+        slots_before += is_group(c, b) || kt > len ? k : 0;
     }
     __syncthreads();
     for (int b = b0; b < b1; ++b) start[b] += before;
-    if (tid == 511) start[c.B] = before + items, first[c.B] = before + items;
+    if (tid == 511) start[E] = before + items, first[E] = before + items;
     if (!listed) return;
 
     auto item_of = [&](int id, int *own) {
-        int lo = 0, hi = c.B;  // last request whose first item is at most id
+        int lo = 0, hi = E;  // last request whose first item is at most id
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
             if (start[mid] <= id) lo = mid;
