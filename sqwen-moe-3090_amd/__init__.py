@@ -749,9 +749,9 @@ def paged_share(q_start, kv_len, group, shared_len, members, m_start=None, m_pos
 
         T = members.shape[0]
         m_start, m_pos, token_group = new(m_start, shared_len.shape[0] + 1), new(m_pos, T), new(token_group, T)
-    share = PagedShare(members, m_start, m_pos, token_group)
+    share = tuple.__new__(PagedShare, (members, m_start, m_pos, token_group))
     if stream is None:
-        rc = (_host or _load_host()).share(q_start, kv_len, group, shared_len, *share, pos)
+        rc = (_host or _load_host()).share(q_start, kv_len, group, shared_len, members, m_start, m_pos, token_group, pos)
         if rc is not None:
             if rc:
                 _check(rc)

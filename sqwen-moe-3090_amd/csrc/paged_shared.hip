@@ -12,6 +12,9 @@
 #include "paged_merge.hpp"
 #include "paged_work.hpp"
 
+#ifndef FEWROWS
+#define FEWROWS 8192
+#endif
 namespace sqa {
 namespace paged {
 namespace {
@@ -25,38 +28,105 @@ struct Merge {
     const int32_t *token_group;
 };
 
-// A wavefront takes R heads of a token together, 4 dims a lane; 64 / R parts at a time: lane
-// r * 64 / R + i holds part i's weight for head r. The own parts come first, then the prefix's.
+// The parts of a row (R heads of a token): splits of its own keys, then of its group's prefix.
 template <int R>
-__global__ __launch_bounds__(kThreads) void merge_shared_kernel(Merge p) {
-    constexpr int kS = 64 / R, kBatch = R >= 4 ? 2 : 8;
+struct RowParts {
+    Row a[R], b[R];
+    int n1, n;
+    bool whole;  // the own keys are one part, normalised
+    // false: a row of no request, or left as it is
+    __device__ __forceinline__ bool find(const Merge &p, int t, int h0) {
+        const Parts &c = p.parts;
+        const int4 w1 = c.where[t], w2 = c.g_where[t];
+        const int g = p.token_group[t];
+        if (t < c.q_start[0] || t >= c.q_start[c.B]) return false;  // the entry was not written
+        whole = (w1.w & 3) == kWhole;
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            const int h = min(h0 + k, c.H - 1);
+            const int64_t at = (int64_t)t * c.H + h;
+            a[k] = whole ? Row{c.whole + at * 256, c.stats + at * 2, 0, 1} : partials(c, w1, h);
+            b[k] = partials(c, w2, h);
+        }
+        n1 = a[0].n;
+        n = n1 + (g >= 0 && g < c.groups ? b[0].n : 0);
+        return n1 != 0;  // (of the token: all heads alike)
+    }
+    // (m, l) of part s < n, at ml1 and ml2 of the head
+    __device__ __forceinline__ float2 stats(const float *ml1, const float *ml2, int s) const {
+        const float *at = s < n1 ? ml1 + s * (a[0].step / 128) : ml2 + (s - n1) * (b[0].step / 128);
+        return s < n ? *reinterpret_cast<const float2 *>(at) : make_float2(-INFINITY, 0.0f);
+    }
+    __device__ __forceinline__ const float *acc(int k, int s) const {
+        return s < n1 ? a[k].acc + s * a[k].step : b[k].acc + (s - n1) * b[k].step;
+    }
+};
+
+// Few rows of many parts: a workgroup a row, its wavefronts every fourth part, 4 dims a lane, so
+// that 32 parts are on their way together. Every wavefront takes all weights for itself, a part a
+// lane: the maximum over all parts first, then the weights, 64 parts at a time.
+__global__ __launch_bounds__(kThreads) void merge_parts_kernel(Merge p) {
+    constexpr int kBatch = 8;
+    __shared__ floatx4 sum[4][64];
+    const Parts &c = p.parts;
+    const int t = (int)blockIdx.y + (int)(blockIdx.z << 15), h = (int)blockIdx.x;
+    if (t >= c.n_tok) return;
+    const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    RowParts<1> r;
+    if (!r.find(p, t, h)) return;
+    const float *gate = c.gate ? gate_row(c, t, h) + threadIdx.x : nullptr;
+    const float g = gate ? *gate : 0.0f;
+    float2 ml = r.stats(r.a[0].ml, r.b[0].ml, lane);
+    float M = ml.x;
+    for (int s0 = 64; s0 < r.n; s0 += 64) M = fmaxf(M, r.stats(r.a[0].ml, r.b[0].ml, s0 + lane).x);
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) M = fmaxf(M, __shfl_xor(M, x));
+    floatx4 o = {0.f, 0.f, 0.f, 0.f};
+    float L = 0.0f;
+    for (int s0 = 0; s0 < r.n; s0 += 64) {
+        if (s0) ml = r.stats(r.a[0].ml, r.b[0].ml, s0 + lane);
+        const float e = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - M);
+        const float l = ml.x == -INFINITY ? 0.0f : ml.y * e, w = r.whole && s0 + lane == 0 ? l : e;
+        L += l;
+        const int end = min(r.n - s0, 64);
+        for (int s1 = wave; s1 < end; s1 += 4 * kBatch) {
+            floatx4 x[kBatch];
+            float wt[kBatch];
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j) {
+                const int s = s1 + 4 * j;
+                wt[j] = s < end ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), min(s, 63))) : 0.0f;
+                if (wt[j] != 0.0f) x[j] = *reinterpret_cast<const floatx4 *>(r.acc(0, s0 + s) + 4 * lane);
+            }
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j)
+                if (wt[j] != 0.0f) o += x[j] * wt[j];
+        }
+    }
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) L += __shfl_xor(L, x);
+    sum[wave][lane] = o;
+    __syncthreads();
+    const float *s = reinterpret_cast<const float *>(sum) + threadIdx.x;
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L, x = ((s[0] + s[256]) + (s[512] + s[768])) * inv;
+    c.dst[((int64_t)t * c.H + h) * kHeadDim + threadIdx.x] = gate ? gate_by(x, g) : x;
+}
+
+// Many rows: a wavefront takes R heads of a token together, 4 dims a lane; 64 / R parts at a
+// time: lane r * 64 / R + i holds part i's weight for head r.
+template <int R>
+__global__ __launch_bounds__(kThreads) void merge_rows_kernel(Merge p) {
+    constexpr int kS = 64 / R, kBatch = 2;
     const Parts &c = p.parts;
     const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int t = (int)blockIdx.y + (int)(blockIdx.z << 15), h0 = ((int)blockIdx.x * 4 + wave) * R;
     if (t >= c.n_tok || h0 >= c.H) return;
-    // (of no request: the entry was not written)
-    if (t < c.q_start[0] || t >= c.q_start[c.B]) return;
-    const int4 w1 = c.where[t];
-    const int g = p.token_group[t];
-    const bool member = g >= 0 && g < c.groups && c.g_len[g] > 0;
-    const int4 w2 = member ? c.g_where[t] : make_int4(0, 0, 0, kDone);
-    const bool whole = (w1.w & 3) == kWhole;
-    Row a[R], b[R];
+    RowParts<R> r;
+    if (!r.find(p, t, h0)) return;
+    const int k_own = lane / kS, i_own = lane % kS;
+    const float *ml1 = r.a[0].ml, *ml2 = r.b[0].ml;
 #pragma unroll
-    for (int k = 0; k < R; ++k) {
-        const int h = min(h0 + k, c.H - 1);
-        a[k] = partials(c, w1, h);
-        if (whole) {
-            const int64_t at = (int64_t)t * c.H + h;
-            a[k] = Row{c.whole + at * 256, c.stats + at * 2, 0, 1};
-        }
-        b[k] = partials(c, w2, h);
-    }
-    if (a[0].n == 0) return;  // of the token: all heads alike
-    const int n1 = a[0].n, n = n1 + b[0].n, k_own = lane / kS, i_own = lane % kS;
-    const float *ml1 = a[0].ml, *ml2 = b[0].ml;
-#pragma unroll
-    for (int k = 1; k < R; ++k) ml1 = k_own == k ? a[k].ml : ml1, ml2 = k_own == k ? b[k].ml : ml2;
+    for (int k = 1; k < R; ++k) ml1 = k_own == k ? r.a[k].ml : ml1, ml2 = k_own == k ? r.b[k].ml : ml2;
     floatx4 o[R], g4[R];
     float M = -INFINITY, L = 0.0f;  // of head k_own
 #pragma unroll
@@ -64,24 +134,22 @@ __global__ __launch_bounds__(kThreads) void merge_shared_kernel(Merge p) {
         o[k] = floatx4{0.f, 0.f, 0.f, 0.f};
         if (c.gate) g4[k] = *reinterpret_cast<const float4a *>(gate_row(c, t, min(h0 + k, c.H - 1)) + 4 * lane);
     }
-    for (int s0 = 0; s0 < n; s0 += kS) {
-        const int s = s0 + i_own;
-        const float *at = s < n1 ? ml1 + s * (a[0].step / 128) : ml2 + (s - n1) * (b[0].step / 128);
-        const float2 ml = s < n ? *reinterpret_cast<const float2 *>(at) : make_float2(-INFINITY, 0.0f);
+    for (int s0 = 0; s0 < r.n; s0 += kS) {
+        const float2 ml = r.stats(ml1, ml2, s0 + i_own);
         float m = ml.x;
 #pragma unroll
         for (int x = 1; x < kS; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
         const float Mn = fmaxf(M, m), al = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(M - Mn);
         const float e = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - Mn);
         float l = ml.x == -INFINITY ? 0.0f : ml.y * e;
-        const float w = whole && s == 0 ? l : e;  // a whole part comes normalised
+        const float w = r.whole && s0 + i_own == 0 ? l : e;
 #pragma unroll
         for (int x = 1; x < kS; x <<= 1) l += __shfl_xor(l, x);
         L = L * al + l;
         M = Mn;
 #pragma unroll
         for (int k = 0; k < R; ++k) o[k] *= __int_as_float(__builtin_amdgcn_readlane(__float_as_int(al), k * kS));
-        const int end = min(n - s0, kS);
+        const int end = min(r.n - s0, kS);
         for (int s1 = 0; s1 < end; s1 += kBatch) {
             floatx4 x[kBatch][R];
             float wt[kBatch][R];
@@ -89,10 +157,8 @@ __global__ __launch_bounds__(kThreads) void merge_shared_kernel(Merge p) {
             for (int j = 0; j < kBatch; ++j)
 #pragma unroll
                 for (int k = 0; k < R; ++k) {
-                    const int i = s0 + s1 + j;
                     wt[j][k] = s1 + j < end ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), k * kS + min(s1 + j, kS - 1))) : 0.0f;
-                    const float *from = i < n1 ? a[k].acc + i * a[k].step : b[k].acc + (i - n1) * b[k].step;
-                    if (wt[j][k] != 0.0f) x[j][k] = *reinterpret_cast<const floatx4 *>(from + 4 * lane);
+                    if (wt[j][k] != 0.0f) x[j][k] = *reinterpret_cast<const floatx4 *>(r.acc(k, s0 + s1 + j) + 4 * lane);
                 }
 #pragma unroll
             for (int j = 0; j < kBatch; ++j)
@@ -173,11 +239,10 @@ int launch_paged_shared(const SharedArgs &a, hipStream_t s) {
     if (rc) return rc;
 
     const int prof = profile_start("paged_shared_merge", s);
-    const bool four = (int64_t)c.n_tok * c.H > 8192 && c.H >= 16;
-    const dim3 grid((unsigned)((c.H + (four ? 16 : 4) - 1) / (four ? 16 : 4)), (unsigned)(c.n_tok < (1 << 15) ? c.n_tok : 1 << 15),
-                    (unsigned)((c.n_tok + (1 << 15) - 1) >> 15));
-    if (four) merge_shared_kernel<4><<<grid, dim3(kThreads), 0, s>>>(m);
-    else merge_shared_kernel<1><<<grid, dim3(kThreads), 0, s>>>(m);
+    const bool few = (int64_t)c.n_tok * c.H <= FEWROWS;
+    const unsigned y = (unsigned)(c.n_tok < (1 << 15) ? c.n_tok : 1 << 15), z = (unsigned)((c.n_tok + (1 << 15) - 1) >> 15);
+    if (few) merge_parts_kernel<<<dim3((unsigned)c.H, y, z), dim3(kThreads), 0, s>>>(m);
+    else merge_rows_kernel<4><<<dim3((unsigned)((c.H + 15) / 16), y, z), dim3(kThreads), 0, s>>>(m);
     profile_stop(prof, s);
     return hip_status(hipGetLastError(), "paged_attn_shared merge launch");
 }
