@@ -167,7 +167,8 @@ int sqa_supports_rope_norm(const sqa_tensor *dst, const sqa_tensor *src, const s
  * Pairs, sections and directions as in sqa_rope_norm_set_rows_q4_0, angle delta * freq_scale *
  * freq_base^(-2 ic / n_rot) in 64 bits, cos and sin of it rounded to fp32; attn_factor, which the
  * cached values have already, plays no part. Blocks that hold a rotated dim are quantized again
- * (quantize_row_q4_0), the others' bytes stay. D of 64, 128 or 256 with a rope.
+ * (quantize_row_q4_0), the others' bytes stay. D of 64, 128 or 256 with a rope, whose fastest
+ * pair turns by up to 1.25 radians a position (1 with freq_scale 1).
  * In place (dst is src) a row that one entry reads must be no other entry's to[]: from == to is
  * fine, as are ranges that do not meet; otherwise, and where to[] names a row twice, that row is
  * unspecified. dst overlaps nothing else. D * n_head <= 2^17.

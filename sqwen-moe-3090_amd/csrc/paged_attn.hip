@@ -2,7 +2,7 @@
 // call launches, its workspace, and the merge of split partials.
 //
 // Requests of few query rows (up to 16 per KV head; up to 8 where larger ones may be
-// in the call) go to paged_decode.hip, the others to paged_chunk.hip.
+// in the call) go to paged_decode.hip, the others to paged_chunk.hpp's kernel.
 #include <float.h>
 
 #include "paged_merge.hpp"

@@ -18,7 +18,7 @@ typedef float float4a __attribute__((ext_vector_type(4), aligned(4)));
 // heads 1 (kFew) or slots * step (kMany).
 constexpr int kDone = 0;  // nothing to merge: the row is written, or left as it was
 constexpr int kFew = 1, kMany = 2;
-constexpr int kWhole = 3;  // one part, normalised, in OwnCall::dst and ::stats
+constexpr int kWhole = 3;  // one part, normalised, in Parts::whole and ::stats
 
 // P of every partial carries this power of two, l with it (which cancels in a merge).
 constexpr int kPBits = 6;

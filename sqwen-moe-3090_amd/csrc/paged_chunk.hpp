@@ -19,6 +19,7 @@
 // scalar base plus constant offsets) and expand them there for all 128 rows:
 //   iteration t: rows of K tile t + 2 and V tile t + 1 are on their way; K tile t + 1
 //   and V tile t are expanded; P V of tile t - 1.
+// (In a call of shared prefixes the score wavefronts expand K, between their MFMAs: kScoreK.)
 // K codes leave a dword of nibbles by shifts and masks alone: the 8 values of a chunk
 // are its dims in the order 0 2 16 18 1 3 17 19, and Q' is laid out in the same order.
 // V needs the codes of 8 keys side by side: 16-bit reads of 8 rows, packed in pairs.

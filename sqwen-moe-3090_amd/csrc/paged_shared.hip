@@ -1,8 +1,8 @@
 // paged_shared.hip - attention of a batch whose groups of requests share long prefixes: what a
 // call launches, its workspace, and the merge of the two parts.
 //
-// A row's own keys go the way of paged_attn (paged_decode.hip, paged_chunk.hip). The keys of a
-// group's prefix meet the rows of all its tokens at once: the many-row kernel of paged_chunk.hip
+// A row's own keys go the way of paged_attn (paged_decode.hip, paged_chunk.hpp). The keys of a
+// group's prefix meet the rows of all its tokens at once: the many-row kernel of paged_chunk.hpp
 // takes tiles of 128 (or 64) rows out of the group's list of members, so that a key is read and
 // expanded once for that many rows instead of once for every request's 8. An extra workgroup of
 // the few-row launch plans the tiles and splits. Groups of few rows (a token or two) are pieces of
@@ -12,14 +12,16 @@
 #include "paged_merge.hpp"
 #include "paged_work.hpp"
 
-#ifndef FEWROWS
-#define FEWROWS 8192
-#endif
 namespace sqa {
 namespace paged {
 namespace {
 
 constexpr int kThreads = 256;
+
+// Rows up to which the merge takes a workgroup a row (merge_parts_kernel): 640 rows of some 50
+// parts 8.5 us (a wavefront four rows: 25.9), 2048 of 11 parts 11.0 (16.0), 3200 11.1 (11.0),
+// 4096 14.6 (12.7), 16384 39.6 (17.8).
+constexpr int kFewRows = 3000;
 
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 
@@ -239,7 +241,7 @@ int launch_paged_shared(const SharedArgs &a, hipStream_t s) {
     if (rc) return rc;
 
     const int prof = profile_start("paged_shared_merge", s);
-    const bool few = (int64_t)c.n_tok * c.H <= FEWROWS;
+    const bool few = (int64_t)c.n_tok * c.H <= kFewRows;
     const unsigned y = (unsigned)(c.n_tok < (1 << 15) ? c.n_tok : 1 << 15), z = (unsigned)((c.n_tok + (1 << 15) - 1) >> 15);
     if (few) merge_parts_kernel<<<dim3((unsigned)c.H, y, z), dim3(kThreads), 0, s>>>(m);
     else merge_rows_kernel<4><<<dim3((unsigned)((c.H + 15) / 16), y, z), dim3(kThreads), 0, s>>>(m);

@@ -279,3 +279,94 @@ def test_random_batches(sqa, orc, dev):
         want = b.ref(orc, **{{"softcap": "cap", "max_bias": "bias"}[k]: v for k, v in opt.items()})
         print(k, H, Hkv, B, G, opt)
         close(call(sqa, dev, b, **opt), want)
+
+
+@pytest.mark.parametrize("B,G", [(70, 1), (70, 90), (300, 300), (1500, 40), (1300, 2500)])
+@pytest.mark.parametrize("most", [1, 9, 40])
+def test_many_requests_and_groups(sqa, orc, dev, B, G, most):
+    """More requests and groups than a wavefront's lanes, and than the few-row kernel keeps."""
+    r = np.random.default_rng(B + G)
+    new = [int(x) for x in r.choice([0, 1, 1, 1, most], B)]
+    group = [int(x) for x in r.integers(-1, G, B)]
+    b = Batch(orc, B + G, new, [int(x) for x in r.integers(0, 40, B)], [int(x) for x in r.integers(0, 90, G)], group, 4, 4, 16)
+    close(call(sqa, dev, b), b.ref(orc))
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1, 1], [150, 1, 90, 0]])
+def test_two_calls_at_once(sqa, orc, dev, new):
+    """On two streams, each with its own workspace."""
+    pair = [Batch(orc, 40 + i, new, [700 - 300 * i, 2000, 65, 8], [900, 30 + i], [0, i, 0, 1], gate=i == 1) for i in (0, 1)]
+    made = [(b.args(sqa, dev), torch.zeros(b.q.shape, device=dev)) for b in pair]
+    a = made[0][0][0]
+    size = sqa.paged_attn_shared_workspace_size(a[0], a[1], a[3], a[6], max(new))
+    works = [torch.full((size,), 0xFF, dtype=torch.uint8, device=dev) for _ in pair]
+    streams = [torch.cuda.Stream() for _ in pair]
+    torch.cuda.synchronize()
+    for _ in range(8):
+        for ((a, kw), out), work, s in zip(made, works, streams):
+            with torch.cuda.stream(s):
+                sqa.paged_attn_shared(*a, **kw, out=out, workspace=work)
+    torch.cuda.synchronize()
+    for b, (_, out) in zip(pair, made):
+        close(out.cpu().numpy().astype(np.float64), b.ref(orc))
+
+
+@pytest.mark.parametrize("new", [[40, 1, 17, 130], [9, 9, 8, 1]])
+def test_chunks_in_place_and_in_small_workspaces(sqa, orc, dev, new):
+    """dst as q and as the gate, chunks and members that split over many keys; every workspace that a call takes."""
+    b = Batch(orc, 16, new, [300, 20, 0, 64], [1500, 200], [0, 0, 1, -1], gate=True)
+    a, kw = b.args(sqa, dev)
+    full = sqa.paged_attn_shared_workspace_size(a[0], a[1], a[3], a[6], a[9])
+    ws = torch.full((full,), 0xFF, dtype=torch.uint8, device=dev)
+    want = sqa.paged_attn_shared(*a, **kw, out=torch.zeros_like(a[0]), workspace=ws)
+    close(want.cpu().numpy().astype(np.float64), b.ref(orc))
+    x = a[0].clone()
+    sqa.paged_attn_shared(x, *a[1:], **kw, out=x, workspace=ws)
+    assert torch.equal(x, want)
+    g = kw["gate"].clone()
+    sqa.paged_attn_shared(*a, gate=g, out=g, workspace=ws)
+    assert torch.equal(g, want)
+    taken = 0
+    for size in [*range(full // 40 * 40, 0, -full // 40), 256]:
+        ws.fill_(0xFF)
+        y = torch.zeros_like(a[0])
+        try:
+            sqa.paged_attn_shared(*a, **kw, out=y, workspace=ws[:size])
+        except sqa.SqaError as e:
+            assert e.status == 3 and not y.any()
+            continue
+        taken += 1
+        close(y.cpu().numpy().astype(np.float64), b.ref(orc))
+        assert (ws[size:] == 0xFF).all()
+    assert 0 < taken <= 40  # (some 0.6 MB are needed, and 256 bytes are not enough)
+
+
+def test_more_tokens_than_max_q(sqa, orc, dev):
+    """Rows of requests with more than max_q tokens may be left as they were: the others are right."""
+    new = [1, 60, 1, 3]
+    b = Batch(orc, 17, new, [30, 20, 100, 64], [700], [0, 0, 0, -1])
+    want = b.ref(orc)
+    for max_q in (1, 3):
+        b.max_q = max_q
+        got = call(sqa, dev, b)
+        for i, n in enumerate(new):
+            if n <= max_q:
+                at = slice(b.q_start[i], b.q_start[i + 1])
+                close(got[at], want[at])
+
+
+@pytest.mark.parametrize("n", [1, 2, 40])
+def test_bias_over_many_tiles(sqa, orc, dev, n):
+    """Slopes that leave only the last keys, and slopes that leave the whole prefix too."""
+    b = Batch(orc, 18, [n, n, n], [2000, 65, 0], [900, 64], [0, 1, 1], page=64, gate=n == 2)
+    for bias in (1.0, 8.0, 30.0):
+        close(call(sqa, dev, b, max_bias=bias), b.ref(orc, bias=bias))
+
+
+@pytest.mark.parametrize("B,n", [(1, 1), (24, 1), (3, 40)])
+def test_weights_keep_their_bits(sqa, orc, dev, B, n):
+    """As for requests that share nothing: logits within some 3 roundings of 2^-24, P and P d_v at 22 bits, below 1e-6 of
+    the output together; the two parts' weights in the merge add 2^-22."""
+    b = Batch(orc, 19, [n] * B, [100] * B, [4096], [0] * B, page=64)
+    got, want = call(sqa, dev, b), b.ref(orc)
+    assert np.linalg.norm(got - want) <= 1e-6 * np.linalg.norm(want)

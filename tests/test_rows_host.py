@@ -95,3 +95,16 @@ def test_python_refuses_tensors_off_the_gpu(sqa):
     for call in (lambda: sqa.get_rows_q4_0(c, i), lambda: sqa.move_rows_q4_0(c, c, i, i)):
         with pytest.raises(sqa.SqaError):
             call()
+
+
+def test_move_rows_refuses_pairs_that_turn_too_fast(sqa):
+    c = [T(sqa, 2, [D, 2, 40], [18, 144, 288], p) for p in (1 << 20, 1 << 21)]
+    to, frm = T(sqa, 27, [9], [8], 1 << 22), T(sqa, 27, [9], [8], 1 << 23)
+    delta = T(sqa, 26, [36], [4], 1 << 24)
+    # radians a position of the fastest pair: base^-(30/32) * scale where base < 1, else scale
+    for base, scale, ok in ((1e7, 1.25, 1), (1e7, 1.3, 0), (1e7, -1.25, 1), (1e7, -1.3, 0), (1.0, 1.0, 1), (0.8, 1.0, 1), (0.7, 1.0, 0), (0.7, 0.8, 1)):
+        rope = sqa.rope_params(32, (4, 4, 4, 4), base, freq_scale=scale)
+        assert sqa.lib().sqa_supports_move_rows(ref(c[0]), ref(c[1]), ref(to), ref(frm), ref(delta), ref(rope)) == ok, (base, scale)
+        if not ok:
+            assert sqa.lib().sqa_move_rows_q4_0(ref(c[0]), ref(c[1]), ref(to), ref(frm), ref(delta), ref(rope), None) == 2
+            assert "radians" in sqa.last_error()
