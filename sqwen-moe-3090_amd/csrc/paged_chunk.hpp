@@ -35,6 +35,8 @@
 // end are 11 us that nothing overlaps (LDS holds one a CU): Q 2.7, its quantization 2.6,
 // the last tile 1.9, the result 3 to 4 (turned in LDS into whole rows it took 5).
 #pragma once
+#include <type_traits>
+
 #include "paged_work.hpp"
 
 namespace sqa {
@@ -51,7 +53,8 @@ constexpr int kValueWaves = 4;
 constexpr int kThreads = 64 * (kScoreWaves + kValueWaves);
 constexpr int kMaxRG = 2;                // 16-row groups per score wave: 1 or 2 (kRG in the kernel)
 constexpr int rows_per_wg(int rg) { return kScoreWaves * rg * 16; }
-constexpr int kOffDk = kPK * 512;        // K stage: Kc, Dk
+constexpr int kWideRow = 520;            // K stage: Kc (rows of 512 bytes, or of 520), Dk
+constexpr int kOffDk = kPK * kWideRow;
 constexpr int kKStage = kOffDk + 8 * kPK * 2;
 constexpr int kOffDv = kHeadDim * kPK * 2;  // V stage: Vc, Dv
 constexpr int kVStage = kOffDv + 8 * kPK * 2;
@@ -63,7 +66,8 @@ constexpr int kPBuf = kScoreWaves * kMaxRG * 2 * 1024;
 constexpr int kLdsA = kLdsP + 2 * kPBuf;          // [4 waves][kRG][16 rows] f32
 constexpr int kABuf = kScoreWaves * kMaxRG * 16 * 4;
 constexpr int kLdsE = kLdsA + 2 * kABuf;          // [2][4] exponents of the V scales, one per pair of blocks
-constexpr int kLdsRaw = kLdsE + 32;               // [K, V][2][32 rows][144 B]
+constexpr int kLdsF = kLdsE + 32;               // [2][4] whether a maximum of the wave's rows has moved
+constexpr int kLdsRaw = kLdsF + 32;               // [K, V][2][32 rows][144 B]
 constexpr int kLdsBytes = kLdsRaw + 4 * kRawTile + 16;
 static_assert(kLdsBytes <= 160 * 1024, "LDS budget");
 static_assert(kLdsRaw % 16 == 0 && kKStage % 16 == 0 && kVStage % 16 == 0, "alignment of the stages");
@@ -82,9 +86,41 @@ __device__ __forceinline__ float xmax32(float x) {
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-// LDS/record row of key k (0..31) of a tile: the inverse of sigma.
-__device__ __forceinline__ int key_row(int k) { return 16 * ((k >> 2) & 1) + 4 * (k >> 3) + (k & 3); }
+// sa[i] += c[i] * (dk of lane i of every 16 lanes), i = 4 K .. 4 K + 3: the multiplication reads the
+// other lane's register (the compiler makes a move of its own of that). The assembler's lines are
+// no instructions to the compiler that read c, a matrix instruction's result: K = 0 has one of the
+// compiler's own before them, and its waits. s_nop: dk may have been written just before.
+template <int K>
+__device__ __forceinline__ void add_scaled(float (&sa)[16], float c0, float c1, float c2, float c3, float dk) {
+    if constexpr (K == 0) {
+        sa[0] = fmaf(__int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(dk), 0x150, 0xf, 0xf, true)), c0, sa[0]);
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_nop 1\n\t"
+                     "v_fmac_f32_dpp %0, %3, %4 row_newbcast:1 row_mask:0xf bank_mask:0xf\n\t"
+                     "v_fmac_f32_dpp %1, %3, %5 row_newbcast:2 row_mask:0xf bank_mask:0xf\n\t"
+                     "v_fmac_f32_dpp %2, %3, %6 row_newbcast:3 row_mask:0xf bank_mask:0xf"
+                     : "+v"(sa[1]), "+v"(sa[2]), "+v"(sa[3]) : "v"(dk), "v"(c1), "v"(c2), "v"(c3));
+    } else {
+        asm volatile("s_nop 1\n\t"
+                     "v_fmac_f32_dpp %0, %4, %5 row_newbcast:%9 row_mask:0xf bank_mask:0xf\n\t"
+                     "v_fmac_f32_dpp %1, %4, %6 row_newbcast:%10 row_mask:0xf bank_mask:0xf\n\t"
+                     "v_fmac_f32_dpp %2, %4, %7 row_newbcast:%11 row_mask:0xf bank_mask:0xf\n\t"
+                     "v_fmac_f32_dpp %3, %4, %8 row_newbcast:%12 row_mask:0xf bank_mask:0xf"
+                     : "+v"(sa[4 * K]), "+v"(sa[4 * K + 1]), "+v"(sa[4 * K + 2]), "+v"(sa[4 * K + 3])
+                     : "v"(dk), "v"(c0), "v"(c1), "v"(c2), "v"(c3), "n"(4 * K), "n"(4 * K + 1), "n"(4 * K + 2), "n"(4 * K + 3));
+    }
+    __builtin_amdgcn_sched_barrier(0);
+}
 
+// LDS row of key k (0..31) of a tile, such that the logits that a lane holds after S^T are those of
+// the keys of its operands in P V: 8g .. 8g + 7 (16x16 tiles), 8g .. and 16 + 8g .. (32x32).
+template <bool kWide>
+__device__ __forceinline__ int key_row(int k) {
+    return kWide ? (k & 19) | ((k & 4) << 1) | ((k & 8) >> 1) : 16 * ((k >> 2) & 1) + 4 * (k >> 3) + (k & 3);
+}
+// V's chunk c of dim d is at c ^ v_swap(d)
+template <bool kWide>
+__device__ __forceinline__ int v_swap(int d) { return kWide ? ((d >> 1) & 2) | ((d >> 4) & 1) : (d >> 1) & 3; }
 
 // Codes n of the low (bits 0-3, 16-19) or high nibbles (4-7, 20-23) of x as the packed
 // fp16 pair n - 8: 0x6400 | n is exactly 1024 + n and 0x6400 | 16 n is 1024 + 16 n; minus
@@ -140,21 +176,23 @@ __device__ __forceinline__ half8 lds_half8(const uint8_t *base, int off_lo, int 
 // With these maps the 32 lanes that LDS serves at a time store to 32 different pairs of
 // banks (lanes over whole rows of K and over all blocks of V met in 16 of them 16 deep:
 // 3260 LDS cycles a tile, 56% of them conflicts).
+template <bool kWide>
 struct Expand {
     int k_raw, k_sh, k_to, dk_raw, dk_to;   // LDS offsets in the first of two buffers
     int v_raw, v_to, v_odd, dv_raw, dv_to, dv_key;
     uint32_t x[4], k[5], d, dk, magic;
     __device__ __forceinline__ void init(int w, int lane) {
-        const int key = 16 * ((lane >> 4) & 1) + 4 * w + (lane & 3), kb = 4 * (lane >> 5) + ((lane >> 2) & 3), r = key_row(key);
+        const int key = kWide ? 16 * (w >> 1) + 8 * ((lane >> 2) & 1) + 4 * (w & 1) + (lane & 3) : 16 * ((lane >> 4) & 1) + 4 * w + (lane & 3);
+        const int kb = 4 * (lane >> 5) + ((lane >> (kWide ? 3 : 2)) & 3), r = key_row<kWide>(key);
         dk_raw = kLdsRaw + kHeadRowBytes * key + 18 * kb;
         k_raw = kLdsRaw + kHeadRowBytes * key + ((18 * kb + 2) & ~3);  // the codes start 2 bytes off a dword for even blocks
         k_sh = kb & 1 ? 0 : 16;
-        k_to = r * 512 + 16 * ((4 * kb) ^ (r & 7)) + (r & 8);
-        dk_to = kOffDk + (kb * kPK + r) * 2;
+        k_to = kWide ? r * kWideRow + 64 * kb : r * 512 + 16 * ((4 * kb) ^ (r & 7)) + (r & 8);
+        dk_to = kOffDk + (kWide ? key * 8 + kb : kb * kPK + r) * 2;
         const int c = lane & 3, i = (lane >> 2) & 1, m = (lane >> 3) & 3, b = 2 * w + (lane >> 5);
         v_raw = kLdsRaw + 2 * kRawTile + kHeadRowBytes * 8 * c + 18 * b + 2 + 4 * m + 2 * i;
         const int dim = 32 * b + 4 * m + 2 * i;
-        v_to = kLdsV + 64 * dim + 16 * (c ^ ((dim >> 1) & 3)) + (dim & 8);
+        v_to = kLdsV + 64 * dim + 16 * (c ^ v_swap<kWide>(dim)) + (dim & 8);
         v_odd = m & 1;
         dv_key = lane & 31;
         dv_raw = kLdsRaw + 2 * kRawTile + kHeadRowBytes * dv_key + 18 * b;
@@ -186,16 +224,17 @@ struct Expand {
         for (int q = 0; q < 4; ++q) y[q] = x[q] >> (8 * byte);
         *reinterpret_cast<uint2 *>(smem + to) = make_uint2(codes_lo(y[0], magic), codes_lo(y[1], magic));
         *reinterpret_cast<uint2 *>(smem + (to ^ 8)) = make_uint2(codes_lo(y[2], magic), codes_lo(y[3], magic));
-        *reinterpret_cast<uint2 *>(smem + to + 1024) = make_uint2(codes_hi(y[0], magic), codes_hi(y[1], magic));
-        *reinterpret_cast<uint2 *>(smem + (to ^ 8) + 1024) = make_uint2(codes_hi(y[2], magic), codes_hi(y[3], magic));
+        const int hi = (kWide ? to ^ 16 : to) + 1024;  // dims 16 further
+        *reinterpret_cast<uint2 *>(smem + hi) = make_uint2(codes_hi(y[0], magic), codes_hi(y[1], magic));
+        *reinterpret_cast<uint2 *>(smem + (hi ^ 8)) = make_uint2(codes_hi(y[2], magic), codes_hi(y[3], magic));
     }
     // chunk m of the lane's block
     __device__ __forceinline__ void store_k(uint8_t *smem, int t, int m) {
-        const int to = (k_to + (t & 1) * kKStage) ^ (16 * m);
+        const int at = k_to + (t & 1) * kKStage, to = kWide ? at + 16 * m : at ^ (16 * m);
         const uint32_t y = __builtin_amdgcn_alignbit(k[m + 1], k[m], (uint32_t)k_sh), z = y >> 8;
         if (m == 0) *reinterpret_cast<uint16_t *>(smem + dk_to + (t & 1) * kKStage) = (uint16_t)dk;
         *reinterpret_cast<uint2 *>(smem + to) = make_uint2(codes_lo(y, magic), codes_hi(y, magic));
-        *reinterpret_cast<uint2 *>(smem + (to ^ 8)) = make_uint2(codes_lo(z, magic), codes_hi(z, magic));
+        *reinterpret_cast<uint2 *>(smem + (kWide ? to + 8 : to ^ 8)) = make_uint2(codes_lo(z, magic), codes_hi(z, magic));
     }
     // V scales of tile t as d_v 2^e (two blocks of this wavefront), 0 for keys at or past
     // `left`, on pages that are not there, and for NaN or Inf (bytes that are no q4_0):
@@ -227,45 +266,53 @@ struct Expand {
 // rint(x * 127 / amax)), times fp16(d) * scale * log2(e) in fp32, as fp16 hi and
 // lo = fp16(Q' - hi). The loads of a row are one batch (block by block they were 16
 // memory latencies at the start of every workgroup).
+template <bool kWide>
 struct QRow {
-    float4a v[16];
+    static constexpr int kC = kWide ? 2 : 1;  // chunks of 8 dims of a block that a lane holds: g, or g and 2 + g
+    float4a v[16 * kC];
     __device__ __forceinline__ void load(const Call &p, int64_t row, int h, int g) {
         const float *q = reinterpret_cast<const float *>(p.q + row * p.q_nb1 + (int64_t)h * p.q_nb2) + 4 * g;
 #pragma unroll
-        for (int b = 0; b < 16; ++b) v[b] = *reinterpret_cast<const float4a *>(q + 16 * b);
+        for (int b = 0; b < 8 * kC; ++b)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) v[2 * b + k] = *reinterpret_cast<const float4a *>(q + 32 * (b / kC) + 8 * (b % kC) + 16 * k);
     }
-    __device__ __forceinline__ void quantize(float qscale, bool ok, half8 (&hi)[8], half8 (&lo)[8]) const {
+    __device__ __forceinline__ void quantize(float qscale, bool ok, half8 (&hi)[8 * kC], half8 (&lo)[8 * kC]) const {
 #pragma unroll
         for (int b = 0; b < 8; ++b) {
-            const float4a a = v[2 * b], c = v[2 * b + 1];
-            const float x[8] = {a.x, a.z, c.x, c.z, a.y, a.w, c.y, c.w};
             float amax = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(x[j]));
-            amax = xmax32(xmax16(amax));
+            for (int k = 2 * kC * b; k < 2 * kC * (b + 1); ++k)
+                amax = fmaxf(fmaxf(fmaxf(amax, fabsf(v[k].x)), fmaxf(fabsf(v[k].y), fabsf(v[k].z))), fabsf(v[k].w));
+            amax = xmax32(kWide ? amax : xmax16(amax));
             const float d = amax / 127.f;
             const float id = amax != 0.0f ? 127.f / amax : 0.0f;
             const float qd = ok ? (float)(_Float16)d * qscale : 0.0f;
-            float y[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                // y opaque: left visible, the compiler may round code * qd to fp16 twice
-                // (once from the fp32 product for hi, once from the exact product for the
-                // hi it subtracts), and a hi + lo off by one fp16 ulp of hi
-                y[j] = rintf(x[j] * id) * qd;
-                asm volatile("" : "+v"(y[j]));
-                hi[b][j] = (_Float16)y[j];
-            }
-            uint32_t hw[4];
-            __builtin_memcpy(hw, &hi[b], 16);
+            for (int c = kC * b; c < kC * (b + 1); ++c) {
+                const float4a u = v[2 * c], w = v[2 * c + 1];
+                const float x[8] = {u.x, u.z, w.x, w.z, u.y, u.w, w.y, w.w};
+                float y[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {  // the exact residual, hi read from its packed half
-                float r;
-                if (j & 1)
-                    asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel:[0,0,1] op_sel_hi:[0,0,1]" : "=v"(r) : "v"(y[j]), "v"(hw[j >> 1]));
-                else
-                    asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel:[0,0,0] op_sel_hi:[0,0,1]" : "=v"(r) : "v"(y[j]), "v"(hw[j >> 1]));
-                lo[b][j] = (_Float16)r;
+                for (int j = 0; j < 8; ++j) {
+                    // y opaque: left visible, the compiler may round code * qd to fp16 twice
+                    // (once from the fp32 product for hi, once from the exact product for the
+                    // hi it subtracts), and a hi + lo off by one fp16 ulp of hi
+                    y[j] = rintf(x[j] * id) * qd;
+                    asm volatile("" : "+v"(y[j]));
+                    hi[c][j] = (_Float16)y[j];
+                }
+                uint32_t hw[4];
+                __builtin_memcpy(hw, &hi[c], 16);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {  // the exact residual, hi read from its packed half
+                    float r;
+                    if (j & 1)
+                        asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel:[0,0,1] op_sel_hi:[0,0,1]" : "=v"(r) : "v"(y[j]), "v"(hw[j >> 1]));
+                    else
+                        asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel:[0,0,0] op_sel_hi:[0,0,1]" : "=v"(r) : "v"(y[j]), "v"(hw[j >> 1]));
+                    lo[c][j] = (_Float16)r;
+                }
             }
         }
     }
@@ -318,10 +365,16 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(C p) {
     // the score waves: 1278 us where this is 1184 and all in the value waves 1231 (2040 tokens behind
     // 16000 shared keys). (For a plain Call the compiler spills 67 registers in the score waves.)
     constexpr bool kScoreK = kPart && !OPT;
+    constexpr bool kWide = kRG == 2;
+    constexpr int kN = 16 * kRG;          // rows of a wave, a lane's column of the matrix tiles
+    constexpr int kV = 8 * kRG;           // keys of its row that a lane holds, 8 g .. 8 g + 7 (+ 16)
+    constexpr int kT = kHeadDim / kN;     // matrix tiles of O
+    constexpr int kR = kWide ? 16 : 4;    // rows of O that a lane holds
+    typedef float Tile __attribute__((ext_vector_type(kWide ? 16 : 4)));
     extern __shared__ __align__(16) uint8_t smem[];
     const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int lane = tid & 63, g = lane >> 4, n = lane & 15;
+    const int lane = tid & 63, g = lane / kN, n = lane % kN;
     const uint32_t lds0 = (uint32_t)(uintptr_t)smem;
 
     const int qb = uniform(group_of(p, rows_per_wg(kRG)));  // tokens of a query tile
@@ -378,54 +431,44 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(C p) {
     // one before the loop, n_tiles + 1 in it, then two for the hand-over of m and l.
     if (wave < kScoreWaves) {
         const int w = wave;
-        float *ml = reinterpret_cast<float *>(smem + kLdsP) + w * (kRG * 32);  // [rg][row][m, l]
-        // Q' hi and lo of rows r = 16 kRG w + 16rg + n (position q_base + r / G, head
-        // kvh*G + r % G) as B operands, dims 32b + 8g..+7
-        half8 bqh[kRG][8], bql[kRG][8];
-        int my_see[kRG], my_pos[kRG];
-        QRow qrow[kRG];
-        bool row_ok[kRG];
-        float my_slope[kRG];
-        float m_run[kRG], l_part[kRG];
+        float *ml = reinterpret_cast<float *>(smem + kLdsP) + w * (kN * 2);  // [row][m, l]
+        // Q' hi and lo of row r = kN w + n (position q_base + r / G, head kvh*G + r % G) as B
+        // operands: chunk g of every block, or chunks g and 2 + g
+        half8 bqh[8 * kRG], bql[8 * kRG];
+        const int r = kN * w + n, i_tok = group_of(p, r), h = kvh * p.G + r - i_tok * p.G;
+        const bool ok = q_base + i_tok < q_top;
+        const int my_see = ok ? sees(rq, q_base + i_tok) : 0;
+        int my_pos = rq.pos0 + q_base + i_tok;
+        const float my_slope = OPT && p.bias != 0.0f ? slope2(p, h) : 0.0f;
         // The logits are accumulated relative to the row's P reference mref =
         // (m_run, or 0 before the first visible key) - ep: s' = s - mref, so that
         // P = 2^s' needs no subtraction, and the lazy-maximum test s > m_run +
         // ks reads s' > lim_s (ks + ep, or -inf before the first visible key).
         // Both change only when the maximum moves.
-        float mref[kRG], lim_s[kRG];
-#pragma unroll
-        for (int rg = 0; rg < kRG; ++rg) {
-            const int r = 16 * kRG * w + 16 * rg + n;
-            const int i = group_of(p, r), h = kvh * p.G + r - i * p.G;
-            const bool ok = q_base + i < q_top;
-            my_see[rg] = ok ? sees(rq, q_base + i) : 0;
-            const int row = ok ? row_of_token(p, rq, shared, q_base + i) : kPart ? 0 : rq.q0;
-            my_pos[rg] = rq.pos0 + q_base + i;
+        float m_run = -INFINITY, l_part = 0.0f, mref = -(float)kEp, lim_s = -INFINITY;
+        {
+            const int row = ok ? row_of_token(p, rq, shared, q_base + i_tok) : kPart ? 0 : rq.q0;
             if constexpr (kPart && OPT)
-                if (shared) my_pos[rg] = ok ? p.m_pos[rq.q0 + q_base + i] : 0;
-            my_slope[rg] = OPT && p.bias != 0.0f ? slope2(p, h) : 0.0f;
-            qrow[rg].load(p, kPart ? max(row, 0) : row, h, g);
-            row_ok[rg] = ok;
-            m_run[rg] = -INFINITY;
-            l_part[rg] = 0.0f;
-            mref[rg] = -(float)kEp;
-            lim_s[rg] = -INFINITY;
+                if (shared) my_pos = ok ? p.m_pos[rq.q0 + q_base + i_tok] : 0;
+            QRow<kWide> q;
+            q.load(p, kPart ? max(row, 0) : row, h, g);
+            __builtin_amdgcn_sched_barrier(0);  // the loads stay together
+            // raw rows of the first tile: the value waves expand them while Q is quantized
+            if (n_tiles > 0) asm volatile("s_barrier" ::: "memory");
+            q.quantize(p.qscale, ok, bqh, bql);
         }
-        __builtin_amdgcn_sched_barrier(0);  // the loads stay together
-        // raw rows of the first tile: the value waves expand them while Q is quantized
-        if (n_tiles > 0) asm volatile("s_barrier" ::: "memory");
-#pragma unroll
-        for (int rg = 0; rg < kRG; ++rg) qrow[rg].quantize(p.qscale, row_ok[rg], bqh[rg], bql[rg]);
-        // K operand of key row 16kg + n, dims 32b + 8g..+7: chunk (4b + g) ^ (n & 7),
-        // halves swapped when n & 8; the XOR touches bit 2 of 4b + g, so even and odd
-        // b use two bases and b >> 1 adds 128 bytes.
+        // 16x16: K operand of key row 16kg + n, chunk (4b + g) ^ (n & 7), halves swapped when n & 8;
+        // the XOR touches bit 2 of 4b + g, so even and odd b use two bases and b >> 1 adds 128 bytes.
+        // 32x32: row n, chunks 4b + g and 4b + 2 + g, one base.
         int k_off[2][2];  // [b & 1][half]
 #pragma unroll
         for (int bp = 0; bp < 2; ++bp)
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf) k_off[bp][hf] = n * 512 + 16 * ((4 * bp + g) ^ (n & 7)) + 8 * (hf ^ nh);
-        const int p_off = w * (kRG * 2048) + 16 * lane;  // P slots [w][rg][half][lane]
-        Expand ex;
+            for (int hf = 0; hf < 2; ++hf)
+                k_off[bp][hf] = kWide ? n * kWideRow + 16 * g : n * 512 + 16 * ((4 * bp + g) ^ (n & 7)) + 8 * (hf ^ nh);
+        const int p_off = w * (kRG * 2048) + 16 * lane;  // P slots [w][8 keys][hi, lo][lane]
+        const int dk_off = kOffDk + 16 * (16 * ((lane >> 3) & 1) + 8 * g + (lane & 7));
+        Expand<kWide> ex;
         ex.init(w, lane);
 
         int ida = id_of(0, 0), idb = id_of(0, 1);  // pages of the tile's two groups
@@ -438,149 +481,189 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(C p) {
             const bool has_a = there(ida), has_b = there(idb);
             ida = id_of(t + 1, 0);
             idb = id_of(t + 1, 1);
-            // this tile's four per-lane K bases, opaque to the compiler: every K read
+            // this tile's per-lane K bases, opaque to the compiler: every K read
             // is then one of them plus an immediate offset (hoisting all 64
             // base + offset sums out of the loop would need 64 more registers)
             int kb[2][2];
 #pragma unroll
-            for (int bp = 0; bp < 2; ++bp)
+            for (int bp = 0; bp < (kWide ? 1 : 2); ++bp)
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
+                for (int hf = 0; hf < (kWide ? 1 : 2); ++hf) {
                     kb[bp][hf] = (t & 1) * kKStage + k_off[bp][hf];
                     asm volatile("" : "+v"(kb[bp][hf]));
                 }
-            // ---- S^T: sa[rg][kg][i] = S[key kt + 8g + 4kg + i][row n of group rg] ----
-            floatx4 sa[kRG][2];
+            // ---- S^T: the logits of the lane's keys in s --------------------------------
+            // K and d_k of a step are on their way while the one before multiplies (read at its start,
+            // every step waited for LDS: 1147 -> 1125 us for 2040 tokens behind 16000 shared keys). The
+            // value waves' reads, held to the start of their block in the same way, took 1163.
+            // The d_k scaling of a step runs while the next one's MFMAs execute. The scheduling barriers
+            // keep the compiler from pulling it back next to the MFMAs it reads (it did, leaving 4-12
+            // instructions between an MFMA and its consumer).
+            const float start = OPT && p.cap2 != 0.0f ? 0.0f : -mref;
+            float s[kV];  // base-2 logits
+            if constexpr (kWide) {
+                // a step is a block: two chunks, hi and lo, on one sum
+                float sa[16];
+                Tile cp;
 #pragma unroll
-            for (int rg = 0; rg < kRG; ++rg) sa[rg][0] = sa[rg][1] = OPT && p.cap2 != 0.0f ? 0.0f : -mref[rg];
-            // d_k of the lane's four C rows 16kg + 4g + i, block b: 8 bytes at
-            // Dk[b][16kg + 4g]
-            const uint8_t *dkb = smem + (t & 1) * kKStage + kOffDk + 8 * g;
-            // Software-pipelined by one step: step j = (block j >> 1, key group j & 1)
-            // issues its MFMAs, then the d_k scaling of step j - 1 runs while they
-            // execute. The scheduling barrier keeps the compiler from pulling the
-            // scaling back next to the MFMAs it reads (it did, leaving 4-12
-            // instructions between an MFMA and its consumer). The sum into sa keeps
-            // the block order of the plain loop.
-            // K and d_k of step j + 1 are on their way while step j multiplies (read at its start, every
-            // step waited for LDS: 1147 -> 1125 us for 2040 tokens behind 16000 shared keys). The value
-            // waves' reads, held to the start of their block in the same way, took 1163.
-            floatx4 cp[kRG];
-            uint2 dkp, dkn;
-            half8 akn;
-            auto load = [&](int j) {
-                const int b = j >> 1, kg = j & 1, o = kg * 8192 + 128 * (b >> 1);
-                akn = lds_half8(smem, kb[b & 1][0] + o, kb[b & 1][1] + o);
-                dkn = *reinterpret_cast<const uint2 *>(dkb + 64 * b + 32 * kg);
-            };
-            load(0);
+                for (int i = 0; i < 16; ++i) sa[i] = start;
+                // d_k of all blocks, the lane's key that of value lane & 15: the sums take it from there
+                half8 an[2], dkh;
+                float dk[8];
+                auto load = [&](int b) {
 #pragma unroll
-            for (int j = 0; j <= 16; ++j) {
-                floatx4 cn[kRG];
-                uint2 dkj;
-                if (j < 16) {
-                    const int b = j >> 1;
-                    const half8 ak = akn;
-                    dkj = dkn;
-                    if (j < 15) load(j + 1);
-                    __builtin_amdgcn_sched_barrier(0);
+                    for (int m = 0; m < 2; ++m)
+                        an[m] = lds_half8(smem, kb[0][0] + 64 * b + 32 * m, kb[0][0] + 64 * b + 32 * m + 8);
+                };
+                load(0);
+                dkh = *reinterpret_cast<const half8 *>(smem + (t & 1) * kKStage + dk_off);
 #pragma unroll
-                    for (int rg = 0; rg < kRG; ++rg) {
-                        const floatx4 c = __builtin_amdgcn_mfma_f32_16x16x32_f16(ak, bqh[rg][b],
-                                                                                 floatx4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-                        cn[rg] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ak, bql[rg][b], c, 0, 0, 0);
+                for (int b = 0; b <= 8; ++b) {
+                    Tile c = 0.0f;
+                    half8 a0, a1;
+                    if (b < 8) {
+                        a0 = an[0], a1 = an[1];
+                        if (b < 7) load(b + 1);
+                        __builtin_amdgcn_sched_barrier(0);
                     }
-                }
-                __builtin_amdgcn_sched_barrier(0);
-                if (j > 0) {
-                    const int kg = (j - 1) & 1;
-                    _Float16 dk[4];
-                    __builtin_memcpy(dk, &dkp, 8);
+                    // between two MFMAs four of the sums of the block before
+                    auto step = [&](auto k_) {
+                        constexpr int k = decltype(k_)::value;
+                        if (b < 8) c = __builtin_amdgcn_mfma_f32_32x32x16_f16(k < 2 ? a0 : a1, (k & 1 ? bql : bqh)[2 * b + (k >> 1)], c, 0, 0, 0);
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (b > 0) add_scaled<k>(sa, cp[4 * k], cp[4 * k + 1], cp[4 * k + 2], cp[4 * k + 3], dk[b - 1]);
+                    };
+                    step(std::integral_constant<int, 0>{});
+                    step(std::integral_constant<int, 1>{});
+                    step(std::integral_constant<int, 2>{});
+                    step(std::integral_constant<int, 3>{});
+                    if (b == 0) {
 #pragma unroll
-                    for (int rg = 0; rg < kRG; ++rg)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) sa[rg][kg][i] = fmaf(cp[rg][i], (float)dk[i], sa[rg][kg][i]);
+                        for (int i = 0; i < 8; ++i) {
+                            dk[i] = (float)dkh[i];
+                            asm volatile("" : "+v"(dk[i]));
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    cp = c;
+                    // the expansion of the next K tile goes between the MFMAs (the value waves do the first)
+                    if (kScoreK && b == 0) ex.read_k(smem, t + 1);
+                    if (kScoreK && b >= 4 && b < 8) ex.store_k(smem, t + 1, b - 4);
                 }
-                if (j < 16) {
-                    dkp = dkj;
 #pragma unroll
-                    for (int rg = 0; rg < kRG; ++rg) cp[rg] = cn[rg];
+                for (int jj = 0; jj < kV; ++jj) s[jj] = sa[jj];
+            } else {
+                // step j is (block j >> 1, key group j & 1): sa[kg][i] of key 8g + 4kg + i
+                Tile sa[2];
+                sa[0] = sa[1] = start;
+                // d_k of the lane's four C rows 16kg + 4g + i, block b: 8 bytes at Dk[b][16kg + 4g]
+                const uint8_t *dkb = smem + (t & 1) * kKStage + kOffDk + 8 * g;
+                Tile cp;
+                uint2 dkp, dkn;
+                half8 akn;
+                auto load = [&](int j) {
+                    const int b = j >> 1, kg = j & 1, o = kg * 8192 + 128 * (b >> 1);
+                    akn = lds_half8(smem, kb[b & 1][0] + o, kb[b & 1][1] + o);
+                    dkn = *reinterpret_cast<const uint2 *>(dkb + 64 * b + 32 * kg);
+                };
+                load(0);
+#pragma unroll
+                for (int j = 0; j <= 16; ++j) {
+                    Tile cn;
+                    uint2 dkj;
+                    if (j < 16) {
+                        const int b = j >> 1;
+                        const half8 ak = akn;
+                        dkj = dkn;
+                        if (j < 15) load(j + 1);
+                        __builtin_amdgcn_sched_barrier(0);
+                        cn = __builtin_amdgcn_mfma_f32_16x16x32_f16(ak, bqh[b], Tile(0.0f), 0, 0, 0);
+                        cn = __builtin_amdgcn_mfma_f32_16x16x32_f16(ak, bql[b], cn, 0, 0, 0);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (j > 0) {
+                        const int kg = (j - 1) & 1;
+                        _Float16 dk[4];
+                        __builtin_memcpy(dk, &dkp, 8);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) sa[kg][i] = fmaf(cp[i], (float)dk[i], sa[kg][i]);
+                    }
+                    if (j < 16) dkp = dkj, cp = cn;
+                    if (kScoreK && j == 0) ex.read_k(smem, t + 1);
+                    if (kScoreK && j >= 8 && j < 16 && j % 2 == 0) ex.store_k(smem, t + 1, (j - 8) / 2);
                 }
-                // the expansion of the next K tile goes between the MFMAs (the value waves do the first)
-                if (kScoreK && j == 0) ex.read_k(smem, t + 1);
-                if (kScoreK && j >= 8 && j < 16 && j % 2 == 0) ex.store_k(smem, t + 1, (j - 8) / 2);
+#pragma unroll
+                for (int jj = 0; jj < kV; ++jj) s[jj] = sa[jj >> 2][jj & 3];
             }
-            float s[kRG][8];  // keys 8g + jj, base-2 logits
+            if (OPT || kWide) {
+                // the scaled sums before what follows (the compiler moved some behind the cap, and
+                // kept 64 products alive till there)
 #pragma unroll
-            for (int rg = 0; rg < kRG; ++rg)
-#pragma unroll
-                for (int jj = 0; jj < 8; ++jj) s[rg][jj] = sa[rg][jj >> 2][jj & 3];
-            if (OPT) {
-                // one row group after the other (both at once need more registers than there
-                // are), and the scaled sums before (the compiler moved those of the second
-                // group behind the first one's cap, and kept 64 products alive till there)
-#pragma unroll
-                for (int rg = 0; rg < kRG; ++rg)
-#pragma unroll
-                    for (int jj = 0; jj < 8; ++jj) asm volatile("" : "+v"(s[rg][jj]));
-#pragma unroll
-                for (int rg = 0; rg < kRG; ++rg) {
-                    __builtin_amdgcn_sched_barrier(0);
-                    if (p.cap2 != 0.0f) cap_logits(s[rg], p.cap2, p.cap_inv, -mref[rg]);
-                    if (p.bias != 0.0f) {
-                        const float far = (float)(my_pos[rg] - (kt + 8 * g));
-#pragma unroll
-                        for (int jj = 0; jj < 8; ++jj) s[rg][jj] = fmaf(-my_slope[rg], fabsf(far - (float)jj), s[rg][jj]);
-                    }
-                }
+                for (int jj = 0; jj < kV; ++jj) asm volatile("" : "+v"(s[jj]));
                 __builtin_amdgcn_sched_barrier(0);
+            }
+            if (OPT) {
+#pragma unroll
+                for (int u = 0; u < kRG; ++u) {  // eight by eight: all at once need more registers than there are
+                    float (&x)[8] = *reinterpret_cast<float (*)[8]>(s + 8 * u);
+                    if (p.cap2 != 0.0f) cap_logits(x, p.cap2, p.cap_inv, -mref);
+                    if (p.bias != 0.0f) {
+                        const float far = (float)(my_pos - (kt + 16 * u + 8 * g));
+#pragma unroll
+                        for (int jj = 0; jj < 8; ++jj) x[jj] = fmaf(-my_slope, fabsf(far - (float)jj), x[jj]);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
             // ---- causal limit, prefix, last key, pages that are not there: whatever the
             // logit is, NaN of garbage bytes too
             if (kt + kPK > see_all || !has_a || !has_b) {
-                const bool has = g < 2 ? has_a : has_b;  // lanes' keys 8g..8g+7
 #pragma unroll
-                for (int rg = 0; rg < kRG; ++rg) {
-                    const int see = has ? min(my_see[rg], k_end) - (kt + 8 * g) : 0;
+                for (int u = 0; u < kRG; ++u) {
+                    const bool has = (kWide ? u == 0 : g < 2) ? has_a : has_b;
+                    const int see = has ? min(my_see, k_end) - (kt + 16 * u + 8 * g) : 0;
 #pragma unroll
-                    for (int jj = 0; jj < 8; ++jj) s[rg][jj] = jj < see ? s[rg][jj] : -INFINITY;
+                    for (int jj = 0; jj < 8; ++jj) s[8 * u + jj] = jj < see ? s[8 * u + jj] : -INFINITY;
                 }
             }
             // ---- online softmax (base 2); P and the rescale factors to LDS -----------
             uint8_t *pb = smem + kLdsP + (t & 1) * kPBuf + p_off;
-            float *ab = reinterpret_cast<float *>(smem + kLdsA + (t & 1) * kABuf) + w * (kRG * 16);
+            float *ab = reinterpret_cast<float *>(smem + kLdsA + (t & 1) * kABuf) + w * kN;
+            // lazy maximum: the reference moves only when a logit passes it by more
+            // than ks, so P <= 2^ks and most tiles need no rescale of O
+            float alpha = 1.0f;
+            int moved = 0;
+            bool over = false;
 #pragma unroll
-            for (int rg = 0; rg < kRG; ++rg) {
-                // lazy maximum: the reference moves only when a logit passes it by more
-                // than ks, so P <= 2^ks and most tiles need no rescale of O
-                float alpha = 1.0f;
-                bool over = false;
+            for (int jj = 0; jj < kV; ++jj) over |= s[jj] > lim_s;
+            if (__any(over)) {
+                float mt = s[0];
 #pragma unroll
-                for (int jj = 0; jj < 8; ++jj) over |= s[rg][jj] > lim_s[rg];
-                if (__any(over)) {
-                    float mt = fmaxf(fmaxf(fmaxf(s[rg][0], s[rg][1]), fmaxf(s[rg][2], s[rg][3])),
-                                     fmaxf(fmaxf(s[rg][4], s[rg][5]), fmaxf(s[rg][6], s[rg][7])));
-                    mt = xmax16(mt);
-                    mt = xmax32(mt);
-                    const float m_new = fmaxf(m_run[rg], mt + mref[rg]);
-                    alpha = m_run[rg] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run[rg] - m_new);
-                    l_part[rg] *= alpha;
-                    m_run[rg] = m_new;
-                    // onto the new reference: s - mref_new = s' + (mref - mref_new)
-                    const float mref_new = (m_new == -INFINITY ? 0.0f : m_new) - (float)kEp;
-                    const float d = mref[rg] - mref_new;
+                for (int jj = 1; jj < kV; ++jj) mt = fmaxf(mt, s[jj]);
+                if (!kWide) mt = xmax16(mt);
+                mt = xmax32(mt);
+                const float m_new = fmaxf(m_run, mt + mref);
+                alpha = m_run == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m_run - m_new);
+                l_part *= alpha;
+                moved = 1;
+                m_run = m_new;
+                // onto the new reference: s - mref_new = s' + (mref - mref_new)
+                const float mref_new = (m_new == -INFINITY ? 0.0f : m_new) - (float)kEp;
+                const float d = mref - mref_new;
 #pragma unroll
-                    for (int jj = 0; jj < 8; ++jj) s[rg][jj] += d;
-                    mref[rg] = mref_new;
-                    lim_s[rg] = m_new == -INFINITY ? -INFINITY : lim_top;
-                }
+                for (int jj = 0; jj < kV; ++jj) s[jj] += d;
+                mref = mref_new;
+                lim_s = m_new == -INFINITY ? -INFINITY : lim_top;
+            }
+#pragma unroll
+            for (int u = 0; u < kRG; ++u) {
                 float pf[8], psum = 0.0f;
 #pragma unroll
                 for (int jj = 0; jj < 8; ++jj) {
-                    pf[jj] = __builtin_amdgcn_exp2f(s[rg][jj]);
+                    pf[jj] = __builtin_amdgcn_exp2f(s[8 * u + jj]);
                     psum += pf[jj];
                 }
-                l_part[rg] += psum;
+                l_part += psum;
                 // P as an fp16 hi + lo pair (22 bits): the value waves form P d_v from it
                 half8 ph, pl;
 #pragma unroll
@@ -591,42 +674,43 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(C p) {
                 __builtin_memcpy(hw, &ph, 16);
 #pragma unroll
                 for (int jj = 0; jj < 8; ++jj) {
-                    float r;
+                    float x;
                     if (jj & 1)
-                        asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel:[0,0,1] op_sel_hi:[0,0,1]" : "=v"(r) : "v"(pf[jj]), "v"(hw[jj >> 1]));
+                        asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel:[0,0,1] op_sel_hi:[0,0,1]" : "=v"(x) : "v"(pf[jj]), "v"(hw[jj >> 1]));
                     else
-                        asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel:[0,0,0] op_sel_hi:[0,0,1]" : "=v"(r) : "v"(pf[jj]), "v"(hw[jj >> 1]));
-                    pl[jj] = (_Float16)r;
+                        asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel:[0,0,0] op_sel_hi:[0,0,1]" : "=v"(x) : "v"(pf[jj]), "v"(hw[jj >> 1]));
+                    pl[jj] = (_Float16)x;
                 }
-                *reinterpret_cast<half8 *>(pb + rg * 2048) = ph;
-                *reinterpret_cast<half8 *>(pb + rg * 2048 + 1024) = pl;
-                if (g == 0) ab[rg * 16 + n] = alpha;
+                *reinterpret_cast<half8 *>(pb + u * 2048) = ph;
+                *reinterpret_cast<half8 *>(pb + u * 2048 + 1024) = pl;
             }
+            if (g == 0) ab[n] = alpha;
+            if (lane == 0) *reinterpret_cast<int *>(smem + kLdsF + 16 * (t & 1) + 4 * w) = moved;
         }
         // ---- hand m and l of the rows to the value waves ----------------------------
         __syncthreads();
         if (n_tiles > 0) {
-#pragma unroll
-            for (int rg = 0; rg < kRG; ++rg) {
-                float lp = l_part[rg];
-                lp += __shfl_xor(lp, 16);
-                lp += __shfl_xor(lp, 32);
-                if (g == 0) {
-                    ml[rg * 32 + 2 * n] = m_run[rg];
-                    ml[rg * 32 + 2 * n + 1] = lp;
-                }
+            if (!kWide) l_part += __shfl_xor(l_part, 16);
+            l_part += __shfl_xor(l_part, 32);
+            if (g == 0) {
+                ml[2 * n] = m_run;
+                ml[2 * n + 1] = l_part;
             }
         }
         __syncthreads();
         return;
     }
 
-    // ---- value waves: O[row 16 kRG w + 16rg + 4g + i][dim 16T + n] ----------------
+    // ---- value waves: O[row kN w + 8 (k >> 2) + 4g + (k & 3)][dim kN T + n] in acc[T][k] ----------
     const int w = wave - kScoreWaves;
-    const float *ml = reinterpret_cast<const float *>(smem + kLdsP) + w * (kRG * 32);  // [rg][row][m, l]
-    // V operand of dim 16T + n, keys 8g..8g+7: chunk g ^ ((n >> 1) & 3), halves swapped when n & 8.
-    const int v_off0 = 64 * n + 16 * (g ^ ((n >> 1) & 3)) + 8 * nh;
-    const int v_off1 = v_off0 ^ 8;
+    const float *ml = reinterpret_cast<const float *>(smem + kLdsP) + w * (kN * 2);  // [row][m, l]
+    // V operand of dim kN T + n, keys 8g..8g+7: chunk g ^ v_swap, halves swapped when n & 8; of keys
+    // 16 + 8g..: chunk 2 + g
+    int v_off[kRG][2];
+#pragma unroll
+    for (int u = 0; u < kRG; ++u)
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) v_off[u][hf] = 64 * n + 16 * ((2 * u + g) ^ v_swap<kWide>(n)) + 8 * (hf ^ nh);
     const int p_off = w * (kRG * 2048) + 16 * lane;
     // DMA: wave w moves 16 rows of a tile, group w & 1, of K (w < 2) or V. They lie on
     // one page: 9 x 16 bytes a row as two instructions of 64 lanes and one of 16.
@@ -651,7 +735,7 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(C p) {
     // ids of the groups of tiles t, t + 1, t + 2
     int a0 = id_of(0, 0), b0 = id_of(0, 1), a1 = id_of(1, 0), b1 = id_of(1, 1), a2 = id_of(2, 0), b2 = id_of(2, 1);
     auto mine = [&](int a, int b) { return w & 1 ? b : a; };
-    Expand ex;
+    Expand<kWide> ex;
     ex.init(w, lane);
     int e_own = kMaxE;                            // of this wavefront's pair of blocks, up to the tile expanded last
     int4 e_acc = make_int4(kMaxE, kMaxE, kMaxE, kMaxE);  // of O's pairs
@@ -674,11 +758,9 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(C p) {
         ex.store_v(smem, 0, 0);
         ex.store_v(smem, 0, 1);
     }
-    floatx4 acc[kRG][16];
+    Tile acc[kT];
 #pragma unroll
-    for (int rg = 0; rg < kRG; ++rg)
-#pragma unroll
-        for (int T = 0; T < 16; ++T) acc[rg][T] = floatx4{0.f, 0.f, 0.f, 0.f};
+    for (int T = 0; T < kT; ++T) acc[T] = 0.0f;
     // (behind the last tile the expansion works on bytes that are there, into stages that
     // nobody reads any more)
     for (int t = 0; t <= n_tiles && n_tiles > 0; ++t) {
@@ -694,31 +776,36 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(C p) {
         if (t == 0) continue;
         const int tp = t - 1;
         const uint8_t *vs = smem + kLdsV + (tp & 1) * kVStage;
-        // this tile's two per-lane V bases, opaque to the compiler (see the K reads)
-        int vb0 = kLdsV + (tp & 1) * kVStage + v_off0, vb1 = kLdsV + (tp & 1) * kVStage + v_off1;
-        asm volatile("" : "+v"(vb0), "+v"(vb1));
+        // this tile's per-lane V bases, opaque to the compiler (see the K reads)
+        int vb[kRG][2];
+#pragma unroll
+        for (int u = 0; u < kRG; ++u)
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                vb[u][hf] = kLdsV + (tp & 1) * kVStage + v_off[u][hf];
+                asm volatile("" : "+v"(vb[u][hf]));
+            }
         const uint8_t *pb = smem + kLdsP + (tp & 1) * kPBuf + p_off;
-        const float *ab = reinterpret_cast<const float *>(smem + kLdsA + (tp & 1) * kABuf) + w * (kRG * 16);
+        const float *ab = reinterpret_cast<const float *>(smem + kLdsA + (tp & 1) * kABuf) + w * kN + 4 * g;
         // O onto the exponents of this tile's V scales where a larger one has come
         int4 e_t = *reinterpret_cast<const int4 *>(smem + kLdsE + 16 * (tp & 1));
         e_t.x = __builtin_amdgcn_readfirstlane(e_t.x), e_t.y = __builtin_amdgcn_readfirstlane(e_t.y);
         e_t.z = __builtin_amdgcn_readfirstlane(e_t.z), e_t.w = __builtin_amdgcn_readfirstlane(e_t.w);
-        half8 ph[kRG], pl[kRG];
-        bool resc = false;
+        half8 ph[kRG], pl[kRG];  // of the lane's row n
+        const int resc = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const int *>(smem + kLdsF + 16 * (tp & 1) + 4 * w));
 #pragma unroll
-        for (int rg = 0; rg < kRG; ++rg) {
-            // rescale factors of rows 4g..4g+3: exactly 1 unless a maximum moved
-            const floatx4 a4 = *reinterpret_cast<const floatx4 *>(ab + rg * 16 + 4 * g);
-            resc |= (a4[0] != 1.0f) | (a4[1] != 1.0f) | (a4[2] != 1.0f) | (a4[3] != 1.0f);
-            ph[rg] = *reinterpret_cast<const half8 *>(pb + rg * 2048);
-            pl[rg] = *reinterpret_cast<const half8 *>(pb + rg * 2048 + 1024);
+        for (int u = 0; u < kRG; ++u) {
+            ph[u] = *reinterpret_cast<const half8 *>(pb + u * 2048);
+            pl[u] = *reinterpret_cast<const half8 *>(pb + u * 2048 + 1024);
         }
-        if (__any(resc)) {  // rare with the lazy maximum: O = alpha O
+        if (resc) {  // rare with the lazy maximum: O = alpha O, alpha of rows 8q + 4g .. + 3
 #pragma unroll
-            for (int rg = 0; rg < kRG; ++rg) {
-                const floatx4 a4 = *reinterpret_cast<const floatx4 *>(ab + rg * 16 + 4 * g);
+            for (int q = 0; q < kR / 4; ++q) {
+                const floatx4 a4 = *reinterpret_cast<const floatx4 *>(ab + 8 * q);
 #pragma unroll
-                for (int T = 0; T < 16; ++T) acc[rg][T] *= a4;
+                for (int T = 0; T < kT; ++T)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[T][4 * q + i] *= a4[i];
             }
         }
         if ((e_t.x ^ e_acc.x) | (e_t.y ^ e_acc.y) | (e_t.z ^ e_acc.z) | (e_t.w ^ e_acc.w)) {
@@ -727,32 +814,32 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(C p) {
             for (int q = 0; q < 4; ++q) {
                 const float f = __builtin_amdgcn_ldexpf(1.0f, to[q] - from[q]);
 #pragma unroll
-                for (int rg = 0; rg < kRG; ++rg)
-#pragma unroll
-                    for (int T = 4 * q; T < 4 * q + 4; ++T) acc[rg][T] *= f;
+                for (int T = kT / 4 * q; T < kT / 4 * (q + 1); ++T) acc[T] *= f;
             }
             e_acc = e_t;
         }
         // d_v and V of block b + 1 are read while block b computes: the LDS latency stays
         // off the MFMA chain. Between the blocks, parts of the next tiles' expansion.
-        uint4 dvn = *reinterpret_cast<const uint4 *>(vs + kOffDv + 16 * g);
-        half8 bvn[2];
+        half8 dvn[kRG], bvn[2];
+        auto load = [&](int b) {
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) bvn[hf] = lds_half8(smem, vb0 + 1024 * hf, vb1 + 1024 * hf);
+            for (int u = 0; u < kRG; ++u) dvn[u] = *reinterpret_cast<const half8 *>(vs + kOffDv + 64 * b + 32 * u + 16 * g);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {  // the block's 32 dims for 16 keys each, or two times 16 dims
+                const int u = kWide ? k : 0, o = 2048 * b + (kWide ? 0 : 1024 * k);
+                bvn[k] = lds_half8(smem, vb[u][0] + o, vb[u][1] + o);
+            }
+        };
+        load(0);
         ex.read_v(smem, t);
         if (!kScoreK) ex.read_k(smem, t + 1);
 #pragma unroll
         for (int b = 0; b < 8; ++b) {
             const half8 bv[2] = {bvn[0], bvn[1]};
-            const uint4 dvr = dvn;
-            if (b < 7) {
-                dvn = *reinterpret_cast<const uint4 *>(vs + kOffDv + 64 * (b + 1) + 16 * g);
+            half8 dv[kRG];
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf)
-                    bvn[hf] = lds_half8(smem, vb0 + 1024 * (2 * b + 2 + hf), vb1 + 1024 * (2 * b + 2 + hf));
-            }
-            half8 dvb;
-            __builtin_memcpy(&dvb, &dvr, 16);
+            for (int u = 0; u < kRG; ++u) dv[u] = dvn[u];
+            if (b < 7) load(b + 1);
             // A = P 2^ep d_v as an fp16 hi + lo pair (22 bits): the products with the
             // exact V codes are then exact in fp32, so a row that a few keys
             // dominate carries no fp16 rounding of P d_v into its output. Ph d_v has
@@ -761,21 +848,22 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(C p) {
             // rounds once.
             half8 ah[kRG], al[kRG];
 #pragma unroll
-            for (int rg = 0; rg < kRG; ++rg) {
-                ah[rg] = ph[rg] * dvb;
-                const half8 r = __builtin_elementwise_fma(ph[rg], dvb, -ah[rg]);
-                al[rg] = __builtin_elementwise_fma(pl[rg], dvb, r);
+            for (int u = 0; u < kRG; ++u) {
+                ah[u] = ph[u] * dv[u];
+                const half8 x = __builtin_elementwise_fma(ph[u], dv[u], -ah[u]);
+                al[u] = __builtin_elementwise_fma(pl[u], dv[u], x);
             }
+            if constexpr (kWide) {
+                acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[0], bv[0], acc[b], 0, 0, 0);
+                acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[1], bv[1], acc[b], 0, 0, 0);
+                acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[0], bv[0], acc[b], 0, 0, 0);
+                acc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[1], bv[1], acc[b], 0, 0, 0);
+            } else {
 #pragma unroll
-            for (int rg = 0; rg < kRG; ++rg)
+                for (int hf = 0; hf < 2; ++hf) acc[2 * b + hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[0], bv[hf], acc[2 * b + hf], 0, 0, 0);
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf)
-                    acc[rg][2 * b + hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[rg], bv[hf], acc[rg][2 * b + hf], 0, 0, 0);
-#pragma unroll
-            for (int rg = 0; rg < kRG; ++rg)
-#pragma unroll
-                for (int hf = 0; hf < 2; ++hf)
-                    acc[rg][2 * b + hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(al[rg], bv[hf], acc[rg][2 * b + hf], 0, 0, 0);
+                for (int hf = 0; hf < 2; ++hf) acc[2 * b + hf] = __builtin_amdgcn_mfma_f32_16x16x32_f16(al[0], bv[hf], acc[2 * b + hf], 0, 0, 0);
+            }
             if (b == 1) scales(t, x0, y0);
             if (b == 2) ex.store_v(smem, t, 0);
             if (b == 3) ex.store_v(smem, t, 1);
@@ -785,44 +873,43 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(C p) {
     __syncthreads();  // m and l of the rows ...
     __syncthreads();  // ... are in LDS
     const int e_out[4] = {-e_acc.x, -e_acc.y, -e_acc.z, -e_acc.w};
-    // rows 16 kRG w + 16 rg + 4g + i, one after the other; the gate of the next one is on
-    // its way while a row goes out
-    auto token_of = [&](int k, int *h) {  // k = 4 rg + i
-        const int r = 16 * kRG * w + 16 * (k >> 2) + 4 * g + (k & 3), tok = group_of(p, r);
+    // the lane's rows, one after the other; the gate of the next one is on its way while a row goes out
+    auto row_at = [&](int k) { return 8 * (k >> 2) + 4 * g + (k & 3); };
+    auto token_of = [&](int k, int *h) {
+        const int r = kN * w + row_at(k), tok = group_of(p, r);
         *h = kvh * p.G + r - tok * p.G;
         return q_base + tok;
     };
     float *dst = p.dst;
     if constexpr (kPart) dst = p.whole;
-    float gv[2][16];
-    auto load_gate = [&](int k, float (&x)[16]) {
+    float gv[2][kT];
+    auto load_gate = [&](int k, float (&x)[kT]) {
         int h;
         const int tok = token_of(k, &h);
         if (tok < q_top) {
             const float *from = reinterpret_cast<const float *>(p.gate + (int64_t)(rq.q0 + tok) * p.gate_nb2 + h * p.gate_nb1) + n;
 #pragma unroll
-            for (int T = 0; T < 16; ++T) x[T] = from[16 * T];
+            for (int T = 0; T < kT; ++T) x[T] = from[kN * T];
         }
     };
     if (!kPart && whole && p.gate) load_gate(0, gv[0]);
 #pragma unroll
-    for (int k = 0; k < 4 * kRG; ++k) {
-        const int rg = k >> 2, i = k & 3, r = 16 * kRG * w + 16 * rg + 4 * g + i;
-        if (!kPart && whole && p.gate && k + 1 < 4 * kRG) load_gate(k + 1, gv[(k + 1) & 1]);
+    for (int k = 0; k < kR; ++k) {
+        if (!kPart && whole && p.gate && k + 1 < kR) load_gate(k + 1, gv[(k + 1) & 1]);
         int h;
         const int tok = token_of(k, &h);
         if (tok >= q_top) continue;
-        const float mrow = n_tiles > 0 ? ml[rg * 32 + 2 * (4 * g + i)] : -INFINITY;
-        const float lrow = n_tiles > 0 ? ml[rg * 32 + 2 * (4 * g + i) + 1] : 0.0f;
+        const float mrow = n_tiles > 0 ? ml[2 * row_at(k)] : -INFINITY;
+        const float lrow = n_tiles > 0 ? ml[2 * row_at(k) + 1] : 0.0f;
         if (whole) {
             const float inv = lrow == 0.0f ? 0.0f : 1.0f / lrow;
             float *to = dst + ((int64_t)(rq.q0 + tok) * p.H + h) * kHeadDim + n;
-            float o[16];
+            float o[kT];
 #pragma unroll
-            for (int T = 0; T < 16; ++T) o[T] = __builtin_amdgcn_ldexpf(acc[rg][T][i], e_out[T >> 2]) * inv;
+            for (int T = 0; T < kT; ++T) o[T] = __builtin_amdgcn_ldexpf(acc[T][k], e_out[T / (kT / 4)]) * inv;
             if (!kPart && p.gate) {
 #pragma unroll
-                for (int T = 0; T < 16; ++T) o[T] = gate_by(o[T], gv[k & 1][T]);
+                for (int T = 0; T < kT; ++T) o[T] = gate_by(o[T], gv[k & 1][T]);
             }
             if constexpr (kPart)
                 if (n == 0) {
@@ -831,12 +918,12 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(C p) {
                     store_through(ml_to + 1, lrow);
                 }
 #pragma unroll
-            for (int T = 0; T < 16; ++T) store_through(to + 16 * T, o[T]);
+            for (int T = 0; T < kT; ++T) store_through(to + kN * T, o[T]);
         } else {
-            const int64_t at = (int64_t)slot * rows_per_wg(kRG) + r;
+            const int64_t at = (int64_t)slot * rows_per_wg(kRG) + kN * w + row_at(k);
 #pragma unroll
-            for (int T = 0; T < 16; ++T)
-                store_through(p.acc_c + at * kHeadDim + 16 * T + n, __builtin_amdgcn_ldexpf(acc[rg][T][i], e_out[T >> 2]));
+            for (int T = 0; T < kT; ++T)
+                store_through(p.acc_c + at * kHeadDim + kN * T + n, __builtin_amdgcn_ldexpf(acc[T][k], e_out[T / (kT / 4)]));
             if (n == 0) {
                 // (acc and l of every split carry the same 2^kEp, which cancels in the merge; a
                 // row of NaN has seen keys, though none of them moved its maximum)
