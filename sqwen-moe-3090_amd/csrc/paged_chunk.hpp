@@ -7,19 +7,25 @@
 // wavefronts hold Q' (hi and lo) of 32 rows each and make the logits and P of tile t,
 // four value wavefronts hold O of the same rows and add P V of tile t - 1.
 //   S^T = sum over q4_0 blocks b of d_k[b] (Kc_b . Q'h_b + Kc_b . Q'l_b): exact codes as
-//   fp16 on v_mfma_f32_16x16x32_f16, Q' = q8_0(Q) * scale * log2(e) as an fp16 hi + lo
-//   pair, the scaling by d_k in fp32; softmax base 2 with a reference maximum that
-//   moves only when a logit passes it by kSlack; O += (P d_v) V with P d_v as an fp16
-//   hi + lo pair and exact codes.
+//   fp16 on v_mfma_f32_32x32x16_f16 (64 rows: 16x16x32), Q' = q8_0(Q) * scale * log2(e) as
+//   an fp16 hi + lo pair, the scaling by d_k in fp32; softmax base 2 with a reference
+//   maximum that moves only when a logit passes it by kSlack; O += (P d_v) V with P d_v as
+//   an fp16 hi + lo pair and exact codes.
+// The 32x32 tiles leave the vector unit more of their time than 16x16 ones (two wavefronts
+// with 8 fmas for every two 16x16x32: 21.4 ns a pair, for one 32x32x16 18.2), a lane holds one
+// row, and LDS serves them without conflicts. Cycles are 8% fewer; how much of that is time is
+// up to the card's power: 2040 tokens behind 16000 shared keys 1163 -> 1129 us on one card, as
+// long as before on another, 2048 behind 30001 2290 -> 2170 and 2264.
 //
 // There is no pre-pass: the contiguous kernel expands K and V into 2112 bytes per key
 // in its workspace, which for a batch would have to hold every request's keys. Here
 // the value wavefronts bring the q4_0 rows themselves into LDS (288 bytes per key and
 // head; a 16-key group lies on one page, so its id is one scalar load and its rows a
-// scalar base plus constant offsets) and expand them there for all 128 rows:
+// scalar base plus constant offsets), which are expanded there for all 128 rows, K by the
+// score and V by the value wavefronts between their MFMAs (K by the value wavefronts too:
+// 2200 us where this is 2170):
 //   iteration t: rows of K tile t + 2 and V tile t + 1 are on their way; K tile t + 1
 //   and V tile t are expanded; P V of tile t - 1.
-// (In a call of shared prefixes the score wavefronts expand K, between their MFMAs: kScoreK.)
 // K codes leave a dword of nibbles by shifts and masks alone: the 8 values of a chunk
 // are its dims in the order 0 2 16 18 1 3 17 19, and Q' is laid out in the same order.
 // V needs the codes of 8 keys side by side: 16-bit reads of 8 rows, packed in pairs.
@@ -29,9 +35,10 @@
 // A = P d_v stays below 2^14 and the parts that count stay clear of fp16's subnormals for
 // V of any size.
 //
-// Bound: the issue of vector (0.53 of the cycles) and matrix instructions (0.38), which add
-// up; exact products take two MFMAs for each useful one. 2048 tokens behind 30001, 16 heads
-// on 2 KV heads: 2.30 ms, 453 TFLOP/s, 2.4 us a tile of 128 x 32. A workgroup's start and
+// Bound: the issue of instructions by one wavefront of each kind a SIMD: vector 0.56 of the
+// cycles, matrix 0.43, both at once 0.23, LDS at work in 0.40. Exact products take two MFMAs for
+// each useful one; without any the tile still takes 0.64 of its time. 2048 tokens behind 30001, 16
+// heads on 2 KV heads: 2.17 ms, 480 TFLOP/s, 2.2 us a tile of 128 x 32. A workgroup's start and
 // end are 11 us that nothing overlaps (LDS holds one a CU): Q 2.7, its quantization 2.6,
 // the last tile 1.9, the result 3 to 4 (turned in LDS into whole rows it took 5).
 #pragma once
@@ -87,7 +94,8 @@ __device__ __forceinline__ float xmax32(float x) {
 }
 
 // sa[i] += c[i] * (dk of lane i of every 16 lanes), i = 4 K .. 4 K + 3: the multiplication reads the
-// other lane's register (the compiler makes a move of its own of that). The assembler's lines are
+// other lane's register (the compiler makes a move of its own of that; every lane reading all its
+// scales from LDS, 16 reads of 16 bytes a tile instead of one, took 3% longer). These lines are
 // no instructions to the compiler that read c, a matrix instruction's result: K = 0 has one of the
 // compiler's own before them, and its waits. s_nop: dk may have been written just before.
 template <int K>
@@ -360,11 +368,6 @@ __device__ __forceinline__ Item many_item(const C &c, int lin, int qb) {
 template <int kRG, bool OPT, class C>
 __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(C p) {
     constexpr bool kPart = kIsParts<C>;
-    // Who expands K: the score waves, between their MFMAs, or with the options, whose score waves have
-    // no registers left for it (spills: 45 us became 74), the value waves as they do V. Both tensors in
-    // the score waves: 1278 us where this is 1184 and all in the value waves 1231 (2040 tokens behind
-    // 16000 shared keys). (For a plain Call the compiler spills 67 registers in the score waves.)
-    constexpr bool kScoreK = kPart && !OPT;
     constexpr bool kWide = kRG == 2;
     constexpr int kN = 16 * kRG;          // rows of a wave, a lane's column of the matrix tiles
     constexpr int kV = 8 * kRG;           // keys of its row that a lane holds, 8 g .. 8 g + 7 (+ 16)
@@ -493,12 +496,10 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(C p) {
                     asm volatile("" : "+v"(kb[bp][hf]));
                 }
             // ---- S^T: the logits of the lane's keys in s --------------------------------
-            // K and d_k of a step are on their way while the one before multiplies (read at its start,
-            // every step waited for LDS: 1147 -> 1125 us for 2040 tokens behind 16000 shared keys). The
-            // value waves' reads, held to the start of their block in the same way, took 1163.
-            // The d_k scaling of a step runs while the next one's MFMAs execute. The scheduling barriers
-            // keep the compiler from pulling it back next to the MFMAs it reads (it did, leaving 4-12
-            // instructions between an MFMA and its consumer).
+            // K of a step is on its way while the one before multiplies (read at its start, every step
+            // waited for LDS: 2% more). The d_k scaling of a step runs while the next one's MFMAs execute;
+            // the scheduling barriers keep the compiler from pulling it back next to the MFMAs it reads (it
+            // did, leaving 4-12 instructions between an MFMA and its consumer).
             const float start = OPT && p.cap2 != 0.0f ? 0.0f : -mref;
             float s[kV];  // base-2 logits
             if constexpr (kWide) {
@@ -547,8 +548,8 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(C p) {
                     }
                     cp = c;
                     // the expansion of the next K tile goes between the MFMAs (the value waves do the first)
-                    if (kScoreK && b == 0) ex.read_k(smem, t + 1);
-                    if (kScoreK && b >= 4 && b < 8) ex.store_k(smem, t + 1, b - 4);
+                    if (b == 0) ex.read_k(smem, t + 1);
+                    if (b >= 4 && b < 8) ex.store_k(smem, t + 1, b - 4);
                 }
 #pragma unroll
                 for (int jj = 0; jj < kV; ++jj) s[jj] = sa[jj];
@@ -589,8 +590,8 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(C p) {
                         for (int i = 0; i < 4; ++i) sa[kg][i] = fmaf(cp[i], (float)dk[i], sa[kg][i]);
                     }
                     if (j < 16) dkp = dkj, cp = cn;
-                    if (kScoreK && j == 0) ex.read_k(smem, t + 1);
-                    if (kScoreK && j >= 8 && j < 16 && j % 2 == 0) ex.store_k(smem, t + 1, (j - 8) / 2);
+                    if (j == 0) ex.read_k(smem, t + 1);
+                    if (j >= 8 && j < 16 && j % 2 == 0) ex.store_k(smem, t + 1, (j - 8) / 2);
                 }
 #pragma unroll
                 for (int jj = 0; jj < kV; ++jj) s[jj] = sa[jj >> 2][jj & 3];
@@ -747,12 +748,9 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(C p) {
         issue(0, mine(a0, b0));
         if (w < 2 && n_tiles > 1) issue(1, mine(a1, b1));
         asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+        ex.read_k(smem, 0);
 #pragma unroll
-        for (int k = 0; k < (kScoreK ? 1 : 2); ++k) {
-            ex.read_k(smem, k);
-#pragma unroll
-            for (int m = 0; m < 4; ++m) ex.store_k(smem, k, m);
-        }
+        for (int m = 0; m < 4; ++m) ex.store_k(smem, 0, m);
         ex.read_v(smem, 0);
         scales(0, a0, b0);
         ex.store_v(smem, 0, 0);
@@ -832,7 +830,6 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(C p) {
         };
         load(0);
         ex.read_v(smem, t);
-        if (!kScoreK) ex.read_k(smem, t + 1);
 #pragma unroll
         for (int b = 0; b < 8; ++b) {
             const half8 bv[2] = {bvn[0], bvn[1]};
@@ -867,7 +864,7 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(C p) {
             if (b == 1) scales(t, x0, y0);
             if (b == 2) ex.store_v(smem, t, 0);
             if (b == 3) ex.store_v(smem, t, 1);
-            if (!kScoreK && b >= 4) ex.store_k(smem, t + 1, b - 4);
+            if (!b >= 4) ex.store_k(smem, t + 1, b - 4);
         }
     }
     __syncthreads();  // m and l of the rows ...
