@@ -99,15 +99,19 @@ __device__ __forceinline__ Request request(const Call &c, int b) {
     return r;
 }
 
-// Of entry b; a group's tokens are counted by their places among the members.
+// Of entry b; a group's tokens are counted by their places among the members. (Either's numbers come
+// by the same loads: one wait for lanes that hold both.)
 __device__ __forceinline__ Request request(const Parts &c, int b) {
-    if (!is_group(c, b)) return request(static_cast<const Call &>(c), b);
+    const bool group = is_group(c, b);
+    const int i = group ? b - c.B : b;
+    const int32_t *starts = group ? c.m_start : c.q_start, *lens = group ? c.g_len : c.kv_len;
+    const int s0 = starts[i], s1 = starts[i + 1], len = lens[i], prefix = c.prefix ? c.prefix[min(b, c.B - 1)] : 0;
     Request r;
-    const int g = b - c.B, s0 = c.m_start[g], s1 = c.m_start[g + 1], len = c.g_len[g];
-    r.prefix = INT32_MAX, r.pos0 = 0;
-    r.kv = (int)min((int64_t)max(len, 0), c.g_most_kv);
+    r.prefix = group ? INT32_MAX : prefix;
+    r.kv = (int)min((int64_t)max(len, 0), group ? c.g_most_kv : c.most_kv);
     r.q0 = min(max(s0, 0), c.n_tok);
-    r.n = r.kv ? min(max(s1, r.q0), c.n_tok) - r.q0 : 0;
+    r.n = group && !r.kv ? 0 : min(max(s1, r.q0), c.n_tok) - r.q0;
+    r.pos0 = group ? 0 : max(len, 0) - r.n;
     return r;
 }
 
