@@ -42,7 +42,9 @@ struct RowParts {
         const int4 w1 = c.where[t], w2 = c.g_where[t];
         const int g = p.token_group[t];
         if (t < c.q_start[0] || t >= c.q_start[c.B]) return false;  // the entry was not written
-        whole = (w1.w & 3) == kWhole;
+        // (where requests' ranges overlap, more of them than there are slots, an entry may be what the
+        // workspace held: there is no `whole` without the chunk kernel)
+        whole = c.rows_c && (w1.w & 3) == kWhole;
 #pragma unroll
         for (int k = 0; k < R; ++k) {
             const int h = min(h0 + k, c.H - 1);

@@ -370,3 +370,29 @@ def test_weights_keep_their_bits(sqa, orc, dev, B, n):
     b = Batch(orc, 19, [n] * B, [100] * B, [4096], [0] * B, page=64)
     got, want = call(sqa, dev, b), b.ref(orc)
     assert np.linalg.norm(got - want) <= 1e-6 * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("max_q", [1, 4, 40])
+def test_ranges_that_overlap_stay_inside(sqa, orc, dev, max_q):
+    """q_start that goes up and down, more requests than the workspace has slots for: unspecified rows, nothing else is
+    touched whatever the workspace held, later calls are right."""
+    b = Batch(orc, 20, [1, 2, 1, 40], [9, 30, 0, 5], [70, 20], [0, 1, 0, 1], pad=2)
+    a, _ = b.args(sqa, dev)
+    T, n = b.q.shape[0], 600
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    starts, lens = i32([0, 4] * (n // 2) + [0]), i32([40] * n)
+    starts[n] = T
+    table = a[3][:1].repeat(n, 1)
+    ws = torch.empty(sqa.paged_attn_shared_workspace_size(a[0], a[1], table, a[6], max_q), dtype=torch.uint8, device=dev)
+    guard = torch.full((T + 8, 16, D), 3.0, device=dev)
+    r = torch.Generator(device=dev).manual_seed(2)
+    for fill in (0xFF, None):
+        if fill is None:
+            ws.copy_(torch.randint(0, 256, ws.shape, generator=r, device=dev, dtype=torch.uint8))
+        else:
+            ws.fill_(fill)
+        share = sqa.paged_share(starts, lens, i32([0, 1, -1] * (n // 3)), a[7], torch.zeros(T, dtype=torch.int32, device=dev))
+        sqa.paged_attn_shared(a[0], a[1], a[2], table, starts, lens, a[6], a[7], share, max_q, out=guard[4:T + 4], workspace=ws)
+        torch.cuda.synchronize()
+        assert (guard[:4] == 3.0).all() and (guard[T + 4:] == 3.0).all()
+    close(call(sqa, dev, b), b.ref(orc))
