@@ -169,21 +169,23 @@ __device__ __forceinline__ half8 lds_half8(const uint8_t *base, int off_lo, int 
 }
 
 
-// The expansion of a tile by the 256 value lanes, in 9 parts that the wavefronts place
-// between the MFMAs of P V. Stores are 8 bytes, the halves of a 16-byte chunk at
-// addresses that differ in bit 3 (which first is a matter of the row: no selects).
+// The expansion of a tile, K by the 256 lanes of the score and V by those of the value wavefronts,
+// in parts that they place between their MFMAs. Stores are 8 bytes, the halves of a 16-byte chunk
+// at addresses that differ in bit 3 (which first is a matter of the row: no selects).
 //   K: lane takes block b of key k: k & 3, b & 3, k >> 4, b >> 2 from the lane's bits 0-1,
 //      2-3, 4, 5, the middle bits of k from the wavefront. Row r = key_row(k) of the
 //      stage, chunk 4b + m (dims 32b + 4m + {0, 2, 16, 18, 1, 3, 17, 19}) at
 //      (4b + m) ^ (r & 7), halves swapped when r & 8.
+//      32x32: k & 3, bit 3 of k, b & 3, b >> 2 from bits 0-1, 2, 3-4, 5, the others from the
+//      wavefront; rows of 520 bytes, chunk 4b + m at its place.
 //   V: lane takes bytes 4m + 2i, 4m + 2i + 1 of block b's codes for the keys 8c .. 8c + 7
 //      (c, i, m from the lane's bits 0-1, 2, 3-4, b = 2w + bit 5) and stores those keys'
-//      chunk of the bytes' 4 dims, chunk c of dim d at c ^ ((d >> 1) & 3), halves
+//      chunk of the bytes' 4 dims, chunk c of dim d at c ^ v_swap(d), halves
 //      swapped when d & 8; odd m the second byte first.
 //   V scales: lane takes key lane & 31 of block 2w + (lane >> 5).
 // With these maps the 32 lanes that LDS serves at a time store to 32 different pairs of
 // banks (lanes over whole rows of K and over all blocks of V met in 16 of them 16 deep:
-// 3260 LDS cycles a tile, 56% of them conflicts).
+// 3260 LDS cycles a tile, 56% of them conflicts; now 1800, 27%, of the reads of raw rows).
 template <bool kWide>
 struct Expand {
     int k_raw, k_sh, k_to, dk_raw, dk_to;   // LDS offsets in the first of two buffers
@@ -864,7 +866,6 @@ __global__ __launch_bounds__(kThreads, 1) void paged_many_kernel(C p) {
             if (b == 1) scales(t, x0, y0);
             if (b == 2) ex.store_v(smem, t, 0);
             if (b == 3) ex.store_v(smem, t, 1);
-            if (!b >= 4) ex.store_k(smem, t + 1, b - 4);
         }
     }
     __syncthreads();  // m and l of the rows ...
