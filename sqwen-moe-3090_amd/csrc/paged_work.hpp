@@ -79,7 +79,7 @@ constexpr int kCounted = 64, kLevels = 8, kRounds = 4;
 // Groups of a shared prefix are requests whose tokens all see all keys and whose parts all go
 // through the merge.
 //
-// Run by all 512 threads of one workgroup; lds: 512 + 6 * 2600 + 1 words, or 512 + B + 1.
+// Run by all 512 threads of one workgroup; lds: 513 + 7 * 2300 words, or 512 + B + 1.
 // Lanes are requests (a run of them above 512), then lengths that are tried, then items.
 template <class C>
 __device__ __forceinline__ void plan_chunks(const C &c, int *lds) {
@@ -90,8 +90,10 @@ __device__ __forceinline__ void plan_chunks(const C &c, int *lds) {
     Item *list = reinterpret_cast<Item *>(c.work + kListAt);
     int *sums = lds, *start = lds + 512;                      // start: first item of every request
     Request *known = reinterpret_cast<Request *>(start + E + 1);
+    int *slot_of = reinterpret_cast<int *>(known + E);
+    int4 *tried = reinterpret_cast<int4 *>(lds + 1024);  // [E][choices] of up to kCounted: tiles, splits, their length, those all see
     const int per = (E + 511) / 512, b0 = min(tid * per, E), b1 = min(b0 + per, E);
-    const bool kept = E <= 2600;  // in LDS; larger batches read them again
+    const bool kept = E <= 2300, counted = E <= kCounted;  // in LDS; larger batches read them again
     auto load = [&](int b) {
         return kept ? known[b] : request(c, b);
     };
@@ -141,7 +143,14 @@ __device__ __forceinline__ void plan_chunks(const C &c, int *lds) {
     int n_j = 0, split_j = 0;
     for (int b = 4 * wave + (lane >> 4); b < E; b += 32) {
         int kt;
-        const int T = chunk_tiles(c, load(b), qb, &kt), n = T * div_ceil(kt, l_j);
+        const Request r = load(b);
+        const int T = chunk_tiles(c, r, qb, &kt), S = div_ceil(kt, l_j), n = T * S;
+        if (counted) {
+            // (made here, an entry and a length once, not by each of the wavefronts below: the plan of
+            // 24 drafts and two groups 11.5 -> 9.4 us, with the slots in LDS)
+            const int most = div_ceil(kt, max(S, 1)), past = max(r.kv - r.n, 0);
+            tried[b * kChoices + j] = make_int4(T, S, most, min(div_floor(past / kChunkKeys, max(most, 1)), S));
+        }
         n_j += n;
         split_j += is_group(c, b) || kt > l_j ? n : 0;
     }
@@ -154,23 +163,22 @@ __device__ __forceinline__ void plan_chunks(const C &c, int *lds) {
     const int64_t N = (int64_t)n_j * c.Hkv, slots_j = (int64_t)split_j * c.Hkv;
     const int part_j = min(l_j, longest);
     const float part = (float)part_j, cus = (float)c.cus;
-    const bool counted = E <= kCounted;
     if (counted) {  // wavefront w: query tiles times splits of at least (w + 1) / 8 of a part
         const int x = div_ceil(part_j * (wave + 1), kLevels);
         int n_x = 0;
         for (int b = lane >> 4; b < E && N > c.cus && N <= kRounds * c.cus; b += 4) {
-            const Request r = load(b);
-            if (r.n * c.G <= c.most_d) continue;
-            int kt;
-            const int T = chunk_tiles(c, r, qb, &kt), S = div_ceil(kt, l_j), past = r.kv - r.n;
-            const int most = div_ceil(kt, max(S, 1)), prefix = (min(r.prefix, r.kv) + kChunkKeys - 1) / kChunkKeys;
+            const int4 v = tried[b * kChoices + j];
+            const int T = v.x, S = v.y, most = v.z, whole = v.w;  // most: 0 of an entry without chunks
             if (most < x) continue;
             // splits that the first query tile sees whole, and the others
-            const int whole = min(div_floor(max(past, 0) / kChunkKeys, most), S);
             n_x += whole * T;
+            if (whole == S) continue;
+            const Request r = load(b);
+            const int kt = max((r.kv + kChunkKeys - 1) / kChunkKeys, 1), past = r.kv - r.n;
+            const int prefix = (min(r.prefix, r.kv) + kChunkKeys - 1) / kChunkKeys;
+            const int q = most - (most * S > kt), rest = kt - q * S;  // as split_range
             for (int s = whole; s < S; ++s) {
-                int t0, t1;
-                split_range(kt, S, s, &t0, &t1);
+                const int t0 = s * q + min(s, rest), t1 = t0 + q + (s < rest);
                 if (t1 - t0 < x) break;
                 // tiles that end in or behind the x-th key tile of the split
                 const int need = kChunkKeys * (t0 + x - 1) - past + 1;
@@ -229,6 +237,7 @@ __device__ __forceinline__ void plan_chunks(const C &c, int *lds) {
         (void)chunk_tiles(c, load(b), qb, &kt);
         first[b] = start[b] + before;
         slot[b] = slots_before;
+        if (kept) slot_of[b] = slots_before;
         slots_before += is_group(c, b) || kt > len ? k : 0;
     }
     __syncthreads();
@@ -254,7 +263,7 @@ __device__ __forceinline__ void plan_chunks(const C &c, int *lds) {
         it.kvh = div_floor(q, it.splits);
         it.split = q - it.kvh * it.splits;
         split_range(kt, it.splits, it.split, &it.t0, &it.t1);
-        it.slot = slot[lo];
+        it.slot = kept ? slot_of[lo] : slot[lo];
         it.spare[0] = it.spare[1] = 0;
         const int keys = sees(it.rq, min((it.tile + 1) * qb, it.rq.n) - 1);
         *own = max(min(it.t1, (keys + kChunkKeys - 1) / kChunkKeys) - it.t0, 0);
