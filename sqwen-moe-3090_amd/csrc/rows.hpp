@@ -40,9 +40,10 @@ struct MoveRows {
     // of every rotation pair: radians a position, which position (t, h, w, e) turns it
     double freq[kMostRot / 2];
     uint8_t component[kMostRot / 2];
-    // set by the launch: its first row, rows of a workgroup, reciprocals of what its threads divide by
+    // set by the launch: its first row, rows of a workgroup, units that its threads rotate in one pass,
+    // reciprocals of what they divide by
     int64_t first;
-    int rows;
+    int rows, pass;
     float recip_half, recip_turned, recip_lanes, recip_copy, recip_rest;
 };
 int launch_move_rows_q4_0(MoveRows p, hipStream_t s);

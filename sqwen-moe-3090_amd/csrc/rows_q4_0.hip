@@ -105,8 +105,9 @@ __device__ __forceinline__ float2 cos_sin(double x) {
 // move_rows: the rows' places and the (cos, sin) of their rotation pairs go to LDS; a rotated
 // block is 8 lanes of 4 values, which read their own codes and their partners' (half dims away,
 // both 4 bytes at one place) and quantize again; the other blocks are copied. A thread has the loads
-// of kTurns rotated units, or kCopies copied ones, in flight together. In place all loads of a row's
-// rotated blocks stand before its stores (a row's lanes may be in two wavefronts).
+// of kTurns rotated units, or kCopies copied ones, in flight together. In place a head's partners must
+// all be read before a block of it is stored: a pass of the threads then takes whole heads, and a
+// barrier stands between its loads and its stores (a head's lanes may be in two wavefronts).
 typedef uint32_t Bytes12 __attribute__((ext_vector_type(3), aligned(4)));
 constexpr int kTurns = 2, kCopies = 4;
 
@@ -139,14 +140,15 @@ __global__ __launch_bounds__(kThreads) void move_rows_q4_0_kernel(MoveRows p) {
     const int turned = (p.n_rot + 31) >> 5, head_bytes = p.head_dim / SQA_QK4_0 * SQA_Q4_0_BLOCK_BYTES;
     const int lanes = 8 * turned, per_row = lanes * p.heads;
     __syncthreads();
-    for (int u0 = tid; u0 - tid < rows * per_row; u0 += kTurns * kThreads) {
+    for (int u0 = 0; u0 < rows * per_row; u0 += p.pass) {
         float out[kTurns][4];
         uint8_t *to[kTurns];
 #pragma unroll
         for (int n = 0; n < kTurns; ++n) {
-            const int u = u0 + n * kThreads, k = div_by(u, p.recip_turned), hl = u - mul(k, per_row), h = div_by(hl, p.recip_lanes);
+            const int i = tid + n * kThreads, u = u0 + i;
+            const int k = div_by(u, p.recip_turned), hl = u - mul(k, per_row), h = div_by(hl, p.recip_lanes);
             const int d0 = 4 * (hl - mul(h, lanes));
-            const int64_t at = k < rows ? places[2 * k] : -1;
+            const int64_t at = i < p.pass && k < rows ? places[2 * k] : -1;
             to[n] = nullptr;
             if (at < 0) continue;
             to[n] = p.dst + places[2 * k + 1] + mul(h, head_bytes) + (d0 >> 5) * SQA_Q4_0_BLOCK_BYTES;
@@ -257,6 +259,9 @@ int launch_move_rows_q4_0(MoveRows p, hipStream_t s) {
     p.rows = rows_of_workgroup(p.n, (lanes + rest) * p.heads, 8, 32);
     p.recip_half = recip(p.n_rot / 2);
     p.recip_turned = recip(lanes * p.heads), p.recip_lanes = recip(lanes);
+    // (between two caches a head may lie across two passes)
+    p.pass = kTurns * kThreads;
+    if (p.src == p.dst && lanes) p.pass -= p.pass % (int)lanes;
     p.recip_copy = recip(rest * p.heads), p.recip_rest = recip(rest);
     const size_t lds = (size_t)p.rows * (16 + (p.n_rot / 2) * sizeof(float2));
     const auto kernel = step == 16   ? move_rows_q4_0_kernel<uint32x4, 16>
