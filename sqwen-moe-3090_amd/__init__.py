@@ -303,16 +303,17 @@ def set_rows_q4_0(cache, src, idx, stream=None):
 def get_rows_q4_0(cache, idx, out=None, dtype=torch.float32, stream=None):
     """out[i] = the values of cache row idx[i] (GGML_OP_GET_ROWS of a q4_0 cache): set_rows_q4_0's counterpart.
 
-    cache: uint8 (rows, ..., row_bytes) contiguous; idx: int64 (n,), an index outside the cache reads as zeros;
-    out: float32 or float16 (n, ne0) with contiguous elements, made here of dtype where it is not given."""
+    cache: uint8 (rows, ..., row_bytes) contiguous, rows of whole blocks; idx: int64 (n,), an index outside the cache
+    reads as zeros; out: float32 or float16 (n, ne0) with contiguous elements, made here of dtype where it is not given."""
     if stream is None and out is not None:
         rc = (_host or _load_host()).get_rows(cache, idx, out)
         if rc is not None:
             if rc:
                 _check(rc)
             return out
+    _need(cache.dim() >= 2 and cache.dtype == torch.uint8 and cache.is_contiguous() and
+          math.prod(cache.shape[1:]) % Q4_0_BLOCK == 0, "cache must be contiguous uint8 (rows, ...), rows of whole 18-byte blocks")
     with _on(cache.device, idx=idx, out=out):
-        _need(cache.dim() >= 2 and cache.dtype == torch.uint8 and cache.is_contiguous(), "cache must be contiguous uint8 (rows, ...)")
         _need(idx.dim() == 1 and idx.dtype == torch.int64, "idx must be int64 (n,)")
         rb, n = math.prod(cache.shape[1:]), idx.shape[0]
         ne0 = rb // Q4_0_BLOCK * QK4_0

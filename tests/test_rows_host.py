@@ -108,3 +108,14 @@ def test_move_rows_refuses_pairs_that_turn_too_fast(sqa):
         if not ok:
             assert sqa.lib().sqa_move_rows_q4_0(ref(c[0]), ref(c[1]), ref(to), ref(frm), ref(delta), ref(rope), None) == 2
             assert "radians" in sqa.last_error()
+
+
+@pytest.mark.parametrize("shape", [(4, 20), (4, 2, 143), (4, 17), (4, 3, 10)])
+def test_get_rows_refuses_rows_of_broken_blocks(sqa, shape):
+    import torch
+
+    c, i = torch.zeros(shape, dtype=torch.uint8), torch.zeros(2, dtype=torch.int64)
+    ne0 = c[0].numel() // 18 * 32
+    for kw in ({}, {"out": torch.zeros((2, ne0))}, {"dtype": torch.float16}):
+        with pytest.raises(sqa.SqaError, match="whole 18-byte blocks"):
+            sqa.get_rows_q4_0(c, i, **kw)
