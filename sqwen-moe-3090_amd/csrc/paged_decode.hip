@@ -78,7 +78,8 @@ constexpr float kPShift = -(float)kPBits;
 constexpr int kMaxDvExp = 18;
 static_assert(2 * kMaxRequests * 4 <= kLdsBytes, "tiles of every request and group");
 static_assert(2 * kLdsBytes <= 160 * 1024, "two workgroups per CU");
-static_assert((513 + 7 * 2300) * 4 <= kLdsBytes && 4 * 1024 + 64 * 16 * 16 <= kLdsBytes && 513 + 7 * 64 <= 1024 && (512 + kMaxRequests + 8) * 4 <= kLdsBytes, "the plan's LDS");
+static_assert((513 + 7 * kPlanKept) * 4 <= kLdsBytes && (513 + 2 * kMaxRequests) * 4 <= kLdsBytes, "the plan's LDS");
+static_assert(513 + 7 * kCounted <= kTriedAt && kTriedAt * 4 + kCounted * kChoices * 16 <= kLdsBytes, "its tried lengths");
 static_assert(4 * 2 * 64 * 32 <= (kVStages - 1) * kTensorBytes, "Q operands must fit in V stages 1..2");
 
 typedef const __attribute__((address_space(3))) uint32_t lds_u32;  // LDS dword from a raw LDS address

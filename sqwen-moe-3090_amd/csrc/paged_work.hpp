@@ -75,11 +75,13 @@ __device__ constexpr int kTried[kChoices] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20
 // batches, this costs 0.3% on average and 7% at most.
 constexpr float kWg = 4.5f, kMerge = 0.7f, kMergeSlot = 0.014f;
 constexpr int kCounted = 64, kLevels = 8, kRounds = 4;
+constexpr int kPlanKept = 2300, kTriedAt = 1024;  // entries that LDS holds whole; where the tried lengths stand in it
 
 // Groups of a shared prefix are requests whose tokens all see all keys and whose parts all go
 // through the merge.
 //
-// Run by all 512 threads of one workgroup; lds: 513 + 7 * 2300 words, or 512 + B + 1.
+// Run by all 512 threads of one workgroup; lds: 513 + 7 E words for E entries, 513 + E above kPlanKept, and the
+// tried lengths.
 // Lanes are requests (a run of them above 512), then lengths that are tried, then items.
 template <class C>
 __device__ __forceinline__ void plan_chunks(const C &c, int *lds) {
@@ -91,9 +93,9 @@ __device__ __forceinline__ void plan_chunks(const C &c, int *lds) {
     int *sums = lds, *start = lds + 512;                      // start: first item of every request
     Request *known = reinterpret_cast<Request *>(start + E + 1);
     int *slot_of = reinterpret_cast<int *>(known + E);
-    int4 *tried = reinterpret_cast<int4 *>(lds + 1024);  // [E][choices] of up to kCounted: tiles, splits, their length, those all see
+    int4 *tried = reinterpret_cast<int4 *>(lds + kTriedAt);  // [E][choices] of up to kCounted: tiles, splits, their length, those all see
     const int per = (E + 511) / 512, b0 = min(tid * per, E), b1 = min(b0 + per, E);
-    const bool kept = E <= 2300, counted = E <= kCounted;  // in LDS; larger batches read them again
+    const bool kept = E <= kPlanKept, counted = E <= kCounted;  // in LDS; larger batches read them again
     auto load = [&](int b) {
         return kept ? known[b] : request(c, b);
     };
