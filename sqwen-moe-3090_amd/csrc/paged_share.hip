@@ -6,7 +6,8 @@
 // rather than wait for another one's sums; then it writes the request's own tokens.
 //
 // Bound by latency: arrays, sums, stores. 8 requests 3.0 us, where an empty launch is 2.2; 1024
-// with 8192 tokens 4.8 (6.2 with a length loaded behind every group id, and sums through LDS).
+// with 8192 tokens 4.8 (6.2 with a length loaded behind every group id, and sums through LDS). The
+// reads of all by all grow with the square: 4096 requests 20 us, with as many groups 59.
 #include "paged_attn.hpp"
 
 namespace sqa {
